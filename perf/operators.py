@@ -192,7 +192,7 @@ def prepare(case, seed):
         state["values"], state["row_scales"] = _values8(x)
     if own:
         from rust_deeplearning_b200.kernels import ops
-        state["matrix"] = ops.mx4_weight(state["codes"], state["scales"], case["in"])
+        state["matrix"] = ops.mx4_weight(state["codes"], state["scales"], case["in"], gated=case["form"] == "gated")
         if case["op"] == "product":
             groups = -(-case["in"] // GROUP)
             state["packed"] = ops.mx8_rows(state["values"].contiguous(), state["row_scales"].reshape(case["rows"], -1)[:, :groups].contiguous())
