@@ -10,6 +10,7 @@
 // dtype codes of the C interface
 #define RDL_F32 0
 #define RDL_BF16 1
+#define RDL_MX8 2     // rows of 8-bit values with a scale a group (microscaling.cuh); where an operand says that it takes them
 
 // Launchers return 0 on success.  On failure they return non-zero and leave a message
 // that rdl_last_error() hands to the caller.
@@ -43,6 +44,8 @@ void rdl_set_error(const char* fmt, ...);
 
 // About a second of clock cycles: the default limit of a wait inside a kernel.
 #define RDL_WAIT_CYCLES 2000000000LL
+// About 0.1 ms: what a block that has given up a wait leaves its own copies to arrive in before it ends.
+#define RDL_COPY_DRAIN_CYCLES 200000LL
 extern int g_rdl_wait_test_code;
 extern long long g_rdl_wait_test_cycles;
 extern int g_rdl_wait_test_extra;

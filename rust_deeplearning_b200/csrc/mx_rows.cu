@@ -1,0 +1,349 @@
+// Rows and weights into the microscaling formats (microscaling.cuh), and weights back.
+//
+// rdl_norm_mx8: what stands before a product of 8-bit rows, in one pass over the row:
+//     t = first ? rms_norm(x; first) : x;  h = residual + t (written to residual_out);  y = second ? rms_norm(h; second) : h
+//     y -> e4m3 with a scale a group
+// Bound by memory: x is read once, the residual read and written once, a byte a column is written.  A block takes a row, held in
+// registers between its passes (rows of up to 8,192 columns; wider ones are read again).  A thread holds four neighbouring columns, so
+// a group is eight lanes of a warp and a block of 128 columns one warp: the largest magnitude is three shuffles away and the four
+// scale codes of a block leave as one word.  The threads a row gets depend on its width alone, so its result does
+// not depend on how many rows a step has.
+//
+// rdl_pack_mx4: a lane takes eight columns (16 bytes of bfloat16 in, 4 bytes of codes out), a group is four lanes.  Memory bound.
+// rdl_expand_mx4: the values the codes stand for; exact in bfloat16 for scales from 2^-125 up to 2^125.
+#include <cuda_fp16.h>
+
+#include "api.h"
+#include "launch.cuh"
+#include "microscaling.cuh"
+#include "row_vec.cuh"
+
+namespace {
+
+struct NormMxArgs {
+    const void* x; int x_dtype;
+    const void* w1; int w1_dtype; float eps1, off1;
+    const float* res; float* res_out;
+    const void* w2; int w2_dtype; float eps2, off2;
+    uint8_t* values; uint8_t* scales;
+    int rows, width, blocks, padded_rows;
+};
+
+// four consecutive columns from column c of a row that starts at element `base`; zeros beyond the width
+template <bool VEC>
+__device__ __forceinline__ void load_columns(const void* p, long long base, int c, int width, int dtype, float (&v)[4]) {
+    if (VEC) {
+        if (c < width) rn_load4(p, base + c, dtype, v);
+        else v[0] = v[1] = v[2] = v[3] = 0.f;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = c + k < width ? rdl_load(p, base + c + k, dtype) : 0.f;
+    }
+}
+
+// a warp's 128 columns of one row, four a lane: codes and the block's four scale codes
+__device__ __forceinline__ void store_block(const float (&v)[4], uint8_t* values, uint8_t* scales, int lane) {
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = mx_larger(m, v[k]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = mx_larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t c = mx8_scale_code(m);
+    const float inv = mx_inverse_scale(c);
+    *reinterpret_cast<uint32_t*>(values + lane * 4) = mx_to_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    uint32_t word = c << (lane & 24);                       // the group's byte of the word
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    word |= __shfl_xor_sync(0xffffffffu, word, 16);
+    if (lane == 0) *reinterpret_cast<uint32_t*>(scales) = word;
+}
+
+template <int ITER, bool VEC>
+__global__ void __launch_bounds__(256) norm_mx8_kernel(const __grid_constant__ NormMxArgs a) {
+    __shared__ float scratch[33];
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const int r = blockIdx.x, lane = threadIdx.x & 31;
+    const long long base = (long long)r * a.width;
+    float v[ITER][4], h[ITER][4];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 4;
+        load_columns<VEC>(a.x, base, c, a.width, a.x_dtype, v[i]);
+        if (a.res) load_columns<VEC>(a.res, base, c, a.width, RDL_F32, h[i]);
+        else h[i][0] = h[i][1] = h[i][2] = h[i][3] = 0.f;
+    }
+    if (a.w1) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ss = fmaf(v[i][k], v[i][k], ss);
+        const float inv = 1.0f / sqrtf(block_sum(ss, scratch) / (float)a.width + a.eps1);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            float w[4];
+            load_columns<VEC>(a.w1, 0, (i * (int)blockDim.x + (int)threadIdx.x) * 4, a.width, a.w1_dtype, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = v[i][k] * inv * (w[k] + a.off1);
+        }
+    }
+    float s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (a.res) v[i][k] = h[i][k] + v[i][k];
+            s2 = fmaf(v[i][k], v[i][k], s2);
+        }
+        if (a.res_out) {
+            if (VEC) {
+                if (c < a.width) rn_store4(a.res_out + base + c, v[i]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c + k < a.width) a.res_out[base + c + k] = v[i][k];
+            }
+        }
+    }
+    float inv2 = 1.f;
+    if (a.w2) inv2 = 1.0f / sqrtf(block_sum(s2, scratch) / (float)a.width + a.eps2);
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 4;
+        const int block = c / MX_BLOCK;                     // one for the whole warp
+        if (block >= a.blocks) break;
+        if (a.w2) {
+            float w[4];
+            load_columns<VEC>(a.w2, 0, c, a.width, a.w2_dtype, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = c + k < a.width ? v[i][k] * inv2 * (w[k] + a.off2) : 0.f;
+        }
+        store_block(v[i], a.values + (long long)r * a.blocks * MX_BLOCK + block * MX_BLOCK,
+                    a.scales + ((long long)block * a.padded_rows + r) * 4, lane);
+    }
+}
+
+// Rows wider than the registers of a block: the row is read once a pass.
+template <bool VEC>
+__global__ void __launch_bounds__(256) norm_mx8_wide_kernel(const __grid_constant__ NormMxArgs a) {
+    __shared__ float scratch[33];
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const int r = blockIdx.x, lane = threadIdx.x & 31, step = blockDim.x * 4;
+    const long long base = (long long)r * a.width;
+    float inv = 1.f;
+    if (a.w1) {
+        float ss = 0.f;
+        for (int c = threadIdx.x * 4; c < a.width; c += step) {
+            float v[4];
+            load_columns<VEC>(a.x, base, c, a.width, a.x_dtype, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ss = fmaf(v[k], v[k], ss);
+        }
+        inv = 1.0f / sqrtf(block_sum(ss, scratch) / (float)a.width + a.eps1);
+    }
+    // h of four columns: the sum of x's norm and the residual
+    auto sum_at = [&](int c, float (&v)[4]) {
+        load_columns<VEC>(a.x, base, c, a.width, a.x_dtype, v);
+        if (a.w1) {
+            float w[4];
+            load_columns<VEC>(a.w1, 0, c, a.width, a.w1_dtype, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = v[k] * inv * (w[k] + a.off1);
+        }
+        if (a.res) {
+            float h[4];
+            load_columns<VEC>(a.res, base, c, a.width, RDL_F32, h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = h[k] + v[k];
+        }
+    };
+    float s2 = 0.f;
+    if (a.w2 || a.res_out) {
+        for (int c = threadIdx.x * 4; c < a.width; c += step) {
+            float v[4];
+            sum_at(c, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s2 = fmaf(v[k], v[k], s2);
+                if (a.res_out && c + k < a.width) a.res_out[base + c + k] = v[k];
+            }
+        }
+    }
+    float inv2 = 1.f;
+    if (a.w2) inv2 = 1.0f / sqrtf(block_sum(s2, scratch) / (float)a.width + a.eps2);
+    for (int c = threadIdx.x * 4; c < a.blocks * MX_BLOCK; c += step) {      // whole warps: both sides are multiples of 128
+        float v[4];
+        // the sum may have replaced the residual it was formed from: this thread reads what it wrote itself
+        if (a.res_out) load_columns<VEC>(a.res_out, base, c, a.width, RDL_F32, v);
+        else sum_at(c, v);
+        if (a.w2) {
+            float w[4];
+            load_columns<VEC>(a.w2, 0, c, a.width, a.w2_dtype, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = c + k < a.width ? v[k] * inv2 * (w[k] + a.off2) : 0.f;
+        }
+        const int block = c / MX_BLOCK;
+        store_block(v, a.values + (long long)r * a.blocks * MX_BLOCK + block * MX_BLOCK,
+                    a.scales + ((long long)block * a.padded_rows + r) * 4, lane);
+    }
+}
+
+struct PackArgs {
+    const void* w; int dtype;
+    uint8_t* codes; uint8_t* scales;
+    int rows, columns, blocks;
+    int half, half_padded;                                  // gated: source rows from `half` on lie from `half_padded` on
+};
+
+// a warp takes 256 columns of one row
+template <bool VEC>
+__global__ void __launch_bounds__(256) pack_mx4_kernel(const __grid_constant__ PackArgs a) {
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int pieces = (a.blocks + 1) / 2;
+    const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (item >= (long long)a.rows * pieces) return;
+    const int row = (int)(item / pieces), piece = (int)(item - (long long)row * pieces);
+    const int to = a.half > 0 && row >= a.half ? row - a.half + a.half_padded : row;
+    const int c = piece * 256 + lane * 8;
+    const long long base = (long long)row * a.columns;
+    float v[8];
+    float (&lo)[4] = reinterpret_cast<float (&)[4]>(v[0]);
+    float (&hi)[4] = reinterpret_cast<float (&)[4]>(v[4]);
+    load_columns<VEC>(a.w, base, c, a.columns, a.dtype, lo);
+    load_columns<VEC>(a.w, base, c + 4, a.columns, a.dtype, hi);
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = mx_larger(m, v[k]);
+    m = mx_larger(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = mx_larger(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t code = mx4_scale_code(m);
+    const float inv = mx_inverse_scale(code);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= inv;
+    uint32_t word = code << ((lane & 12) * 2);              // lanes 4 q to 4 q + 3: byte q of the block's word
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    const int block = c / MX_BLOCK;
+    if (block >= a.blocks) return;
+    *reinterpret_cast<uint32_t*>(a.codes + ((long long)to * a.blocks * MX_BLOCK + c) / 2) = mx_to_e2m1(v);
+    if ((lane & 15) == 0)
+        *reinterpret_cast<uint32_t*>(a.scales + (((long long)(to / MX_UNIT) * a.blocks + block) * MX_UNIT + to % MX_UNIT) * 4) = word;
+}
+
+struct ExpandArgs {
+    const uint8_t* codes; const uint8_t* scales;
+    void* out; int dtype;
+    int rows, columns, blocks, half, half_padded;
+};
+
+template <bool VEC>
+__global__ void __launch_bounds__(256) expand_mx4_kernel(const __grid_constant__ ExpandArgs a) {
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const int words = a.blocks * (MX_BLOCK / 8);            // of eight codes, a row
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (long long)a.rows * words) return;
+    const int row = (int)(i / words), word = (int)(i - (long long)row * words), c = word * 8;
+    const int from = a.half > 0 && row >= a.half ? row - a.half + a.half_padded : row;
+    uint32_t h[4];
+    mx_from_e2m1(*reinterpret_cast<const uint32_t*>(a.codes + (long long)from * words * 4 + word * 4), h);
+    const int block = c / MX_BLOCK;
+    const float s = mx_scale(a.scales[(((long long)(from / MX_UNIT) * a.blocks + block) * MX_UNIT + from % MX_UNIT) * 4 + c % MX_BLOCK / MX_GROUP]);
+    const long long base = (long long)row * a.columns + c;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        v[2 * k] = f.x * s;
+        v[2 * k + 1] = f.y * s;
+    }
+    if (VEC && c + 8 <= a.columns) {
+        if (a.dtype == RDL_BF16) {
+            uint4 raw;
+            __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+            *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + base) = raw;
+        } else {
+            *reinterpret_cast<float4*>((float*)a.out + base) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>((float*)a.out + base + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + k < a.columns) rdl_store(a.out, base + k, a.dtype, v[k]);
+    }
+}
+
+}  // namespace
+
+extern "C" int rdl_norm_mx8(const void* x, int x_dtype, const void* w1, int w1_dtype, float eps1, float off1,
+                            const float* residual, float* residual_out, const void* w2, int w2_dtype, float eps2, float off2,
+                            void* values, void* scales, int n_rows, int width, void* stream) {
+    if (n_rows == 0) return 0;
+    RDL_REQUIRE(x && values && scales, "norm_mx8: missing operand");
+    RDL_REQUIRE(rdl_valid_dtype(x_dtype) && (!w1 || rdl_valid_dtype(w1_dtype)) && (!w2 || rdl_valid_dtype(w2_dtype)), "norm_mx8: bad dtype");
+    RDL_REQUIRE(n_rows >= 0 && width > 0, "norm_mx8: bad sizes rows=%d width=%d", n_rows, width);
+    RDL_REQUIRE((uintptr_t)values % 4 == 0 && (uintptr_t)scales % 4 == 0, "norm_mx8: the results must start on 4-byte boundaries");
+    const NormMxArgs a{x, x_dtype, w1, w1_dtype, eps1, off1, residual, residual_out, w2, w2_dtype, eps2, off2,
+                       (uint8_t*)values, (uint8_t*)scales, n_rows, width, mx_blocks(width), (n_rows + 3) / 4 * 4};
+    const bool vec = width % 4 == 0 && aligned16(x) && aligned16(w1) && aligned16(w2) && aligned16(residual) && aligned16(residual_out);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int quads = a.blocks * (MX_BLOCK / 4);
+    // the fewest whole warps that hold the row with the fewest columns a thread, up to 256 threads
+    const int iter = quads <= 256 ? 1 : (quads <= 512 ? 2 : (quads <= 1024 ? 4 : 8));
+    const int threads = ((quads + iter - 1) / iter + 31) / 32 * 32;
+    cudaError_t e;
+#define RDL_NORM_MX8(I) (e = vec ? rdl_launch(norm_mx8_kernel<I, true>, dim3(n_rows), dim3(threads), 0, st, a) \
+                                 : rdl_launch(norm_mx8_kernel<I, false>, dim3(n_rows), dim3(threads), 0, st, a))
+    if (quads > 256 * RN_MAX_IT)
+        e = vec ? rdl_launch(norm_mx8_wide_kernel<true>, dim3(n_rows), dim3(256), 0, st, a) : rdl_launch(norm_mx8_wide_kernel<false>, dim3(n_rows), dim3(256), 0, st, a);
+    else if (iter == 1) RDL_NORM_MX8(1);
+    else if (iter == 2) RDL_NORM_MX8(2);
+    else if (iter == 4) RDL_NORM_MX8(4);
+    else RDL_NORM_MX8(8);
+#undef RDL_NORM_MX8
+    RDL_CHECK_EX(e, "norm_mx8");
+    return 0;
+}
+
+extern "C" int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales, int rows, int columns, int gated, void* stream) {
+    RDL_REQUIRE(w && codes && scales, "pack_mx4: missing operand");
+    RDL_REQUIRE(rdl_valid_dtype(dtype), "pack_mx4: bad dtype %d", dtype);
+    RDL_REQUIRE(rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "pack_mx4: bad sizes rows=%d columns=%d", rows, columns);
+    RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "pack_mx4: the results must start on 16-byte boundaries");
+    const int half = gated ? rows / 2 : 0;
+    const PackArgs a{w, dtype, (uint8_t*)codes, (uint8_t*)scales, rows, columns, mx_blocks(columns), half, (half + MX_UNIT - 1) / MX_UNIT * MX_UNIT};
+    const long long warps = (long long)rows * ((a.blocks + 1) / 2), grid = (warps + 7) / 8;
+    RDL_REQUIRE(grid <= 0x7fffffffLL, "pack_mx4: %d x %d is too large", rows, columns);
+    cudaStream_t st = (cudaStream_t)stream;
+    const cudaError_t e = columns % 4 == 0 && aligned16(w) ? rdl_launch(pack_mx4_kernel<true>, dim3((unsigned)grid), dim3(256), 0, st, a)
+                                                           : rdl_launch(pack_mx4_kernel<false>, dim3((unsigned)grid), dim3(256), 0, st, a);
+    RDL_CHECK_EX(e, "pack_mx4");
+    // The products read weights before the kernel ahead of them has ended (launch.cuh).  Something that is launched the ordinary way
+    // comes in between, so that a product right behind this call finds the codes written.
+    const long long units = gated ? 2LL * (a.half_padded / MX_UNIT) : (rows + MX_UNIT - 1) / MX_UNIT;
+    RDL_CUDA(cudaMemsetAsync((uint8_t*)scales + units * a.blocks * (MX_UNIT * 4), 0, 16, st), "pack_mx4");
+    return 0;
+}
+
+extern "C" int rdl_expand_mx4(const void* codes, const void* scales, void* out, int dtype, int rows, int columns, int gated, void* stream) {
+    RDL_REQUIRE(codes && scales && out, "expand_mx4: missing operand");
+    RDL_REQUIRE(rdl_valid_dtype(dtype), "expand_mx4: bad dtype %d", dtype);
+    RDL_REQUIRE(rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "expand_mx4: bad sizes rows=%d columns=%d", rows, columns);
+    RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "expand_mx4: the codes must start on 16-byte boundaries");
+    const int half = gated ? rows / 2 : 0;
+    const ExpandArgs a{(const uint8_t*)codes, (const uint8_t*)scales, out, dtype, rows, columns, mx_blocks(columns), half,
+                       (half + MX_UNIT - 1) / MX_UNIT * MX_UNIT};
+    const long long words = (long long)rows * a.blocks * (MX_BLOCK / 8), grid = (words + 255) / 256;
+    RDL_REQUIRE(grid <= 0x7fffffffLL, "expand_mx4: %d x %d is too large", rows, columns);
+    cudaStream_t st = (cudaStream_t)stream;
+    const cudaError_t e = columns % 8 == 0 && aligned16(out) ? rdl_launch(expand_mx4_kernel<true>, dim3((unsigned)grid), dim3(256), 0, st, a)
+                                                             : rdl_launch(expand_mx4_kernel<false>, dim3((unsigned)grid), dim3(256), 0, st, a);
+    RDL_CHECK_EX(e, "expand_mx4");
+    return 0;
+}

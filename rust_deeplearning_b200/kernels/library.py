@@ -23,7 +23,7 @@ from concurrent.futures import ThreadPoolExecutor
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(_PKG, "csrc")
 LIB_NAME = "librdl_b200_kernels.so"
-ABI_VERSION = 25
+ABI_VERSION = 26
 
 # fast math is never enabled: the 32-bit path relies on exact tanhf/expf/sqrtf and plain FMA
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -188,6 +188,8 @@ FAULTS = {
     5: "attention_prefill_tc: a tile copy or a product did not complete",
     6: "gemm_tc (pairs of blocks): a stage or an accumulator was not handed over",
     7: "gemm_skinny: a weight copy did not complete",
+    8: "mx_stream: a weight copy did not complete",
+    9: "mx_tc: a stage or an accumulator was not handed over",
 }
 
 
@@ -429,6 +431,12 @@ _SIGNATURES = {
     "rdl_gemm_skinny_norm": [_P, _I, _P, _P, _I, _I, _I, _I, _I, _F, ctypes.POINTER(DeferredNormArgs), _P, _F, _P],
     "rdl_stream_rows": [_P, _I, _F, _P, _P, _P, _P, _I, _F, _P, _I, _I, _P],
     "rdl_gemm_tc": [_P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _F, _P],
+    "rdl_norm_mx8": [_P, _I, _P, _I, _F, _F, _P, _P, _P, _I, _F, _F, _P, _P, _I, _I, _P],
+    "rdl_pack_mx4": [_P, _I, _P, _P, _I, _I, _I, _P],
+    "rdl_expand_mx4": [_P, _P, _P, _I, _I, _I, _I, _P],
+    "rdl_mx_stream": [_P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _LL, _P, _P],
+    "rdl_mx_stream_slices": [_I, _I, _I],
+    "rdl_mx_tc": [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P],
     "rdl_random_normal": [_P, _I, _LL, ctypes.c_ulonglong, ctypes.c_double, _P],
     "rdl_sample": [_P, _P, _P, _I, _I, ctypes.POINTER(SamplingArgs), _P, _P, _P, _P, _P, _P],
     "rdl_upload_batch": [_P, _P, _I, _P, _I, _I, _I, _P],

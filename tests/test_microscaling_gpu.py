@@ -1,0 +1,379 @@
+"""4-bit weights, 8-bit rows and what is computed with them, against float64 (tests/plain_microscaling.py).
+
+Tolerances, from the formats and the arithmetic:
+  rounding to 4 or 8 bits of values that are given is exact: the same values, bit for bit;
+  a norm's result in 8 bits is off by half a step (2^-4 of the value, or 2^-10 of the scale where the value is small) and by what
+  float32 statistics move it (2^-18 of the value, generously);
+  a sum of K products in float: each of G groups is summed by the tensor core (32 terms, 2^-23 each) and joins a float sum:
+  (64 + G) 2^-23 of the sum of magnitudes; float32 rows enter with 22 bits: 2^-21 of the same more;
+  a bfloat16 result: 2^-8 of the value (and of the largest value of the row where a gate's hardware tanh, 2^-11, came before)."""
+import numpy as np
+import pytest
+import torch
+
+import plain_microscaling as plain
+from rust_deeplearning_b200.kernels import library, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def rnd(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def rows_for(m, k, kind, seed):
+    """Rows with quiet and loud ones, a row of zeros, a group of zeros."""
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(seed))
+    x *= torch.exp2(torch.arange(m).float() % 5 * 3 - 6)[:, None]
+    if m > 2:
+        x[m // 2] = 0
+    x[:, 32:64] = 0
+    x = x.to(DEV)
+    if kind == "mx8":
+        r = ops.pack_mx8(x)
+        return r, f64(r.dequantise())
+    x = x.to(torch.bfloat16 if kind == "bfloat16" else torch.float32)
+    return x, f64(x)
+
+
+def sum_tolerance(x, w, kind):
+    groups = -(-x.shape[1] // 32)
+    return (np.abs(x) @ np.abs(w).T) * ((64 + groups) * 2.0 ** -23 + (2.0 ** -21 if kind == "float32" else 0.0))
+
+
+def check(got, want, tol, what):
+    err = np.abs(f64(got) - want) - tol
+    assert np.isfinite(f64(got)).all(), f"{what}: non-finite output"
+    assert (err <= 0).all(), f"{what}: {float(err.max()):.3e} beyond the tolerance"
+
+
+# ---- the formats ----
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,columns,gated", [(1, 1, False), (3, 31, False), (17, 33, False), (16, 128, False), (50, 1003, False),
+                                                (30, 260, True), (2, 32, True)])
+def test_pack_mx4(rows, columns, gated, dtype):
+    w = rnd((rows, columns), dtype, rows, 0.02)
+    w *= torch.exp2(torch.randint(-30, 30, (rows, 1), generator=torch.Generator().manual_seed(1)).to(DEV)).to(dtype)
+    w[rows // 2, :32] = 0
+    want, codes = plain.quantise(f64(w), plain.E2M1)
+    packed = ops.pack_mx4(w, gated)
+    assert np.array_equal(f64(ops.expand_mx4(packed, torch.float32)), want)
+    assert np.array_equal(f64(ops.expand_mx4(packed)), want)             # exact in bfloat16 too
+    # the scales, and zeros in the padding
+    part = rows // 2 if gated else rows
+    by_row = packed.scales.permute(0, 2, 1, 3).reshape(packed.padded_rows, -1).cpu().numpy()
+    halves = np.split(by_row, 2) if gated else [by_row]
+    assert np.array_equal(np.concatenate([h[:part, :codes.shape[1]] for h in halves]), codes)
+    assert not any(h[part:].any() or h[:, codes.shape[1]:].any() for h in halves)
+    assert int(packed.codes.count_nonzero()) <= rows * -(-columns // 2)
+
+
+def test_pack_mx4_ties_and_edges():
+    """Every tie between two codes, both signs, the largest value, a group that is not finite, the smallest scales."""
+    w = torch.zeros((6, 64), device=DEV)
+    w[0, :16] = torch.tensor([6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5, -6.0])
+    w[1, 0], w[1, 32] = float("inf"), 1.0
+    w[2, 5] = float("nan")
+    w[3, 0], w[3, 1] = 2.0 ** -130, 2.0 ** -149
+    w[4, 0], w[4, 1] = 3.0e38, 1.0
+    w[5, 0], w[5, 32] = 6.0, 6.0000005
+    want, codes = plain.quantise(f64(w), plain.E2M1)
+    got = f64(ops.expand_mx4(ops.pack_mx4(w), torch.float32))
+    with np.errstate(over="ignore"):
+        want = want.astype(np.float32)                                   # 4 x 2^126 is not a float32: it comes back as an infinity
+    assert np.array_equal(got[[0, 3, 4, 5]], want[[0, 3, 4, 5]])
+    for r in (1, 2):
+        assert np.isnan(got[r, :32]).all() and np.array_equal(got[r, 32:], want[r, 32:])
+    assert codes[5, 0] == 127 and codes[5, 1] == 128
+
+
+def test_mx4_weight_from_codes_is_the_packed_one():
+    for rows, columns, gated in ((20, 75, False), (26, 128, True)):
+        w = rnd((rows, columns), torch.float32, 3)
+        packed = ops.pack_mx4(w, gated)
+        q, codes = plain.quantise(f64(w), plain.E2M1)
+        scale = 2.0 ** (codes - 127.0)
+        wide = plain.groups_of(q) / scale[..., None]
+        nib = (plain.nearest(wide, plain.E2M1) + 8 * (np.signbit(wide) & (wide != 0))).reshape(rows, -1)[:, :columns + columns % 2].astype(np.uint8)
+        if columns % 2:
+            nib[:, -1] = 13                                              # what lies behind the last column does not count
+        given = ops.mx4_weight(torch.from_numpy(nib[:, 0::2] | nib[:, 1::2] << 4).to(DEV), torch.from_numpy(codes.astype(np.uint8)).to(DEV), columns, gated)
+        assert torch.equal(given.scales, packed.scales)
+        assert np.array_equal(f64(ops.expand_mx4(given, torch.float32)), q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,columns", [(1, 1), (5, 31), (3, 128), (7, 1003), (2, 8192), (2, 8197), (3, 20000)])
+def test_pack_mx8(rows, columns, dtype):
+    x = rnd((rows, columns), dtype, 5, 3.0)
+    x[0, :1] = 448.0
+    want, codes = plain.quantise(f64(x), plain.E4M3)
+    got = ops.pack_mx8(x)
+    assert np.array_equal(f64(got.dequantise()), want)
+    padded = np.zeros((rows, -(-columns // 128) * 4))
+    padded[:, :codes.shape[1]] = codes
+    assert np.array_equal(got.scales.reshape(rows, -1).cpu().numpy(), padded)
+    again = ops.mx8_rows(got.values.contiguous(), got.scales.reshape(rows, -1)[:, :codes.shape[1]].contiguous())
+    assert torch.equal(again.values.view(torch.uint8), got.values.view(torch.uint8)) and torch.equal(again.scales, got.scales)
+
+
+def test_pack_mx8_groups_that_are_not_finite():
+    x = rnd((3, 96), torch.float32, 6)
+    x[0, 40], x[1, 0], x[1, 95] = float("inf"), float("nan"), float("-inf")
+    got = f64(ops.pack_mx8(x).dequantise())
+    want = plain.quantise(f64(x), plain.E4M3)[0]
+    bad = np.zeros((3, 3), bool)
+    bad[0, 1] = bad[1, 0] = bad[1, 2] = True
+    bad = np.repeat(bad, 32, axis=1)
+    assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,width", [(1, 64), (5, 80), (3, 131), (4, 2304), (2, 4608), (3, 8192), (2, 8196), (2, 10007)])
+def test_norm_mx8(rows, width, dtype):
+    x, res = rnd((rows, width), dtype, 1, 3.0), rnd((rows, width), torch.float32, 4, 2.0)
+    w1 = ops.NormParams(rnd((width,), dtype, 2, 0.5), 1e-5, 1.0)
+    w2 = ops.NormParams(rnd((width,), torch.float32, 3, 0.5), 1e-6, 0.0)
+    for first, second, with_res in ((w1, w2, True), (None, w2, True), (w1, None, True), (None, w2, False), (w1, w2, False)):
+        h = plain.rms_norm(f64(x), f64(w1.weight), 1e-5, 1.0) if first else f64(x)
+        own = res.clone() if with_res else None
+        h = h + f64(res) if with_res else h
+        y = plain.rms_norm(h, f64(w2.weight), 1e-6, 0.0) if second else h
+        got = ops.norm_mx8(x, first=first, residual=own, second=second)
+        scale = 2.0 ** (got.scales.reshape(rows, -1).cpu().numpy().astype(np.float64) - 127)
+        per_value = np.repeat(scale, 32, axis=1)[:, :width]
+        check(got.dequantise(), y, np.abs(y) * (2.0 ** -4 + 2.0 ** -18) + per_value * 2.0 ** -10, "rows")
+        amax = np.abs(plain.groups_of(y)).max(-1)
+        used = scale[:, :amax.shape[1]]
+        assert (amax <= 448 * used * (1 + 2.0 ** -18)).all() and (amax >= 224 * used * (1 - 2.0 ** -18)).all()
+        if with_res:
+            check(own, h, 2.0 ** -18 * np.abs(h) + 2.0 ** -18 * np.abs(f64(res)), "sum")
+            out = torch.full_like(own, float("nan"))
+            keep = res.clone()
+            again = ops.norm_mx8(x, first=first, residual=keep, second=second, residual_out=out)
+            assert torch.equal(out, own) and torch.equal(keep, res) and torch.equal(again.values.view(torch.uint8), got.values.view(torch.uint8))
+
+
+def test_norm_mx8_is_the_same_row_by_row():
+    x, res = rnd((9, 2304), torch.bfloat16, 1), rnd((9, 2304), torch.float32, 2)
+    w = ops.NormParams(rnd((2304,), torch.bfloat16, 3), 1e-6, 1.0)
+    whole = ops.norm_mx8(x, first=w, residual=res.clone(), second=w)
+    for r in range(9):
+        one = ops.norm_mx8(x[r:r + 1], first=w, residual=res[r:r + 1].clone(), second=w)
+        assert torch.equal(one.values.view(torch.uint8), whole.values[r:r + 1].view(torch.uint8)) and torch.equal(one.scales[0], whole.scales[r])
+
+
+def test_norm_mx8_beyond_32_bits():
+    """2.4e9 values: the last rows lie behind what 32 bits can count."""
+    rows, width = 600_000, 4096
+    x = torch.zeros((rows, width), dtype=torch.bfloat16, device=DEV)
+    x[-3:] = rnd((3, width), torch.bfloat16, 8)
+    got = ops.pack_mx8(x)
+    want = ops.pack_mx8(x[-3:].clone())
+    assert torch.equal(got.values[-3:].view(torch.uint8), want.values.view(torch.uint8)) and torch.equal(got.scales[-3:], want.scales)
+
+
+# ---- the products ----
+
+SHAPES = [(1, 1, 1), (1, 3, 32), (2, 16, 33), (5, 777, 1003), (8, 100, 128), (9, 17, 2304), (16, 333, 640), (16, 40, 14336)]
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mx8"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_few_rows(m, n, k, kind):
+    w = ops.pack_mx4(rnd((n, k), torch.float32, 7, 0.05))
+    x, x64 = rows_for(m, k, kind, 8)
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    want = x64 @ w64.T
+    tol = sum_tolerance(x64, w64, kind)
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32), want, tol, "float32")
+    check(ops.linear_mx4(x, w, out_dtype=torch.bfloat16), want, tol + np.abs(want) * 2.0 ** -8, "bfloat16")
+
+
+@pytest.mark.parametrize("m,n,k", [(17, 1, 1), (17, 40, 32), (100, 777, 1003), (128, 256, 128), (129, 257, 300), (300, 130, 2304), (40, 600, 14336)])
+def test_many_rows(m, n, k):
+    w = ops.pack_mx4(rnd((n, k), torch.float32, 7, 0.05))
+    x, x64 = rows_for(m, k, "mx8", 8)
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    want = x64 @ w64.T
+    tol = sum_tolerance(x64, w64, "mx8")
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32, status=status), want, tol, "float32")
+    check(ops.linear_mx4(x, w, status=status), want, tol + np.abs(want) * 2.0 ** -8, "bfloat16")
+    assert status.item() == 0
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_more_rows_of_a_tensor(kind):
+    w = ops.pack_mx4(rnd((70, 200), torch.float32, 7, 0.05))
+    x, x64 = rows_for(37, 200, kind, 8)
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32), x64 @ w64.T, sum_tolerance(x64, w64, kind), "rows")
+
+
+@pytest.mark.parametrize("act", ["gelu_pytorch_tanh", "silu", "swish_limit"])
+@pytest.mark.parametrize("m,n,k,kind", [(1, 1, 32, "bfloat16"), (7, 37, 300, "bfloat16"), (16, 100, 5000, "float32"), (9, 64, 128, "mx8"), (17, 65, 128, "mx8"),
+                                        (140, 190, 1003, "mx8"), (64, 33, 40, "mx8")])
+def test_gated(m, n, k, kind, act):
+    w = ops.pack_mx4(rnd((2 * n, k), torch.float32, 9, 0.1), gated=True)
+    x, x64 = rows_for(m, k, kind, 10)
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    param = 7.0 if act == "swish_limit" else 0.0
+    want = plain.gated(x64 @ w64.T, act, param)
+    got = ops.linear_gated_mx4(x, w, act, param)
+    # the activations' slopes are at most 1.2 (1.8 with the factor 1.702), so an error of a half moves the result by 2 (|g| + |u| + 1) times it
+    t = sum_tolerance(x64, w64, kind)
+    g, u = np.split(np.abs(x64 @ w64.T), 2, axis=-1)
+    tol = 2 * (g + u + 1) * (t[:, :n] + t[:, n:])
+    fast = 2.0 ** -10 * np.maximum(g, 1) * (u + 1)                       # the hardware's tanh and exponential
+    exact_kind = kind == "float32"
+    check(got, want, tol + (2.0 ** -21 * np.abs(want) if exact_kind else np.abs(want) * 2.0 ** -8 + fast), act)
+    rows = ops.linear_gated_mx4(x, w, act, param, out_mx8=True)
+    scale = np.repeat(2.0 ** (rows.scales.reshape(m, -1).cpu().numpy().astype(np.float64) - 127), 32, axis=1)[:, :n]
+    check(rows.dequantise(), want, tol + fast + np.abs(want) * 2.0 ** -4 * (1 + 2.0 ** -6) + scale * 2.0 ** -10, act + " in 8 bits")
+    # the padding of the 8-bit result is zeros: the product behind it reads it
+    assert not rows._values[:m, n:].any() and not rows.scales.reshape(m, -1)[:, -(-n // 32):].any()
+
+
+@pytest.mark.parametrize("m,kind", [(3, "bfloat16"), (12, "float32"), (16, "mx8"), (50, "mx8")])
+def test_epilogues(m, kind):
+    w = ops.pack_mx4(rnd((90, 256), torch.float32, 11, 0.2))
+    x, x64 = rows_for(m, 256, kind, 12)
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    y, tol = x64 @ w64.T, sum_tolerance(x64, w64, kind)
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32, softcap=5.0), 5.0 * np.tanh(y / 5.0), tol + 2.0 ** -20 * 5, "soft-cap")
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32, activation="relu2"), np.maximum(y, 0) ** 2, 2 * np.abs(y) * tol + tol ** 2 + 2.0 ** -22 * y * y, "relu2")
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32, activation="silu_plain"), plain.act(y, "silu"), 2 * tol + 2.0 ** -20 * np.abs(y), "silu")
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_rows_of_any_size(kind):
+    """Values near the ends of the float range, and scales that undo them."""
+    w = rnd((40, 128), torch.float32, 13)
+    dtype = getattr(torch, kind)
+    for factor in (2.0 ** 100, 2.0 ** -100, 2.0 ** -126):
+        x = (rnd((6, 128), torch.float32, 14) * factor).to(dtype)
+        packed = ops.pack_mx4(w / (factor if factor > 1 else max(factor, 2.0 ** -100)))
+        w64 = f64(ops.expand_mx4(packed, torch.float32))
+        check(ops.linear_mx4(x, packed, out_dtype=torch.float32), f64(x) @ w64.T, sum_tolerance(f64(x), w64, kind) + 2.0 ** -149 * 128, str(factor))
+
+
+@pytest.mark.parametrize("m,kind", [(4, "bfloat16"), (4, "float32"), (4, "mx8"), (40, "mx8")])
+def test_infinities_and_nan(m, kind):
+    """What is not finite reaches the outputs of its own row, and only those; a NaN scale of a weight reaches its own column."""
+    w = torch.full((20, 96), 0.5, device=DEV)
+    packed = ops.pack_mx4(w)
+    x = rnd((m, 96), torch.float32, 15)
+    x[1, 3] = float("nan")
+    x[2, 50] = float("inf")
+    x = ops.pack_mx8(x) if kind == "mx8" else x.to(getattr(torch, kind))
+    got = f64(ops.linear_mx4(x, packed, out_dtype=torch.float32))
+    assert np.isnan(got[1]).all()
+    assert np.isnan(got[2]).all() if kind == "mx8" else np.isposinf(got[2]).all()
+    assert np.isfinite(got[[0, 3] + list(range(4, m))]).all()
+    w[7, 40] = float("nan")
+    x = rnd((m, 96), torch.float32, 15)
+    x = ops.pack_mx8(x) if kind == "mx8" else x.to(getattr(torch, kind))
+    got = f64(ops.linear_mx4(x, ops.pack_mx4(w), out_dtype=torch.float32))
+    assert np.isnan(got[:, 7]).all() and np.isfinite(np.delete(got, 7, axis=1)).all()
+
+
+def test_a_row_does_not_depend_on_the_others():
+    w = ops.pack_mx4(rnd((300, 1000), torch.float32, 16))
+    x, _ = rows_for(16, 1000, "bfloat16", 17)
+    whole = ops.linear_mx4(x[:8].contiguous(), w)
+    other = x[:8].clone()
+    other[1:] = float("nan")
+    assert torch.equal(ops.linear_mx4(other, w)[0], whole[0])
+    r, _ = rows_for(200, 1000, "mx8", 18)
+    first = ops.linear_mx4(r, w)
+    assert torch.equal(first, ops.linear_mx4(r, w))                      # the same bits every time
+    r._values[40:] = 0x7f                                                # NaN
+    assert torch.equal(ops.linear_mx4(r, w)[:40], first[:40])
+
+
+def test_another_stream_and_a_graph():
+    w = ops.pack_mx4(rnd((256, 512), torch.float32, 19))
+    gw = ops.pack_mx4(rnd((512, 512), torch.float32, 20), gated=True)
+    x = rnd((40, 512), torch.bfloat16, 21)
+
+    def chain(x):
+        rows = ops.norm_mx8(x, second=ops.NormParams(norm, 1e-6, 0.0))
+        return ops.linear_mx4(ops.linear_gated_mx4(rows, gw2, "silu", out_mx8=True), w), ops.linear_mx4(x[:9].contiguous(), w)
+
+    norm, gw2 = torch.ones(512, device=DEV), ops.pack_mx4(rnd((1024, 512), torch.float32, 22), gated=True)
+    want = [t.clone() for t in chain(x)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = chain(x)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(x)
+    x.copy_(rnd((40, 512), torch.bfloat16, 23))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, chain(x)))
+    assert gw.gated
+
+
+def test_a_product_right_behind_the_packing():
+    """The weights are read before the kernel ahead has ended: the packing keeps that safe by itself."""
+    x = rnd((8, 2304), torch.bfloat16, 24)
+    for seed in range(5):
+        w = rnd((4096, 2304), torch.bfloat16, 30 + seed)
+        first = ops.linear_mx4(x, ops.pack_mx4(w))
+        packed = ops.pack_mx4(w)
+        torch.cuda.synchronize()
+        assert torch.equal(first, ops.linear_mx4(x, packed))
+
+
+@pytest.mark.parametrize("m,code,name", [(8, 8, "mx_stream"), (40, 9, "mx_tc")])
+def test_a_wait_that_runs_out(m, code, name):
+    lib = library.load()
+    w = ops.pack_mx4(rnd((300, 512), torch.float32, 25))
+    x, x64 = rows_for(m, 512, "mx8", 26)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    try:
+        lib.rdl_set_wait_test(code, 200_000, 64)
+        ops.linear_mx4(x, w, status=status)
+        torch.cuda.synchronize()
+    finally:
+        lib.rdl_set_wait_test(0, 0, 0)
+    assert status.item() == code and name in library.FAULTS[code]
+    status.zero_()
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32, status=status), x64 @ w64.T, sum_tolerance(x64, w64, "mx8"), "the launch after")
+    assert status.item() == 0
+
+
+# ---- refusals ----
+
+def test_refusals():
+    w = ops.pack_mx4(rnd((32, 64), torch.float32, 27))
+    g = ops.pack_mx4(rnd((32, 64), torch.float32, 27), gated=True)
+    x = rnd((4, 64), torch.bfloat16, 28)
+    for call in (lambda: ops.linear_mx4(x, rnd((32, 64), torch.bfloat16, 1)), lambda: ops.linear_mx4(x, g), lambda: ops.linear_gated_mx4(x, w, "silu"),
+                 lambda: ops.linear_mx4(x[:, :32], w), lambda: ops.linear_mx4(rnd((4, 128), torch.bfloat16, 1)[:, ::2], w),
+                 lambda: ops.linear_mx4(x.to(torch.float16), w), lambda: ops.linear_mx4(x, w, softcap=3.0),
+                 lambda: ops.linear_mx4(x, w, activation="tanh"), lambda: ops.linear_gated_mx4(x, g, "relu2"),
+                 lambda: ops.linear_mx4(x, w, out_dtype=torch.float32, softcap=-1.0),
+                 lambda: ops.linear_mx4(x.cpu(), w), lambda: ops.linear_mx4(x[0], w),
+                 lambda: ops.pack_mx4(x.to(torch.float16)), lambda: ops.pack_mx4(x[:3], gated=True), lambda: ops.pack_mx4(x[:, ::2]), lambda: ops.pack_mx4(x[0]),
+                 lambda: ops.norm_mx8(x, residual=x), lambda: ops.norm_mx8(x, second=ops.NormParams(x[0, :32], 1e-6, 0.0)), lambda: ops.norm_mx8(x[:, ::2]),
+                 lambda: ops.norm_mx8(x, residual_out=torch.empty(3, 64, device=DEV)), lambda: ops.norm_mx8(x.to(torch.float16)),
+                 lambda: ops.mx8_rows(x, x), lambda: ops.mx4_weight(torch.zeros(4, 4, dtype=torch.uint8, device=DEV), torch.zeros(4, 2, dtype=torch.uint8, device=DEV), 8),
+                 lambda: ops.expand_mx4(w, torch.float16)):
+        with pytest.raises(library.KernelError):
+            call()
+    assert ops.linear_mx4(x[:0], w).shape == (0, 32) and ops.linear_mx4(ops.pack_mx8(x[:0]), w).shape == (0, 32)
+    assert ops.linear_gated_mx4(x[:0], g, "silu", out_mx8=True).shape == (0, 16)
