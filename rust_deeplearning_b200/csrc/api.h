@@ -28,14 +28,14 @@ void rdl_set_programmatic_launch(int on);
 #define RDL_FAULT_ATTENTION_TC 5       // attention_prefill_tc: a tile copy or a product did not complete
 #define RDL_FAULT_GEMM_TC_PAIR 6       // gemm_tc, pairs of blocks: as 4
 #define RDL_FAULT_GEMM_STREAM 7        // gemm_skinny: a weight copy did not complete
-#define RDL_FAULT_MX_STREAM 8          // mx_stream: a weight copy did not complete
-#define RDL_FAULT_MX_TC 9              // mx_tc: a stage or an accumulator was not handed over
+#define RDL_FAULT_MX_FEW 8             // mx_few_rows: a weight copy or a product did not complete
+#define RDL_FAULT_MX_MANY 9            // mx_many_rows: a stage or an accumulator was not handed over
 
 // For tests of the bounded waits: the kernel whose fault code is `code` gives up a wait after `cycles`
 // clock cycles instead of about a second, and announces `extra_tx_bytes` more bytes to the barrier of
 // its first copy than that copy delivers, so that this one wait cannot complete.  The block then
 // records its code and returns normally.  code 0 switches the test off.  Kernels with the codes
-// RDL_FAULT_ATTENTION_DECODE, RDL_FAULT_GEMM_STREAM, RDL_FAULT_MX_STREAM and RDL_FAULT_MX_TC honour it.
+// RDL_FAULT_ATTENTION_DECODE, RDL_FAULT_GEMM_STREAM, RDL_FAULT_MX_FEW and RDL_FAULT_MX_MANY honour it.
 void rdl_set_wait_test(int code, long long cycles, int extra_tx_bytes);
 
 // One attention call over a batch of sequences: the new tokens of this step are the queries,
@@ -438,21 +438,22 @@ int rdl_gemm_tc(void* out, int out_dtype, const void* x, const void* w, int m, i
 int rdl_norm_mx8(const void* x, int x_dtype, const void* w1, int w1_dtype, float eps1, float off1,
                  const float* residual, float* residual_out, const void* w2, int w2_dtype, float eps2, float off2,
                  void* values, void* scales, int n_rows, int width, void* stream);
-// A [rows, columns] matrix to 4 bits: codes [padded rows][padded columns / 2], scales [padded rows / 16][blocks][16][4] and 16 bytes more.
-// gated: the two halves of the rows are padded on their own.  The padding is left as it is (the products want zeros there).
+// A [rows, columns] matrix to 4 bits, in tiles of 128 x 128: codes of 8 KB a tile, scales of 512 bytes a tile and 16 bytes more.
+// gated: a [gate; up] matrix.  The padding is left as it is (the products want zeros there).
 int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales, int rows, int columns, int gated, void* stream);
 // the values of a 4-bit matrix, [rows, columns]
 int rdl_expand_mx4(const void* codes, const void* scales, void* out, int dtype, int rows, int columns, int gated, void* stream);
+// What the products take as `weight`: a block of host memory of rdl_mx4_matrix_bytes bytes on a 64-byte boundary, filled once by
+// rdl_mx4_describe.  It holds the addresses of the codes (on a 32-byte boundary) and the scales (16) and their tensor maps.
+int rdl_mx4_matrix_bytes(void);
+int rdl_mx4_describe(void* matrix, const void* codes, const void* scales, int rows, int columns, int gated);
 // out[m, n] = epilogue(sum_k x[m, k] w[n, k]) for up to 16 rows and a 4-bit matrix.  x_kind: RDL_F32 or RDL_BF16 ([m, k]), or RDL_MX8
-// with row_scales.  gated: act(gate) * up of the two halves of the matrix (n outputs each).  scratch: floats, where
-// rdl_mx_stream_slices is above 1 (slices * m * (gated ? 2 n : n) of them).
-int rdl_mx_stream(void* out, int out_dtype, const void* x, int x_kind, const void* row_scales, const void* codes, const void* scales,
-                  int m, int n, int k, int gated, int activation, float act_param, float softcap, float* scratch, long long scratch_floats,
-                  int* status, void* stream);
-int rdl_mx_stream_slices(int m, int k, int x_kind);
-// the same for any number of 8-bit rows on the tensor cores; out_kind RDL_MX8: 8-bit rows of n columns with out_scales
-int rdl_mx_tc(void* out, int out_kind, void* out_scales, const void* x, const void* row_scales, const void* codes, const void* scales,
-              int m, int n, int k, int gated, int activation, float act_param, float softcap, int* status, void* stream);
+// with row_scales.  A gated matrix: act(gate) * up.
+int rdl_mx_few_rows(void* out, int out_dtype, const void* x, int x_kind, const void* row_scales, const void* weight, int m,
+                    int activation, float act_param, float softcap, int* status, void* stream);
+// the same for any number of 8-bit rows, in tensor-core tiles; out_kind RDL_MX8: 8-bit rows of n columns with out_scales
+int rdl_mx_many_rows(void* out, int out_kind, void* out_scales, const void* x, const void* row_scales, const void* weight, int m,
+                     int activation, float act_param, float softcap, int* status, void* stream);
 
 // ---- latent attention (csrc/latent.cu) ----
 // One call per layer run and step: rotates the rotated part of every query head (in place, or into

@@ -7,16 +7,32 @@
 // infinity or a NaN has c = 255.  Codes are value * 2^(127 - c) rounded to nearest, ties to even.
 //
 // Columns are padded to whole blocks of 128 (four groups) with zero codes.
-//   weights  codes [padded rows][padded columns / 2]; scales [padded rows / 16][blocks][16][4]: a few-row product, which takes 16
-//            rows at a time, reads its scales in one piece, and 128 rows of a block are 8 pieces of 64 bytes for a tensor-core
-//            tile.  Rows are padded to 16; a [gate; up] matrix pads each half.
+//   weights  tiles of 128 rows x 128 columns, one after another along the columns: codes [rows / 128][blocks][128][64 bytes], scales
+//            [rows / 128][blocks][32][4][4]: the four scales of row 32 c + l at [l][c], the order a tensor-core product wants.
+//            A tile is 8 KB and 512 bytes in one piece.  (Rows in one piece each were read 64 bytes at a time: the output head
+//            of the 2B shape took 133 us.)  Rows are padded to 128.  A [gate; up] matrix lays 16 gate rows before the 16 up rows
+//            of the same outputs, so that a tile holds both halves of 64 outputs.
 //   rows     values [rows padded to 4][padded columns]; scales [blocks][rows padded to 4][4].
 #pragma once
 
 #include "common.cuh"
 
-constexpr int MX_GROUP = 32, MX_BLOCK = 128, MX_UNIT = 16;
+constexpr int MX_GROUP = 32, MX_BLOCK = 128, MX_ROWS = 128, MX_UNIT = 16;
 static inline int mx_blocks(int columns) { return (columns + MX_BLOCK - 1) / MX_BLOCK; }
+
+// where row `row` of a weight lies; half: outputs of a [gate; up] matrix, 0: not one
+__device__ __forceinline__ int mx_place(int row, int half) {
+    if (half == 0) return row;
+    const int up = row >= half, o = row - (up ? half : 0);
+    return o / MX_UNIT * (2 * MX_UNIT) + up * MX_UNIT + o % MX_UNIT;
+}
+// bytes from the start of the codes to the one of (place, column), and of the scales to the one of its group
+__device__ __forceinline__ long long mx_code_at(int place, int column, int blocks) {
+    return (((long long)(place / MX_ROWS) * blocks + column / MX_BLOCK) * MX_ROWS + place % MX_ROWS) * (MX_BLOCK / 2) + column % MX_BLOCK / 2;
+}
+__device__ __forceinline__ long long mx_scale_at(int place, int column, int blocks) {
+    return ((long long)(place / MX_ROWS) * blocks + column / MX_BLOCK) * (MX_ROWS * 4) + place % 32 * 16 + place % MX_ROWS / 32 * 4 + column % MX_BLOCK / MX_GROUP;
+}
 
 // The scale code of a group from its largest magnitude; TOP_EXP, TOP_MANT: the format's largest value is 1.TOP_MANT x 2^TOP_EXP.
 template <int TOP_EXP, uint32_t TOP_MANT>

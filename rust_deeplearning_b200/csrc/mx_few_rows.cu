@@ -1,0 +1,534 @@
+// Few rows times a 4-bit weight matrix (formats: microscaling.cuh):  out[m, n] = epilogue(sum_k x[m, k] w[n, k]),  m <= 16.
+//
+// Decode: bound by the bytes of the weights, 4.25 bits each, read once.  Anything a thread does per weight would cost more than the
+// weight's transfer, so no thread touches one: TMA brings codes to shared memory in the form the block-scaled tcgen05 product reads
+// (mx_tensor.cuh), with 128 weight rows as its M side and the few rows as its N side.
+//
+// The rows have to be 8-bit values with a power of two a group, too.  Rows that are in that form enter as they are.  A bfloat16 value
+// has 8 significant bits and e4m3 has 4: it enters as the sum of two, its leading four bits and the rest, with a scale 2^3
+// smaller.  This is exact for values above 2^-14 of the largest of their group (below it, it is off by at most 2^-18 of that
+// largest one).  A float32 value enters as six parts, 24 bits.  The parts are columns of the one product and are added up in its epilogue.
+// Rows that hold an infinity or a NaN, which parts cannot, or nothing but numbers so small that a part's scale would fall
+// below 2^-127, are computed again by plain arithmetic.
+//
+// Warp 0 loads weights: they depend on nothing an earlier kernel of the step writes, so it starts while that kernel is still running.
+// Warp 1 issues scales and products.  Sixteen warps turn the rows into parts (once, where a block's columns fit shared memory), a block of columns after
+// another so that the products can begin; eight of them then take finished sums out of tensor memory.  A wide matrix: a block takes 128 rows of weights after another.  One with fewer tiles than
+// multiprocessors: a cluster of up to 8 blocks shares a tile, each with its part of the columns, and its blocks send their sums through
+// distributed shared memory to the one that adds up that part of the outputs, in rank order.  Every wait is bounded.
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "activations.cuh"
+#include "api.h"
+#include "launch.cuh"
+#include "mx_tensor.cuh"
+
+namespace {
+
+// A stage of the ring is two blocks of columns: what a stage costs the issuing warp beside its products (a wait, a commit) is about as long
+// as the products of one.
+constexpr int WORKERS = 512, THREADS = 64 + WORKERS, MAX_STAGES = 8, STEP = 2, SCALE_BUFS = 4, MAX_PASS = 64;
+
+struct FewArgs {
+    const void* x; const uint8_t* row_scales;
+    const uint8_t* codes; const uint8_t* scales;
+    void* out; int out_dtype;
+    int M, N, K;                                 // N: outputs
+    int blocks, row_pad;                         // blocks of 128 columns; the rows' padded count (8-bit rows)
+    int tiles, split, slice_blocks, pass_blocks, stages;
+    int share;                                   // outputs of a tile that a block of a cluster adds up
+    int gated, activation; float act_param, softcap;
+    bool vec;                                    // rows lie on 16-byte boundaries
+    long long wait_cycles; int test_extra_tx;
+    int* status;
+};
+
+__device__ __forceinline__ void tma_codes(uint32_t dst, const CUtensorMap* map, int y, uint32_t bar, unsigned long long policy) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(bar), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void bulk_scales(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, unsigned long long policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// N accumulator columns of the warp's lanes, as bits; there after mx_tmem_wait_ld
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
+    static_assert(N == 4 || N == 8, "four or eight columns");
+    if constexpr (N == 4)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t map_to_block(uint32_t addr, uint32_t rank) {      // the same place in the shared memory of block `rank`
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ float finish(const FewArgs& a, float y, float up) {
+    if (a.gated) y = rdl_gated(y, up, a.activation, a.act_param);
+    else if (a.activation >= 16) y = rdl_unary(y, a.activation);
+    if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
+    return y;
+}
+
+// ---- eight columns of a row, as they lie and in parts; the four lanes of a group hold neighbouring ones ----
+template <int PARTS>
+struct Chunk {
+    uint32_t w[PARTS == 6 ? 8 : (PARTS == 2 ? 4 : 2)];
+    uint32_t code;                               // the group's scale, of 8-bit rows
+};
+
+template <int PARTS>
+__device__ __forceinline__ void load_chunk(const FewArgs& a, int m, int k, Chunk<PARTS>& d) {
+    if constexpr (PARTS == 1) {
+        const uint2 v = *reinterpret_cast<const uint2*>((const uint8_t*)a.x + (long long)m * a.blocks * MX_BLOCK + k);
+        d.w[0] = v.x; d.w[1] = v.y;
+        d.code = a.row_scales[((long long)(k / MX_BLOCK) * a.row_pad + m) * 4 + k % MX_BLOCK / MX_GROUP];
+    } else {
+        const long long base = (long long)m * a.K + k;
+#pragma unroll
+        for (int i = 0; i < (PARTS == 6 ? 8 : 4); ++i) d.w[i] = 0;
+        if (a.vec) {
+            if (k < a.K) {
+                const uint4* p = reinterpret_cast<const uint4*>((const char*)a.x + base * (PARTS == 2 ? 2 : 4));
+#pragma unroll
+                for (int i = 0; i < (PARTS == 6 ? 2 : 1); ++i) *reinterpret_cast<uint4*>(&d.w[4 * i]) = p[i];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (k + e >= a.K) continue;
+                if (PARTS == 2) d.w[e >> 1] |= (uint32_t)((const unsigned short*)a.x)[base + e] << (16 * (e & 1));
+                else d.w[PARTS == 2 ? 0 : e] = ((const uint32_t*)a.x)[base + e];
+            }
+        }
+    }
+}
+
+constexpr int ROW_FINE = 0, ROW_ZERO = 1, ROW_TINY = 2, ROW_BAD = 3;
+
+// The parts of a chunk as e4m3 bytes, and the scale codes of its group; the four lanes of a group come here together.  A part is the
+// leading four bits of what the parts before it leave, cut off and not rounded, so that what it leaves is exact; each lies at least 2^3
+// below the one before, and so does its scale.
+template <int PARTS>
+__device__ __forceinline__ int make_parts(const Chunk<PARTS>& d, uint2 (&bytes)[PARTS], uint32_t (&code)[PARTS]) {
+    if constexpr (PARTS == 1) {
+        bytes[0] = make_uint2(d.w[0], d.w[1]);
+        code[0] = d.code;
+        return ROW_ZERO;
+    } else {
+        uint32_t top = 0;                                    // magnitudes are in order as integers
+        if constexpr (PARTS == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = __vmaxu2(top, d.w[i] & 0x7fff7fffu);
+            top = max(top & 0xffff0000u, top << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, d.w[i] & 0x7fffffffu);
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const bool bad = top >= 0x7f800000u;
+        const uint32_t c = bad ? 0u : mx8_scale_code(__uint_as_float(top));
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(PARTS == 6 ? d.w[PARTS == 6 ? e : 0] : (e & 1 ? d.w[e >> 1] & 0xffff0000u : d.w[e >> 1] << 16));
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            code[part] = c > 3u * part ? c - 3u * part : 0u;
+            const float f = mx_inverse_scale(code[part]);
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (part + 1 < PARTS) {
+                    const float cut = __uint_as_float(__float_as_uint(v[e]) & 0xfff00000u);
+                    y[e] = cut * f;
+                    v[e] -= cut;
+                } else {
+                    y[e] = v[e] * f;
+                }
+            }
+            bytes[part] = make_uint2(mx_to_e4m3(y[0], y[1], y[2], y[3]), mx_to_e4m3(y[4], y[5], y[6], y[7]));
+            if (bad) bytes[part] = make_uint2(0, 0);         // the row is computed again: zeros keep its columns quiet
+        }
+        return bad ? ROW_BAD : (top == 0 ? ROW_ZERO : (c >= 3u * (PARTS - 1) ? ROW_FINE : ROW_TINY));
+    }
+}
+
+// PARTS: 1 (8-bit rows), 2 (bfloat16), 6 (float32); R: rows the product has place for
+template <int PARTS, int R>
+__global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs a) {
+    constexpr int NB = PARTS * R;                            // columns of the product: part p of row m is column p R + m
+    constexpr int X_BLOCK = NB * MX_BLOCK;                   // bytes of a block of 128 columns of the rows
+    constexpr int TMEM_COLS = 2 * NB + SCALE_BUFS * 8 <= 128 ? 128 : 256;
+    constexpr int AHEAD = PARTS == 6 ? 2 : 4;                // chunks a lane asks for before it works on the first
+    static_assert(NB % 16 == 0 && 2 * NB + SCALE_BUFS * 8 <= TMEM_COLS, "the sums of two tiles and the scales share tensor memory");
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], x_ready[MAX_PASS], x_free;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up;
+    // rows with an infinity or a NaN here; rows with a group too small for its last parts; rows with one that is not
+    __shared__ unsigned bad_rows, tiny_rows, fine_rows;
+    // shared memory: rows | ring of codes | the rows' scales | ring of scales | sums of a cluster's blocks
+    const uint32_t x_s = mx_smem(smem), ring_s = x_s + (uint32_t)(a.pass_blocks * X_BLOCK);
+    const uint32_t xs_s = ring_s + (uint32_t)(a.stages * STEP * MX_TILE_BYTES), ws_s = xs_s + (uint32_t)(a.pass_blocks * MX_SCALE_BYTES);
+    const uint32_t y_off = (uint32_t)(a.pass_blocks * (X_BLOCK + MX_SCALE_BYTES) + a.stages * STEP * (MX_TILE_BYTES + MX_SCALE_BYTES));
+
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // the compiler may know it uniform
+    const int rank = a.split > 1 ? (int)(blockIdx.x % a.split) : 0;
+    const int first_tile = blockIdx.x / a.split, tile_step = gridDim.x / a.split;
+    const int b0 = min(rank * a.slice_blocks, a.blocks), b1 = min(b0 + a.slice_blocks, a.blocks);
+    const int passes = (b1 - b0 + a.pass_blocks - 1) / a.pass_blocks;
+    {   // every barrier by a thread of its own
+        const int t = threadIdx.x;
+        if (t < MAX_STAGES) { mx_bar_init(mx_smem(&full_bar[t]), 1); mx_bar_init(mx_smem(&empty_bar[t]), 1); }
+        else if (t < MAX_STAGES + 2) { mx_bar_init(mx_smem(&acc_full[t - MAX_STAGES]), 1); mx_bar_init(mx_smem(&acc_empty[t - MAX_STAGES]), 8); }
+        else if (t == MAX_STAGES + 2) { mx_bar_init(mx_smem(&x_free), 1); gave_up = 0; bad_rows = tiny_rows = fine_rows = 0; }
+        else if (t >= 64 && t < 64 + MAX_PASS) mx_bar_init(mx_smem(&x_ready[t - 64]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mx_smem(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    mx_fence_before();
+    __syncthreads();
+    if (a.split > 1) cluster_arrive();                       // "this block runs"; waited for before anything is stored in another one
+    mx_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+    volatile int* gave_up_v = &gave_up;
+    bool ok = true;
+
+    if (warp == 0) {
+        // ---- weights ----
+        unsigned long long policy;                           // read once a step: first to leave L2
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        int s = 0, piece = first_tile * a.blocks + b0;       // place in the ring; block of columns over all tiles
+        uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
+        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, piece += (tile_step - 1) * a.blocks + (a.blocks - (b1 - b0))) {
+            for (int kb = b0; kb < b1;) {
+                // a stage is up to STEP blocks; none reaches into the next pass over the rows
+                const int n = min(STEP, min(b0 + ((kb - b0) / a.pass_blocks + 1) * a.pass_blocks, b1) - kb);
+                if (!mx_warp_wait(mx_smem(&empty_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
+                if (mx_elect()) {
+                    const uint32_t full = mx_smem(&full_bar[s]), at = ring_s + (uint32_t)(s * STEP * MX_TILE_BYTES);
+                    mx_bar_expect(full, (uint32_t)n * (MX_TILE_TX + MX_SCALE_BYTES) + extra);
+                    tma_codes(at, &map_w, piece * MX_ROWS, full, policy);
+                    if (n > 1) tma_codes(at + MX_TILE_BYTES, &map_w, (piece + 1) * MX_ROWS, full, policy);
+                    bulk_scales(ws_s + (uint32_t)(s * STEP * MX_SCALE_BYTES), a.scales + (long long)piece * MX_SCALE_BYTES, (uint32_t)n * MX_SCALE_BYTES, full, policy);
+                }
+                __syncwarp();
+                extra = 0;
+                kb += n;
+                piece += n;
+                if (++s == a.stages) { s = 0; parity ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        // ---- scales to tensor memory, and the products ----
+        int s = 0, lt = 0, n_pass = 0, scale_buf = 0;
+        uint32_t parity = 0;
+        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++lt) {
+            const int buf = lt & 1;
+            if (!mx_warp_wait(mx_smem(&acc_empty[buf]), ((lt >> 1) & 1) ^ 1, a.wait_cycles, gave_up_v)) { ok = false; break; }
+            for (int p = 0; p < passes && ok; ++p) {
+                const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
+                const bool fresh = passes > 1 || lt == 0;            // the rows are being made ready, block by block
+                for (int kb = p0; kb < p1;) {
+                    const int n = min(STEP, p1 - kb);
+                    for (int j = 0; j < n && fresh && ok; ++j) ok = mx_warp_wait(mx_smem(&x_ready[kb - p0 + j]), n_pass & 1, a.wait_cycles, gave_up_v);
+                    if (!ok || !mx_warp_wait(mx_smem(&full_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
+                    mx_fence_after();
+                    if (mx_elect()) {
+#pragma unroll
+                        for (int j = 0; j < STEP; ++j) {
+                            if (j >= n) break;
+                            const uint32_t sa = tmem + 2 * NB + (uint32_t)((scale_buf + j) & (SCALE_BUFS - 1)) * 8, sb = sa + 4;
+                            copy_scales(sa, mx_scale_desc(ws_s + (uint32_t)((s * STEP + j) * MX_SCALE_BYTES)));
+                            copy_scales(sb, mx_scale_desc(xs_s + (uint32_t)((kb + j - p0) * MX_SCALE_BYTES)));
+                            const uint64_t ad = mx_operand_desc(ring_s + (uint32_t)((s * STEP + j) * MX_TILE_BYTES)), bd = mx_operand_desc(x_s + (uint32_t)((kb + j - p0) * X_BLOCK));
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_mx(tmem + buf * NB, ad + (uint32_t)(k * 2), bd + (uint32_t)(k * 2), mx_idesc(MX_E2M1, MX_E4M3, MX_ROWS, NB, k), sa, sb, kb + j != b0 || k != 0);
+                        }
+                        commit(mx_smem(&empty_bar[s]));
+                    }
+                    __syncwarp();
+                    kb += n;
+                    scale_buf = (scale_buf + n) & (SCALE_BUFS - 1);
+                    if (++s == a.stages) { s = 0; parity ^= 1; }
+                }
+                ++n_pass;
+                if (ok && passes > 1 && mx_elect()) commit(mx_smem(&x_free));
+                __syncwarp();
+            }
+            if (ok && mx_elect()) commit(mx_smem(&acc_full[buf]));
+            __syncwarp();
+        }
+    } else {
+        // ---- rows to parts; then the sums ----
+        rdl_grid_wait();
+        rdl_grid_launch_dependents();
+        const int q = warp & 3, half = (warp - 2) >> 2;      // the first eight of these warps take the sums out
+        // a lane's chunk of row 0 (lanes 16 to 31: of row 1) of a block, and its group's scale: the two halves of a warp hold neighbouring rows
+        const uint32_t my_place = x_s + (uint32_t)((lane >> 4) * 128 + ((((lane & 15) >> 1) ^ (lane >> 4)) << 4) + (lane & 1) * 8);
+        const uint32_t my_scale = xs_s + (uint32_t)((lane >> 4) * 16 + ((lane & 15) >> 2));
+        int lt = 0, n_pass = 0;
+        // (a wait in vain ends no loop here: the blocks of a cluster meet again below)
+        for (int tile = first_tile; tile < a.tiles; tile += tile_step, ++lt) {
+            for (int p = 0; p < passes && (passes > 1 || lt == 0); ++p, ++n_pass) {
+                if (n_pass > 0 && !mx_bar_wait(mx_smem(&x_free), (n_pass - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
+                const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
+                // A warp takes every sixteenth block of columns, and hands each over on its own: the products begin with the first.
+                // Every block's barrier takes part in every pass, so that its phase is the number of the pass.
+                for (int pb = warp - 2; pb < a.pass_blocks; pb += WORKERS / 32) {
+                    const int block = p0 + pb, chunks = block < p1 ? a.M * (MX_BLOCK / 8) : 0;
+                    const uint32_t at = my_place + (uint32_t)(pb * X_BLOCK), sc_at = my_scale + (uint32_t)(pb * MX_SCALE_BYTES);
+                    uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
+#pragma unroll
+                    for (int c0 = 0; c0 < R * (MX_BLOCK / 8); c0 += 32 * AHEAD) {
+                        if (c0 >= chunks) break;
+                        Chunk<PARTS> d[AHEAD];
+#pragma unroll
+                        for (int u = 0; u < AHEAD; ++u) {
+                            const int i = c0 + u * 32 + lane;                            // 16 chunks a row
+#pragma unroll
+                            for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
+                            d[u].code = 0;
+                            if (i < chunks) load_chunk<PARTS>(a, i >> 4, block * MX_BLOCK + (lane & 15) * 8, d[u]);
+                        }
+#pragma unroll
+                        for (int u = 0; u < AHEAD; ++u) {
+                            const int m0 = c0 / 16 + u * 2;                              // this lane's row: m0 or m0 + 1
+                            if (c0 + u * 32 >= chunks) break;                            // none of this warp's
+                            uint2 bytes[PARTS];
+                            uint32_t code[PARTS];
+                            const int kind = make_parts<PARTS>(d[u], bytes, code);
+                            if (c0 + u * 32 + lane < chunks) {
+                                // swizzled by the row: rows m0 and m0 + 1 of eight flip the pieces by m0 & 6 beside what my_place has of the lane's own
+                                const uint32_t to = (at ^ (uint32_t)((m0 & 6) << 4)) + (uint32_t)((m0 >> 3) * 1024 + (m0 & 6) * 128);
+#pragma unroll
+                                for (int part = 0; part < PARTS; ++part)
+                                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (uint32_t)(part * R * 128)), "r"(bytes[part].x), "r"(bytes[part].y) : "memory");
+                                if ((lane & 3) == 0) {
+#pragma unroll
+                                    for (int part = 0; part < PARTS; ++part)
+                                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(sc_at + (uint32_t)(m0 * 16 + (part * R & 31) * 16 + (part * R >> 5) * 4)), "r"(code[part]) : "memory");
+                                }
+                                if (PARTS > 1) {
+#pragma unroll
+                                    for (int kd = 0; kd < 4; ++kd)
+                                        if (kd != ROW_ZERO && kind == kd) seen[kd] |= 1u << (m0 + (lane >> 4));
+                                }
+                            }
+                        }
+                    }
+                    if (PARTS > 1) {
+                        const uint32_t fine = __reduce_or_sync(0xffffffffu, seen[ROW_FINE]), rare = seen[ROW_TINY] | seen[ROW_BAD];
+                        if (lane == 0 && fine) atomicOr(&fine_rows, fine);
+                        if (rare) { atomicOr(&tiny_rows, seen[ROW_TINY]); atomicOr(&bad_rows, seen[ROW_BAD]); }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the products read what was stored here
+                    __syncwarp();
+                    if (lane == 0) mx_bar_arrive(mx_smem(&x_ready[pb]));
+                }
+            }
+            const int buf = lt & 1;
+            if (!mx_bar_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
+            mx_fence_after();
+            float* y = reinterpret_cast<float*>(smem + y_off);       // a cluster's sums (one tile each)
+            if (warp < 10) {
+                // lane l of quarter q: weight row 32 q + l of the tile; this warp takes half of the rows
+                constexpr int MINE = R / 2;
+                float sum[MINE];
+#pragma unroll
+                for (int j = 0; j < MINE; ++j) sum[j] = 0.f;
+                if (passes > 0) {
+                    uint32_t v[PARTS][MINE];
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * NB + part * R + half * MINE), v[part]);
+                    mx_tmem_wait_ld();
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part)                            // the smallest first
+#pragma unroll
+                        for (int j = 0; j < MINE; ++j) sum[j] += __uint_as_float(v[part][j]);
+                }
+                mx_fence_before();
+                __syncwarp();
+                if (lane == 0) mx_bar_arrive(mx_smem(&acc_empty[buf]));
+                // all of a row too small for its last parts (below 2^-103): they would be lost
+                const unsigned bad = *(volatile unsigned*)&bad_rows | (*(volatile unsigned*)&tiny_rows & ~*(volatile unsigned*)&fine_rows);
+                if (PARTS > 1 && bad) {                          // plain arithmetic, for what the parts cannot hold
+                    const int wr = tile * MX_ROWS + 32 * q + lane;
+                    for (int j = 0; j < MINE; ++j) {
+                        const int m = half * MINE + j;
+                        if (!(bad >> m & 1)) continue;
+                        float y = 0.f;
+                        for (int k = b0 * MX_BLOCK; k < min(b1 * MX_BLOCK, a.K); ++k) {
+                            const uint32_t code = a.codes[mx_code_at(wr, k, a.blocks)] >> (4 * (k & 1));
+                            uint32_t h[4];
+                            mx_from_e2m1(code & 15u, h);
+                            const float w = __half2float(__ushort_as_half((unsigned short)(h[0] & 0xffffu)))
+                                            * mx_scale(a.scales[mx_scale_at(wr, k, a.blocks)]);
+                            y = fmaf(rdl_load(a.x, (long long)m * a.K + k, PARTS == 2 ? RDL_BF16 : RDL_F32), w, y);
+                        }
+#pragma unroll
+                        for (int i = 0; i < MINE; ++i)
+                            if (i == j) sum[i] = y;
+                    }
+                }
+                if (a.split == 1) {
+                    // neighbouring lanes have neighbouring outputs; gated: 16 gate rows, then their 16 up rows
+                    const int n = a.gated ? tile * (MX_ROWS / 2) + 16 * q + lane : tile * MX_ROWS + 32 * q + lane;
+#pragma unroll
+                    for (int j = 0; j < MINE; ++j) {
+                        const int m = half * MINE + j;
+                        const float up = a.gated ? __shfl_down_sync(0xffffffffu, sum[j], 16) : 0.f;
+                        if (m < a.M && n < a.N && (!a.gated || lane < 16)) rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, finish(a, sum[j], up));
+                    }
+                } else {
+                    // each block adds up a part of the outputs: this row's sums go to its block, to this rank's place there
+                    const int r = 32 * q + lane, o = a.gated ? (r >> 5) * 16 + (r & 15) : r, owner = o / a.share;
+                    const int at = a.gated ? (o - owner * a.share) * 2 + ((r >> 4) & 1) : o - owner * a.share, outs = a.gated ? 2 * a.share : a.share;
+                    cluster_wait();                              // every block of the cluster runs
+                    const uint32_t to = map_to_block(mx_smem(y), owner) + (uint32_t)(rank * R * outs + at) * 4;
+#pragma unroll
+                    for (int j = 0; j < MINE; ++j)
+                        if (half * MINE + j < a.M) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (uint32_t)((half * MINE + j) * outs) * 4), "f"(sum[j]) : "memory");
+                }
+            } else if (a.split > 1) {
+                cluster_wait();
+            }
+        }
+    }
+    if (!ok && a.status) atomicExch(a.status, RDL_FAULT_MX_FEW);
+    if (a.split > 1) {
+        __syncwarp();
+        if (warp < 2) cluster_wait();                        // the first barrier: the workers are past it
+        cluster_arrive();
+        cluster_wait();                                      // every block's sums are where they are added up
+        if (warp >= 2) {
+            const int tid = threadIdx.x - 64, per_tile = a.gated ? MX_ROWS / 2 : MX_ROWS, outs = a.gated ? 2 * a.share : a.share;
+            const float* y = reinterpret_cast<const float*>(smem + y_off);
+            for (int idx = tid; idx < a.M * a.share; idx += WORKERS) {
+                const int m = idx / a.share, o = idx - m * a.share, of_tile = rank * a.share + o, n = first_tile * per_tile + of_tile;
+                if (of_tile >= per_tile || n >= a.N) continue;
+                float v[2] = {0.f, 0.f};
+                for (int s = 0; s < a.split; ++s) {
+                    const float* ys = y + (s * R + m) * outs;
+                    if (a.gated) { v[0] += ys[2 * o]; v[1] += ys[2 * o + 1]; }
+                    else v[0] += ys[o];
+                }
+                rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, finish(a, v[0], v[1]));
+            }
+        }
+    }
+    if (*gave_up_v && threadIdx.x == 0) mx_drain();
+    mx_fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+// Clusters of `size` blocks, each block with a multiprocessor to itself, that run at the same time on the current device.  Fewer than
+// multiprocessors / size: a cluster lies within one group of them, and what is left of a group stays empty (18 clusters of 8 on 148
+// multiprocessors took two turns, 14 us where one took 6).
+int clusters_at_once(int size) {
+    static std::atomic<int> known[64][9];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (const int k = known[dev][size].load(std::memory_order_relaxed)) return k - 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size * 32);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = 200 * 1024;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (rdl_allow_shared<mx_few_rows_kernel<2, 8>>(200 * 1024) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, mx_few_rows_kernel<2, 8>, &cfg) != cudaSuccess) {
+        cudaGetLastError();                                  // an answer of none is safe: the tile is not shared
+        n = 0;
+    }
+    known[dev][size].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
+template <int PARTS, int R>
+int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
+    constexpr int NB = PARTS * R, PER_BLOCK = NB * MX_BLOCK + MX_SCALE_BYTES, PER_STAGE = STEP * (MX_TILE_BYTES + MX_SCALE_BYTES);
+    const int sms = rdl_sm_count();
+    a.tiles = w.tiles;
+    // as many blocks a tile as keeps every tile on the device at once, each with two blocks of columns or more
+    a.split = 1;
+    if (a.tiles * 2 <= sms)
+        for (a.split = 8; a.split > 1; --a.split)
+            if (a.blocks >= 2 * a.split && a.tiles <= clusters_at_once(a.split)) break;
+    a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
+    a.slice_blocks = (a.blocks + a.split - 1) / a.split;
+    const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - 1024 - sums;      // alignment, static shared memory
+    // the rows of all of a block's columns beside a ring of three stages, or of as many as fit
+    a.pass_blocks = a.slice_blocks;
+    if (a.pass_blocks * PER_BLOCK + 3 * PER_STAGE > most) a.pass_blocks = (most - 3 * PER_STAGE) / PER_BLOCK;
+    if (a.pass_blocks > MAX_PASS) a.pass_blocks = MAX_PASS;
+    a.stages = (most - a.pass_blocks * PER_BLOCK) / PER_STAGE;
+    if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
+    // no deeper than the block's work: what shared memory is left lets the next kernel's blocks begin
+    const int turns = a.split > 1 ? 1 : (a.tiles + sms - 1) / sms;
+    const int steps = (a.slice_blocks + STEP - 1) / STEP + (a.slice_blocks - 1) / a.pass_blocks;
+    if ((long long)a.stages > (long long)turns * steps) a.stages = turns * steps;
+    const int smem = 1024 + a.pass_blocks * PER_BLOCK + a.stages * PER_STAGE + sums;
+    RDL_CUDA((rdl_allow_shared<mx_few_rows_kernel<PARTS, R>>(smem)), "mx_few_rows");
+    const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
+    RDL_CHECK_EX(rdl_launch_cluster(mx_few_rows_kernel<PARTS, R>, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, w.codes_map, a), "mx_few_rows");
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int rdl_mx_few_rows(void* out, int out_dtype, const void* x, int x_kind, const void* row_scales, const void* weight, int m,
+                               int activation, float act_param, float softcap, int* status, void* stream) {
+    const Mx4Matrix* w = (const Mx4Matrix*)weight;
+    RDL_REQUIRE(w && w->codes, "mx_few_rows: missing weight");
+    RDL_REQUIRE(m >= 0 && m <= 16, "mx_few_rows: %d rows, at most 16 are supported", m);
+    if (m == 0) return 0;
+    RDL_REQUIRE(out && x, "mx_few_rows: missing operand");
+    RDL_REQUIRE(rdl_valid_dtype(out_dtype), "mx_few_rows: bad output dtype %d", out_dtype);
+    RDL_REQUIRE(rdl_valid_dtype(x_kind) || (x_kind == RDL_MX8 && row_scales && (uintptr_t)x % 8 == 0), "mx_few_rows: bad rows (kind %d)", x_kind);
+    RDL_REQUIRE(!w->gated || rdl_gated_known(activation), "mx_few_rows: unknown activation %d", activation);
+    RDL_REQUIRE(softcap >= 0.f, "mx_few_rows: soft-cap must not be negative");
+    FewArgs a{};
+    a.x = x; a.row_scales = (const uint8_t*)row_scales;
+    a.codes = w->codes; a.scales = w->scales;
+    a.out = out; a.out_dtype = out_dtype;
+    a.M = m; a.N = w->gated ? w->rows / 2 : w->rows; a.K = w->columns;
+    a.blocks = w->blocks; a.row_pad = (m + 3) / 4 * 4;
+    a.gated = w->gated; a.activation = activation; a.act_param = act_param; a.softcap = softcap;
+    a.vec = a.K % 8 == 0 && (uintptr_t)x % 16 == 0;
+    a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_FEW); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_FEW);
+    a.status = status;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (x_kind == RDL_MX8) return launch<1, 16>(a, *w, st);
+    if (x_kind == RDL_BF16) return m <= 8 ? launch<2, 8>(a, *w, st) : launch<2, 16>(a, *w, st);
+    return m <= 8 ? launch<6, 8>(a, *w, st) : launch<6, 16>(a, *w, st);
+}

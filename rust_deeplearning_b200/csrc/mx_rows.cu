@@ -16,6 +16,7 @@
 #include "api.h"
 #include "launch.cuh"
 #include "microscaling.cuh"
+#include "mx_tensor.cuh"
 #include "row_vec.cuh"
 
 namespace {
@@ -194,7 +195,7 @@ struct PackArgs {
     const void* w; int dtype;
     uint8_t* codes; uint8_t* scales;
     int rows, columns, blocks;
-    int half, half_padded;                                  // gated: source rows from `half` on lie from `half_padded` on
+    int half;                                               // gated: outputs (source rows of each half); 0: not gated
 };
 
 // a warp takes 256 columns of one row
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(256) pack_mx4_kernel(const __grid_constant__ P
     const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (item >= (long long)a.rows * pieces) return;
     const int row = (int)(item / pieces), piece = (int)(item - (long long)row * pieces);
-    const int to = a.half > 0 && row >= a.half ? row - a.half + a.half_padded : row;
+    const int to = mx_place(row, a.half);
     const int c = piece * 256 + lane * 8;
     const long long base = (long long)row * a.columns;
     float v[8];
@@ -229,15 +230,15 @@ __global__ void __launch_bounds__(256) pack_mx4_kernel(const __grid_constant__ P
     word |= __shfl_xor_sync(0xffffffffu, word, 8);
     const int block = c / MX_BLOCK;
     if (block >= a.blocks) return;
-    *reinterpret_cast<uint32_t*>(a.codes + ((long long)to * a.blocks * MX_BLOCK + c) / 2) = mx_to_e2m1(v);
+    *reinterpret_cast<uint32_t*>(a.codes + mx_code_at(to, c, a.blocks)) = mx_to_e2m1(v);
     if ((lane & 15) == 0)
-        *reinterpret_cast<uint32_t*>(a.scales + (((long long)(to / MX_UNIT) * a.blocks + block) * MX_UNIT + to % MX_UNIT) * 4) = word;
+        *reinterpret_cast<uint32_t*>(a.scales + mx_scale_at(to, c, a.blocks)) = word;
 }
 
 struct ExpandArgs {
     const uint8_t* codes; const uint8_t* scales;
     void* out; int dtype;
-    int rows, columns, blocks, half, half_padded;
+    int rows, columns, blocks, half;
 };
 
 template <bool VEC>
@@ -248,11 +249,10 @@ __global__ void __launch_bounds__(256) expand_mx4_kernel(const __grid_constant__
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= (long long)a.rows * words) return;
     const int row = (int)(i / words), word = (int)(i - (long long)row * words), c = word * 8;
-    const int from = a.half > 0 && row >= a.half ? row - a.half + a.half_padded : row;
+    const int from = mx_place(row, a.half);
     uint32_t h[4];
-    mx_from_e2m1(*reinterpret_cast<const uint32_t*>(a.codes + (long long)from * words * 4 + word * 4), h);
-    const int block = c / MX_BLOCK;
-    const float s = mx_scale(a.scales[(((long long)(from / MX_UNIT) * a.blocks + block) * MX_UNIT + from % MX_UNIT) * 4 + c % MX_BLOCK / MX_GROUP]);
+    mx_from_e2m1(*reinterpret_cast<const uint32_t*>(a.codes + mx_code_at(from, c, a.blocks)), h);
+    const float s = mx_scale(a.scales[mx_scale_at(from, c, a.blocks)]);
     const long long base = (long long)row * a.columns + c;
     float v[8];
 #pragma unroll
@@ -317,7 +317,7 @@ extern "C" int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales,
     RDL_REQUIRE(rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "pack_mx4: bad sizes rows=%d columns=%d", rows, columns);
     RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "pack_mx4: the results must start on 16-byte boundaries");
     const int half = gated ? rows / 2 : 0;
-    const PackArgs a{w, dtype, (uint8_t*)codes, (uint8_t*)scales, rows, columns, mx_blocks(columns), half, (half + MX_UNIT - 1) / MX_UNIT * MX_UNIT};
+    const PackArgs a{w, dtype, (uint8_t*)codes, (uint8_t*)scales, rows, columns, mx_blocks(columns), half};
     const long long warps = (long long)rows * ((a.blocks + 1) / 2), grid = (warps + 7) / 8;
     RDL_REQUIRE(grid <= 0x7fffffffLL, "pack_mx4: %d x %d is too large", rows, columns);
     cudaStream_t st = (cudaStream_t)stream;
@@ -326,8 +326,8 @@ extern "C" int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales,
     RDL_CHECK_EX(e, "pack_mx4");
     // The products read weights before the kernel ahead of them has ended (launch.cuh).  Something that is launched the ordinary way
     // comes in between, so that a product right behind this call finds the codes written.
-    const long long units = gated ? 2LL * (a.half_padded / MX_UNIT) : (rows + MX_UNIT - 1) / MX_UNIT;
-    RDL_CUDA(cudaMemsetAsync((uint8_t*)scales + units * a.blocks * (MX_UNIT * 4), 0, 16, st), "pack_mx4");
+    const long long tiles = ((gated ? 2LL * ((half + MX_UNIT - 1) / MX_UNIT) * MX_UNIT : rows) + MX_ROWS - 1) / MX_ROWS;
+    RDL_CUDA(cudaMemsetAsync((uint8_t*)scales + tiles * a.blocks * (MX_ROWS * 4), 0, 16, st), "pack_mx4");
     return 0;
 }
 
@@ -337,8 +337,7 @@ extern "C" int rdl_expand_mx4(const void* codes, const void* scales, void* out, 
     RDL_REQUIRE(rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "expand_mx4: bad sizes rows=%d columns=%d", rows, columns);
     RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "expand_mx4: the codes must start on 16-byte boundaries");
     const int half = gated ? rows / 2 : 0;
-    const ExpandArgs a{(const uint8_t*)codes, (const uint8_t*)scales, out, dtype, rows, columns, mx_blocks(columns), half,
-                       (half + MX_UNIT - 1) / MX_UNIT * MX_UNIT};
+    const ExpandArgs a{(const uint8_t*)codes, (const uint8_t*)scales, out, dtype, rows, columns, mx_blocks(columns), half};
     const long long words = (long long)rows * a.blocks * (MX_BLOCK / 8), grid = (words + 255) / 256;
     RDL_REQUIRE(grid <= 0x7fffffffLL, "expand_mx4: %d x %d is too large", rows, columns);
     cudaStream_t st = (cudaStream_t)stream;
@@ -346,4 +345,23 @@ extern "C" int rdl_expand_mx4(const void* codes, const void* scales, void* out, 
                                                              : rdl_launch(expand_mx4_kernel<false>, dim3((unsigned)grid), dim3(256), 0, st, a);
     RDL_CHECK_EX(e, "expand_mx4");
     return 0;
+}
+
+extern "C" int rdl_mx4_matrix_bytes(void) { return (int)sizeof(Mx4Matrix); }
+
+extern "C" int rdl_mx4_describe(void* matrix, const void* codes, const void* scales, int rows, int columns, int gated) {
+    RDL_REQUIRE(matrix && (uintptr_t)matrix % 64 == 0, "mx4_describe: the description must lie on a 64-byte boundary");
+    RDL_REQUIRE(codes && scales && rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "mx4_describe: bad sizes rows=%d columns=%d", rows, columns);
+    RDL_REQUIRE((uintptr_t)codes % 32 == 0 && (uintptr_t)scales % 16 == 0, "mx4_describe: the codes must start on a 32-byte boundary, the scales on a 16-byte boundary");
+    Mx4Matrix* w = (Mx4Matrix*)matrix;
+    const int part = gated ? rows / 2 : rows;
+    *w = Mx4Matrix{};
+    w->codes = (const uint8_t*)codes; w->scales = (const uint8_t*)scales;
+    w->rows = rows; w->columns = columns; w->gated = gated ? 1 : 0;
+    w->blocks = mx_blocks(columns);
+    w->tiles = ((gated ? 2 * ((part + MX_UNIT - 1) / MX_UNIT * MX_UNIT) : part) + MX_ROWS - 1) / MX_ROWS;
+    const cuuint64_t pieces = (cuuint64_t)w->tiles * w->blocks * MX_ROWS;
+    RDL_REQUIRE(pieces <= 0x7fffffffULL, "mx4_describe: %d x %d is too large", rows, columns);      // a tile's coordinate is an int
+    return mx_make_map(&w->codes_map, codes, {CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, {MX_BLOCK, pieces}, {MX_BLOCK / 2}, {MX_BLOCK, MX_ROWS},
+                                              CU_TENSOR_MAP_SWIZZLE_128B}, "the codes of a 4-bit matrix");
 }

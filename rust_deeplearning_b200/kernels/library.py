@@ -188,8 +188,8 @@ FAULTS = {
     5: "attention_prefill_tc: a tile copy or a product did not complete",
     6: "gemm_tc (pairs of blocks): a stage or an accumulator was not handed over",
     7: "gemm_skinny: a weight copy did not complete",
-    8: "mx_stream: a weight copy did not complete",
-    9: "mx_tc: a stage or an accumulator was not handed over",
+    8: "mx_few_rows: a weight copy or a product did not complete",
+    9: "mx_many_rows: a stage or an accumulator was not handed over",
 }
 
 
@@ -434,9 +434,10 @@ _SIGNATURES = {
     "rdl_norm_mx8": [_P, _I, _P, _I, _F, _F, _P, _P, _P, _I, _F, _F, _P, _P, _I, _I, _P],
     "rdl_pack_mx4": [_P, _I, _P, _P, _I, _I, _I, _P],
     "rdl_expand_mx4": [_P, _P, _P, _I, _I, _I, _I, _P],
-    "rdl_mx_stream": [_P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _LL, _P, _P],
-    "rdl_mx_stream_slices": [_I, _I, _I],
-    "rdl_mx_tc": [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P],
+    "rdl_mx4_matrix_bytes": [],
+    "rdl_mx4_describe": [_P, _P, _P, _I, _I, _I],
+    "rdl_mx_few_rows": [_P, _I, _P, _I, _P, _P, _I, _I, _F, _F, _P, _P],
+    "rdl_mx_many_rows": [_P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_random_normal": [_P, _I, _LL, ctypes.c_ulonglong, ctypes.c_double, _P],
     "rdl_sample": [_P, _P, _P, _I, _I, ctypes.POINTER(SamplingArgs), _P, _P, _P, _P, _P, _P],
     "rdl_upload_batch": [_P, _P, _I, _P, _I, _I, _I, _P],

@@ -1783,37 +1783,53 @@ def delta_rule_scan(rows: torch.Tensor, *, v_col: int, q_f, k_f, g_f, beta_f, n_
 # e2m1 (0 0.5 1 1.5 2 3 4 6 and a sign), rows of activations e4m3 (up to 448).  A scale is the smallest power of two that brings the
 # group's largest magnitude to at most 6 or 448; values are rounded to nearest, ties to even; a group that holds an infinity or
 # a NaN is NaN.  `csrc/microscaling.cuh` has the layouts.
+#
+# A call of these in a decode step costs the host more than the device, so they ask for what they need once (a weight keeps its
+# description, its sizes and its device) and build no message unless something is wrong.
 
-MX_GROUP, MX_BLOCK = 32, 128
-MX_FEW_ROWS = 16         # up to this many rows the kernel that streams the 4-bit weights runs; above, the tensor-core tiles
+MX_GROUP, MX_BLOCK, MX_ROWS = 32, 128, 128
+MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs; above, the tensor-core tiles of 128 rows
+_MX8 = 2                 # rows of 8 bits, where a kernel's argument says of what kind its rows are
+_KINDS = {torch.float32: 0, torch.bfloat16: 1}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _blocks(columns: int) -> int:
     return -(-columns // MX_BLOCK)
 
 
+def _refuse(msg):
+    raise KernelError(msg)
+
+
 class Mx4Weight:
     """A [rows, columns] matrix in 4 bits, laid out for the products (`pack_mx4`, `mx4_weight` make it).
-    gated: it is [gate; up] for `linear_gated_mx4`, each half padded on its own."""
+    gated: it is [gate; up] for `linear_gated_mx4`; 16 gate rows lie before the 16 up rows of the same outputs."""
 
     def __init__(self, rows: int, columns: int, gated: bool, device):
+        device = torch.device(device)
         _need(rows > 0 and columns > 0 and (not gated or rows % 2 == 0), f"a 4-bit weight of {rows} x {columns}{', gated' if gated else ''}")
+        _need(device.type == "cuda", "kernels run on CUDA tensors only; there is no CPU path")
         self.rows, self.columns, self.gated = rows, columns, bool(gated)
-        part = rows // 2 if gated else rows
-        self.padded_rows = -(-part // 16) * 16 * (2 if gated else 1)
+        self.outputs = rows // 2 if gated else rows
+        self.tiles = -(-(-(-self.outputs // 16) * 32 if gated else rows) // MX_ROWS)
         self.shape = (rows, columns)
-        # the padding's codes are zeros; the scales have 16 bytes more, which the packing kernel's launcher clears last
-        self.codes = torch.zeros((self.padded_rows, _blocks(columns) * (MX_BLOCK // 2)), dtype=torch.uint8, device=device)
-        self._scales = torch.zeros((self.padded_rows * _blocks(columns) * 4 + 16,), dtype=torch.uint8, device=device)
+        blocks = _blocks(columns)
+        # what the packing does not write has to be zeros; without padding there is none of it
+        make = torch.empty if self.tiles * MX_ROWS == rows and columns == blocks * MX_BLOCK else torch.zeros
+        self.codes = make((self.tiles, blocks, MX_ROWS, MX_BLOCK // 2), dtype=torch.uint8, device=device)
+        self._scales = make((self.tiles * blocks * MX_ROWS * 4 + 16,), dtype=torch.uint8, device=device)    # 16 bytes more, which the packing clears last
+        self.device = self.codes.device
+        self._index = self.device.index
+        lib = library.load()
+        self._host = ctypes.create_string_buffer(lib.rdl_mx4_matrix_bytes() + 64)
+        self.handle = -(-ctypes.addressof(self._host) // 64) * 64
+        library.check(lib.rdl_mx4_describe(self.handle, self.codes.data_ptr(), self._scales.data_ptr(), rows, columns, int(self.gated)), 0)
 
     @property
     def scales(self) -> torch.Tensor:
-        """uint8 [padded rows / 16, blocks, 16, 4]"""
-        return self._scales[:-16].view(self.padded_rows // 16, _blocks(self.columns), 16, 4)
-
-    @property
-    def device(self):
-        return self.codes.device
+        """uint8 [tiles, blocks, 32, 4, 4]: the four scales of row 32 c + l of a tile at [l, c]"""
+        return self._scales[:-16].view(self.tiles, _blocks(self.columns), 32, 4, 4)
 
     @property
     def nbytes(self) -> int:
@@ -1824,32 +1840,32 @@ class Mx8Rows:
     """Rows of activations in 8 bits with a scale a group: what `norm_mx8`, `pack_mx8` and `linear_gated_mx4` make and
     `linear_mx4` and `linear_gated_mx4` take in place of a tensor."""
 
+    __slots__ = ("rows", "columns", "shape", "device", "_values", "_scales")
+
     def __init__(self, rows: int, columns: int, device):
-        self.rows, self.columns = rows, columns
-        self.shape = (rows, columns)
-        padded, blocks = -(-rows // 4) * 4, _blocks(columns)
+        self.rows, self.columns, self.shape = rows, columns, (rows, columns)
+        padded, blocks = (rows + 3) // 4 * 4, (columns + MX_BLOCK - 1) // MX_BLOCK
         # the padding rows hold whatever the memory held: nothing reads a result that comes of them
-        self._values = torch.empty((padded, blocks * MX_BLOCK), dtype=torch.uint8, device=device)
+        self._values = torch.empty((padded, blocks * MX_BLOCK), dtype=torch.float8_e4m3fn, device=device)
         self._scales = torch.empty((blocks, padded, 4), dtype=torch.uint8, device=device)
+        self.device = self._values.device
 
     @property
     def values(self) -> torch.Tensor:
         """float8_e4m3fn [rows, columns], before the scales (a view)"""
-        return self._values.view(torch.float8_e4m3fn)[:self.rows, :self.columns]
+        v = self._values
+        return v if v.shape == self.shape else v.as_strided(self.shape, (v.shape[1], 1))
 
     @property
     def scales(self) -> torch.Tensor:
         """uint8 exponents + 127, [rows, blocks of 128 columns, 4 groups] (a view)"""
-        return self._scales.permute(1, 0, 2)[:self.rows]
-
-    @property
-    def device(self):
-        return self._values.device
+        blocks, padded, _ = self._scales.shape
+        return self._scales.as_strided((self.rows, blocks, 4), (4, padded * 4, 1))
 
     def dequantise(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the rows stand for, [rows, columns] (for looking at them; the products take the rows as they are)."""
         scale = self.scales.contiguous().view(torch.float8_e8m0fnu).float()          # 255 is that type's NaN
-        wide = self._values.view(torch.float8_e4m3fn)[:self.rows].float().view(self.rows, -1, MX_GROUP)
+        wide = self._values[:self.rows].float().view(self.rows, -1, MX_GROUP)
         return (wide * scale.reshape(self.rows, -1, 1)).view(self.rows, -1)[:, :self.columns].to(dtype)
 
 
@@ -1857,10 +1873,10 @@ def pack_mx4(weight: torch.Tensor, gated: bool = False) -> Mx4Weight:
     """A [rows, columns] matrix (float32 or bfloat16) rounded to 4 bits."""
     _need(weight.dim() == 2, "pack_mx4: a matrix [rows, columns]")
     _dense(weight, "weight")
-    stream = _stream(weight)
+    dtype = _dtype_code(weight)
     w = Mx4Weight(weight.shape[0], weight.shape[1], gated, weight.device)
-    library.check(library.load().rdl_pack_mx4(_ptr(weight), _dtype_code(weight), _ptr(w.codes), _ptr(w._scales), w.rows, w.columns,
-                                              int(w.gated), stream))
+    library.check(library.load().rdl_pack_mx4(weight.data_ptr(), dtype, w.codes.data_ptr(), w._scales.data_ptr(), w.rows, w.columns,
+                                              int(w.gated), _raw_stream(w._index)))
     return w
 
 
@@ -1869,71 +1885,85 @@ def mx4_weight(codes: torch.Tensor, scales: torch.Tensor, columns: int, gated: b
     low half of a byte; scales uint8 [rows, ceil(columns / 32)], exponent + 127."""
     _need(codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.dim() == 2 and scales.dim() == 2,
           "mx4_weight: codes and scales are uint8 matrices")
-    rows, groups = codes.shape[0], -(-columns // MX_GROUP)
+    rows, groups, used = codes.shape[0], -(-columns // MX_GROUP), -(-columns // 2)
     # codes that came padded to whole groups are taken too
-    _need(columns > 0 and codes.shape[1] in (-(-columns // 2), groups * MX_GROUP // 2) and tuple(scales.shape) == (rows, groups),
+    _need(columns > 0 and codes.shape[1] in (used, groups * MX_GROUP // 2) and tuple(scales.shape) == (rows, groups),
           f"mx4_weight: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit {columns} columns")
-    _need(codes.is_cuda and codes.device == scales.device, "mx4_weight: codes and scales lie on one CUDA device")
+    _need(codes.device == scales.device, "mx4_weight: codes and scales lie on one device")
     w = Mx4Weight(rows, columns, gated, codes.device)
     if columns % 2:          # the half byte behind an odd row's last column is padding, whatever it held
         codes = codes.clone()
-        codes[:, columns // 2] &= 15
-    used = -(-columns // 2)
-    halves = 2 if gated else 1
-    for h in range(halves):
-        n, to = rows // halves, h * (w.padded_rows // halves)
-        w.codes[to:to + n, :used] = codes[h * n:(h + 1) * n, :used]
-        by_row = torch.zeros((w.padded_rows // halves, _blocks(columns) * 4), dtype=torch.uint8, device=codes.device)
-        by_row[:n, :groups] = scales[h * n:(h + 1) * n]
-        w.scales[to // 16:(to + by_row.shape[0]) // 16] = by_row.view(-1, 16, _blocks(columns), 4).permute(0, 2, 1, 3)
+        codes[:, used - 1] &= 15
+    blocks = _blocks(columns)
+
+    def laid_out(t, per_block):          # [rows, some] -> [tiles, blocks, 128, per_block]
+        if gated:                        # 16 gate rows, then their 16 up rows
+            halves = torch.zeros((2, -(-w.outputs // 16) * 16, t.shape[1]), dtype=torch.uint8, device=t.device)
+            halves[:, :w.outputs] = t.reshape(2, w.outputs, -1)
+            t = halves.view(2, -1, 16, t.shape[1]).transpose(0, 1).reshape(-1, t.shape[1])
+        wide = torch.zeros((w.tiles * MX_ROWS, blocks * per_block), dtype=torch.uint8, device=t.device)
+        wide[:t.shape[0], :t.shape[1]] = t
+        return wide.view(w.tiles, MX_ROWS, blocks, per_block).transpose(1, 2)
+
+    w.codes.copy_(laid_out(codes[:, :used], MX_BLOCK // 2))
+    w.scales.copy_(laid_out(scales, 4).reshape(w.tiles, blocks, 4, 32, 4).transpose(2, 3))
     return w
 
 
 def expand_mx4(weight: Mx4Weight, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values a 4-bit matrix stands for, [rows, columns]."""
-    stream = _stream(weight.codes)
+    _need(dtype in _KINDS, f"kernels write float32 or bfloat16 tensors, not {dtype}")
     out = torch.empty(weight.shape, dtype=dtype, device=weight.device)
-    library.check(library.load().rdl_expand_mx4(_ptr(weight.codes), _ptr(weight._scales), _ptr(out), _dtype_code(out), weight.rows, weight.columns,
-                                                int(weight.gated), stream))
+    library.check(library.load().rdl_expand_mx4(weight.codes.data_ptr(), weight._scales.data_ptr(), out.data_ptr(), _KINDS[dtype], weight.rows,
+                                                weight.columns, int(weight.gated), _raw_stream(weight._index)))
     return out
 
 
 def mx8_rows(values: torch.Tensor, scales: torch.Tensor) -> Mx8Rows:
     """Rows that are in 8 bits already: values float8_e4m3fn [rows, columns], scales uint8 [rows, ceil(columns / 32)], exponent + 127."""
-    _need(values.dtype is torch.float8_e4m3fn and scales.dtype is torch.uint8 and values.dim() == 2
+    _need(values.dtype is torch.float8_e4m3fn and scales.dtype is torch.uint8 and values.dim() == 2 and values.shape[1] > 0
           and tuple(scales.shape) == (values.shape[0], -(-values.shape[1] // MX_GROUP)),
           "mx8_rows: float8_e4m3fn [rows, columns] and uint8 [rows, groups of 32 columns]")
     _need(values.is_cuda and values.device == scales.device, "mx8_rows: values and scales lie on one CUDA device")
     r = Mx8Rows(values.shape[0], values.shape[1], values.device)
-    r._values.zero_()
-    r._scales.zero_()
-    r._values[:r.rows, :r.columns] = values.view(torch.uint8)
+    if r.columns % MX_BLOCK:
+        r._values.zero_()
+    r.values.copy_(values)
     padded = torch.zeros((r.rows, _blocks(r.columns) * 4), dtype=torch.uint8, device=r.device)
     padded[:, :scales.shape[1]] = scales
     r.scales.copy_(padded.view(r.rows, -1, 4))
     return r
 
 
+def _norm_weight(p: Optional[NormParams], width: int, name: str):
+    """address, dtype code, eps, offset"""
+    if p is None:
+        return None, 0, 0.0, 0.0
+    w = p.weight
+    if not (w.is_contiguous() and w.numel() == width and w.is_cuda):
+        _refuse(f"norm_mx8: the {name} norm's weight must hold {width} contiguous values on the device")
+    return w.data_ptr(), _dtype_code(w), p.eps, p.offset
+
+
 def norm_mx8(x: torch.Tensor, *, first: Optional[NormParams] = None, residual: Optional[torch.Tensor] = None,
              second: Optional[NormParams] = None, residual_out: Optional[torch.Tensor] = None) -> Mx8Rows:
     """`norm_residual_norm` with its result in 8 bits: t = first ? rms_norm(x; first) : x;  h = residual + t (float32, written
     to `residual_out`, by default back to `residual`) or t;  returns second ? rms_norm(h; second) : h as 8-bit rows."""
-    _dense(x, "x")
-    _need(x.dim() == 2 and x.shape[1] > 0, "norm_mx8: x must be [rows, width]")
+    if x.dim() != 2 or not x.is_contiguous() or x.shape[1] == 0:
+        _refuse("norm_mx8: x must be contiguous [rows, width]")
+    if not x.is_cuda:
+        _refuse("kernels run on CUDA tensors only; there is no CPU path")
     rows, width = x.shape
-    for p, name in ((first, "first"), (second, "second")):
-        _need(p is None or (p.weight.is_contiguous() and p.weight.numel() == width), f"norm_mx8: the {name} norm's weight must hold {width} values")
-    for t, name in ((residual, "residual"), (residual_out, "residual_out")):
-        _need(t is None or (t.dtype is torch.float32 and t.is_contiguous() and t.shape == x.shape), f"norm_mx8: {name} must be contiguous float32 [rows, width]")
     if residual_out is None:
         residual_out = residual
-    stream = _stream(x)
+    for t in (residual, residual_out):
+        if t is not None and not (t.dtype is torch.float32 and t.is_contiguous() and t.shape == x.shape and t.device == x.device):
+            _refuse("norm_mx8: residual and residual_out must be contiguous float32 [rows, width]")
     y = Mx8Rows(rows, width, x.device)
     library.check(library.load().rdl_norm_mx8(
-        _ptr(x), _dtype_code(x), _ptr(first.weight) if first else None, _dtype_code(first.weight) if first else 0,
-        float(first.eps) if first else 0.0, float(first.offset) if first else 0.0, _ptr(residual), _ptr(residual_out),
-        _ptr(second.weight) if second else None, _dtype_code(second.weight) if second else 0,
-        float(second.eps) if second else 0.0, float(second.offset) if second else 0.0, _ptr(y._values), _ptr(y._scales), rows, width, stream))
+        x.data_ptr(), _dtype_code(x), *_norm_weight(first, width, "first"), residual.data_ptr() if residual is not None else None,
+        residual_out.data_ptr() if residual_out is not None else None, *_norm_weight(second, width, "second"),
+        y._values.data_ptr(), y._scales.data_ptr(), rows, width, _raw_stream(y.device.index)))
     return y
 
 
@@ -1942,45 +1972,45 @@ def pack_mx8(x: torch.Tensor) -> Mx8Rows:
     return norm_mx8(x)
 
 
-def _mx_stream(out, x, weight: Mx4Weight, n: int, gated: bool, activation: int, param: float, softcap: float, status):
-    lib = library.load()
-    if isinstance(x, Mx8Rows):
-        kind, data, row_scales = 2, x._values, x._scales
-    else:
-        kind, data, row_scales = _dtype_code(x), x, None
-    rows = out.shape[0]
-    slices = lib.rdl_mx_stream_slices(rows, weight.columns, kind)
-    scratch = torch.empty((slices * rows * n * (2 if gated else 1),), dtype=torch.float32, device=out.device) if slices > 1 else None
-    library.check(lib.rdl_mx_stream(_ptr(out), _dtype_code(out), _ptr(data), kind, _ptr(row_scales), _ptr(weight.codes), _ptr(weight._scales),
-                                    rows, n, weight.columns, int(gated), activation, float(param), float(softcap), _ptr(scratch),
-                                    scratch.numel() if scratch is not None else 0, _status(status), _stream(out)), 2 if slices > 1 else 1)
-
-
-def _product_mx4(x, weight: Mx4Weight, n: int, out_dtype, gated: bool, activation: int, param: float, softcap: float, status):
-    rows, few = x.shape[0], x.shape[0] <= MX_FEW_ROWS
-    out = torch.empty((rows, n), dtype=out_dtype, device=weight.device)
-    if rows == 0:
-        return out
-    if few:
-        _mx_stream(out, x, weight, n, gated, activation, param, softcap, status)
-    elif isinstance(x, Mx8Rows):
-        library.check(library.load().rdl_mx_tc(_ptr(out), _dtype_code(out), None, _ptr(x._values), _ptr(x._scales), _ptr(weight.codes),
-                                               _ptr(weight._scales), rows, n, weight.columns, int(gated), activation, float(param),
-                                               float(softcap), _status(status), _stream(out)))
-    else:
-        for r in range(0, rows, MX_FEW_ROWS):
-            _mx_stream(out[r:r + MX_FEW_ROWS], x[r:r + MX_FEW_ROWS], weight, n, gated, activation, param, softcap, status)
-    return out
-
-
-def _mx4_operands(x, weight: Mx4Weight, gated: bool, who: str):
+def _mx4_refuse(x, weight, gated: bool, who: str):
+    """Says what is wrong with a call that `_product_mx4` will not take."""
     _need(isinstance(weight, Mx4Weight), f"{who}: the weight must be an Mx4Weight (pack_mx4, mx4_weight)")
     _need(weight.gated == gated, f"{who}: the weight was packed {'as [gate; up]' if weight.gated else 'without its gated form'}")
     _need(len(x.shape) == 2 and x.shape[1] == weight.columns, f"{who}: shapes {tuple(x.shape)} and {weight.shape} do not fit")
     _need(x.device == weight.device, f"{who}: rows on {x.device}, weight on {weight.device}")
-    if not isinstance(x, Mx8Rows):
-        _dtype_code(x)
-        _dense(x, "x")
+    _dtype_code(x)
+    _dense(x, "x")
+    _refuse(f"{who}: these operands do not fit")
+
+
+def _product_mx4(x, weight: Mx4Weight, gated: bool, out_dtype, out_mx8: bool, activation: int, param: float, softcap: float, status, who: str):
+    packed = type(x) is Mx8Rows
+    if type(weight) is not Mx4Weight or weight.gated is not gated or len(x.shape) != 2 or x.shape[1] != weight.columns or x.device != weight.device or not (
+            packed or (x.dtype in _KINDS and x.is_contiguous())):
+        _mx4_refuse(x, weight, gated, who)
+    rows, n, device = x.shape[0], weight.outputs, weight.device
+    status = status if status is not None else _step_status
+    status = status.data_ptr() if status is not None else None
+    lib, stream = library.load(), _raw_stream(weight._index)
+    if packed:
+        data, scales, kind = x._values.data_ptr(), x._scales.data_ptr(), _MX8
+    else:
+        data, scales, kind = x.data_ptr(), None, _KINDS[x.dtype]
+    if packed and rows > MX_FEW_ROWS:
+        if out_mx8:
+            out = Mx8Rows(rows, n, device)
+            to, to_scales, out_kind = out._values.data_ptr(), out._scales.data_ptr(), _MX8
+        else:
+            out = torch.empty((rows, n), dtype=out_dtype or torch.bfloat16, device=device)
+            to, to_scales, out_kind = out.data_ptr(), None, _KINDS[out.dtype]
+        library.check(lib.rdl_mx_many_rows(to, out_kind, to_scales, data, scales, weight.handle, rows, activation, param, softcap, status, stream))
+        return out
+    out = torch.empty((rows, n), dtype=torch.float32 if out_mx8 else out_dtype or (torch.bfloat16 if packed else x.dtype), device=device)
+    to, out_kind, row, out_row = out.data_ptr(), _KINDS[out.dtype], weight.columns * x.element_size() if not packed else 0, n * out.element_size()
+    for r in range(0, rows, MX_FEW_ROWS):
+        library.check(lib.rdl_mx_few_rows(to + r * out_row, out_kind, data + r * row, kind, scales, weight.handle, min(rows - r, MX_FEW_ROWS),
+                                          activation, param, softcap, status, stream))
+    return norm_mx8(out) if out_mx8 else out
 
 
 def linear_mx4(x, weight: Mx4Weight, out_dtype: Optional[torch.dtype] = None, softcap: Optional[float] = None,
@@ -1991,29 +2021,23 @@ def linear_mx4(x, weight: Mx4Weight, out_dtype: Optional[torch.dtype] = None, so
     x is a float32 or bfloat16 tensor or `Mx8Rows` (whose result is bfloat16 unless out_dtype says otherwise).  Up to 16 rows the weights
     are streamed once; more rows of a tensor are taken 16 at a time (pack them to 8 bits, `pack_mx8`, to have them on the tensor
     cores' 8-bit rate); more 8-bit rows run in tensor-core tiles.
-    The weight is a constant, as `linear` has it."""
-    _mx4_operands(x, weight, False, "linear_mx4")
-    _need(activation is None or (activation in UNARY_FORMS and softcap is None),
-          f"linear_mx4: activation '{activation}' is not one of {sorted(UNARY_FORMS)} (and comes without a soft-cap)")
-    out_dtype = out_dtype or (torch.bfloat16 if isinstance(x, Mx8Rows) else x.dtype)
-    _need(softcap is None or out_dtype is torch.float32, "linear_mx4: the soft-cap is applied to float32 results")
-    return _product_mx4(x, weight, weight.rows, out_dtype, False, UNARY_FORMS[activation] if activation else 0, 0.0, softcap or 0.0, status)
+    The weight is a constant, as `linear` has it (one that `pack_mx4` has just made may be used at once)."""
+    form = 0
+    if activation is not None or softcap is not None or out_dtype is not None:
+        _need(activation is None or (activation in UNARY_FORMS and softcap is None),
+              f"linear_mx4: activation '{activation}' is not one of {sorted(UNARY_FORMS)} (and comes without a soft-cap)")
+        _need(out_dtype is None or out_dtype in _KINDS, f"linear_mx4: results are float32 or bfloat16, not {out_dtype}")
+        _need(softcap is None or out_dtype is torch.float32 or (out_dtype is None and getattr(x, "dtype", None) is torch.float32),
+              "linear_mx4: the soft-cap is applied to float32 results")
+        form = UNARY_FORMS[activation] if activation else 0
+    return _product_mx4(x, weight, False, out_dtype, False, form, 0.0, softcap or 0.0, status, "linear_mx4")
 
 
 def linear_gated_mx4(x, weight: Mx4Weight, activation: str, param: float = 0.0, out_mx8: bool = False,
                      status: Optional[torch.Tensor] = None):
     """act(x Wg^T) * (x Wu^T) for a 4-bit [Wg; Wu] packed with gated=True (or another form of `GATED_FORMS`; param: its parameter)
     -> [rows, I] in x's dtype (bfloat16 for 8-bit rows), or, with out_mx8, as 8-bit rows for the product that follows."""
-    _mx4_operands(x, weight, True, "linear_gated_mx4")
-    _need(activation in GATED_FORMS, f"unknown activation '{activation}', known: {sorted(GATED_FORMS)}")
-    n, form = weight.rows // 2, GATED_FORMS[activation]
-    out_dtype = torch.bfloat16 if isinstance(x, Mx8Rows) else x.dtype
-    if not out_mx8:
-        return _product_mx4(x, weight, n, out_dtype, True, form, param, 0.0, status)
-    if isinstance(x, Mx8Rows) and x.rows > MX_FEW_ROWS:
-        y = Mx8Rows(x.rows, n, x.device)
-        library.check(library.load().rdl_mx_tc(_ptr(y._values), 2, _ptr(y._scales), _ptr(x._values), _ptr(x._scales), _ptr(weight.codes),
-                                               _ptr(weight._scales), x.rows, n, weight.columns, 1, form, float(param), 0.0, _status(status),
-                                               _stream(y._values)))
-        return y
-    return pack_mx8(_product_mx4(x, weight, n, torch.float32, True, form, param, 0.0, status))
+    form = GATED_FORMS.get(activation)
+    if form is None:
+        _refuse(f"unknown activation '{activation}', known: {sorted(GATED_FORMS)}")
+    return _product_mx4(x, weight, True, None, out_mx8, form, param, 0.0, status, "linear_gated_mx4")
