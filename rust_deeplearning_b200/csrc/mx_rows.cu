@@ -362,6 +362,8 @@ extern "C" int rdl_mx4_describe(void* matrix, const void* codes, const void* sca
     w->tiles = ((gated ? 2 * ((part + MX_UNIT - 1) / MX_UNIT * MX_UNIT) : part) + MX_ROWS - 1) / MX_ROWS;
     const cuuint64_t pieces = (cuuint64_t)w->tiles * w->blocks * MX_ROWS;
     RDL_REQUIRE(pieces <= 0x7fffffffULL, "mx4_describe: %d x %d is too large", rows, columns);      // a tile's coordinate is an int
-    return mx_make_map(&w->codes_map, codes, {CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, {MX_BLOCK, pieces}, {MX_BLOCK / 2}, {MX_BLOCK, MX_ROWS},
-                                              CU_TENSOR_MAP_SWIZZLE_128B}, "the codes of a 4-bit matrix");
+    if (int e = mx_make_map(&w->codes_map, codes, {CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, {MX_BLOCK, pieces}, {MX_BLOCK / 2}, {MX_BLOCK, MX_ROWS},
+                                                   CU_TENSOR_MAP_SWIZZLE_128B}, "the codes of a 4-bit matrix")) return e;
+    return mx_make_map(&w->scales_map, scales, {CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, {MX_ROWS, pieces / MX_ROWS}, {MX_SCALE_BYTES}, {MX_ROWS, 1},
+                                                CU_TENSOR_MAP_SWIZZLE_NONE}, "the scales of a 4-bit matrix");
 }

@@ -17,6 +17,7 @@
 // A 4-bit weight on the host's side: made once, when the weight is laid out.
 struct Mx4Matrix {
     CUtensorMap codes_map;                       // [tile x block x row][128 codes], a box is a tile
+    CUtensorMap scales_map;                      // [tile x block][128 words], a box is a tile's
     const uint8_t* codes; const uint8_t* scales;
     int rows, columns, gated;                    // as packed (gated: rows / 2 outputs)
     int blocks, tiles;                           // of 128 columns, of 128 rows
