@@ -30,12 +30,13 @@ void rdl_set_programmatic_launch(int on);
 #define RDL_FAULT_GEMM_STREAM 7        // gemm_skinny: a weight copy did not complete
 #define RDL_FAULT_MX_FEW 8             // mx_few_rows: a weight copy or a product did not complete
 #define RDL_FAULT_MX_MANY 9            // mx_many_rows: a stage or an accumulator was not handed over
+#define RDL_FAULT_MX_SOME 10           // mx_some_rows: as 9
 
 // For tests of the bounded waits: the kernel whose fault code is `code` gives up a wait after `cycles`
 // clock cycles instead of about a second, and announces `extra_tx_bytes` more bytes to the barrier of
 // its first copy than that copy delivers, so that this one wait cannot complete.  The block then
 // records its code and returns normally.  code 0 switches the test off.  Kernels with the codes
-// RDL_FAULT_ATTENTION_DECODE, RDL_FAULT_GEMM_STREAM, RDL_FAULT_MX_FEW and RDL_FAULT_MX_MANY honour it.
+// RDL_FAULT_ATTENTION_DECODE, RDL_FAULT_GEMM_STREAM, RDL_FAULT_MX_FEW, RDL_FAULT_MX_MANY and RDL_FAULT_MX_SOME honour it.
 void rdl_set_wait_test(int code, long long cycles, int extra_tx_bytes);
 
 // One attention call over a batch of sequences: the new tokens of this step are the queries,
@@ -451,7 +452,10 @@ int rdl_mx4_describe(void* matrix, const void* codes, const void* scales, int ro
 // with row_scales.  A gated matrix: act(gate) * up.
 int rdl_mx_few_rows(void* out, int out_dtype, const void* x, int x_kind, const void* row_scales, const void* weight, int m,
                     int activation, float act_param, float softcap, int* status, void* stream);
-// the same for any number of 8-bit rows, in tensor-core tiles; out_kind RDL_MX8: 8-bit rows of n columns with out_scales
+// the same for up to 128 rows of 8 bits
+int rdl_mx_some_rows(void* out, int out_dtype, const void* x, const void* row_scales, const void* weight, int m,
+                     int activation, float act_param, float softcap, int* status, void* stream);
+// the same for any number of 8-bit rows, in tensor-core tiles (up to 128 rows by rdl_mx_some_rows where that is faster); out_kind RDL_MX8: 8-bit rows of n columns with out_scales
 int rdl_mx_many_rows(void* out, int out_kind, void* out_scales, const void* x, const void* row_scales, const void* weight, int m,
                      int activation, float act_param, float softcap, int* status, void* stream);
 

@@ -18,8 +18,6 @@
 // distributed shared memory to the one that adds up that part of the outputs, in rank order.  Every wait is bounded.
 #include <cuda_fp16.h>
 
-#include <atomic>
-
 #include "activations.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -83,7 +81,7 @@ __device__ __forceinline__ uint32_t map_to_block(uint32_t addr, uint32_t rank) {
 }
 
 __device__ __forceinline__ float finish(const FewArgs& a, float y, float up) {
-    if (a.gated) y = rdl_gated(y, up, a.activation, a.act_param);
+    if (a.gated) y = a.out_dtype == RDL_F32 ? rdl_gated(y, up, a.activation, a.act_param) : rdl_gated_near(y, up, a.activation, a.act_param);
     else if (a.activation >= 16) y = rdl_unary(y, a.activation);
     if (a.softcap > 0.f) y = a.softcap * tanhf(y / a.softcap);
     return y;
@@ -432,13 +430,17 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             for (int idx = tid; idx < a.M * a.share; idx += WORKERS) {
                 const int m = idx / a.share, o = idx - m * a.share, of_tile = rank * a.share + o, n = first_tile * per_tile + of_tile;
                 if (of_tile >= per_tile || n >= a.N) continue;
-                float v[2] = {0.f, 0.f};
-                for (int s = 0; s < a.split; ++s) {
-                    const float* ys = y + (s * R + m) * outs;
-                    if (a.gated) { v[0] += ys[2 * o]; v[1] += ys[2 * o + 1]; }
-                    else v[0] += ys[o];
+                const float* ys = y + m * outs + (a.gated ? 2 * o : o);
+                float v[8], u[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {                // all asked for before the first is used
+                    v[s] = s < a.split ? ys[s * R * outs] : 0.f;
+                    u[s] = a.gated && s < a.split ? ys[s * R * outs + 1] : 0.f;
                 }
-                rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, finish(a, v[0], v[1]));
+                float sum = 0.f, up = 0.f;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) { sum += v[s]; up += u[s]; }
+                rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, finish(a, sum, up));
             }
         }
     }
@@ -448,42 +450,12 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
-// Clusters of `size` blocks, each block with a multiprocessor to itself, that run at the same time on the current device.  Fewer than
-// multiprocessors / size: a cluster lies within one group of them, and what is left of a group stays empty (18 clusters of 8 on 148
-// multiprocessors took two turns, 14 us where one took 6).
-int clusters_at_once(int size) {
-    static std::atomic<int> known[64][9];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if (const int k = known[dev][size].load(std::memory_order_relaxed)) return k - 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(size * 32);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = 200 * 1024;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)size;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (rdl_allow_shared<mx_few_rows_kernel<2, 8>>(200 * 1024) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, mx_few_rows_kernel<2, 8>, &cfg) != cudaSuccess) {
-        cudaGetLastError();                                  // an answer of none is safe: the tile is not shared
-        n = 0;
-    }
-    known[dev][size].store(n + 1, std::memory_order_relaxed);
-    return n;
-}
-
 template <int PARTS, int R>
 int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
     constexpr int NB = PARTS * R, PER_BLOCK = NB * MX_BLOCK + MX_SCALE_BYTES, PER_STAGE = STEP * (MX_TILE_BYTES + MX_SCALE_BYTES);
     const int sms = rdl_sm_count();
     a.tiles = w.tiles;
-    // as many blocks a tile as keeps every tile on the device at once, each with two blocks of columns or more
-    a.split = 1;
-    if (a.tiles * 2 <= sms)
-        for (a.split = 8; a.split > 1; --a.split)
-            if (a.blocks >= 2 * a.split && a.tiles <= clusters_at_once(a.split)) break;
+    a.split = mx_split(a.tiles, a.blocks, sms);
     a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
     a.slice_blocks = (a.blocks + a.split - 1) / a.split;
     const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - 1024 - sums;      // alignment, static shared memory

@@ -19,8 +19,6 @@
 // row lie in one thread, which is a group.
 //
 // Every wait is bounded; a block that gives up sets `status` and every path ends in the common tear-down.
-#include <cstdlib>
-
 #include "activations.cuh"
 #include "api.h"
 #include "launch.cuh"
@@ -111,20 +109,15 @@ __device__ __forceinline__ void finish(const ManyArgs& a, float (&y)[32], const 
         if (a.out_kind == RDL_F32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = rdl_gated(y[i], u[i], a.activation, a.act_param);
-        } else if (a.activation == RDL_ACT_GELU_TANH) {
-            // 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z)) by the hardware's powers of two and reciprocal: good to 2^-20, where its tanh, at
-            // 2^-11, would move one 8-bit code in a thousand
+        } else if (a.activation == RDL_ACT_GELU_TANH) {      // the choice is made once a piece
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float g = y[i], t = g * fmaf(-0.10294324f, g * g, -2.3022082f);      // -2 z log2(e)
-                float e, r;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-                y[i] = g * r * u[i];
-            }
+            for (int i = 0; i < 32; ++i) y[i] = rdl_gated_near(y[i], u[i], RDL_ACT_GELU_TANH, 0.f);
+        } else if (a.activation == RDL_ACT_SILU) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = rdl_gated_near(y[i], u[i], RDL_ACT_SILU, 0.f);
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = rdl_gated_fast(y[i], u[i], a.activation, a.act_param);
+            for (int i = 0; i < 32; ++i) y[i] = rdl_gated_near(y[i], u[i], RDL_ACT_SWISH_LIMIT, a.act_param);
         }
     } else if (a.activation >= 16) {
 #pragma unroll
@@ -326,12 +319,21 @@ __global__ void __launch_bounds__(THREADS, 1) mx_many_rows_kernel(const __grid_c
                             const uint4 raw = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
                             if (row < a.M && col < a.N) *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (long long)row * a.N + col) = raw;
                         }
-                    } else {                                              // rows that begin anywhere
-#pragma unroll 8
-                        for (int r = 0; r < 32; ++r) {
-                            const int row = m0 + 4 * r + q;
-                            const __nv_bfloat16 e = *reinterpret_cast<const __nv_bfloat16*>(stage + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-                            if (row < a.M && n + lane < a.N) ((__nv_bfloat16*)a.out)[(long long)row * a.N + n + lane] = e;
+                    } else {                                              // rows that begin anywhere: a column a lane, 16 rows in flight
+                        __nv_bfloat16* o = (__nv_bfloat16*)a.out + (long long)(m0 + q) * a.N + n + lane;
+                        const long long step = 4LL * a.N;
+                        const int there = n + lane < a.N ? (a.M - m0 - q + 3) / 4 : 0;      // rows 4 r + q of the tile that are there
+#pragma unroll
+                        for (int r0 = 0; r0 < 32; r0 += 16) {
+                            __nv_bfloat16 e[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const int r = r0 + j;
+                                e[j] = *reinterpret_cast<const __nv_bfloat16*>(stage + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (r0 + j < there) o[(r0 + j) * step] = e[j];
                         }
                     }
                     __syncwarp();
@@ -391,6 +393,8 @@ extern "C" int rdl_mx_many_rows(void* out, int out_kind, void* out_scales, const
     RDL_REQUIRE((uintptr_t)x % 16 == 0 && (uintptr_t)row_scales % 16 == 0 && (uintptr_t)out % 16 == 0, "mx_many_rows: operands must start on 16-byte boundaries");
     RDL_REQUIRE(!w->gated || rdl_gated_known(activation), "mx_many_rows: unknown activation %d", activation);
     RDL_REQUIRE(softcap >= 0.f, "mx_many_rows: soft-cap must not be negative");
+    if (m <= 128 && out_kind != RDL_MX8 && mx_some_rows_pay(*w, m))
+        return rdl_mx_some_rows(out, out_kind, x, row_scales, weight, m, activation, act_param, softcap, status, stream);
     const int n = w->gated ? w->rows / 2 : w->rows;
     const cuuint64_t blocks = w->blocks, cols = blocks * MX_BLOCK, rows4 = (m + 3LL) / 4 * 4;
     CUtensorMap mx, mxs;
@@ -405,8 +409,6 @@ extern "C" int rdl_mx_many_rows(void* out, int out_kind, void* out_scales, const
     a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_MANY); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_MANY);
     a.status = status;
     cudaStream_t st = (cudaStream_t)stream;
-    static const int forced = getenv("RDL_MX_PAIR") ? atoi(getenv("RDL_MX_PAIR")) : -1;
-    const bool pair = forced >= 0 ? forced : m > BM;
-    if (pair) return w->gated ? launch<true, 2>(mx, mxs, *w, a, st) : launch<false, 2>(mx, mxs, *w, a, st);
+    if (m > BM) return w->gated ? launch<true, 2>(mx, mxs, *w, a, st) : launch<false, 2>(mx, mxs, *w, a, st);
     return w->gated ? launch<true, 1>(mx, mxs, *w, a, st) : launch<false, 1>(mx, mxs, *w, a, st);
 }

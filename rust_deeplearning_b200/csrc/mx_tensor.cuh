@@ -23,6 +23,11 @@ struct Mx4Matrix {
     int blocks, tiles;                           // of 128 columns, of 128 rows
 };
 
+// Blocks that share a tile, each with its part of the columns: as many as keep every tile on the device at once (in clusters of up to 8),
+// each with two blocks of columns or more.
+int mx_split(int tiles, int blocks, int sms);
+bool mx_some_rows_pay(const Mx4Matrix& w, int m);
+
 namespace {
 
 constexpr int MX_TILE_BYTES = MX_ROWS * MX_BLOCK, MX_TILE_TX = MX_TILE_BYTES / 2;      // in shared memory; read (what a 4-bit transfer counts)

@@ -190,6 +190,7 @@ FAULTS = {
     7: "gemm_skinny: a weight copy did not complete",
     8: "mx_few_rows: a weight copy or a product did not complete",
     9: "mx_many_rows: a stage or an accumulator was not handed over",
+    10: "mx_some_rows: a stage or an accumulator was not handed over",
 }
 
 
@@ -437,6 +438,7 @@ _SIGNATURES = {
     "rdl_mx4_matrix_bytes": [],
     "rdl_mx4_describe": [_P, _P, _P, _I, _I, _I],
     "rdl_mx_few_rows": [_P, _I, _P, _I, _P, _P, _I, _I, _F, _F, _P, _P],
+    "rdl_mx_some_rows": [_P, _I, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_mx_many_rows": [_P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_random_normal": [_P, _I, _LL, ctypes.c_ulonglong, ctypes.c_double, _P],
     "rdl_sample": [_P, _P, _P, _I, _I, ctypes.POINTER(SamplingArgs), _P, _P, _P, _P, _P, _P],

@@ -1788,7 +1788,7 @@ def delta_rule_scan(rows: torch.Tensor, *, v_col: int, q_f, k_f, g_f, beta_f, n_
 # description, its sizes and its device) and build no message unless something is wrong.
 
 MX_GROUP, MX_BLOCK, MX_ROWS = 32, 128, 128
-MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs; above, the tensor-core tiles of 128 rows
+MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs, which also takes tensors; above, 8-bit rows only
 _MX8 = 2                 # rows of 8 bits, where a kernel's argument says of what kind its rows are
 _KINDS = {torch.float32: 0, torch.bfloat16: 1}
 _raw_stream = torch._C._cuda_getCurrentRawStream

@@ -200,7 +200,7 @@ def test_few_rows(m, n, k, kind):
     check(ops.linear_mx4(x, w, out_dtype=torch.bfloat16), want, tol + np.abs(want) * 2.0 ** -8, "bfloat16")
 
 
-@pytest.mark.parametrize("m,n,k", [(17, 1, 1), (17, 40, 32), (100, 777, 1003), (128, 256, 128), (129, 257, 300), (300, 130, 2304), (40, 600, 14336)])
+@pytest.mark.parametrize("m,n,k", [(17, 1, 1), (17, 40, 32), (33, 2304, 2304), (64, 4096, 1280), (100, 777, 1003), (128, 20000, 160), (127, 19001, 300), (130, 777, 1003), (128, 256, 128), (129, 257, 300), (300, 130, 2304), (40, 600, 14336)])
 def test_many_rows(m, n, k):
     w = ops.pack_mx4(rnd((n, k), torch.float32, 7, 0.05))
     x, x64 = rows_for(m, k, "mx8", 8)
@@ -340,11 +340,11 @@ def test_a_product_right_behind_the_packing():
         assert torch.equal(first, ops.linear_mx4(x, packed))
 
 
-@pytest.mark.parametrize("m,code,name", [(8, 8, "mx_few_rows"), (40, 9, "mx_many_rows")])
-def test_a_wait_that_runs_out(m, code, name):
+@pytest.mark.parametrize("m,k,code,name", [(8, 512, 8, "mx_few_rows"), (140, 512, 9, "mx_many_rows"), (40, 4096, 10, "mx_some_rows")])
+def test_a_wait_that_runs_out(m, k, code, name):
     lib = library.load()
-    w = ops.pack_mx4(rnd((300, 512), torch.float32, 25))
-    x, x64 = rows_for(m, 512, "mx8", 26)
+    w = ops.pack_mx4(rnd((300, k), torch.float32, 25))
+    x, x64 = rows_for(m, k, "mx8", 26)
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
     try:
         lib.rdl_set_wait_test(code, 200_000, 64)
