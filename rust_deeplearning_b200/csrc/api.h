@@ -440,7 +440,7 @@ int rdl_norm_mx8(const void* x, int x_dtype, const void* w1, int w1_dtype, float
                  const float* residual, float* residual_out, const void* w2, int w2_dtype, float eps2, float off2,
                  void* values, void* scales, int n_rows, int width, void* stream);
 // A [rows, columns] matrix to 4 bits, in tiles of 128 x 128: codes of 8 KB a tile, scales of 512 bytes a tile and 16 bytes more.
-// gated: a [gate; up] matrix.  The padding is left as it is (the products want zeros there).
+// gated: a [gate; up] matrix.  The padding becomes zeros.
 int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales, int rows, int columns, int gated, void* stream);
 // the values of a 4-bit matrix, [rows, columns]
 int rdl_expand_mx4(const void* codes, const void* scales, void* out, int dtype, int rows, int columns, int gated, void* stream);

@@ -20,11 +20,11 @@
 constexpr int MX_GROUP = 32, MX_BLOCK = 128, MX_ROWS = 128, MX_UNIT = 16;
 static inline int mx_blocks(int columns) { return (columns + MX_BLOCK - 1) / MX_BLOCK; }
 
-// where row `row` of a weight lies; half: outputs of a [gate; up] matrix, 0: not one
-__device__ __forceinline__ int mx_place(int row, int half) {
-    if (half == 0) return row;
-    const int up = row >= half, o = row - (up ? half : 0);
-    return o / MX_UNIT * (2 * MX_UNIT) + up * MX_UNIT + o % MX_UNIT;
+// which row of a weight lies at `place`, or -1: padding; rows: of the matrix, half: outputs of a [gate; up] matrix, 0: not one
+__device__ __forceinline__ int mx_row_at(int place, int rows, int half) {
+    if (half == 0) return place < rows ? place : -1;
+    const int up = place / MX_UNIT & 1, o = place / (2 * MX_UNIT) * MX_UNIT + place % MX_UNIT;
+    return o < half ? o + up * half : -1;
 }
 // bytes from the start of the codes to the one of (place, column), and of the scales to the one of its group
 __device__ __forceinline__ long long mx_code_at(int place, int column, int blocks) {

@@ -369,14 +369,14 @@ __global__ void __launch_bounds__(THREADS, 1) mx_many_rows_kernel(const __grid_c
 }
 
 template <bool GATED, int CTAS>
-int launch(const CUtensorMap& mx, const CUtensorMap& mxs, const Mx4Matrix& w, const ManyArgs& a, cudaStream_t st) {
+int launch(const MxRowsMaps& maps, const Mx4Matrix& w, const ManyArgs& a, cudaStream_t st) {
     constexpr int OUT_BN = GATED ? BN / 2 : BN;
     const long long tiles = (long long)((a.N + OUT_BN - 1) / OUT_BN) * ((a.M + BM * CTAS - 1) / (BM * CTAS));
     RDL_REQUIRE(tiles <= 0x3fffffffLL, "mx_many_rows: %lld tiles are too many", tiles);
     const int at_once = rdl_sm_count() / CTAS > 0 ? rdl_sm_count() / CTAS : 1;
     RDL_CUDA((rdl_allow_shared<mx_many_rows_kernel<GATED, CTAS>>(smem_bytes(CTAS))), "mx_many_rows");
     RDL_CHECK_EX(rdl_launch_cluster(mx_many_rows_kernel<GATED, CTAS>, dim3((tiles < at_once ? (int)tiles : at_once) * CTAS), dim3(THREADS), CTAS,
-                                    (size_t)smem_bytes(CTAS), st, mx, mxs, w.codes_map, w.scales_map, a), "mx_many_rows");
+                                    (size_t)smem_bytes(CTAS), st, maps.values, maps.scales, w.codes_map, w.scales_map, a), "mx_many_rows");
     return 0;
 }
 
@@ -396,11 +396,9 @@ extern "C" int rdl_mx_many_rows(void* out, int out_kind, void* out_scales, const
     if (m <= 128 && out_kind != RDL_MX8 && mx_some_rows_pay(*w, m))
         return rdl_mx_some_rows(out, out_kind, x, row_scales, weight, m, activation, act_param, softcap, status, stream);
     const int n = w->gated ? w->rows / 2 : w->rows;
-    const cuuint64_t blocks = w->blocks, cols = blocks * MX_BLOCK, rows4 = (m + 3LL) / 4 * 4;
-    CUtensorMap mx, mxs;
-    if (int e = mx_make_map(&mx, x, {CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, {cols, rows4 / 4, 4}, {cols * 4, cols}, {BK, 32, 4}, CU_TENSOR_MAP_SWIZZLE_128B}, "8-bit rows")) return e;
-    if (int e = mx_make_map(&mxs, row_scales, {CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, {rows4, blocks}, {rows4 * 4}, {BM, 1}, CU_TENSOR_MAP_SWIZZLE_NONE},
-                            "the scales of 8-bit rows")) return e;
+    const long long blocks = w->blocks, rows4 = (m + 3LL) / 4 * 4;
+    MxRowsMaps maps;
+    if (int e = mx_rows_maps(&maps, x, row_scales, blocks, rows4)) return e;
     ManyArgs a{};
     a.out = out; a.out_kind = out_kind; a.out_scales = (uint8_t*)out_scales;
     a.M = m; a.N = n; a.blocks = (int)blocks;
@@ -409,6 +407,6 @@ extern "C" int rdl_mx_many_rows(void* out, int out_kind, void* out_scales, const
     a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_MANY); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_MANY);
     a.status = status;
     cudaStream_t st = (cudaStream_t)stream;
-    if (m > BM) return w->gated ? launch<true, 2>(mx, mxs, *w, a, st) : launch<false, 2>(mx, mxs, *w, a, st);
-    return w->gated ? launch<true, 1>(mx, mxs, *w, a, st) : launch<false, 1>(mx, mxs, *w, a, st);
+    if (m > BM) return w->gated ? launch<true, 2>(maps, *w, a, st) : launch<false, 2>(maps, *w, a, st);
+    return w->gated ? launch<true, 1>(maps, *w, a, st) : launch<false, 1>(maps, *w, a, st);
 }

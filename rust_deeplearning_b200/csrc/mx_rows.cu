@@ -9,7 +9,7 @@
 // scale codes of a block leave as one word.  The threads a row gets depend on its width alone, so its result does
 // not depend on how many rows a step has.
 //
-// rdl_pack_mx4: a lane takes eight columns (16 bytes of bfloat16 in, 4 bytes of codes out), a group is four lanes.  Memory bound.
+// rdl_pack_mx4: a matrix to 4 bits, padding and all.  Memory bound.
 // rdl_expand_mx4: the values the codes stand for; exact in bfloat16 for scales from 2^-125 up to 2^125.
 #include <cuda_fp16.h>
 
@@ -29,6 +29,23 @@ struct NormMxArgs {
     uint8_t* values; uint8_t* scales;
     int rows, width, blocks, padded_rows;
 };
+
+// 1 / sqrt(sum over the block / n + eps) for every thread; `part` holds a float a warp and is used for this sum alone, so that one barrier
+// is enough.  The order of additions depends on the block's size alone.  The hardware's reciprocal root and one Newton step: an
+// error of this factor would move every value of the row the same way, and 8-bit codes with them.
+__device__ __forceinline__ float row_factor(float v, float* part, int n, float eps) {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int warps = blockDim.x >> 5;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+        if (w < warps) t += part[w];
+    const float a = t / (float)n + eps, r = rsqrtf(a);
+    const float step = 0.5f * r * fmaf(-(a * r), r, 1.0f);
+    return a > 0.f && isfinite(a) && isfinite(r) ? r + step : r;      // nothing to mend of an infinity or a NaN
+}
 
 // four consecutive columns from column c of a row that starts at element `base`; zeros beyond the width
 template <bool VEC>
@@ -58,43 +75,64 @@ __device__ __forceinline__ void store_block(const float (&v)[4], uint8_t* values
     if (lane == 0) *reinterpret_cast<uint32_t*>(scales) = word;
 }
 
-template <int ITER, bool VEC>
-__global__ void __launch_bounds__(256) norm_mx8_kernel(const __grid_constant__ NormMxArgs a) {
-    __shared__ float scratch[33];
+// HALF: bfloat16 rows, kept as they are between the passes: two registers a group of four columns, which lets one block more run.
+template <int ITER, bool VEC, bool HALF>
+__global__ void __launch_bounds__(256, ITER <= 4 ? 5 : (ITER <= 6 ? 4 : 3)) norm_mx8_kernel(const __grid_constant__ NormMxArgs a) {
+    static_assert(VEC || !HALF, "rows of any width are read value by value");
+    __shared__ float part[2][8];
     rdl_grid_wait();
     rdl_grid_launch_dependents();
     const int r = blockIdx.x, lane = threadIdx.x & 31;
     const long long base = (long long)r * a.width;
-    float v[ITER][4], h[ITER][4];
+    uint2 raw[HALF ? ITER : 1];
+    float v[ITER][4];                                       // HALF: the residual, then the sum; else x, then the sum
+    float h[HALF ? 1 : ITER][4];                            // the residual
+    auto column = [&](int i) { return (i * (int)blockDim.x + (int)threadIdx.x) * 4; };
+    auto value = [&](int i, float (&x)[4]) {                // x as float
+        if (HALF) {
+            const uint2 w = raw[HALF ? i : 0];
+            x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u); x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = v[i][k];
+        }
+    };
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 4;
-        load_columns<VEC>(a.x, base, c, a.width, a.x_dtype, v[i]);
-        if (a.res) load_columns<VEC>(a.res, base, c, a.width, RDL_F32, h[i]);
-        else h[i][0] = h[i][1] = h[i][2] = h[i][3] = 0.f;
+        const int c = column(i);
+        if (HALF) raw[HALF ? i : 0] = c < a.width ? *reinterpret_cast<const uint2*>((const __nv_bfloat16*)a.x + base + c) : make_uint2(0, 0);
+        else load_columns<VEC>(a.x, base, c, a.width, a.x_dtype, v[i]);
+        float (&res)[4] = HALF ? v[i] : h[HALF ? 0 : i];
+        if (a.res) load_columns<VEC>(a.res, base, c, a.width, RDL_F32, res);
+        else res[0] = res[1] = res[2] = res[3] = 0.f;
     }
+    float inv = 1.f;
     if (a.w1) {
         float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < ITER; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) ss = fmaf(v[i][k], v[i][k], ss);
-        const float inv = 1.0f / sqrtf(block_sum(ss, scratch) / (float)a.width + a.eps1);
-#pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            float w[4];
-            load_columns<VEC>(a.w1, 0, (i * (int)blockDim.x + (int)threadIdx.x) * 4, a.width, a.w1_dtype, w);
+            float x[4];
+            value(i, x);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = v[i][k] * inv * (w[k] + a.off1);
+            for (int k = 0; k < 4; ++k) ss = fmaf(x[k], x[k], ss);
         }
+        inv = row_factor(ss, part[0], a.width, a.eps1);
     }
     float s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 4;
+        const int c = column(i);
+        float x[4];
+        value(i, x);
+        if (a.w1) {
+            float w[4];
+            load_columns<VEC>(a.w1, 0, c, a.width, a.w1_dtype, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = x[k] * inv * (w[k] + a.off1);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (a.res) v[i][k] = h[i][k] + v[i][k];
+            v[i][k] = a.res ? (HALF ? v[i][k] : h[HALF ? 0 : i][k]) + x[k] : x[k];
             s2 = fmaf(v[i][k], v[i][k], s2);
         }
         if (a.res_out) {
@@ -107,11 +145,10 @@ __global__ void __launch_bounds__(256) norm_mx8_kernel(const __grid_constant__ N
             }
         }
     }
-    float inv2 = 1.f;
-    if (a.w2) inv2 = 1.0f / sqrtf(block_sum(s2, scratch) / (float)a.width + a.eps2);
+    const float inv2 = a.w2 ? row_factor(s2, part[1], a.width, a.eps2) : 1.f;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 4;
+        const int c = column(i);
         const int block = c / MX_BLOCK;                     // one for the whole warp
         if (block >= a.blocks) break;
         if (a.w2) {
@@ -128,7 +165,7 @@ __global__ void __launch_bounds__(256) norm_mx8_kernel(const __grid_constant__ N
 // Rows wider than the registers of a block: the row is read once a pass.
 template <bool VEC>
 __global__ void __launch_bounds__(256) norm_mx8_wide_kernel(const __grid_constant__ NormMxArgs a) {
-    __shared__ float scratch[33];
+    __shared__ float part[2][8];
     rdl_grid_wait();
     rdl_grid_launch_dependents();
     const int r = blockIdx.x, lane = threadIdx.x & 31, step = blockDim.x * 4;
@@ -142,7 +179,7 @@ __global__ void __launch_bounds__(256) norm_mx8_wide_kernel(const __grid_constan
 #pragma unroll
             for (int k = 0; k < 4; ++k) ss = fmaf(v[k], v[k], ss);
         }
-        inv = 1.0f / sqrtf(block_sum(ss, scratch) / (float)a.width + a.eps1);
+        inv = row_factor(ss, part[0], a.width, a.eps1);
     }
     // h of four columns: the sum of x's norm and the residual
     auto sum_at = [&](int c, float (&v)[4]) {
@@ -173,7 +210,7 @@ __global__ void __launch_bounds__(256) norm_mx8_wide_kernel(const __grid_constan
         }
     }
     float inv2 = 1.f;
-    if (a.w2) inv2 = 1.0f / sqrtf(block_sum(s2, scratch) / (float)a.width + a.eps2);
+    if (a.w2) inv2 = row_factor(s2, part[1], a.width, a.eps2);
     for (int c = threadIdx.x * 4; c < a.blocks * MX_BLOCK; c += step) {      // whole warps: both sides are multiples of 128
         float v[4];
         // the sum may have replaced the residual it was formed from: this thread reads what it wrote itself
@@ -191,48 +228,71 @@ __global__ void __launch_bounds__(256) norm_mx8_wide_kernel(const __grid_constan
     }
 }
 
+// Packing and expanding: a block takes a tile of 128 x 128, 8 warps two rows at a time, a lane eight columns of one: 256 bytes of bfloat16
+// and 64 bytes of codes of a row in one piece, four rows of a lane in flight.
+constexpr int TILE_AHEAD = 4;
+
 struct PackArgs {
     const void* w; int dtype;
     uint8_t* codes; uint8_t* scales;
-    int rows, columns, blocks;
-    int half;                                               // gated: outputs (source rows of each half); 0: not gated
+    int rows, columns, blocks, half;                        // half: outputs of a [gate; up] matrix, 0: not one
 };
 
-// a warp takes 256 columns of one row
-template <bool VEC>
+// VEC 2: bfloat16 rows of whole 16-byte pieces; 1: rows of whole groups of four columns; 0: any
+template <int VEC>
 __global__ void __launch_bounds__(256) pack_mx4_kernel(const __grid_constant__ PackArgs a) {
     rdl_grid_wait();
     rdl_grid_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int pieces = (a.blocks + 1) / 2;
-    const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (item >= (long long)a.rows * pieces) return;
-    const int row = (int)(item / pieces), piece = (int)(item - (long long)row * pieces);
-    const int to = mx_place(row, a.half);
-    const int c = piece * 256 + lane * 8;
-    const long long base = (long long)row * a.columns;
-    float v[8];
-    float (&lo)[4] = reinterpret_cast<float (&)[4]>(v[0]);
-    float (&hi)[4] = reinterpret_cast<float (&)[4]>(v[4]);
-    load_columns<VEC>(a.w, base, c, a.columns, a.dtype, lo);
-    load_columns<VEC>(a.w, base, c + 4, a.columns, a.dtype, hi);
-    float m = 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x / a.blocks, block = blockIdx.x - tile * a.blocks, c = block * MX_BLOCK + (lane & 15) * 8;
+    uint8_t* codes = a.codes + (long long)blockIdx.x * (MX_ROWS * MX_BLOCK / 2);
+    uint8_t* scales = a.scales + (long long)blockIdx.x * (MX_ROWS * 4);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = mx_larger(m, v[k]);
-    m = mx_larger(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = mx_larger(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t code = mx4_scale_code(m);
-    const float inv = mx_inverse_scale(code);
+    for (int r0 = 0; r0 < MX_ROWS; r0 += 16 * TILE_AHEAD) {
+        float v[TILE_AHEAD][8];
+        uint4 raw[TILE_AHEAD];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= inv;
-    uint32_t word = code << ((lane & 12) * 2);              // lanes 4 q to 4 q + 3: byte q of the block's word
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    const int block = c / MX_BLOCK;
-    if (block >= a.blocks) return;
-    *reinterpret_cast<uint32_t*>(a.codes + mx_code_at(to, c, a.blocks)) = mx_to_e2m1(v);
-    if ((lane & 15) == 0)
-        *reinterpret_cast<uint32_t*>(a.scales + mx_scale_at(to, c, a.blocks)) = word;
+        for (int i = 0; i < TILE_AHEAD; ++i) {
+            const int src = mx_row_at(tile * MX_ROWS + r0 + i * 16 + warp * 2 + (lane >> 4), a.rows, a.half);
+            const int width = src < 0 ? 0 : a.columns;      // padding: nothing of the row is there
+            const long long base = (long long)src * a.columns;
+            if (VEC == 2) {
+                raw[i] = c < width ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.w + base + c) : make_uint4(0, 0, 0, 0);
+            } else {
+                load_columns<VEC != 0>(a.w, base, c, width, a.dtype, reinterpret_cast<float (&)[4]>(v[i][0]));
+                load_columns<VEC != 0>(a.w, base, c + 4, width, a.dtype, reinterpret_cast<float (&)[4]>(v[i][4]));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < TILE_AHEAD; ++i) {
+            const int r = r0 + i * 16 + warp * 2 + (lane >> 4);
+            uint32_t top = 0;                               // magnitudes are in order as integers, NaN the largest
+            if (VEC == 2) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    top = __vmaxu2(top, w[k] & 0x7fff7fffu);
+                    v[i][2 * k] = __uint_as_float(w[k] << 16);
+                    v[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                }
+                top = max(top & 0xffff0000u, top << 16);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const uint32_t code = mx4_scale_code(__uint_as_float(top));
+            const float inv = mx_inverse_scale(code);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[i][k] *= inv;
+            uint32_t word = code << ((lane & 12) * 2);      // lanes 4 q to 4 q + 3 of a row: byte q of the row's word
+            word |= __shfl_xor_sync(0xffffffffu, word, 4);
+            word |= __shfl_xor_sync(0xffffffffu, word, 8);
+            *reinterpret_cast<uint32_t*>(codes + r * (MX_BLOCK / 2) + (lane & 15) * 4) = mx_to_e2m1(v[i]);
+            if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + r % 32 * 16 + r / 32 * 4) = word;
+        }
+    }
 }
 
 struct ExpandArgs {
@@ -245,38 +305,59 @@ template <bool VEC>
 __global__ void __launch_bounds__(256) expand_mx4_kernel(const __grid_constant__ ExpandArgs a) {
     rdl_grid_wait();
     rdl_grid_launch_dependents();
-    const int words = a.blocks * (MX_BLOCK / 8);            // of eight codes, a row
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (long long)a.rows * words) return;
-    const int row = (int)(i / words), word = (int)(i - (long long)row * words), c = word * 8;
-    const int from = mx_place(row, a.half);
-    uint32_t h[4];
-    mx_from_e2m1(*reinterpret_cast<const uint32_t*>(a.codes + mx_code_at(from, c, a.blocks)), h);
-    const float s = mx_scale(a.scales[mx_scale_at(from, c, a.blocks)]);
-    const long long base = (long long)row * a.columns + c;
-    float v[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x / a.blocks, block = blockIdx.x - tile * a.blocks, c = block * MX_BLOCK + (lane & 15) * 8;
+    const uint8_t* codes = a.codes + (long long)blockIdx.x * (MX_ROWS * MX_BLOCK / 2);
+    const uint8_t* scales = a.scales + (long long)blockIdx.x * (MX_ROWS * 4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
-        v[2 * k] = f.x * s;
-        v[2 * k + 1] = f.y * s;
-    }
-    if (VEC && c + 8 <= a.columns) {
-        if (a.dtype == RDL_BF16) {
-            uint4 raw;
-            __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(&raw);
+    for (int r0 = 0; r0 < MX_ROWS; r0 += 16 * TILE_AHEAD) {
+        uint32_t w[TILE_AHEAD], sc[TILE_AHEAD];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-            *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + base) = raw;
-        } else {
-            *reinterpret_cast<float4*>((float*)a.out + base) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>((float*)a.out + base + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        for (int i = 0; i < TILE_AHEAD; ++i) {
+            const int r = r0 + i * 16 + warp * 2 + (lane >> 4);
+            w[i] = *reinterpret_cast<const uint32_t*>(codes + r * (MX_BLOCK / 2) + (lane & 15) * 4);
+            sc[i] = scales[r % 32 * 16 + r / 32 * 4 + (lane & 15) / 4];
         }
-    } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (c + k < a.columns) rdl_store(a.out, base + k, a.dtype, v[k]);
+        for (int i = 0; i < TILE_AHEAD; ++i) {
+            const int row = mx_row_at(tile * MX_ROWS + r0 + i * 16 + warp * 2 + (lane >> 4), a.rows, a.half);
+            if (row < 0) continue;
+            uint32_t h[4];
+            mx_from_e2m1(w[i], h);
+            const float s = mx_scale(sc[i]);
+            const long long base = (long long)row * a.columns + c;
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+                v[2 * k] = f.x * s;
+                v[2 * k + 1] = f.y * s;
+            }
+            if (VEC) {
+                if (c >= a.columns) continue;
+                if (a.dtype == RDL_BF16) {
+                    uint4 raw;
+                    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                    *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + base) = raw;
+                } else {
+                    *reinterpret_cast<float4*>((float*)a.out + base) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>((float*)a.out + base + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + k < a.columns) rdl_store(a.out, base + k, a.dtype, v[k]);
+            }
+        }
     }
+}
+
+// tiles of 128 rows of a weight
+int weight_tiles(int rows, int gated) {
+    const int places = gated ? (rows / 2 + MX_UNIT - 1) / MX_UNIT * (2 * MX_UNIT) : rows;
+    return (places + MX_ROWS - 1) / MX_ROWS;
 }
 
 }  // namespace
@@ -293,19 +374,25 @@ extern "C" int rdl_norm_mx8(const void* x, int x_dtype, const void* w1, int w1_d
                        (uint8_t*)values, (uint8_t*)scales, n_rows, width, mx_blocks(width), (n_rows + 3) / 4 * 4};
     const bool vec = width % 4 == 0 && aligned16(x) && aligned16(w1) && aligned16(w2) && aligned16(residual) && aligned16(residual_out);
     cudaStream_t st = (cudaStream_t)stream;
-    const int quads = a.blocks * (MX_BLOCK / 4);
-    // the fewest whole warps that hold the row with the fewest columns a thread, up to 256 threads
-    const int iter = quads <= 256 ? 1 : (quads <= 512 ? 2 : (quads <= 1024 ? 4 : 8));
-    const int threads = ((quads + iter - 1) / iter + 31) / 32 * 32;
-    cudaError_t e;
-#define RDL_NORM_MX8(I) (e = vec ? rdl_launch(norm_mx8_kernel<I, true>, dim3(n_rows), dim3(threads), 0, st, a) \
-                                 : rdl_launch(norm_mx8_kernel<I, false>, dim3(n_rows), dim3(threads), 0, st, a))
+    const int quads = a.blocks * (MX_BLOCK / 4);            // groups of four columns
+    // the threads, 128 to 256, and the groups of each that leave the fewest of them without one; on the width alone
+    int threads = 32, iter = 1;
+    if (quads > 32) {
+        int best = 1 << 30;
+        for (int t = quads < 256 ? (quads + 31) / 32 * 32 : 256; t >= (quads < 128 ? 32 : 128); t -= 32) {
+            const int i = (quads + t - 1) / t;
+            if (i <= RN_MAX_IT && i * t < best) { best = i * t; threads = t; iter = i; }
+        }
+    }
+    cudaError_t e = cudaErrorInvalidValue;
+    const bool half = vec && x_dtype == RDL_BF16;
+#define RDL_NORM_MX8(I) case I: e = half ? rdl_launch(norm_mx8_kernel<I, true, true>, dim3(n_rows), dim3(threads), 0, st, a) \
+                                    : vec ? rdl_launch(norm_mx8_kernel<I, true, false>, dim3(n_rows), dim3(threads), 0, st, a) \
+                                          : rdl_launch(norm_mx8_kernel<I, false, false>, dim3(n_rows), dim3(threads), 0, st, a); break
     if (quads > 256 * RN_MAX_IT)
         e = vec ? rdl_launch(norm_mx8_wide_kernel<true>, dim3(n_rows), dim3(256), 0, st, a) : rdl_launch(norm_mx8_wide_kernel<false>, dim3(n_rows), dim3(256), 0, st, a);
-    else if (iter == 1) RDL_NORM_MX8(1);
-    else if (iter == 2) RDL_NORM_MX8(2);
-    else if (iter == 4) RDL_NORM_MX8(4);
-    else RDL_NORM_MX8(8);
+    else
+        switch (iter) { RDL_NORM_MX8(1); RDL_NORM_MX8(2); RDL_NORM_MX8(3); RDL_NORM_MX8(4); RDL_NORM_MX8(5); RDL_NORM_MX8(6); RDL_NORM_MX8(7); RDL_NORM_MX8(8); }
 #undef RDL_NORM_MX8
     RDL_CHECK_EX(e, "norm_mx8");
     return 0;
@@ -316,18 +403,18 @@ extern "C" int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales,
     RDL_REQUIRE(rdl_valid_dtype(dtype), "pack_mx4: bad dtype %d", dtype);
     RDL_REQUIRE(rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "pack_mx4: bad sizes rows=%d columns=%d", rows, columns);
     RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "pack_mx4: the results must start on 16-byte boundaries");
-    const int half = gated ? rows / 2 : 0;
-    const PackArgs a{w, dtype, (uint8_t*)codes, (uint8_t*)scales, rows, columns, mx_blocks(columns), half};
-    const long long warps = (long long)rows * ((a.blocks + 1) / 2), grid = (warps + 7) / 8;
+    const PackArgs a{w, dtype, (uint8_t*)codes, (uint8_t*)scales, rows, columns, mx_blocks(columns), gated ? rows / 2 : 0};
+    const long long grid = (long long)weight_tiles(rows, gated) * a.blocks;
     RDL_REQUIRE(grid <= 0x7fffffffLL, "pack_mx4: %d x %d is too large", rows, columns);
     cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = columns % 4 == 0 && aligned16(w) ? rdl_launch(pack_mx4_kernel<true>, dim3((unsigned)grid), dim3(256), 0, st, a)
-                                                           : rdl_launch(pack_mx4_kernel<false>, dim3((unsigned)grid), dim3(256), 0, st, a);
+    const int vec = columns % 4 == 0 && aligned16(w) ? (dtype == RDL_BF16 && columns % 8 == 0 ? 2 : 1) : 0;
+    const cudaError_t e = vec == 2 ? rdl_launch(pack_mx4_kernel<2>, dim3((unsigned)grid), dim3(256), 0, st, a)
+                          : vec == 1 ? rdl_launch(pack_mx4_kernel<1>, dim3((unsigned)grid), dim3(256), 0, st, a)
+                                     : rdl_launch(pack_mx4_kernel<0>, dim3((unsigned)grid), dim3(256), 0, st, a);
     RDL_CHECK_EX(e, "pack_mx4");
     // The products read weights before the kernel ahead of them has ended (launch.cuh).  Something that is launched the ordinary way
     // comes in between, so that a product right behind this call finds the codes written.
-    const long long tiles = ((gated ? 2LL * ((half + MX_UNIT - 1) / MX_UNIT) * MX_UNIT : rows) + MX_ROWS - 1) / MX_ROWS;
-    RDL_CUDA(cudaMemsetAsync((uint8_t*)scales + tiles * a.blocks * (MX_ROWS * 4), 0, 16, st), "pack_mx4");
+    RDL_CUDA(cudaMemsetAsync((uint8_t*)scales + grid * (MX_ROWS * 4), 0, 16, st), "pack_mx4");
     return 0;
 }
 
@@ -336,9 +423,8 @@ extern "C" int rdl_expand_mx4(const void* codes, const void* scales, void* out, 
     RDL_REQUIRE(rdl_valid_dtype(dtype), "expand_mx4: bad dtype %d", dtype);
     RDL_REQUIRE(rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "expand_mx4: bad sizes rows=%d columns=%d", rows, columns);
     RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "expand_mx4: the codes must start on 16-byte boundaries");
-    const int half = gated ? rows / 2 : 0;
-    const ExpandArgs a{(const uint8_t*)codes, (const uint8_t*)scales, out, dtype, rows, columns, mx_blocks(columns), half};
-    const long long words = (long long)rows * a.blocks * (MX_BLOCK / 8), grid = (words + 255) / 256;
+    const ExpandArgs a{(const uint8_t*)codes, (const uint8_t*)scales, out, dtype, rows, columns, mx_blocks(columns), gated ? rows / 2 : 0};
+    const long long grid = (long long)weight_tiles(rows, gated) * a.blocks;
     RDL_REQUIRE(grid <= 0x7fffffffLL, "expand_mx4: %d x %d is too large", rows, columns);
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = columns % 8 == 0 && aligned16(out) ? rdl_launch(expand_mx4_kernel<true>, dim3((unsigned)grid), dim3(256), 0, st, a)
@@ -354,12 +440,11 @@ extern "C" int rdl_mx4_describe(void* matrix, const void* codes, const void* sca
     RDL_REQUIRE(codes && scales && rows > 0 && columns > 0 && (!gated || rows % 2 == 0), "mx4_describe: bad sizes rows=%d columns=%d", rows, columns);
     RDL_REQUIRE((uintptr_t)codes % 32 == 0 && (uintptr_t)scales % 16 == 0, "mx4_describe: the codes must start on a 32-byte boundary, the scales on a 16-byte boundary");
     Mx4Matrix* w = (Mx4Matrix*)matrix;
-    const int part = gated ? rows / 2 : rows;
     *w = Mx4Matrix{};
     w->codes = (const uint8_t*)codes; w->scales = (const uint8_t*)scales;
     w->rows = rows; w->columns = columns; w->gated = gated ? 1 : 0;
     w->blocks = mx_blocks(columns);
-    w->tiles = ((gated ? 2 * ((part + MX_UNIT - 1) / MX_UNIT * MX_UNIT) : part) + MX_ROWS - 1) / MX_ROWS;
+    w->tiles = weight_tiles(rows, gated);
     const cuuint64_t pieces = (cuuint64_t)w->tiles * w->blocks * MX_ROWS;
     RDL_REQUIRE(pieces <= 0x7fffffffULL, "mx4_describe: %d x %d is too large", rows, columns);      // a tile's coordinate is an int
     if (int e = mx_make_map(&w->codes_map, codes, {CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, {MX_BLOCK, pieces}, {MX_BLOCK / 2}, {MX_BLOCK, MX_ROWS},

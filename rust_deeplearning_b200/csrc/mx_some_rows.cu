@@ -269,11 +269,9 @@ extern "C" int rdl_mx_some_rows(void* out, int out_dtype, const void* x, const v
     RDL_REQUIRE((uintptr_t)x % 16 == 0 && (uintptr_t)row_scales % 16 == 0, "mx_some_rows: the rows must start on 16-byte boundaries");
     RDL_REQUIRE(!w->gated || rdl_gated_known(activation), "mx_some_rows: unknown activation %d", activation);
     RDL_REQUIRE(softcap >= 0.f, "mx_some_rows: soft-cap must not be negative");
-    const cuuint64_t blocks = w->blocks, cols = blocks * MX_BLOCK, rows4 = (m + 3) / 4 * 4;
-    CUtensorMap mx, mxs;
-    if (int e = mx_make_map(&mx, x, {CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, {cols, rows4 / 4, 4}, {cols * 4, cols}, {MX_BLOCK, 32, 4}, CU_TENSOR_MAP_SWIZZLE_128B}, "8-bit rows")) return e;
-    if (int e = mx_make_map(&mxs, row_scales, {CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, {rows4, blocks}, {rows4 * 4}, {ROWS, 1}, CU_TENSOR_MAP_SWIZZLE_NONE},
-                            "the scales of 8-bit rows")) return e;
+    const long long blocks = w->blocks, rows4 = (m + 3LL) / 4 * 4;
+    MxRowsMaps maps;
+    if (int e = mx_rows_maps(&maps, x, row_scales, blocks, rows4)) return e;
     SomeArgs a{};
     a.out = out; a.out_dtype = out_dtype;
     a.M = m; a.N = w->gated ? w->rows / 2 : w->rows; a.blocks = w->blocks; a.tiles = w->tiles;
@@ -292,6 +290,6 @@ extern "C" int rdl_mx_some_rows(void* out, int out_dtype, const void* x, const v
     cudaStream_t st = (cudaStream_t)stream;
     RDL_CUDA(rdl_allow_shared<mx_some_rows_kernel>(smem), "mx_some_rows");
     const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
-    RDL_CHECK_EX(rdl_launch_cluster(mx_some_rows_kernel, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, mx, mxs, w->codes_map, w->scales_map, a), "mx_some_rows");
+    RDL_CHECK_EX(rdl_launch_cluster(mx_some_rows_kernel, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, maps.values, maps.scales, w->codes_map, w->scales_map, a), "mx_some_rows");
     return 0;
 }

@@ -15,7 +15,7 @@
 #include "microscaling.cuh"
 
 // A 4-bit weight on the host's side: made once, when the weight is laid out.
-struct Mx4Matrix {
+struct alignas(64) Mx4Matrix {
     CUtensorMap codes_map;                       // [tile x block x row][128 codes], a box is a tile
     CUtensorMap scales_map;                      // [tile x block][128 words], a box is a tile's
     const uint8_t* codes; const uint8_t* scales;
@@ -118,6 +118,15 @@ inline int mx_make_map(CUtensorMap* map, const void* p, const MxMapShape& s, con
                               s.swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     RDL_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with driver error %d for %s", (int)r, what);
     return 0;
+}
+
+// The maps of 8-bit rows: values as [4][rows / 4][columns] in boxes of 4 x 32 rows, scales as [blocks][rows] words in boxes of 128.
+struct MxRowsMaps { CUtensorMap values, scales; };
+inline int mx_rows_maps(MxRowsMaps* maps, const void* x, const void* row_scales, long long blocks, long long rows4) {
+    const cuuint64_t cols = (cuuint64_t)blocks * MX_BLOCK, rows = (cuuint64_t)rows4;
+    if (int e = mx_make_map(&maps->values, x, {CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, {cols, rows / 4, 4}, {cols * 4, cols}, {MX_BLOCK, 32, 4}, CU_TENSOR_MAP_SWIZZLE_128B}, "8-bit rows")) return e;
+    return mx_make_map(&maps->scales, row_scales, {CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, {rows, (cuuint64_t)blocks}, {rows * 4}, {MX_ROWS, 1}, CU_TENSOR_MAP_SWIZZLE_NONE},
+                       "the scales of 8-bit rows");
 }
 
 }  // namespace

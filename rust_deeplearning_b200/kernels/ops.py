@@ -1815,10 +1815,8 @@ class Mx4Weight:
         self.tiles = -(-(-(-self.outputs // 16) * 32 if gated else rows) // MX_ROWS)
         self.shape = (rows, columns)
         blocks = _blocks(columns)
-        # what the packing does not write has to be zeros; without padding there is none of it
-        make = torch.empty if self.tiles * MX_ROWS == rows and columns == blocks * MX_BLOCK else torch.zeros
-        self.codes = make((self.tiles, blocks, MX_ROWS, MX_BLOCK // 2), dtype=torch.uint8, device=device)
-        self._scales = make((self.tiles * blocks * MX_ROWS * 4 + 16,), dtype=torch.uint8, device=device)    # 16 bytes more, which the packing clears last
+        self.codes = torch.empty((self.tiles, blocks, MX_ROWS, MX_BLOCK // 2), dtype=torch.uint8, device=device)
+        self._scales = self.codes.new_empty((self.tiles * blocks * MX_ROWS * 4 + 16,))       # 16 bytes more, which the packing clears last
         self.device = self.codes.device
         self._index = self.device.index
         lib = library.load()
@@ -1840,32 +1838,39 @@ class Mx8Rows:
     """Rows of activations in 8 bits with a scale a group: what `norm_mx8`, `pack_mx8` and `linear_gated_mx4` make and
     `linear_mx4` and `linear_gated_mx4` take in place of a tensor."""
 
-    __slots__ = ("rows", "columns", "shape", "device", "_values", "_scales")
+    __slots__ = ("rows", "columns", "shape", "device", "_data", "_layout")
 
-    def __init__(self, rows: int, columns: int, device):
+    def __init__(self, rows: int, columns: int, like: torch.Tensor):
+        """Place for so many rows, on the device of `like`."""
         self.rows, self.columns, self.shape = rows, columns, (rows, columns)
         padded, blocks = (rows + 3) // 4 * 4, (columns + MX_BLOCK - 1) // MX_BLOCK
-        # the padding rows hold whatever the memory held: nothing reads a result that comes of them
-        self._values = torch.empty((padded, blocks * MX_BLOCK), dtype=torch.float8_e4m3fn, device=device)
-        self._scales = torch.empty((blocks, padded, 4), dtype=torch.uint8, device=device)
-        self.device = self._values.device
+        # values [padded rows][padded columns], then scales [blocks][padded rows][4], a 32nd of that.  The padding rows hold whatever the
+        # memory held: nothing reads a result that comes of them.
+        self._layout = (padded, blocks)
+        self._data = like.new_empty((padded + (padded + 31) // 32, blocks * MX_BLOCK), dtype=torch.float8_e4m3fn)
+        self.device = like.device
+
+    @property
+    def _addresses(self):
+        """of the values and of the scales"""
+        p = self._data.data_ptr()
+        return p, p + self._layout[0] * self._layout[1] * MX_BLOCK
 
     @property
     def values(self) -> torch.Tensor:
         """float8_e4m3fn [rows, columns], before the scales (a view)"""
-        v = self._values
-        return v if v.shape == self.shape else v.as_strided(self.shape, (v.shape[1], 1))
+        return self._data.as_strided(self.shape, (self._layout[1] * MX_BLOCK, 1))
 
     @property
     def scales(self) -> torch.Tensor:
         """uint8 exponents + 127, [rows, blocks of 128 columns, 4 groups] (a view)"""
-        blocks, padded, _ = self._scales.shape
-        return self._scales.as_strided((self.rows, blocks, 4), (4, padded * 4, 1))
+        padded, blocks = self._layout
+        return self._data.view(torch.uint8).as_strided((self.rows, blocks, 4), (4, padded * 4, 1), padded * blocks * MX_BLOCK)
 
     def dequantise(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the rows stand for, [rows, columns] (for looking at them; the products take the rows as they are)."""
         scale = self.scales.contiguous().view(torch.float8_e8m0fnu).float()          # 255 is that type's NaN
-        wide = self._values[:self.rows].float().view(self.rows, -1, MX_GROUP)
+        wide = self._data[:self.rows].float().view(self.rows, -1, MX_GROUP)
         return (wide * scale.reshape(self.rows, -1, 1)).view(self.rows, -1)[:, :self.columns].to(dtype)
 
 
@@ -1925,9 +1930,9 @@ def mx8_rows(values: torch.Tensor, scales: torch.Tensor) -> Mx8Rows:
           and tuple(scales.shape) == (values.shape[0], -(-values.shape[1] // MX_GROUP)),
           "mx8_rows: float8_e4m3fn [rows, columns] and uint8 [rows, groups of 32 columns]")
     _need(values.is_cuda and values.device == scales.device, "mx8_rows: values and scales lie on one CUDA device")
-    r = Mx8Rows(values.shape[0], values.shape[1], values.device)
+    r = Mx8Rows(values.shape[0], values.shape[1], values)
     if r.columns % MX_BLOCK:
-        r._values.zero_()
+        r._data.view(torch.uint8).zero_()
     r.values.copy_(values)
     padded = torch.zeros((r.rows, _blocks(r.columns) * 4), dtype=torch.uint8, device=r.device)
     padded[:, :scales.shape[1]] = scales
@@ -1939,31 +1944,36 @@ def _norm_weight(p: Optional[NormParams], width: int, name: str):
     """address, dtype code, eps, offset"""
     if p is None:
         return None, 0, 0.0, 0.0
-    w = p.weight
-    if not (w.is_contiguous() and w.numel() == width and w.is_cuda):
-        _refuse(f"norm_mx8: the {name} norm's weight must hold {width} contiguous values on the device")
-    return w.data_ptr(), _dtype_code(w), p.eps, p.offset
+    w, eps, offset = p
+    code = _KINDS.get(w.dtype)
+    if code is None or not (w.is_contiguous() and w.numel() == width and w.is_cuda):
+        _refuse(f"norm_mx8: the {name} norm's weight must hold {width} contiguous float32 or bfloat16 values on the device")
+    return w.data_ptr(), code, eps, offset
+
+
+def _norm_sum(t: Optional[torch.Tensor], shape, name: str):
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or not t.is_contiguous() or t.shape != shape or not t.is_cuda:
+        _refuse(f"norm_mx8: {name} must be contiguous float32 [rows, width] on the device")
+    return t.data_ptr()
 
 
 def norm_mx8(x: torch.Tensor, *, first: Optional[NormParams] = None, residual: Optional[torch.Tensor] = None,
              second: Optional[NormParams] = None, residual_out: Optional[torch.Tensor] = None) -> Mx8Rows:
     """`norm_residual_norm` with its result in 8 bits: t = first ? rms_norm(x; first) : x;  h = residual + t (float32, written
     to `residual_out`, by default back to `residual`) or t;  returns second ? rms_norm(h; second) : h as 8-bit rows."""
-    if x.dim() != 2 or not x.is_contiguous() or x.shape[1] == 0:
-        _refuse("norm_mx8: x must be contiguous [rows, width]")
+    shape, kind = x.shape, _KINDS.get(x.dtype)
+    if kind is None or len(shape) != 2 or not x.is_contiguous() or shape[1] == 0:
+        _refuse("norm_mx8: x must be contiguous float32 or bfloat16 [rows, width]")
     if not x.is_cuda:
         _refuse("kernels run on CUDA tensors only; there is no CPU path")
-    rows, width = x.shape
-    if residual_out is None:
-        residual_out = residual
-    for t in (residual, residual_out):
-        if t is not None and not (t.dtype is torch.float32 and t.is_contiguous() and t.shape == x.shape and t.device == x.device):
-            _refuse("norm_mx8: residual and residual_out must be contiguous float32 [rows, width]")
-    y = Mx8Rows(rows, width, x.device)
-    library.check(library.load().rdl_norm_mx8(
-        x.data_ptr(), _dtype_code(x), *_norm_weight(first, width, "first"), residual.data_ptr() if residual is not None else None,
-        residual_out.data_ptr() if residual_out is not None else None, *_norm_weight(second, width, "second"),
-        y._values.data_ptr(), y._scales.data_ptr(), rows, width, _raw_stream(y.device.index)))
+    rows, width = shape
+    res = _norm_sum(residual, shape, "residual")
+    to = res if residual_out is None else _norm_sum(residual_out, shape, "residual_out")
+    y = Mx8Rows(rows, width, x)
+    library.check(library.load().rdl_norm_mx8(x.data_ptr(), kind, *_norm_weight(first, width, "first"), res, to, *_norm_weight(second, width, "second"),
+                                              *y._addresses, rows, width, _raw_stream(x.get_device())))
     return y
 
 
@@ -1988,25 +1998,29 @@ def _product_mx4(x, weight: Mx4Weight, gated: bool, out_dtype, out_mx8: bool, ac
     if type(weight) is not Mx4Weight or weight.gated is not gated or len(x.shape) != 2 or x.shape[1] != weight.columns or x.device != weight.device or not (
             packed or (x.dtype in _KINDS and x.is_contiguous())):
         _mx4_refuse(x, weight, gated, who)
-    rows, n, device = x.shape[0], weight.outputs, weight.device
+    rows, n = x.shape[0], weight.outputs
     status = status if status is not None else _step_status
     status = status.data_ptr() if status is not None else None
     lib, stream = library.load(), _raw_stream(weight._index)
     if packed:
-        data, scales, kind = x._values.data_ptr(), x._scales.data_ptr(), _MX8
+        (data, scales), kind = x._addresses, _MX8
     else:
         data, scales, kind = x.data_ptr(), None, _KINDS[x.dtype]
     if packed and rows > MX_FEW_ROWS:
         if out_mx8:
-            out = Mx8Rows(rows, n, device)
-            to, to_scales, out_kind = out._values.data_ptr(), out._scales.data_ptr(), _MX8
+            out = Mx8Rows(rows, n, weight.codes)
+            (to, to_scales), out_kind = out._addresses, _MX8
         else:
-            out = torch.empty((rows, n), dtype=out_dtype or torch.bfloat16, device=device)
+            out = weight.codes.new_empty((rows, n), dtype=out_dtype or torch.bfloat16)
             to, to_scales, out_kind = out.data_ptr(), None, _KINDS[out.dtype]
         library.check(lib.rdl_mx_many_rows(to, out_kind, to_scales, data, scales, weight.handle, rows, activation, param, softcap, status, stream))
         return out
-    out = torch.empty((rows, n), dtype=torch.float32 if out_mx8 else out_dtype or (torch.bfloat16 if packed else x.dtype), device=device)
-    to, out_kind, row, out_row = out.data_ptr(), _KINDS[out.dtype], weight.columns * x.element_size() if not packed else 0, n * out.element_size()
+    out = weight.codes.new_empty((rows, n), dtype=torch.float32 if out_mx8 else out_dtype or (torch.bfloat16 if packed else x.dtype))
+    to, out_kind = out.data_ptr(), _KINDS[out.dtype]
+    if 0 < rows <= MX_FEW_ROWS:
+        library.check(lib.rdl_mx_few_rows(to, out_kind, data, kind, scales, weight.handle, rows, activation, param, softcap, status, stream))
+        return norm_mx8(out) if out_mx8 else out
+    out_row, row = n * out.element_size(), weight.columns * x.element_size() if not packed else 0
     for r in range(0, rows, MX_FEW_ROWS):
         library.check(lib.rdl_mx_few_rows(to + r * out_row, out_kind, data + r * row, kind, scales, weight.handle, min(rows - r, MX_FEW_ROWS),
                                           activation, param, softcap, status, stream))

@@ -242,7 +242,7 @@ def test_gated(m, n, k, kind, act):
     scale = np.repeat(2.0 ** (rows.scales.reshape(m, -1).cpu().numpy().astype(np.float64) - 127), 32, axis=1)[:, :n]
     check(rows.dequantise(), want, tol + fast + np.abs(want) * 2.0 ** -4 * (1 + 2.0 ** -6) + scale * 2.0 ** -10, act + " in 8 bits")
     # the padding of the 8-bit result is zeros: the product behind it reads it
-    assert not rows._values.view(torch.uint8)[:m, n:].any() and not rows.scales.reshape(m, -1)[:, -(-n // 32):].any()
+    assert not rows._data.view(torch.uint8)[:m, n:].any() and not rows.scales.reshape(m, -1)[:, -(-n // 32):].any()
 
 
 @pytest.mark.parametrize("m,kind", [(3, "bfloat16"), (12, "float32"), (16, "mx8"), (50, "mx8")])
@@ -298,7 +298,7 @@ def test_a_row_does_not_depend_on_the_others():
     r, _ = rows_for(200, 1000, "mx8", 18)
     first = ops.linear_mx4(r, w)
     assert torch.equal(first, ops.linear_mx4(r, w))                      # the same bits every time
-    r._values.view(torch.uint8)[40:] = 0x7f                              # NaN
+    r._data.view(torch.uint8)[40:200] = 0x7f                            # NaN
     assert torch.equal(ops.linear_mx4(r, w)[:40], first[:40])
 
 
