@@ -46,6 +46,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=0, help="Seed of the sampler.")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16",
                    help="bfloat16: the serving kernels; float32: everything in true 32-bit.")
+    p.add_argument("--weights", choices=["as-stored", "mx4", "mx4+head"], default="as-stored",
+                   help="mx4: the projections in 4 bits with a scale a group of 32 (mx4+head: the output head too).")
     p.add_argument("--stop-ids", default=None, help="Stop token ids (default: the model's end-of-sequence ids).")
     p.add_argument("--max-context", type=int, default=None, help="Longest sequence the cache is sized for.")
     p.add_argument("--timings", action="store_true", help="Print the device time of every step (CUDA events) to stderr.")
@@ -91,6 +93,7 @@ def main(argv: Optional[List[str]] = None, stdin=None, stdout=None) -> int:
     from .weights.loader import WeightError
     from .weights.safetensors_io import SafetensorsError
 
+    weight_format = None if args.weights == "as-stored" else args.weights
     try:
         if args.random_config is not None:
             weights_seed = args.seed if args.weights_seed is None else args.weights_seed
@@ -101,11 +104,11 @@ def main(argv: Optional[List[str]] = None, stdin=None, stdout=None) -> int:
             except (OSError, ValueError) as e:
                 print(f"error: cannot read {args.random_config}: {e}", file=sys.stderr)
                 return 1
-            model = random_model(raw, weights_seed, args.dtype)
+            model = random_model(raw, weights_seed, args.dtype, weight_format=weight_format)
         else:
             print(f"Loading {args.model_dir} ({args.dtype})...", file=sys.stderr)
-            model = load_model(args.model_dir, args.dtype)
-    except (ConfigError, WeightError, SafetensorsError, RuntimeError) as e:
+            model = load_model(args.model_dir, args.dtype, weight_format=weight_format)
+    except (ConfigError, WeightError, SafetensorsError, RuntimeError, ValueError) as e:
         print(f"error: {e}", file=sys.stderr)
         return 1
     spec = model.spec

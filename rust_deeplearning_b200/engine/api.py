@@ -27,28 +27,30 @@ def _require_cuda(device):
     return dev
 
 
-def load_model(folder: str, dtype: Union[str, torch.dtype] = "bfloat16", device="cuda:0", strict: bool = True) -> Model:
+def load_model(folder: str, dtype: Union[str, torch.dtype] = "bfloat16", device="cuda:0", strict: bool = True,
+               weight_format: Optional[str] = None) -> Model:
     """A model folder (config.json + model.safetensors) -> a model on the device.  The model class
     is chosen by config.json.  dtype "bfloat16": the serving kernels; "float32": everything in
     true 32-bit.  strict False: tensors the model does not read are skipped with a warning instead
-    of being an error."""
+    of being an error.  weight_format: "mx4" rounds the projections to 4 bits with a scale a group of 32 as they are loaded, "mx4+head"
+    the output head too (None: as they are; see `Model`)."""
     dev = _require_cuda(device)
     dtype = parse_dtype(dtype)
     raw = read_config_json(folder)
     arch = architecture_for(raw)
     spec = arch.build_spec(arch.parse_config(raw))
     weights = load_weights(spec, folder, dtype, dev, strict)
-    return Model(spec, weights, dtype, dev)
+    return Model(spec, weights, dtype, dev, weight_format)
 
 
 def random_model(config: Dict[str, Any], seed: int = 0, dtype: Union[str, torch.dtype] = "bfloat16",
-                 device="cuda:0") -> Model:
+                 device="cuda:0", weight_format: Optional[str] = None) -> Model:
     """A model with N(0, 0.02) weights made on the device from (config, seed), without files."""
     dev = _require_cuda(device)
     dtype = parse_dtype(dtype)
     arch = architecture_for(config)
     spec = arch.build_spec(arch.parse_config(config))
-    return Model(spec, random_weights(spec, seed, dtype, dev), dtype, dev)
+    return Model(spec, random_weights(spec, seed, dtype, dev), dtype, dev, weight_format)
 
 
 class Generator:

@@ -501,7 +501,7 @@ def deferred_ok(rows: int, width: int, dtype: torch.dtype) -> bool:
 
 def linear_branch(x: torch.Tensor, weight: torch.Tensor, sink: Optional[BranchSink], status: Optional[torch.Tensor] = None):
     """x W^T as a branch of a residual stream: a `Branch` where the split form applies, else the plain result."""
-    if sink is None or not (_skinny_ok(x, weight) and deferred_ok(x.shape[0], weight.shape[0], x.dtype)
+    if type(weight) is Mx4Weight or sink is None or not (_skinny_ok(x, weight) and deferred_ok(x.shape[0], weight.shape[0], x.dtype)
                             and tuple(sink.residual.shape) == (x.shape[0], weight.shape[0])):
         return linear(x, weight, status=status)
     rows, width = x.shape[0], weight.shape[0]
@@ -560,7 +560,12 @@ def linear(x, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
     bfloat16: up to 16 rows (decode) the weight-streaming tensor-core kernels, from 128 rows the TMA +
     tcgen05 kernels, all with float accumulation and the soft-cap in their epilogue.  17 to 127 rows, and
     operands that do not meet the alignment rules, go to a library product (cuBLAS through torch), which
-    is what the reference's engine uses for all its products."""
+    is what the reference's engine uses for all its products.
+
+    A 4-bit weight (`Mx4Weight`): `linear_mx4`.  Up to 16 rows of a tensor enter as they are, more bfloat16 rows are rounded to 8 bits
+    first (`pack_mx8`); x may be rows that are in 8 bits already."""
+    if type(weight) is Mx4Weight:
+        return linear_mx4(_rows_for_mx4(x), weight, out_dtype, softcap, status, activation)
     _need(activation is None or (activation in UNARY_FORMS and softcap is None),
           f"linear: activation '{activation}' is not one of {sorted(UNARY_FORMS)} (and comes without a soft-cap)")
     if isinstance(x, DeferredRows):
@@ -596,7 +601,10 @@ def linear_gated(x, weight_gate_up: torch.Tensor, activation: str, status: Optio
     """act(x Wg^T) * (x Wu^T) for the row-concatenated matrix [Wg; Wu] ([2I, in]) -> [rows, I]; or another form of
     `GATED_FORMS` (param: its parameter).
     In bfloat16 this is one kernel (the activation is the product's epilogue); otherwise a product
-    and the gated activation kernel."""
+    and the gated activation kernel.  A 4-bit weight: as in `linear`; rows in 8 bits give a result in 8 bits, for the product behind."""
+    if type(weight_gate_up) is Mx4Weight:
+        x = _rows_for_mx4(x)
+        return linear_gated_mx4(x, weight_gate_up, activation, param, type(x) is Mx8Rows, status)
     _need(activation in GATED_FORMS, f"unknown activation '{activation}', known: {sorted(GATED_FORMS)}")
     _need(weight_gate_up.shape[0] % 2 == 0, "linear_gated: the weight must hold gate rows and as many up rows")
     if isinstance(x, DeferredRows):
@@ -1791,6 +1799,7 @@ MX_GROUP, MX_BLOCK, MX_ROWS = 32, 128, 128
 MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs, which also takes tensors; above, 8-bit rows only
 _MX8 = 2                 # rows of 8 bits, where a kernel's argument says of what kind its rows are
 _KINDS = {torch.float32: 0, torch.bfloat16: 1}
+MX8 = "mx8"              # in place of a dtype: rows wanted as `Mx8Rows`
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -1819,10 +1828,23 @@ class Mx4Weight:
         self._scales = self.codes.new_empty((self.tiles * blocks * MX_ROWS * 4 + 16,))       # 16 bytes more, which the packing clears last
         self.device = self.codes.device
         self._index = self.device.index
+        self._describe()
+
+    def _describe(self):
         lib = library.load()
         self._host = ctypes.create_string_buffer(lib.rdl_mx4_matrix_bytes() + 64)
         self.handle = -(-ctypes.addressof(self._host) // 64) * 64
-        library.check(lib.rdl_mx4_describe(self.handle, self.codes.data_ptr(), self._scales.data_ptr(), rows, columns, int(self.gated)), 0)
+        library.check(lib.rdl_mx4_describe(self.handle, self.codes.data_ptr(), self._scales.data_ptr(), self.rows, self.columns, int(self.gated)), 0)
+
+    def first(self, rows: int) -> "Mx4Weight":
+        """The weight's first rows as a weight of their own, on the same memory."""
+        _need(not self.gated and 0 < rows <= self.rows, f"first: {rows} rows of a {'gated ' if self.gated else ''}weight of {self.rows}")
+        w = Mx4Weight.__new__(Mx4Weight)
+        w.rows, w.columns, w.gated, w.outputs, w.shape = rows, self.columns, False, rows, (rows, self.columns)
+        w.tiles = -(-rows // MX_ROWS)
+        w.codes, w._scales, w.device, w._index = self.codes[:w.tiles], self._scales[:w.tiles * _blocks(self.columns) * MX_ROWS * 4 + 16], self.device, self._index
+        w._describe()
+        return w
 
     @property
     def scales(self) -> torch.Tensor:
@@ -1839,6 +1861,7 @@ class Mx8Rows:
     `linear_mx4` and `linear_gated_mx4` take in place of a tensor."""
 
     __slots__ = ("rows", "columns", "shape", "device", "_data", "_layout")
+    dtype = torch.bfloat16       # of what a product makes of them
 
     def __init__(self, rows: int, columns: int, like: torch.Tensor):
         """Place for so many rows, on the device of `like`."""
@@ -2025,6 +2048,15 @@ def _product_mx4(x, weight: Mx4Weight, gated: bool, out_dtype, out_mx8: bool, ac
         library.check(lib.rdl_mx_few_rows(to + r * out_row, out_kind, data + r * row, kind, scales, weight.handle, min(rows - r, MX_FEW_ROWS),
                                           activation, param, softcap, status, stream))
     return norm_mx8(out) if out_mx8 else out
+
+
+def _rows_for_mx4(x):
+    """What `linear` hands a 4-bit weight: many bfloat16 rows in 8 bits, everything else as it is."""
+    if isinstance(x, DeferredRows):
+        x = x.materialise()
+    if type(x) is not Mx8Rows and x.dtype is torch.bfloat16 and x.shape[0] > MX_FEW_ROWS:
+        x = pack_mx8(x)
+    return x
 
 
 def linear_mx4(x, weight: Mx4Weight, out_dtype: Optional[torch.dtype] = None, softcap: Optional[float] = None,

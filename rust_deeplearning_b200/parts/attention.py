@@ -41,7 +41,8 @@ different sizes share the attention kernels by zero padding: the heads of q, k, 
 with max(head_dim, value_dim) values, the padding made by zero rows of the product's matrix (and zero columns of
 W_o), so that scores and outputs are unchanged and no kernel needs to know.
 Optional offers for the split form of the norms around few-row products (`parts/norm.py`):
-`takes_deferred_rows` (x may be `ops.DeferredRows`) and `delivers_branch` (forward takes `sink`).
+`takes_deferred_rows` (x may be `ops.DeferredRows`) and `delivers_branch` (forward takes `sink`).  `use_mx4()`: the projections go to
+4 bits (`ops.Mx4Weight`); the mixer then says `takes_mx8_rows` (x may be `ops.Mx8Rows`) and gives up the split form.
 """
 from __future__ import annotations
 
@@ -291,6 +292,15 @@ class Attention:
         if pos is not None and hasattr(pos, "tables") and hasattr(pos, "rotary_dim"):
             return pos.tables(), pos.rotary_dim
         return None, 0
+
+    def use_mx4(self) -> int:
+        """The projections in 4 bits from now on (`ops.Mx4Weight`); how many matrices."""
+        self.w_qkv, self.w_o = ops.pack_mx4(self.w_qkv), ops.pack_mx4(self.w_o)
+        if not self.extended:
+            self.w_q = self.w_qkv.first(self.q_width)
+        self.takes_deferred_rows = self.delivers_branch = False
+        self.takes_mx8_rows = not self.extended
+        return 2
 
     takes_deferred_rows = True     # x goes into the q/k/v (or q) product and nowhere else
     delivers_branch = True         # the output projection may deliver the result through a stream's sink

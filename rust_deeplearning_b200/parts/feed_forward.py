@@ -9,7 +9,8 @@ Interface of a feed-forward: `forward(x [rows, hidden] normed) -> [rows, hidden]
 independent of each other, so packing and batching never concern it.  Two optional offers, for the split
 form of the norms around few-row products (`parts/norm.py`): `takes_deferred_rows` (x may be
 `ops.DeferredRows`; it goes into `ops.linear` / `ops.linear_gated` only) and `delivers_branch` (forward takes
-`sink` and ends in `ops.linear_branch`).
+`sink` and ends in `ops.linear_branch`).  `use_mx4()`: the part's matrices go to 4 bits (`ops.Mx4Weight`); it then says
+`takes_mx8_rows` (x may be `ops.Mx8Rows`) and gives up the split form.
 """
 from __future__ import annotations
 
@@ -31,6 +32,13 @@ class GatedMLP:
 
     takes_deferred_rows = True     # x goes into one product and nowhere else
     delivers_branch = True         # the last product may deliver the result through a stream's sink
+
+    def use_mx4(self) -> int:
+        """The matrices in 4 bits from now on; how many."""
+        self.w_gate_up, self.w_down = ops.pack_mx4(self.w_gate_up, gated=True), ops.pack_mx4(self.w_down)
+        self.takes_deferred_rows = self.delivers_branch = False
+        self.takes_mx8_rows = True
+        return 2
 
     def forward(self, x, sink=None):
         return ops.linear_branch(ops.linear_gated(x, self.w_gate_up, self.activation, **self.form), self.w_down, sink)
@@ -54,6 +62,12 @@ class PlainMLP:
 
     takes_deferred_rows = True
     delivers_branch = True
+
+    def use_mx4(self) -> int:
+        self.w_up, self.w_down = ops.pack_mx4(self.w_up), ops.pack_mx4(self.w_down)
+        self.takes_deferred_rows = self.delivers_branch = False
+        self.takes_mx8_rows = True
+        return 2
 
     def forward(self, x, sink=None):
         return ops.linear_branch(ops.linear(x, self.w_up, activation=self.activation), self.w_down, sink)

@@ -64,6 +64,11 @@ class LinearHead:
 
     takes_deferred_rows = True      # n goes into one product and nowhere else
 
+    def use_mx4(self) -> int:
+        self.weight = ops.pack_mx4(self.weight)
+        self.takes_deferred_rows = False
+        return 1
+
     def forward(self, n) -> torch.Tensor:
         z = ops.linear(n, self.weight, out_dtype=torch.float32, softcap=self.softcap)
         return ops.scale_(z, self.scale) if self.scale != 1.0 else z
@@ -93,11 +98,25 @@ class SandwichBlock:
         split form (`ops.DeferredRows`); the model tells the block before, so that its last product can prepare them."""
         return self.pre_mixer if getattr(self.mixer, "takes_deferred_rows", False) else None
 
+    def _in_8_bits(self, stream) -> bool:
+        """Whether a part's products want this step's rows in 8 bits: more of them than the few-row kernel takes, 4-bit weights."""
+        return (self.act_dtype is torch.bfloat16 and stream.x.shape[0] > ops.MX_FEW_ROWS
+                and any(getattr(p, "takes_mx8_rows", False) for p in (self.mixer, self.feed_forward)))
+
+    def _input(self, stream, norm, part):
+        return stream.normed_mx8(norm) if getattr(part, "takes_mx8_rows", False) else stream.normed(norm, self.act_dtype)
+
     def forward(self, stream: ResidualStream, batch, cache, run: int):
         # Parts say what they can do with the split form of the norms (few rows; see ResidualStream):
         # takes_deferred_rows - x goes into ops.linear / ops.linear_gated only; delivers_branch - forward takes
         # `sink` and ends in ops.linear_branch.  Everything else runs through the norm kernels.
         mixer, ff = self.mixer, self.feed_forward
+        if self._in_8_bits(stream):
+            stream.norm_after_block = None
+            stream.add(mixer.forward(self._input(stream, self.pre_mixer, mixer), batch, cache, run), self.post_mixer)
+            if ff is not None:
+                stream.add(ff.forward(self._input(stream, self.pre_ff, ff)), self.post_ff)
+            return
         m_in, m_out = getattr(mixer, "takes_deferred_rows", False), getattr(mixer, "delivers_branch", False)
         f_in, f_out = getattr(ff, "takes_deferred_rows", False), getattr(ff, "delivers_branch", False)
         after, stream.norm_after_block = stream.norm_after_block, None
@@ -252,11 +271,21 @@ def _build_parallel(layer: LayerSpec, ctx: BuildContext) -> ParallelBlock:
 register_part("block", "parallel", _build_parallel, replace=True)
 
 
-class Model:
-    """A model built from a ModelSpec and loaded tensors.  Nothing here names an architecture."""
+WEIGHT_FORMATS = ("mx4", "mx4+head")
 
-    def __init__(self, spec: ModelSpec, weights: Dict[str, torch.Tensor], dtype: torch.dtype, device):
+
+class Model:
+    """A model built from a ModelSpec and loaded tensors.  Nothing here names an architecture.
+
+    weight_format: "mx4" keeps the matrices of every part that offers it (`use_mx4() -> how many`) in 4 bits with a scale a group of
+    32; "mx4+head" the output head's too.  Steps of up to 16 rows multiply them with the activations as they are, larger ones with
+    activations rounded to 8 bits.  Parts without the offer keep theirs as they were loaded."""
+
+    def __init__(self, spec: ModelSpec, weights: Dict[str, torch.Tensor], dtype: torch.dtype, device, weight_format: Optional[str] = None):
         spec.validate()
+        if weight_format not in (None, *WEIGHT_FORMATS):
+            raise ValueError(f"unknown weight format '{weight_format}', known: {list(WEIGHT_FORMATS)}")
+        self.weight_format, packed = weight_format, 0
         self.spec, self.dtype, self.device = spec, dtype, torch.device(device)
         ctx = BuildContext(weights, dtype, self.device)
         self.embedding = build_part("embedding", spec.embedding, ctx)
@@ -264,6 +293,8 @@ class Model:
         self.layers = []
         for layer in spec.layers:
             self.layers.append(build_block(layer, ctx))
+            if weight_format is not None:
+                packed += sum(p.use_mx4() for p in (getattr(self.layers[-1], n, None) for n in ("mixer", "feed_forward")) if hasattr(p, "use_mx4"))
             # parts hold what they need (fused copies or the tensors themselves)
             for p in (q for top in (layer.mixer, layer.feed_forward, *layer.norms.values()) if top is not None for q in top.walk()):
                 for t in p.tensors.values():
@@ -275,6 +306,10 @@ class Model:
         self.final_norm = build_part("norm", spec.final_norm, ctx)
         self.start_stream = build_part("stream", spec.stream, ctx)     # the embedded rows -> the stream the blocks work on
         self.head = build_part("head", spec.head, ctx)
+        if weight_format == "mx4+head":
+            packed += self.head.use_mx4() if hasattr(self.head, "use_mx4") else 0
+        if weight_format is not None and packed == 0:
+            raise ValueError(f"{spec.architecture}: none of its parts keeps its matrices in 4 bits")
         self.schedule = list(spec.schedule)
         # what joins the stream before a run: (whether the embedded rows do, a float32 vector or None)
         self.entries = {e: (s.enters.embedding, None if s.enters.vectors is None else

@@ -23,8 +23,10 @@ For blocks that norm AFTER the sum the stream offers `rows(dtype)` (the stream i
 `renorm(branch, norm, alpha, dtype)`: x <- norm(alpha x + branch) in float32, in place, in one kernel that also
 leaves x in the activations' dtype for the next part.
 
+For products with 4-bit weights the stream offers `normed_mx8(norm)`: the same rows in 8 bits (`ops.Mx8Rows`).
+
 Interface of a norm: `apply(x [rows, hidden], out_dtype) -> [rows, hidden]`;
-optionally `fused_params() -> ops.NormParams`.
+optionally `fused_params() -> ops.NormParams` and `apply_mx8(x) -> ops.Mx8Rows`.
 """
 from __future__ import annotations
 
@@ -51,6 +53,10 @@ class RMSNorm:
 
     def apply(self, x: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
         return ops.norm_residual_norm(x, second=self.params, out_dtype=out_dtype)
+
+    def apply_mx8(self, x: torch.Tensor):
+        """The same as 8-bit rows for products with 4-bit weights."""
+        return ops.norm_mx8(x, second=self.params)
 
 
 def _build_rms_norm(spec: PartSpec, ctx: BuildContext) -> RMSNorm:
@@ -229,6 +235,21 @@ class ResidualStream:
         self._flush()
         self._prepare(upcoming, out_dtype)
         return norm.apply(self.x, out_dtype)
+
+    def normed_mx8(self, norm):
+        """norm(x) after any waiting branch has been added, as 8-bit rows for products with 4-bit weights: "norm the branch, add it,
+        norm the sum, round to 8 bits" in one kernel where both norms are fusable and nothing else waits."""
+        self._settled()
+        self._operand = None
+        if self._pending is not None and self._entering is None and not isinstance(self._pending[0], ops.Branch) and _fusable(norm):
+            branch, post = self._pending
+            if post is None or _fusable(post):
+                self._pending = None
+                return ops.norm_mx8(branch, first=post.fused_params() if post else None, residual=self.x, second=norm.fused_params())
+        self._flush()
+        if callable(getattr(norm, "apply_mx8", None)):
+            return norm.apply_mx8(self.x)
+        return ops.pack_mx8(norm.apply(self.x, torch.bfloat16))
 
     def normed_rows(self, norm, rows: torch.Tensor, out_dtype: torch.dtype, deferred_ok: bool = False):
         """norm(x[rows]) for an int32 list of rows."""
