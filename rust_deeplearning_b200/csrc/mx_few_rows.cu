@@ -25,8 +25,7 @@
 
 namespace {
 
-// A stage of the ring is two blocks of columns: what a stage costs the issuing warp beside its products (a wait, a commit) is about as long
-// as the products of one.
+// A stage of the ring is STEP blocks of columns: a stage costs the issuing thread a wait beside its products, about as long as those of a block.
 constexpr int WORKERS = 512, THREADS = 64 + WORKERS, MAX_STAGES = 8, STEP = 2, SCALE_BUFS = 4, MAX_PASS = 64;
 
 struct FewArgs {
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     static_assert(NB % 16 == 0 && 2 * NB + SCALE_BUFS * 8 <= TMEM_COLS, "the sums of two tiles and the scales share tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], x_ready[MAX_PASS], x_free;
+    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], x_ready[MAX_PASS / STEP], x_free;
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     // rows with an infinity or a NaN here; rows with a group too small for its last parts; rows with one that is not
@@ -201,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         if (t < MAX_STAGES) { mx_bar_init(mx_smem(&full_bar[t]), 1); mx_bar_init(mx_smem(&empty_bar[t]), 1); }
         else if (t < MAX_STAGES + 2) { mx_bar_init(mx_smem(&acc_full[t - MAX_STAGES]), 1); mx_bar_init(mx_smem(&acc_empty[t - MAX_STAGES]), 8); }
         else if (t == MAX_STAGES + 2) { mx_bar_init(mx_smem(&x_free), 1); gave_up = 0; bad_rows = tiny_rows = fine_rows = 0; }
-        else if (t >= 64 && t < 64 + MAX_PASS) mx_bar_init(mx_smem(&x_ready[t - 64]), 1);
+        else if (t >= 64 && t < 64 + MAX_PASS / STEP) mx_bar_init(mx_smem(&x_ready[t - 64]), STEP);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -218,45 +217,47 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
 
     if (warp == 0) {
         // ---- weights ----
-        unsigned long long policy;                           // read once a step: first to leave L2
-        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-        int s = 0, piece = first_tile * a.blocks + b0;       // place in the ring; block of columns over all tiles
-        uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
-        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, piece += (tile_step - 1) * a.blocks + (a.blocks - (b1 - b0))) {
-            for (int kb = b0; kb < b1;) {
-                // a stage is up to STEP blocks; none reaches into the next pass over the rows
-                const int n = min(STEP, min(b0 + ((kb - b0) / a.pass_blocks + 1) * a.pass_blocks, b1) - kb);
-                if (!mx_warp_wait(mx_smem(&empty_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
-                if (mx_elect()) {
+        if (mx_elect()) {
+            unsigned long long policy;                       // read once a step: first to leave L2
+            asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+            int s = 0, piece = first_tile * a.blocks + b0;   // place in the ring; block of columns over all tiles
+            uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
+            for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, piece += (tile_step - 1) * a.blocks + (a.blocks - (b1 - b0))) {
+                for (int kb = b0, pass_end = min(b0 + a.pass_blocks, b1); kb < b1;) {
+                    // a stage is up to STEP blocks; none reaches into the next pass over the rows
+                    const int n = min(STEP, pass_end - kb);
+                    if (!mx_bar_wait(mx_smem(&empty_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
                     const uint32_t full = mx_smem(&full_bar[s]), at = ring_s + (uint32_t)(s * STEP * MX_TILE_BYTES);
                     mx_bar_expect(full, (uint32_t)n * (MX_TILE_TX + MX_SCALE_BYTES) + extra);
-                    tma_codes(at, &map_w, piece * MX_ROWS, full, policy);
-                    if (n > 1) tma_codes(at + MX_TILE_BYTES, &map_w, (piece + 1) * MX_ROWS, full, policy);
+#pragma unroll
+                    for (int j = 0; j < STEP; ++j)
+                        if (j < n) tma_codes(at + (uint32_t)(j * MX_TILE_BYTES), &map_w, (piece + j) * MX_ROWS, full, policy);
                     bulk_scales(ws_s + (uint32_t)(s * STEP * MX_SCALE_BYTES), a.scales + (long long)piece * MX_SCALE_BYTES, (uint32_t)n * MX_SCALE_BYTES, full, policy);
+                    extra = 0;
+                    kb += n;
+                    piece += n;
+                    if (kb == pass_end) pass_end = min(pass_end + a.pass_blocks, b1);
+                    if (++s == a.stages) { s = 0; parity ^= 1; }
                 }
-                __syncwarp();
-                extra = 0;
-                kb += n;
-                piece += n;
-                if (++s == a.stages) { s = 0; parity ^= 1; }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         // ---- scales to tensor memory, and the products ----
-        int s = 0, lt = 0, n_pass = 0, scale_buf = 0;
-        uint32_t parity = 0;
-        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++lt) {
-            const int buf = lt & 1;
-            if (!mx_warp_wait(mx_smem(&acc_empty[buf]), ((lt >> 1) & 1) ^ 1, a.wait_cycles, gave_up_v)) { ok = false; break; }
-            for (int p = 0; p < passes && ok; ++p) {
-                const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
-                const bool fresh = passes > 1 || lt == 0;            // the rows are being made ready, block by block
-                for (int kb = p0; kb < p1;) {
-                    const int n = min(STEP, p1 - kb);
-                    for (int j = 0; j < n && fresh && ok; ++j) ok = mx_warp_wait(mx_smem(&x_ready[kb - p0 + j]), n_pass & 1, a.wait_cycles, gave_up_v);
-                    if (!ok || !mx_warp_wait(mx_smem(&full_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
-                    mx_fence_after();
-                    if (mx_elect()) {
+        if (mx_elect()) {
+            int s = 0, lt = 0, n_pass = 0, scale_buf = 0;
+            uint32_t parity = 0;
+            for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++lt) {
+                const int buf = lt & 1;
+                if (!mx_bar_wait(mx_smem(&acc_empty[buf]), ((lt >> 1) & 1) ^ 1, a.wait_cycles, gave_up_v)) { ok = false; break; }
+                for (int p = 0; p < passes && ok; ++p, ++n_pass) {
+                    const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
+                    const bool fresh = passes > 1 || lt == 0;            // the rows are being made ready, STEP blocks at a time
+                    for (int kb = p0; kb < p1;) {
+                        const int n = min(STEP, p1 - kb);
+                        const uint32_t full = mx_smem(&full_bar[s]);
+                        if (!mx_bar_wait_both(full, parity, fresh ? mx_smem(&x_ready[(kb - p0) / STEP]) : full, fresh ? (uint32_t)(n_pass & 1) : parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
+                        mx_fence_after();
 #pragma unroll
                         for (int j = 0; j < STEP; ++j) {
                             if (j >= n) break;
@@ -269,19 +270,16 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                                 mma_mx(tmem + buf * NB, ad + (uint32_t)(k * 2), bd + (uint32_t)(k * 2), mx_idesc(MX_E2M1, MX_E4M3, MX_ROWS, NB, k), sa, sb, kb + j != b0 || k != 0);
                         }
                         commit(mx_smem(&empty_bar[s]));
+                        kb += n;
+                        scale_buf = (scale_buf + n) & (SCALE_BUFS - 1);
+                        if (++s == a.stages) { s = 0; parity ^= 1; }
                     }
-                    __syncwarp();
-                    kb += n;
-                    scale_buf = (scale_buf + n) & (SCALE_BUFS - 1);
-                    if (++s == a.stages) { s = 0; parity ^= 1; }
+                    if (ok && passes > 1) commit(mx_smem(&x_free));
                 }
-                ++n_pass;
-                if (ok && passes > 1 && mx_elect()) commit(mx_smem(&x_free));
-                __syncwarp();
+                if (ok) commit(mx_smem(&acc_full[buf]));
             }
-            if (ok && mx_elect()) commit(mx_smem(&acc_full[buf]));
-            __syncwarp();
         }
+        __syncwarp();
     } else {
         // ---- rows to parts; then the sums ----
         rdl_grid_wait();
@@ -296,9 +294,9 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             for (int p = 0; p < passes && (passes > 1 || lt == 0); ++p, ++n_pass) {
                 if (n_pass > 0 && !mx_bar_wait(mx_smem(&x_free), (n_pass - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
                 const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
-                // A warp takes every sixteenth block of columns, and hands each over on its own: the products begin with the first.
+                // A warp takes every sixteenth block of columns, and hands it over: the products begin with the first STEP of them.
                 // Every block's barrier takes part in every pass, so that its phase is the number of the pass.
-                for (int pb = warp - 2; pb < a.pass_blocks; pb += WORKERS / 32) {
+                for (int pb = warp - 2; pb < (a.pass_blocks + STEP - 1) / STEP * STEP; pb += WORKERS / 32) {
                     const int block = p0 + pb, chunks = block < p1 ? a.M * (MX_BLOCK / 8) : 0;
                     const uint32_t at = my_place + (uint32_t)(pb * X_BLOCK), sc_at = my_scale + (uint32_t)(pb * MX_SCALE_BYTES);
                     uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
@@ -347,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the products read what was stored here
                     __syncwarp();
-                    if (lane == 0) mx_bar_arrive(mx_smem(&x_ready[pb]));
+                    if (lane == 0) mx_bar_arrive(mx_smem(&x_ready[pb / STEP]));
                 }
             }
             const int buf = lt & 1;

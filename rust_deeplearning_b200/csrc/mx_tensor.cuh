@@ -56,7 +56,7 @@ __device__ __forceinline__ bool mx_bar_wait(uint32_t bar, uint32_t parity, long 
 }
 // One thread of a warp that has come here as a whole.  What tcgen05 and TMA instructions take has to be uniform over the warp: behind this
 // choice the compiler knows that one thread issues them; behind `lane == 0` it does not and goes through the lanes, which cost 90
-// clock cycles an instruction (a block of 128 columns, four products and two copies of scales: 538 cycles, and 182 so).
+// clock cycles an instruction (a block of 128 columns, four products and two copies of scales: 538 cycles, and 185 so).
 __device__ __forceinline__ bool mx_elect() {
     uint32_t one;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
@@ -65,6 +65,14 @@ __device__ __forceinline__ bool mx_elect() {
 // the wait of a whole warp; the same answer in all of its lanes
 __device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, long long limit, volatile int* gave_up) {
     return __all_sync(0xffffffffu, mx_bar_wait(bar, parity, limit, gave_up));
+}
+// Two barriers at once: a wait takes 110 to 190 cycles to answer even if it is long over, as long as the products of a block, and these
+// two answer together.
+__device__ __forceinline__ bool mx_bar_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, long long limit, volatile int* gave_up) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p, q;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nmbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n"
+                 "and.pred p, p, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1) : "memory");
+    return ok != 0 || (mx_bar_wait(bar0, parity0, limit, gave_up) && mx_bar_wait(bar1, parity1, limit, gave_up));
 }
 // copies that are on their way when a block gives up still write to its shared memory: they get the time to arrive
 __device__ __forceinline__ void mx_drain() {
