@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         if (t < MAX_STAGES) { mx_bar_init(mx_smem(&full_bar[t]), 1); mx_bar_init(mx_smem(&empty_bar[t]), 1); }
         else if (t < MAX_STAGES + 2) { mx_bar_init(mx_smem(&acc_full[t - MAX_STAGES]), 1); mx_bar_init(mx_smem(&acc_empty[t - MAX_STAGES]), 8); }
         else if (t == MAX_STAGES + 2) { mx_bar_init(mx_smem(&x_free), 1); gave_up = 0; bad_rows = tiny_rows = fine_rows = 0; }
-        else if (t >= 64 && t < 64 + MAX_PASS / STEP) mx_bar_init(mx_smem(&x_ready[t - 64]), STEP);
+        else if (t >= 64 && t < 64 + MAX_PASS / STEP) mx_bar_init(mx_smem(&x_ready[t - 64]), STEP * (R / 8));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -294,14 +294,15 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             for (int p = 0; p < passes && (passes > 1 || lt == 0); ++p, ++n_pass) {
                 if (n_pass > 0 && !mx_bar_wait(mx_smem(&x_free), (n_pass - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
                 const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
-                // A warp takes every sixteenth block of columns, and hands it over: the products begin with the first STEP of them.
-                // Every block's barrier takes part in every pass, so that its phase is the number of the pass.
-                for (int pb = warp - 2; pb < (a.pass_blocks + STEP - 1) / STEP * STEP; pb += WORKERS / 32) {
-                    const int block = p0 + pb, chunks = block < p1 ? a.M * (MX_BLOCK / 8) : 0;
-                    const uint32_t at = my_place + (uint32_t)(pb * X_BLOCK), sc_at = my_scale + (uint32_t)(pb * MX_SCALE_BYTES);
+                // A warp takes every sixteenth piece, eight rows of a block of columns, and hands it over: the products begin with the first
+                // STEP blocks.  Every block's barrier takes part in every pass, so that its phase is the number of the pass.
+                for (int piece = warp - 2; piece < (a.pass_blocks + STEP - 1) / STEP * STEP * (R / 8); piece += WORKERS / 32) {
+                    const int pb = piece / (R / 8), first = piece % (R / 8) * 8, block = p0 + pb;
+                    const int chunks = block < p1 ? (min(a.M - first, 8)) * (MX_BLOCK / 8) : 0;
+                    const uint32_t at = my_place + (uint32_t)(pb * X_BLOCK + first * 128), sc_at = my_scale + (uint32_t)(pb * MX_SCALE_BYTES + first * 16);
                     uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
 #pragma unroll
-                    for (int c0 = 0; c0 < R * (MX_BLOCK / 8); c0 += 32 * AHEAD) {
+                    for (int c0 = 0; c0 < 8 * (MX_BLOCK / 8); c0 += 32 * AHEAD) {
                         if (c0 >= chunks) break;
                         Chunk<PARTS> d[AHEAD];
 #pragma unroll
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
 #pragma unroll
                             for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
                             d[u].code = 0;
-                            if (i < chunks) load_chunk<PARTS>(a, i >> 4, block * MX_BLOCK + (lane & 15) * 8, d[u]);
+                            if (i < chunks) load_chunk<PARTS>(a, first + (i >> 4), block * MX_BLOCK + (lane & 15) * 8, d[u]);
                         }
 #pragma unroll
                         for (int u = 0; u < AHEAD; ++u) {
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                                 if (PARTS > 1) {
 #pragma unroll
                                     for (int kd = 0; kd < 4; ++kd)
-                                        if (kd != ROW_ZERO && kind == kd) seen[kd] |= 1u << (m0 + (lane >> 4));
+                                        if (kd != ROW_ZERO && kind == kd) seen[kd] |= 1u << (first + m0 + (lane >> 4));
                                 }
                             }
                         }

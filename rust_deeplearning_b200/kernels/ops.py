@@ -1800,7 +1800,7 @@ MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs, which a
 _MX8 = 2                 # rows of 8 bits, where a kernel's argument says of what kind its rows are
 _KINDS = {torch.float32: 0, torch.bfloat16: 1}
 MX8 = "mx8"              # in place of a dtype: rows wanted as `Mx8Rows`
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # what torch.cuda.current_stream(i).cuda_stream gives, in a thirtieth of the time
 
 
 def _blocks(columns: int) -> int:

@@ -359,6 +359,44 @@ def test_a_wait_that_runs_out(m, k, code, name):
     assert status.item() == 0
 
 
+def test_tensors_that_start_anywhere():
+    """Contiguous rows at an odd place of their memory: the same results as aligned ones."""
+    w = rnd((70, 200), torch.float32, 33, 0.05)
+    packed = ops.pack_mx4(w)
+    norm = ops.NormParams(rnd((201,), torch.float32, 35)[1:], 1e-6, 1.0)
+    for dtype in (torch.bfloat16, torch.float32):
+        flat = rnd((1 + 6 * 200,), dtype, 34)
+        odd = flat[1:].view(6, 200)
+        even = odd.clone()
+        assert odd.data_ptr() % 8 != 0 and even.data_ptr() % 16 == 0
+        assert torch.equal(ops.linear_mx4(odd, packed), ops.linear_mx4(even, packed))
+        a, b = ops.norm_mx8(odd, second=norm), ops.norm_mx8(even, second=ops.NormParams(norm.weight.clone(), 1e-6, 1.0))
+        assert torch.equal(a.dequantise(), b.dequantise())
+        flat = torch.cat([flat[:1], w.to(dtype).reshape(-1)])
+        assert torch.equal(ops.expand_mx4(ops.pack_mx4(flat[1:].view(70, 200))), ops.expand_mx4(ops.pack_mx4(w.to(dtype))))
+
+
+def test_a_weight_beyond_32_bits():
+    """2.5e9 bytes of codes: the last rows' outputs come from behind what 32 bits can count."""
+    rows, columns = 600_064, 8192
+    w = torch.zeros((rows, columns), dtype=torch.bfloat16, device=DEV)
+    tail = rnd((64, columns), torch.bfloat16, 36, 0.1)
+    w[-64:] = tail
+    packed, small = ops.pack_mx4(w), ops.pack_mx4(tail)
+    del w
+    x = rnd((3, columns), torch.bfloat16, 37)
+    got = ops.linear_mx4(x, packed, out_dtype=torch.float32)
+    want = f64(x) @ f64(ops.expand_mx4(small, torch.float32)).T
+    check(got[:, -64:], want, sum_tolerance(f64(x), f64(ops.expand_mx4(small, torch.float32)), "bfloat16"), "last outputs")
+    assert not got[:, :-64].any()
+    rows8 = ops.pack_mx8(rnd((20, columns), torch.bfloat16, 38))
+    got = ops.linear_mx4(rows8, packed)
+    assert torch.equal(got[:, -64:], ops.linear_mx4(rows8, packed)[:, -64:]) and not got[:, :-64].any()
+    w64, x64 = f64(ops.expand_mx4(small, torch.float32)), f64(rows8.dequantise())
+    want = x64 @ w64.T
+    check(got[:, -64:], want, sum_tolerance(x64, w64, "mx8") + np.abs(want) * 2.0 ** -8, "last outputs of 8-bit rows")
+
+
 # ---- refusals ----
 
 def test_refusals():
