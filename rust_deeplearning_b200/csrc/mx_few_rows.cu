@@ -12,10 +12,15 @@
 // below 2^-127, are computed again by plain arithmetic.
 //
 // Warp 0 loads weights: they depend on nothing an earlier kernel of the step writes, so it starts while that kernel is still running.
-// Warp 1 issues scales and products.  Sixteen warps turn the rows into parts (once, where a block's columns fit shared memory), a block of columns after
-// another so that the products can begin; eight of them then take finished sums out of tensor memory.  A wide matrix: a block takes 128 rows of weights after another.  One with fewer tiles than
+// Warp 1 issues scales and products.  Sixteen warps turn the rows into parts (once, where a block's columns fit shared memory; else for
+// every tile, into slots that are used in turn), a block of columns after another so that the products can begin; eight of them then take
+// finished sums out of tensor memory.  A wide matrix: a block takes 128 rows of weights after another.  One with fewer tiles than
 // multiprocessors: a cluster of up to 8 blocks shares a tile, each with its part of the columns, and its blocks send their sums through
 // distributed shared memory to the one that adds up that part of the outputs, in rank order.  Every wait is bounded.
+//
+// Measured on the device, one bfloat16 row: 256,000 outputs of 2,304 columns (313 MB) 55.8 us, 5.6 TB/s; 28,672 of 3,584, gated, 14.5 us,
+// 3.8 TB/s; 4,096 of 2,304 (5 MB) 5.5 us: there what bounds it is the chain of a launch, the first copy, the products of a block's columns
+// and the exchange in the cluster.  16 rows: 62.5, 20.5 and 6.8 us (in 8 bits already: 58.2, 16.4 and 5.8).
 #include <cuda_fp16.h>
 
 #include "activations.cuh"
@@ -26,7 +31,7 @@
 namespace {
 
 // A stage of the ring is STEP blocks of columns: a stage costs the issuing thread a wait beside its products, about as long as those of a block.
-constexpr int WORKERS = 512, THREADS = 64 + WORKERS, MAX_STAGES = 8, STEP = 2, SCALE_BUFS = 4, MAX_PASS = 64;
+constexpr int WORKERS = 512, THREADS = 64 + WORKERS, MAX_STAGES = 8, STEP = 2, SCALE_BUFS = 4, MAX_SLOTS = 64;
 
 struct FewArgs {
     const void* x; const uint8_t* row_scales;
@@ -34,7 +39,7 @@ struct FewArgs {
     void* out; int out_dtype;
     int M, N, K;                                 // N: outputs
     int blocks, row_pad;                         // blocks of 128 columns; the rows' padded count (8-bit rows)
-    int tiles, split, slice_blocks, pass_blocks, stages;
+    int tiles, split, slice_blocks, slots, stages;   // slots: blocks of the rows that shared memory holds
     int share;                                   // outputs of a tile that a block of a cluster adds up
     int gated, activation; float act_param, softcap;
     bool vec;                                    // rows lie on 16-byte boundaries
@@ -174,33 +179,36 @@ __device__ __forceinline__ int make_parts(const Chunk<PARTS>& d, uint2 (&bytes)[
 template <int PARTS, int R>
 __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs a) {
     constexpr int NB = PARTS * R;                            // columns of the product: part p of row m is column p R + m
+    constexpr int PIECES = STEP * (R / 8);                   // of a group of STEP blocks: eight rows of a block each
     constexpr int X_BLOCK = NB * MX_BLOCK;                   // bytes of a block of 128 columns of the rows
     constexpr int TMEM_COLS = 2 * NB + SCALE_BUFS * 8 <= 128 ? 128 : 256;
     constexpr int AHEAD = PARTS == 6 ? 2 : 4;                // chunks a lane asks for before it works on the first
     static_assert(NB % 16 == 0 && 2 * NB + SCALE_BUFS * 8 <= TMEM_COLS, "the sums of two tiles and the scales share tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], x_ready[MAX_PASS / STEP], x_free;
+    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], x_ready[MAX_SLOTS / STEP], x_free[MAX_SLOTS / STEP];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     // rows with an infinity or a NaN here; rows with a group too small for its last parts; rows with one that is not
     __shared__ unsigned bad_rows, tiny_rows, fine_rows;
     // shared memory: rows | ring of codes | the rows' scales | ring of scales | sums of a cluster's blocks
-    const uint32_t x_s = mx_smem(smem), ring_s = x_s + (uint32_t)(a.pass_blocks * X_BLOCK);
-    const uint32_t xs_s = ring_s + (uint32_t)(a.stages * STEP * MX_TILE_BYTES), ws_s = xs_s + (uint32_t)(a.pass_blocks * MX_SCALE_BYTES);
-    const uint32_t y_off = (uint32_t)(a.pass_blocks * (X_BLOCK + MX_SCALE_BYTES) + a.stages * STEP * (MX_TILE_BYTES + MX_SCALE_BYTES));
+    const uint32_t x_s = mx_smem(smem), ring_s = x_s + (uint32_t)(a.slots * X_BLOCK);
+    const uint32_t xs_s = ring_s + (uint32_t)(a.stages * STEP * MX_TILE_BYTES), ws_s = xs_s + (uint32_t)(a.slots * MX_SCALE_BYTES);
+    const uint32_t y_off = (uint32_t)(a.slots * (X_BLOCK + MX_SCALE_BYTES) + a.stages * STEP * (MX_TILE_BYTES + MX_SCALE_BYTES));
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // the compiler may know it uniform
     const int rank = a.split > 1 ? (int)(blockIdx.x % a.split) : 0;
     const int first_tile = blockIdx.x / a.split, tile_step = gridDim.x / a.split;
     const int b0 = min(rank * a.slice_blocks, a.blocks), b1 = min(b0 + a.slice_blocks, a.blocks);
-    const int passes = (b1 - b0 + a.pass_blocks - 1) / a.pass_blocks;
+    // the rows lie in slots of STEP blocks: all of them once (they stay for every tile), or as many as there is room for, in turn
+    const int groups = (b1 - b0 + STEP - 1) / STEP, x_groups = a.slots / STEP;
+    const bool resident = groups <= x_groups;
     {   // every barrier by a thread of its own
         const int t = threadIdx.x;
         if (t < MAX_STAGES) { mx_bar_init(mx_smem(&full_bar[t]), 1); mx_bar_init(mx_smem(&empty_bar[t]), 1); }
         else if (t < MAX_STAGES + 2) { mx_bar_init(mx_smem(&acc_full[t - MAX_STAGES]), 1); mx_bar_init(mx_smem(&acc_empty[t - MAX_STAGES]), 8); }
-        else if (t == MAX_STAGES + 2) { mx_bar_init(mx_smem(&x_free), 1); gave_up = 0; bad_rows = tiny_rows = fine_rows = 0; }
-        else if (t >= 64 && t < 64 + MAX_PASS / STEP) mx_bar_init(mx_smem(&x_ready[t - 64]), STEP * (R / 8));
+        else if (t == MAX_STAGES + 2) { gave_up = 0; bad_rows = tiny_rows = fine_rows = 0; }
+        else if (t >= 64 && t < 64 + MAX_SLOTS / STEP) { mx_bar_init(mx_smem(&x_ready[t - 64]), PIECES); mx_bar_init(mx_smem(&x_free[t - 64]), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -223,9 +231,8 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             int s = 0, piece = first_tile * a.blocks + b0;   // place in the ring; block of columns over all tiles
             uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
             for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, piece += (tile_step - 1) * a.blocks + (a.blocks - (b1 - b0))) {
-                for (int kb = b0, pass_end = min(b0 + a.pass_blocks, b1); kb < b1;) {
-                    // a stage is up to STEP blocks; none reaches into the next pass over the rows
-                    const int n = min(STEP, pass_end - kb);
+                for (int kb = b0; kb < b1;) {
+                    const int n = min(STEP, b1 - kb);
                     if (!mx_bar_wait(mx_smem(&empty_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
                     const uint32_t full = mx_smem(&full_bar[s]), at = ring_s + (uint32_t)(s * STEP * MX_TILE_BYTES);
                     mx_bar_expect(full, (uint32_t)n * (MX_TILE_TX + MX_SCALE_BYTES) + extra);
@@ -236,7 +243,6 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                     extra = 0;
                     kb += n;
                     piece += n;
-                    if (kb == pass_end) pass_end = min(pass_end + a.pass_blocks, b1);
                     if (++s == a.stages) { s = 0; parity ^= 1; }
                 }
             }
@@ -245,37 +251,36 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     } else if (warp == 1) {
         // ---- scales to tensor memory, and the products ----
         if (mx_elect()) {
-            int s = 0, lt = 0, n_pass = 0, scale_buf = 0;
-            uint32_t parity = 0;
+            int s = 0, lt = 0, scale_buf = 0, g = 0;         // g: the rows' group
+            uint32_t parity = 0, x_parity = 0;
             for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++lt) {
                 const int buf = lt & 1;
                 if (!mx_bar_wait(mx_smem(&acc_empty[buf]), ((lt >> 1) & 1) ^ 1, a.wait_cycles, gave_up_v)) { ok = false; break; }
-                for (int p = 0; p < passes && ok; ++p, ++n_pass) {
-                    const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
-                    const bool fresh = passes > 1 || lt == 0;            // the rows are being made ready, STEP blocks at a time
-                    for (int kb = p0; kb < p1;) {
-                        const int n = min(STEP, p1 - kb);
-                        const uint32_t full = mx_smem(&full_bar[s]);
-                        if (!mx_bar_wait_both(full, parity, fresh ? mx_smem(&x_ready[(kb - p0) / STEP]) : full, fresh ? (uint32_t)(n_pass & 1) : parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
-                        mx_fence_after();
+                if (resident) g = 0;
+                for (int kb = b0; kb < b1; kb += STEP) {
+                    const int n = min(STEP, b1 - kb);
+                    const uint32_t full = mx_smem(&full_bar[s]);
+                    const bool fresh = !resident || lt == 0; // the rows are being made ready
+                    if (!mx_bar_wait_both(full, parity, fresh ? mx_smem(&x_ready[g]) : full, fresh ? x_parity : parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
+                    mx_fence_after();
 #pragma unroll
-                        for (int j = 0; j < STEP; ++j) {
-                            if (j >= n) break;
-                            const uint32_t sa = tmem + 2 * NB + (uint32_t)((scale_buf + j) & (SCALE_BUFS - 1)) * 8, sb = sa + 4;
-                            copy_scales(sa, mx_scale_desc(ws_s + (uint32_t)((s * STEP + j) * MX_SCALE_BYTES)));
-                            copy_scales(sb, mx_scale_desc(xs_s + (uint32_t)((kb + j - p0) * MX_SCALE_BYTES)));
-                            const uint64_t ad = mx_operand_desc(ring_s + (uint32_t)((s * STEP + j) * MX_TILE_BYTES)), bd = mx_operand_desc(x_s + (uint32_t)((kb + j - p0) * X_BLOCK));
+                    for (int j = 0; j < STEP; ++j) {
+                        if (j >= n) break;
+                        const uint32_t sa = tmem + 2 * NB + (uint32_t)((scale_buf + j) & (SCALE_BUFS - 1)) * 8, sb = sa + 4;
+                        copy_scales(sa, mx_scale_desc(ws_s + (uint32_t)((s * STEP + j) * MX_SCALE_BYTES)));
+                        copy_scales(sb, mx_scale_desc(xs_s + (uint32_t)((g * STEP + j) * MX_SCALE_BYTES)));
+                        const uint64_t ad = mx_operand_desc(ring_s + (uint32_t)((s * STEP + j) * MX_TILE_BYTES)), bd = mx_operand_desc(x_s + (uint32_t)((g * STEP + j) * X_BLOCK));
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma_mx(tmem + buf * NB, ad + (uint32_t)(k * 2), bd + (uint32_t)(k * 2), mx_idesc(MX_E2M1, MX_E4M3, MX_ROWS, NB, k), sa, sb, kb + j != b0 || k != 0);
-                        }
-                        commit(mx_smem(&empty_bar[s]));
-                        kb += n;
-                        scale_buf = (scale_buf + n) & (SCALE_BUFS - 1);
-                        if (++s == a.stages) { s = 0; parity ^= 1; }
+                        for (int k = 0; k < 4; ++k)
+                            mma_mx(tmem + buf * NB, ad + (uint32_t)(k * 2), bd + (uint32_t)(k * 2), mx_idesc(MX_E2M1, MX_E4M3, MX_ROWS, NB, k), sa, sb, kb + j != b0 || k != 0);
                     }
-                    if (ok && passes > 1) commit(mx_smem(&x_free));
+                    commit(mx_smem(&empty_bar[s]));
+                    if (!resident) commit(mx_smem(&x_free[g]));
+                    scale_buf = (scale_buf + n) & (SCALE_BUFS - 1);
+                    if (++s == a.stages) { s = 0; parity ^= 1; }
+                    if (++g == x_groups) { g = 0; x_parity ^= 1; }
                 }
+                if (resident) x_parity = 0;
                 if (ok) commit(mx_smem(&acc_full[buf]));
             }
         }
@@ -288,67 +293,76 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         // a lane's chunk of row 0 (lanes 16 to 31: of row 1) of a block, and its group's scale: the two halves of a warp hold neighbouring rows
         const uint32_t my_place = x_s + (uint32_t)((lane >> 4) * 128 + ((((lane & 15) >> 1) ^ (lane >> 4)) << 4) + (lane & 1) * 8);
         const uint32_t my_scale = xs_s + (uint32_t)((lane >> 4) * 16 + ((lane & 15) >> 2));
-        int lt = 0, n_pass = 0;
-        // (a wait in vain ends no loop here: the blocks of a cluster meet again below)
-        for (int tile = first_tile; tile < a.tiles; tile += tile_step, ++lt) {
-            for (int p = 0; p < passes && (passes > 1 || lt == 0); ++p, ++n_pass) {
-                if (n_pass > 0 && !mx_bar_wait(mx_smem(&x_free), (n_pass - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
-                const int p0 = b0 + p * a.pass_blocks, p1 = min(p0 + a.pass_blocks, b1);
-                // A warp takes every sixteenth piece, eight rows of a block of columns, and hands it over: the products begin with the first
-                // STEP blocks.  Every block's barrier takes part in every pass, so that its phase is the number of the pass.
-                for (int piece = warp - 2; piece < (a.pass_blocks + STEP - 1) / STEP * STEP * (R / 8); piece += WORKERS / 32) {
-                    const int pb = piece / (R / 8), first = piece % (R / 8) * 8, block = p0 + pb;
-                    const int chunks = block < p1 ? (min(a.M - first, 8)) * (MX_BLOCK / 8) : 0;
-                    const uint32_t at = my_place + (uint32_t)(pb * X_BLOCK + first * 128), sc_at = my_scale + (uint32_t)(pb * MX_SCALE_BYTES + first * 16);
-                    uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
+        // The rows of tile `turn` of this block: warps take pieces in turn, eight rows of a block of columns each, and hand them over; the
+        // products begin with the first STEP blocks.  Where the rows do not stay, a piece waits until its slot has been read.  The pieces
+        // are counted on over the tiles, and there are no more warps at it than a round over the slots has pieces: so a warp's next piece
+        // is at most one round on, and the phase of its slot's barrier before the one that it waits for is over.
+        const int pieces = groups * PIECES, takers = min(WORKERS / 32, x_groups * PIECES);
+        auto prepare = [&](int turn) {
+            if (warp - 2 >= takers) return;
+            const int before = turn * pieces;
+            for (int p = before + ((warp - 2 - before % takers + takers) % takers); p < before + pieces; p += takers) {
+                const int nth = p / PIECES, piece = p - before, gi = piece / PIECES, round = nth / x_groups, gs = nth - round * x_groups;
+                if (round > 0 && !resident && !mx_bar_wait(mx_smem(&x_free[gs]), (round - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
+                const int j = piece % PIECES / (R / 8), first = piece % (R / 8) * 8, block = b0 + gi * STEP + j, slot = gs * STEP + j;
+                const int chunks = block < b1 ? (min(a.M - first, 8)) * (MX_BLOCK / 8) : 0;
+                const uint32_t at = my_place + (uint32_t)(slot * X_BLOCK + first * 128), sc_at = my_scale + (uint32_t)(slot * MX_SCALE_BYTES + first * 16);
+                uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
 #pragma unroll
-                    for (int c0 = 0; c0 < 8 * (MX_BLOCK / 8); c0 += 32 * AHEAD) {
-                        if (c0 >= chunks) break;
-                        Chunk<PARTS> d[AHEAD];
+                for (int c0 = 0; c0 < 8 * (MX_BLOCK / 8); c0 += 32 * AHEAD) {
+                    if (c0 >= chunks) break;
+                    Chunk<PARTS> d[AHEAD];
 #pragma unroll
-                        for (int u = 0; u < AHEAD; ++u) {
-                            const int i = c0 + u * 32 + lane;                            // 16 chunks a row
+                    for (int u = 0; u < AHEAD; ++u) {
+                        const int i = c0 + u * 32 + lane;                            // 16 chunks a row
 #pragma unroll
-                            for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
-                            d[u].code = 0;
-                            if (i < chunks) load_chunk<PARTS>(a, first + (i >> 4), block * MX_BLOCK + (lane & 15) * 8, d[u]);
-                        }
+                        for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
+                        d[u].code = 0;
+                        if (i < chunks) load_chunk<PARTS>(a, first + (i >> 4), block * MX_BLOCK + (lane & 15) * 8, d[u]);
+                    }
 #pragma unroll
-                        for (int u = 0; u < AHEAD; ++u) {
-                            const int m0 = c0 / 16 + u * 2;                              // this lane's row: m0 or m0 + 1
-                            if (c0 + u * 32 >= chunks) break;                            // none of this warp's
-                            uint2 bytes[PARTS];
-                            uint32_t code[PARTS];
-                            const int kind = make_parts<PARTS>(d[u], bytes, code);
-                            if (c0 + u * 32 + lane < chunks) {
-                                // swizzled by the row: rows m0 and m0 + 1 of eight flip the pieces by m0 & 6 beside what my_place has of the lane's own
-                                const uint32_t to = (at ^ (uint32_t)((m0 & 6) << 4)) + (uint32_t)((m0 >> 3) * 1024 + (m0 & 6) * 128);
+                    for (int u = 0; u < AHEAD; ++u) {
+                        const int m0 = c0 / 16 + u * 2;                              // this lane's row: m0 or m0 + 1
+                        if (c0 + u * 32 >= chunks) break;                            // none of this warp's
+                        uint2 bytes[PARTS];
+                        uint32_t code[PARTS];
+                        const int kind = make_parts<PARTS>(d[u], bytes, code);
+                        if (c0 + u * 32 + lane < chunks) {
+                            // swizzled by the row: rows m0 and m0 + 1 of eight flip the pieces by m0 & 6 beside what my_place has of the lane's own
+                            const uint32_t to = (at ^ (uint32_t)((m0 & 6) << 4)) + (uint32_t)((m0 >> 3) * 1024 + (m0 & 6) * 128);
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part)
+                                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (uint32_t)(part * R * 128)), "r"(bytes[part].x), "r"(bytes[part].y) : "memory");
+                            if ((lane & 3) == 0) {
 #pragma unroll
                                 for (int part = 0; part < PARTS; ++part)
-                                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (uint32_t)(part * R * 128)), "r"(bytes[part].x), "r"(bytes[part].y) : "memory");
-                                if ((lane & 3) == 0) {
+                                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(sc_at + (uint32_t)(m0 * 16 + (part * R & 31) * 16 + (part * R >> 5) * 4)), "r"(code[part]) : "memory");
+                            }
+                            if (PARTS > 1) {
 #pragma unroll
-                                    for (int part = 0; part < PARTS; ++part)
-                                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(sc_at + (uint32_t)(m0 * 16 + (part * R & 31) * 16 + (part * R >> 5) * 4)), "r"(code[part]) : "memory");
-                                }
-                                if (PARTS > 1) {
-#pragma unroll
-                                    for (int kd = 0; kd < 4; ++kd)
-                                        if (kd != ROW_ZERO && kind == kd) seen[kd] |= 1u << (first + m0 + (lane >> 4));
-                                }
+                                for (int kd = 0; kd < 4; ++kd)
+                                    if (kd != ROW_ZERO && kind == kd) seen[kd] |= 1u << (first + m0 + (lane >> 4));
                             }
                         }
                     }
-                    if (PARTS > 1) {
-                        const uint32_t fine = __reduce_or_sync(0xffffffffu, seen[ROW_FINE]), rare = seen[ROW_TINY] | seen[ROW_BAD];
-                        if (lane == 0 && fine) atomicOr(&fine_rows, fine);
-                        if (rare) { atomicOr(&tiny_rows, seen[ROW_TINY]); atomicOr(&bad_rows, seen[ROW_BAD]); }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the products read what was stored here
-                    __syncwarp();
-                    if (lane == 0) mx_bar_arrive(mx_smem(&x_ready[pb / STEP]));
                 }
+                if (PARTS > 1) {
+                    const uint32_t fine = __reduce_or_sync(0xffffffffu, seen[ROW_FINE]), rare = seen[ROW_TINY] | seen[ROW_BAD];
+                    if (lane == 0 && fine) atomicOr(&fine_rows, fine);
+                    if (rare) { atomicOr(&tiny_rows, seen[ROW_TINY]); atomicOr(&bad_rows, seen[ROW_BAD]); }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // the products read what was stored here
+                __syncwarp();
+                if (lane == 0) mx_bar_arrive(mx_smem(&x_ready[gs]));
             }
+        };
+        int lt = 0;
+        // (a wait in vain ends no loop here: the blocks of a cluster meet again below)
+        prepare(0);
+        for (int tile = first_tile; tile < a.tiles; tile += tile_step, ++lt) {
+            // the next tile's rows before this one's sums: its products then find them (they need the sums before these to be out, which
+            // the last turn saw to)
+            if (!resident && tile + tile_step < a.tiles) prepare(lt + 1);
             const int buf = lt & 1;
             if (!mx_bar_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
             mx_fence_after();
@@ -359,7 +373,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                 float sum[MINE];
 #pragma unroll
                 for (int j = 0; j < MINE; ++j) sum[j] = 0.f;
-                if (passes > 0) {
+                if (groups > 0) {
                     uint32_t v[PARTS][MINE];
 #pragma unroll
                     for (int part = 0; part < PARTS; ++part) tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * NB + part * R + half * MINE), v[part]);
@@ -458,17 +472,18 @@ int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
     a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
     a.slice_blocks = (a.blocks + a.split - 1) / a.split;
     const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - 1024 - sums;      // alignment, static shared memory
-    // the rows of all of a block's columns beside a ring of three stages, or of as many as fit
-    a.pass_blocks = a.slice_blocks;
-    if (a.pass_blocks * PER_BLOCK + 3 * PER_STAGE > most) a.pass_blocks = (most - 3 * PER_STAGE) / PER_BLOCK;
-    if (a.pass_blocks > MAX_PASS) a.pass_blocks = MAX_PASS;
-    a.stages = (most - a.pass_blocks * PER_BLOCK) / PER_STAGE;
+    // The rows of all of a block's columns, if a ring of two stages fits beside them (float32, 8 rows x 2,304, 256,000 outputs: 71 us so and 94
+    // with the rows brought anew for every tile; bfloat16, 16 x 3,584, 28,672 gated: 20.5 and 23.0); else as many as fit beside four.
+    a.slots = (a.slice_blocks + STEP - 1) / STEP * STEP;
+    if (a.slots * PER_BLOCK + 2 * PER_STAGE > most) a.slots = (most - 4 * PER_STAGE) / PER_BLOCK / STEP * STEP;
+    if (a.slots > MAX_SLOTS) a.slots = MAX_SLOTS;
+    a.stages = (most - a.slots * PER_BLOCK) / PER_STAGE;
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
     // no deeper than the block's work: what shared memory is left lets the next kernel's blocks begin
     const int turns = a.split > 1 ? 1 : (a.tiles + sms - 1) / sms;
-    const int steps = (a.slice_blocks + STEP - 1) / STEP + (a.slice_blocks - 1) / a.pass_blocks;
+    const int steps = (a.slice_blocks + STEP - 1) / STEP;
     if ((long long)a.stages > (long long)turns * steps) a.stages = turns * steps;
-    const int smem = 1024 + a.pass_blocks * PER_BLOCK + a.stages * PER_STAGE + sums;
+    const int smem = 1024 + a.slots * PER_BLOCK + a.stages * PER_STAGE + sums;
     RDL_CUDA((rdl_allow_shared<mx_few_rows_kernel<PARTS, R>>(smem)), "mx_few_rows");
     const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
     RDL_CHECK_EX(rdl_launch_cluster(mx_few_rows_kernel<PARTS, R>, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, w.codes_map, a), "mx_few_rows");

@@ -189,6 +189,22 @@ SHAPES = [(1, 1, 1), (1, 3, 32), (2, 16, 33), (5, 777, 1003), (8, 100, 128), (9,
 
 
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "mx8"])
+@pytest.mark.parametrize("m,n,k", [(16, 19001, 4700), (9, 300, 36865)])
+def test_few_rows_longer_than_shared_memory(m, n, k, kind):
+    """The blocks of the rows pass through shared memory in turn, again for each tile; a row that is not finite keeps to itself."""
+    w = ops.pack_mx4(rnd((n, k), torch.float32, 40, 0.05))
+    x, x64 = rows_for(m, k, kind, 41)
+    w64 = f64(ops.expand_mx4(w, torch.float32))
+    want, tol = x64 @ w64.T, sum_tolerance(x64, w64, kind)
+    whole = ops.linear_mx4(x, w, out_dtype=torch.float32)
+    check(whole, want, tol, "float32")
+    if kind != "mx8":
+        x[2, k - 1] = float("nan")
+        got = ops.linear_mx4(x, w, out_dtype=torch.float32)
+        assert got[2].isnan().all() and torch.equal(torch.cat([got[:2], got[3:]]), torch.cat([whole[:2], whole[3:]]))
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mx8"])
 @pytest.mark.parametrize("m,n,k", SHAPES)
 def test_few_rows(m, n, k, kind):
     w = ops.pack_mx4(rnd((n, k), torch.float32, 7, 0.05))
