@@ -11,7 +11,7 @@ extern "C" {
 #define RDL_ACT_SILU 1
 #define RDL_ACT_SWISH_LIMIT 2   // min(g, L) sigmoid(1.702 min(g, L)) (clamp(u, -L, L) + 1), L a parameter
 
-#define RDL_ABI_VERSION 26
+#define RDL_ABI_VERSION 27
 
 const char* rdl_last_error(void);
 int rdl_abi_version(void);
@@ -396,8 +396,8 @@ int rdl_gemm_skinny(void* out, int out_dtype, const void* x, const void* w, int 
 #define RDL_NORM_DEFERRED 2    // the call is C
 typedef struct {
     int mode;
-    float* sums;                     // [units of 16 columns][8 rows][4]: sum y^2, sum h^2, sum h a', sum a'^2
-    int n_sums;                      // C: the units P had (P: taken from n)
+    float* sums;                     // [units][8 rows][4]: sum y^2, sum h^2, sum h a', sum a'^2; a unit: 16 columns, or what a 4-bit P says
+    int n_sums;                      // C: the units P had (P: taken from n; with a 4-bit matrix the place there is)
     // P
     const float* residual;           // h [rows][n]
     const void* w1; int w1_dtype; float off1;
@@ -452,6 +452,11 @@ int rdl_mx4_describe(void* matrix, const void* codes, const void* scales, int ro
 // with row_scales.  A gated matrix: act(gate) * up.
 int rdl_mx_few_rows(void* out, int out_dtype, const void* x, int x_kind, const void* row_scales, const void* weight, int m,
                     int activation, float act_param, float softcap, int* status, void* stream);
+// The same with one side of a deferred norm (DeferredNormArgs; bfloat16 rows, 1 to 8 of them).  A branch's product (no epilogue; not a
+// gated matrix) writes rdl_mx_branch_units(weight) units of sums, the count of which norm->n_sums repeats; 0: this matrix has no such form.
+int rdl_mx_branch_units(const void* weight);
+int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, const void* weight, int m, int activation, float act_param, float softcap,
+                         const DeferredNormArgs* norm, int* status, void* stream);
 // the same for up to 128 rows of 8 bits
 int rdl_mx_some_rows(void* out, int out_dtype, const void* x, const void* row_scales, const void* weight, int m,
                      int activation, float act_param, float softcap, int* status, void* stream);

@@ -18,9 +18,13 @@
 // multiprocessors: a cluster of up to 8 blocks shares a tile, each with its part of the columns, and its blocks send their sums through
 // distributed shared memory to the one that adds up that part of the outputs, in rank order.  Every wait is bounded.
 //
-// Measured on the device, one bfloat16 row: 256,000 outputs of 2,304 columns (313 MB) 55.8 us, 5.6 TB/s; 28,672 of 3,584, gated, 14.5 us,
-// 3.8 TB/s; 4,096 of 2,304 (5 MB) 5.5 us: there what bounds it is the chain of a launch, the first copy, the products of a block's columns
-// and the exchange in the cluster.  16 rows: 62.5, 20.5 and 6.8 us (in 8 bits already: 58.2, 16.4 and 5.8).
+// Up to 8 bfloat16 rows can have a deferred norm on either side (the algebra: DeferredNormArgs in api.h).  The branch's product writes its
+// partial sums a block of the cluster at a time.  The product behind the norm takes both halves of the operand as its rows; four warps add
+// the partial sums up and see to the stream while it multiplies, and a row's two sums are joined on their way out of tensor memory.
+// (Joining the halves before the product, as x = s2 (ht + s1 at), makes parts of half as many rows, but only after the sums are there: it
+// took 2 us more than a plain product; this way 1 us with up to 4 rows, 1.1 to 2.5 us with 8.)  Output projection, gated product, down
+// projection and next projection of a layer of width 2,304, with the norms between: 1 row 27.0 us, 29.7 with kernels for the norms; 8
+// rows 32.8 and 34.0.
 #include <cuda_fp16.h>
 
 #include "activations.cuh"
@@ -43,6 +47,7 @@ struct FewArgs {
     int share;                                   // outputs of a tile that a block of a cluster adds up
     int gated, activation; float act_param, softcap;
     bool vec;                                    // rows lie on 16-byte boundaries
+    DeferredNormArgs norm; int src_rows;             // one side of a deferred norm; the rows of which sums are wanted (M: rows of the output)
     long long wait_cycles; int test_extra_tx;
     int* status;
 };
@@ -68,9 +73,11 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 }
 // N accumulator columns of the warp's lanes, as bits; there after mx_tmem_wait_ld
 template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
-    static_assert(N == 4 || N == 8, "four or eight columns");
-    if constexpr (N == 4)
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
+    static_assert(N == 2 || N == 4 || N == 8, "two, four or eight columns");
+    if constexpr (N == 2)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr) : "memory");
+    else if constexpr (N == 4)
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
     else
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -125,6 +132,11 @@ __device__ __forceinline__ void load_chunk(const FewArgs& a, int m, int k, Chunk
     }
 }
 
+__device__ __forceinline__ uint32_t raw_load(const void* p, long long i, int dtype) {             // bits now, the value when it is needed
+    return dtype == RDL_BF16 ? (uint32_t)((const unsigned short*)p)[i] : ((const uint32_t*)p)[i];
+}
+__device__ __forceinline__ float raw_value(uint32_t bits, int dtype) { return __uint_as_float(dtype == RDL_BF16 ? bits << 16 : bits); }
+
 constexpr int ROW_FINE = 0, ROW_ZERO = 1, ROW_TINY = 2, ROW_BAD = 3;
 
 // The parts of a chunk as e4m3 bytes, and the scale codes of its group; the four lanes of a group come here together.  A part is the
@@ -175,14 +187,17 @@ __device__ __forceinline__ int make_parts(const Chunk<PARTS>& d, uint2 (&bytes)[
     }
 }
 
-// PARTS: 1 (8-bit rows), 2 (bfloat16), 6 (float32); R: rows the product has place for
-template <int PARTS, int R>
+// PARTS: 1 (8-bit rows), 2 (bfloat16), 6 (float32); R: rows the product has place for; MODE: 0, or the side of a deferred norm
+template <int PARTS, int R, int MODE>
 __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs a) {
     constexpr int NB = PARTS * R;                            // columns of the product: part p of row m is column p R + m
     constexpr int PIECES = STEP * (R / 8);                   // of a group of STEP blocks: eight rows of a block each
     constexpr int X_BLOCK = NB * MX_BLOCK;                   // bytes of a block of 128 columns of the rows
     constexpr int TMEM_COLS = 2 * NB + SCALE_BUFS * 8 <= 128 ? 128 : 256;
     constexpr int AHEAD = PARTS == 6 ? 2 : 4;                // chunks a lane asks for before it works on the first
+    // behind a deferred norm four of the workers see to the sums and to the stream; the others make parts (of 18 blocks of 16 rows, three
+    // pieces each, as sixteen would)
+    constexpr int SIDE = MODE == RDL_NORM_DEFERRED ? 4 : 0, TAKERS = WORKERS / 32 - SIDE;
     static_assert(NB % 16 == 0 && 2 * NB + SCALE_BUFS * 8 <= TMEM_COLS, "the sums of two tiles and the scales share tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -191,6 +206,8 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     __shared__ int gave_up;
     // rows with an infinity or a NaN here; rows with a group too small for its last parts; rows with one that is not
     __shared__ unsigned bad_rows, tiny_rows, fine_rows;
+    __shared__ float4 norm_part[SIDE ? SIDE : 1][8];         // the branch's partial sums, a warp's share of the units
+    __shared__ float2 row_scale[8];                          // a row's two numbers
     // shared memory: rows | ring of codes | the rows' scales | ring of scales | sums of a cluster's blocks
     const uint32_t x_s = mx_smem(smem), ring_s = x_s + (uint32_t)(a.slots * X_BLOCK);
     const uint32_t xs_s = ring_s + (uint32_t)(a.stages * STEP * MX_TILE_BYTES), ws_s = xs_s + (uint32_t)(a.slots * MX_SCALE_BYTES);
@@ -293,11 +310,17 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         // a lane's chunk of row 0 (lanes 16 to 31: of row 1) of a block, and its group's scale: the two halves of a warp hold neighbouring rows
         const uint32_t my_place = x_s + (uint32_t)((lane >> 4) * 128 + ((((lane & 15) >> 1) ^ (lane >> 4)) << 4) + (lane & 1) * 8);
         const uint32_t my_scale = xs_s + (uint32_t)((lane >> 4) * 16 + ((lane & 15) >> 2));
+        // behind a deferred norm the rows are the operand's: R / 2 of the stream, R / 2 of the branch, the first src_rows of each in use
+        auto used_row = [&](int r) { return MODE != RDL_NORM_DEFERRED || (r & (R / 2 - 1)) < a.src_rows; };
         // The rows of tile `turn` of this block: warps take pieces in turn, eight rows of a block of columns each, and hand them over; the
         // products begin with the first STEP blocks.  Where the rows do not stay, a piece waits until its slot has been read.  The pieces
         // are counted on over the tiles, and there are no more warps at it than a round over the slots has pieces: so a warp's next piece
         // is at most one round on, and the phase of its slot's barrier before the one that it waits for is over.
-        const int pieces = groups * PIECES, takers = min(WORKERS / 32, x_groups * PIECES);
+        const int pieces = groups * PIECES, takers = min(TAKERS, x_groups * PIECES);
+        auto shift = [](Chunk<PARTS> (&d)[AHEAD]) {
+#pragma unroll
+            for (int i = 1; i < AHEAD; ++i) d[i - 1] = d[i];
+        };
         auto prepare = [&](int turn) {
             if (warp - 2 >= takers) return;
             const int before = turn * pieces;
@@ -305,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                 const int nth = p / PIECES, piece = p - before, gi = piece / PIECES, round = nth / x_groups, gs = nth - round * x_groups;
                 if (round > 0 && !resident && !mx_bar_wait(mx_smem(&x_free[gs]), (round - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
                 const int j = piece % PIECES / (R / 8), first = piece % (R / 8) * 8, block = b0 + gi * STEP + j, slot = gs * STEP + j;
-                const int chunks = block < b1 ? (min(a.M - first, 8)) * (MX_BLOCK / 8) : 0;
+                const int chunks = block < b1 ? min((MODE == RDL_NORM_DEFERRED ? R : a.M) - first, 8) * (MX_BLOCK / 8) : 0;
                 const uint32_t at = my_place + (uint32_t)(slot * X_BLOCK + first * 128), sc_at = my_scale + (uint32_t)(slot * MX_SCALE_BYTES + first * 16);
                 uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
 #pragma unroll
@@ -318,15 +341,17 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
 #pragma unroll
                         for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
                         d[u].code = 0;
-                        if (i < chunks) load_chunk<PARTS>(a, first + (i >> 4), block * MX_BLOCK + (lane & 15) * 8, d[u]);
+                        if (i < chunks && used_row(first + (i >> 4))) load_chunk<PARTS>(a, first + (i >> 4), block * MX_BLOCK + (lane & 15) * 8, d[u]);
                     }
-#pragma unroll
+#pragma unroll 1                                                                     // short code: see the head of the file
                     for (int u = 0; u < AHEAD; ++u) {
                         const int m0 = c0 / 16 + u * 2;                              // this lane's row: m0 or m0 + 1
                         if (c0 + u * 32 >= chunks) break;                            // none of this warp's
+                        if (MODE == RDL_NORM_DEFERRED && !used_row(first + m0)) { shift(d); continue; }
                         uint2 bytes[PARTS];
                         uint32_t code[PARTS];
-                        const int kind = make_parts<PARTS>(d[u], bytes, code);
+                        const int kind = make_parts<PARTS>(d[0], bytes, code);
+                        shift(d);
                         if (c0 + u * 32 + lane < chunks) {
                             // swizzled by the row: rows m0 and m0 + 1 of eight flip the pieces by m0 & 6 beside what my_place has of the lane's own
                             const uint32_t to = (at ^ (uint32_t)((m0 & 6) << 4)) + (uint32_t)((m0 >> 3) * 1024 + (m0 & 6) * 128);
@@ -359,6 +384,58 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         int lt = 0;
         // (a wait in vain ends no loop here: the blocks of a cluster meet again below)
         prepare(0);
+        if (SIDE > 0 && warp >= 2 + TAKERS) {
+            // a row's two numbers, lane & 7 the row, from the branch's partial sums in a fixed order
+            const DeferredNormArgs& d = a.norm;
+            auto add_lanes = [](float4& v) {                 // over the lanes with the same lane & 7
+#pragma unroll
+                for (int o = 8; o <= 16; o <<= 1) {
+                    v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+                    v.z += __shfl_xor_sync(0xffffffffu, v.z, o); v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
+                }
+            };
+            const int me = warp - 2 - TAKERS;
+            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+            if ((lane & 7) < a.src_rows) {
+                for (int u0 = me * 4 + (lane >> 3); u0 < d.n_sums; u0 += 8 * SIDE * 4) {
+                    float4 v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int u = u0 + i * SIDE * 4;
+                        v[i] = u < d.n_sums ? __ldcg(reinterpret_cast<const float4*>(d.sums) + u * 8 + (lane & 7)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { t.x += v[i].x; t.y += v[i].y; t.z += v[i].z; t.w += v[i].w; }
+                }
+            }
+            add_lanes(t);
+            if (lane < 8) norm_part[me][lane] = t;
+            asm volatile("bar.sync 1, %0;" ::"n"(SIDE * 32) : "memory");
+            static_assert(SIDE == 0 || SIDE == 4, "four shares, one a quarter of the warp");
+            t = norm_part[(lane >> 3) & (SIDE ? SIDE - 1 : 0)][lane & 7];
+            add_lanes(t);
+            const float s1 = rsqrtf(t.x / (float)a.K + d.eps1);
+            const float s2 = rsqrtf(fmaxf(t.y + 2.f * s1 * t.z + s1 * s1 * t.w, 0.f) / (float)a.K + d.eps2);     // of the squares of h + s1 a'
+            if (me == 0 && lane < 8) row_scale[lane] = make_float2(s1, s2);
+            __syncwarp();
+            asm volatile("bar.arrive 2, %0;" ::"n"(SIDE * 32 + 256) : "memory");         // for the warps that take the sums out
+            // this block's slice of the updated stream and of the operand after it
+            if (d.residual_out || d.scaled_next) {
+                const long long total = (long long)a.src_rows * a.K, per = (total + gridDim.x - 1) / gridDim.x;
+                const long long begin = (long long)blockIdx.x * per, end = begin + per < total ? begin + per : total;
+                for (long long e0 = begin + me * 32; e0 < end; e0 += SIDE * 32) {
+                    const long long e = e0 + lane;
+                    const bool in = e < end;
+                    const int m = in ? (int)(e / a.K) : 0;
+                    const float r1 = __shfl_sync(0xffffffffu, s1, m);
+                    if (!in) continue;
+                    const float h = fmaf(r1, raw_value(raw_load(d.branch_in, e, RDL_BF16), RDL_BF16), d.residual_in[e]);
+                    if (d.residual_out) d.residual_out[e] = h;
+                    if (d.scaled_next)
+                        ((__nv_bfloat16*)d.scaled_next)[e] = __float2bfloat16_rn(h * (raw_value(raw_load(d.w_next, e - (long long)m * a.K, d.w_next_dtype), d.w_next_dtype) + d.off_next));
+                }
+            }
+        }
         for (int tile = first_tile; tile < a.tiles; tile += tile_step, ++lt) {
             // the next tile's rows before this one's sums: its products then find them (they need the sums before these to be out, which
             // the last turn saw to)
@@ -366,17 +443,27 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             const int buf = lt & 1;
             if (!mx_bar_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
             mx_fence_after();
+            if (SIDE > 0 && lt == 0 && warp < 10) asm volatile("bar.sync 2, %0;" ::"n"(SIDE * 32 + 256) : "memory");
             float* y = reinterpret_cast<float*>(smem + y_off);       // a cluster's sums (one tile each)
             if (warp < 10) {
                 // lane l of quarter q: weight row 32 q + l of the tile; this warp takes half of the rows
                 constexpr int MINE = R / 2;
+                // which row sum[j] is of: half of the rows, or (deferred) of the stream's the same as of the branch's
+                auto row_of = [&](int j) { return MODE != RDL_NORM_DEFERRED ? half * MINE + j : (j < MINE / 2 ? 0 : MINE / 2) + half * (MINE / 2) + j; };
                 float sum[MINE];
 #pragma unroll
                 for (int j = 0; j < MINE; ++j) sum[j] = 0.f;
                 if (groups > 0) {
                     uint32_t v[PARTS][MINE];
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part) tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * NB + part * R + half * MINE), v[part]);
+                    for (int part = 0; part < PARTS; ++part) {
+                        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * NB + part * R);
+                        if constexpr (MODE != RDL_NORM_DEFERRED) tmem_ld<MINE>(at + half * MINE, v[part]);
+                        else {
+                            tmem_ld<MINE / 2>(at + half * (MINE / 2), v[part]);
+                            tmem_ld<MINE / 2>(at + R / 2 + half * (MINE / 2), v[part] + MINE / 2);
+                        }
+                    }
                     mx_tmem_wait_ld();
 #pragma unroll
                     for (int part = PARTS - 1; part >= 0; --part)                            // the smallest first
@@ -391,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                 if (PARTS > 1 && bad) {                          // plain arithmetic, for what the parts cannot hold
                     const int wr = tile * MX_ROWS + 32 * q + lane;
                     for (int j = 0; j < MINE; ++j) {
-                        const int m = half * MINE + j;
+                        const int m = row_of(j);
                         if (!(bad >> m & 1)) continue;
                         float y = 0.f;
                         for (int k = b0 * MX_BLOCK; k < min(b1 * MX_BLOCK, a.K); ++k) {
@@ -407,14 +494,30 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                             if (i == j) sum[i] = y;
                     }
                 }
+                if constexpr (MODE == RDL_NORM_DEFERRED) {       // both halves joined; sum[j] is row half * MINE / 2 + j of the result
+#pragma unroll
+                    for (int j = 0; j < MINE / 2; ++j) {
+                        const float2 r = row_scale[half * (MINE / 2) + j];
+                        sum[j] = r.y * fmaf(r.x, sum[j + MINE / 2], sum[j]);
+                    }
+                }
+                constexpr int OWN = MODE == RDL_NORM_DEFERRED ? MINE / 2 : MINE;
+                const int m_first = half * OWN, m_end = min(m_first + OWN, a.src_rows);
                 if (a.split == 1) {
                     // neighbouring lanes have neighbouring outputs; gated: 16 gate rows, then their 16 up rows
                     const int n = a.gated ? tile * (MX_ROWS / 2) + 16 * q + lane : tile * MX_ROWS + 32 * q + lane;
+#pragma unroll 1
+                    for (int m = m_first; m < m_end; ++m) {
+                        const float up = a.gated ? __shfl_down_sync(0xffffffffu, sum[0], 16) : 0.f;
+                        if (n < a.N && (!a.gated || lane < 16)) {
+                            const float y = finish(a, sum[0], up);
+                            if (MODE != RDL_NORM_DEFERRED || !a.norm.row_index) rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, y);
+                            else
+                                for (int j = 0; j < a.M; ++j)
+                                    if (a.norm.row_index[j] == m) rdl_store(a.out, (long long)j * a.N + n, a.out_dtype, y);
+                        }
 #pragma unroll
-                    for (int j = 0; j < MINE; ++j) {
-                        const int m = half * MINE + j;
-                        const float up = a.gated ? __shfl_down_sync(0xffffffffu, sum[j], 16) : 0.f;
-                        if (m < a.M && n < a.N && (!a.gated || lane < 16)) rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, finish(a, sum[j], up));
+                        for (int i = 1; i < OWN; ++i) sum[i - 1] = sum[i];
                     }
                 } else {
                     // each block adds up a part of the outputs: this row's sums go to its block, to this rank's place there
@@ -423,8 +526,8 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                     cluster_wait();                              // every block of the cluster runs
                     const uint32_t to = map_to_block(mx_smem(y), owner) + (uint32_t)(rank * R * outs + at) * 4;
 #pragma unroll
-                    for (int j = 0; j < MINE; ++j)
-                        if (half * MINE + j < a.M) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (uint32_t)((half * MINE + j) * outs) * 4), "f"(sum[j]) : "memory");
+                    for (int j = 0; j < OWN; ++j)
+                        if (m_first + j < m_end) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (uint32_t)((m_first + j) * outs) * 4), "f"(sum[j]) : "memory");
                 }
             } else if (a.split > 1) {
                 cluster_wait();
@@ -436,14 +539,54 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         __syncwarp();
         if (warp < 2) cluster_wait();                        // the first barrier: the workers are past it
         cluster_arrive();
+        // the branch of a residual stream: a warp takes a row, and has its elements of the stream and the norms' weights on their way now
+        constexpr int PER_LANE = MODE == RDL_NORM_BRANCH ? 2 : 1;                        // of at most 64 outputs
+        float stream[PER_LANE];
+        uint32_t w1[PER_LANE], w2[PER_LANE];
+        if constexpr (MODE == RDL_NORM_BRANCH) {
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                const int o = lane + 32 * i, of_tile = rank * a.share + o, n = first_tile * MX_ROWS + of_tile, m = warp - 2;
+                stream[i] = 0.f; w1[i] = w2[i] = 0;
+                if (m < 0 || m >= a.M || o >= a.share || of_tile >= MX_ROWS || n >= a.N) continue;
+                stream[i] = a.norm.residual[(long long)m * a.N + n];
+                w1[i] = raw_load(a.norm.w1, n, a.norm.w1_dtype);
+                w2[i] = raw_load(a.norm.w2, n, a.norm.w2_dtype);
+            }
+        }
         cluster_wait();                                      // every block's sums are where they are added up
-        if (warp >= 2) {
+        if constexpr (MODE == RDL_NORM_BRANCH) {
+            const int m = warp - 2;
+            if (m >= 0 && m < 8) {
+                const DeferredNormArgs& d = a.norm;
+                const float* ys = reinterpret_cast<const float*>(smem + y_off) + m * a.share;
+                float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < PER_LANE; ++i) {
+                    const int o = lane + 32 * i, of_tile = rank * a.share + o, n = first_tile * MX_ROWS + of_tile;
+                    if (m >= a.M || o >= a.share || of_tile >= MX_ROWS || n >= a.N) continue;
+                    float v[8], y = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) v[s] = s < a.split ? ys[s * R * a.share + o] : 0.f;
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) y += v[s];
+                    const __nv_bfloat16 b = __float2bfloat16_rn(y * (raw_value(w1[i], d.w1_dtype) + d.off1));
+                    const float bv = __bfloat162float(b);    // what the stream will add, s1 times
+                    t.x = fmaf(y, y, t.x); t.y = fmaf(stream[i], stream[i], t.y); t.z = fmaf(stream[i], bv, t.z); t.w = fmaf(bv, bv, t.w);
+                    ((__nv_bfloat16*)d.branch)[(long long)m * a.N + n] = b;
+                    ((__nv_bfloat16*)d.scaled)[(long long)m * a.N + n] = __float2bfloat16_rn(bv * (raw_value(w2[i], d.w2_dtype) + d.off2));
+                }
+                t.x = warp_sum(t.x); t.y = warp_sum(t.y); t.z = warp_sum(t.z); t.w = warp_sum(t.w);
+                if (lane == 0) reinterpret_cast<float4*>(d.sums)[blockIdx.x * 8 + m] = t;        // rows beyond M: zeros
+            }
+        } else if (warp >= 2) {
             const int tid = threadIdx.x - 64, per_tile = a.gated ? MX_ROWS / 2 : MX_ROWS, outs = a.gated ? 2 * a.share : a.share;
             const float* y = reinterpret_cast<const float*>(smem + y_off);
             for (int idx = tid; idx < a.M * a.share; idx += WORKERS) {
                 const int m = idx / a.share, o = idx - m * a.share, of_tile = rank * a.share + o, n = first_tile * per_tile + of_tile;
-                if (of_tile >= per_tile || n >= a.N) continue;
-                const float* ys = y + m * outs + (a.gated ? 2 * o : o);
+                const int src = MODE == RDL_NORM_DEFERRED && a.norm.row_index ? a.norm.row_index[m] : m;
+                if (of_tile >= per_tile || n >= a.N || src < 0 || src >= a.src_rows) continue;
+                const float* ys = y + src * outs + (a.gated ? 2 * o : o);
                 float v[8], u[8];
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {                // all asked for before the first is used
@@ -463,15 +606,19 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
-template <int PARTS, int R>
+template <int PARTS, int R, int MODE = 0>
 int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
     constexpr int NB = PARTS * R, PER_BLOCK = NB * MX_BLOCK + MX_SCALE_BYTES, PER_STAGE = STEP * (MX_TILE_BYTES + MX_SCALE_BYTES);
     const int sms = rdl_sm_count();
+    a.codes = w.codes; a.scales = w.scales;
+    a.N = w.gated ? w.rows / 2 : w.rows; a.K = w.columns;
+    a.blocks = w.blocks; a.gated = w.gated;
+    a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_FEW); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_FEW);
     a.tiles = w.tiles;
     a.split = mx_split(a.tiles, a.blocks, sms);
     a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
     a.slice_blocks = (a.blocks + a.split - 1) / a.split;
-    const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - 1024 - sums;      // alignment, static shared memory
+    const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - (MODE == RDL_NORM_DEFERRED ? 2048 : 1024) - sums;    // alignment, static shared memory
     // The rows of all of a block's columns, if a ring of two stages fits beside them (float32, 8 rows x 2,304, 256,000 outputs: 71 us so and 94
     // with the rows brought anew for every tile; bfloat16, 16 x 3,584, 28,672 gated: 20.5 and 23.0); else as many as fit beside four.
     a.slots = (a.slice_blocks + STEP - 1) / STEP * STEP;
@@ -484,9 +631,9 @@ int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
     const int steps = (a.slice_blocks + STEP - 1) / STEP;
     if ((long long)a.stages > (long long)turns * steps) a.stages = turns * steps;
     const int smem = 1024 + a.slots * PER_BLOCK + a.stages * PER_STAGE + sums;
-    RDL_CUDA((rdl_allow_shared<mx_few_rows_kernel<PARTS, R>>(smem)), "mx_few_rows");
+    RDL_CUDA((rdl_allow_shared<mx_few_rows_kernel<PARTS, R, MODE>>(smem)), "mx_few_rows");
     const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
-    RDL_CHECK_EX(rdl_launch_cluster(mx_few_rows_kernel<PARTS, R>, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, w.codes_map, a), "mx_few_rows");
+    RDL_CHECK_EX(rdl_launch_cluster(mx_few_rows_kernel<PARTS, R, MODE>, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, w.codes_map, a), "mx_few_rows");
     return 0;
 }
 
@@ -505,16 +652,56 @@ extern "C" int rdl_mx_few_rows(void* out, int out_dtype, const void* x, int x_ki
     RDL_REQUIRE(softcap >= 0.f, "mx_few_rows: soft-cap must not be negative");
     FewArgs a{};
     a.x = x; a.row_scales = (const uint8_t*)row_scales;
-    a.codes = w->codes; a.scales = w->scales;
     a.out = out; a.out_dtype = out_dtype;
-    a.M = m; a.N = w->gated ? w->rows / 2 : w->rows; a.K = w->columns;
-    a.blocks = w->blocks; a.row_pad = (m + 3) / 4 * 4;
-    a.gated = w->gated; a.activation = activation; a.act_param = act_param; a.softcap = softcap;
-    a.vec = a.K % 8 == 0 && (uintptr_t)x % 16 == 0;
-    a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_FEW); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_FEW);
+    a.M = a.src_rows = m; a.row_pad = (m + 3) / 4 * 4;
+    a.activation = activation; a.act_param = act_param; a.softcap = softcap;
+    a.vec = w->columns % 8 == 0 && (uintptr_t)x % 16 == 0;
     a.status = status;
     cudaStream_t st = (cudaStream_t)stream;
     if (x_kind == RDL_MX8) return launch<1, 16>(a, *w, st);
     if (x_kind == RDL_BF16) return m <= 8 ? launch<2, 8>(a, *w, st) : launch<2, 16>(a, *w, st);
     return m <= 8 ? launch<6, 8>(a, *w, st) : launch<6, 16>(a, *w, st);
+}
+
+// The partial sums a branch's product writes for each of its rows: one a block; 0: the matrix is not shared by clusters, no such form
+extern "C" int rdl_mx_branch_units(const void* weight) {
+    const Mx4Matrix* w = (const Mx4Matrix*)weight;
+    if (!w || !w->codes || w->gated) return 0;
+    const int split = mx_split(w->tiles, w->blocks, rdl_sm_count());
+    return split > 1 ? w->tiles * split : 0;
+}
+
+extern "C" int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, const void* weight, int m, int activation, float act_param,
+                                    float softcap, const DeferredNormArgs* norm, int* status, void* stream) {
+    const Mx4Matrix* w = (const Mx4Matrix*)weight;
+    RDL_REQUIRE(w && w->codes && x && norm, "mx_few_rows_norm: missing operand");
+    RDL_REQUIRE(m > 0 && m <= 8, "mx_few_rows_norm: %d rows, 1 to 8 are supported", m);
+    RDL_REQUIRE(norm->sums && (uintptr_t)norm->sums % 16 == 0, "mx_few_rows_norm: the partial sums must lie on a 16-byte boundary");
+    FewArgs a{};
+    a.x = x; a.norm = *norm; a.status = status;
+    a.activation = activation; a.act_param = act_param; a.softcap = softcap;
+    a.M = a.src_rows = m;
+    a.vec = w->columns % 8 == 0 && (uintptr_t)x % 16 == 0;
+    if (norm->mode == RDL_NORM_BRANCH) {
+        RDL_REQUIRE(!w->gated && activation == 0 && softcap == 0.f, "mx_few_rows_norm: a branch's product has the plain epilogue");
+        RDL_REQUIRE(norm->residual && norm->w1 && norm->w2 && norm->branch && norm->scaled, "mx_few_rows_norm: a branch needs the stream, both norms' weights and its two outputs");
+        RDL_REQUIRE(rdl_valid_dtype(norm->w1_dtype) && rdl_valid_dtype(norm->w2_dtype), "mx_few_rows_norm: bad dtype of a norm's weight");
+        const int units = rdl_mx_branch_units(weight);
+        RDL_REQUIRE(units > 0 && norm->n_sums == units, "mx_few_rows_norm: place for %d units of sums, the matrix has %d", norm->n_sums, units);
+        return launch<2, 8, RDL_NORM_BRANCH>(a, *w, (cudaStream_t)stream);
+    }
+    RDL_REQUIRE(norm->mode == RDL_NORM_DEFERRED, "mx_few_rows_norm: unknown mode %d", norm->mode);
+    RDL_REQUIRE(out && rdl_valid_dtype(out_dtype), "mx_few_rows_norm: missing output or bad output dtype %d", out_dtype);
+    RDL_REQUIRE(!w->gated || rdl_gated_known(activation), "mx_few_rows_norm: unknown activation %d", activation);
+    RDL_REQUIRE(softcap >= 0.f, "mx_few_rows_norm: soft-cap must not be negative");
+    RDL_REQUIRE(a.vec, "mx_few_rows_norm: the operand needs a multiple of 8 columns and a 16-byte boundary");
+    RDL_REQUIRE(norm->n_sums > 0 && norm->n_out > 0 && norm->n_out <= 8 && (norm->row_index || norm->n_out <= m), "mx_few_rows_norm: %d units of sums, %d output rows", norm->n_sums, norm->n_out);
+    const bool side = norm->residual_out || norm->scaled_next;
+    RDL_REQUIRE(!side || (norm->branch_in && norm->residual_in), "mx_few_rows_norm: the stream's update needs the branch and the stream");
+    // other blocks still read the old one
+    RDL_REQUIRE(!norm->residual_out || norm->residual_out != norm->residual_in, "mx_few_rows_norm: the updated stream needs a buffer of its own");
+    RDL_REQUIRE(!norm->scaled_next || (norm->w_next && rdl_valid_dtype(norm->w_next_dtype)), "mx_few_rows_norm: the next operand needs the next norm's weight");
+    a.out = out; a.out_dtype = out_dtype;
+    a.M = norm->n_out;
+    return m <= 4 ? launch<2, 8, RDL_NORM_DEFERRED>(a, *w, (cudaStream_t)stream) : launch<2, 16, RDL_NORM_DEFERRED>(a, *w, (cudaStream_t)stream);
 }

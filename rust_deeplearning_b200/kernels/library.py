@@ -23,7 +23,7 @@ from concurrent.futures import ThreadPoolExecutor
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(_PKG, "csrc")
 LIB_NAME = "librdl_b200_kernels.so"
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 # fast math is never enabled: the 32-bit path relies on exact tanhf/expf/sqrtf and plain FMA
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -438,6 +438,8 @@ _SIGNATURES = {
     "rdl_mx4_matrix_bytes": [],
     "rdl_mx4_describe": [_P, _P, _P, _I, _I, _I],
     "rdl_mx_few_rows": [_P, _I, _P, _I, _P, _P, _I, _I, _F, _F, _P, _P],
+    "rdl_mx_branch_units": [_P],
+    "rdl_mx_few_rows_norm": [_P, _I, _P, _P, _I, _I, _F, _F, ctypes.POINTER(DeferredNormArgs), _P, _P],
     "rdl_mx_some_rows": [_P, _I, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_mx_many_rows": [_P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_random_normal": [_P, _I, _LL, ctypes.c_ulonglong, ctypes.c_double, _P],

@@ -395,7 +395,8 @@ def _gemm_bf16(x, weight, n_out, out_dtype, gated, activation, softcap, status, 
 # norms are scalings by one number a row and one number a column, so they can be split (the algebra stands in
 # csrc/api.h at DeferredNormArgs): P's epilogue applies the column factors and writes partial sums of squares,
 # C multiplies an operand of 2 x 8 rows (the stream's rows and the branch's rows, both with the second norm's
-# column factors) and applies the row factors in its epilogue.  Three small types carry this through the parts.
+# column factors) and applies the row factors in its epilogue.  Three small types carry this through the parts.  Either product may have a
+# 4-bit weight (`Mx4Weight`); P then has a unit of partial sums a block instead of one for every 16 columns.
 
 DEFERRED_MAX_ROWS = 8
 # A very wide product (the output head) runs for most of its time in its steady state, where multiplying 16 rows
@@ -415,7 +416,7 @@ class BranchSink(NamedTuple):
 
 class Branch:
     """A branch delivered through a BranchSink: a' = y (post.weight + post.offset) [rows, width] in bfloat16,
-    the partial sums [units, 8, 4] and, in the operand's second half (`second_half_row`), a' (then.weight + then.offset)."""
+    the partial sums [units, 8, 4] (their count is the product's) and, in the operand's second half (`second_half_row`), a' (then.weight + then.offset)."""
 
     def __init__(self, sink: BranchSink, values: torch.Tensor, sums: torch.Tensor):
         self.sink, self.values, self.sums = sink, values, sums
@@ -501,8 +502,8 @@ def deferred_ok(rows: int, width: int, dtype: torch.dtype) -> bool:
 
 def linear_branch(x: torch.Tensor, weight: torch.Tensor, sink: Optional[BranchSink], status: Optional[torch.Tensor] = None):
     """x W^T as a branch of a residual stream: a `Branch` where the split form applies, else the plain result."""
-    if type(weight) is Mx4Weight or sink is None or not (_skinny_ok(x, weight) and deferred_ok(x.shape[0], weight.shape[0], x.dtype)
-                            and tuple(sink.residual.shape) == (x.shape[0], weight.shape[0])):
+    if sink is None or not (_branch_ok_mx4(x, weight) if type(weight) is Mx4Weight else _skinny_ok(x, weight)) or not (
+            deferred_ok(x.shape[0], weight.shape[0], x.dtype) and tuple(sink.residual.shape) == (x.shape[0], weight.shape[0])):
         return linear(x, weight, status=status)
     rows, width = x.shape[0], weight.shape[0]
     for p in (sink.post, sink.then):
@@ -510,22 +511,35 @@ def linear_branch(x: torch.Tensor, weight: torch.Tensor, sink: Optional[BranchSi
     _need(sink.operand.dtype is torch.bfloat16 and tuple(sink.operand.shape) == (2 * DEFERRED_MAX_ROWS, width)
           and sink.operand.is_contiguous(), "the sink's operand must be bfloat16 [16, width]")
     values = torch.empty((rows, width), dtype=torch.bfloat16, device=x.device)
-    sums = torch.empty(((width + 15) // 16, 8, 4), dtype=torch.float32, device=x.device)
+    units = weight.branch_units if type(weight) is Mx4Weight else (width + 15) // 16
+    sums = torch.empty((units, 8, 4), dtype=torch.float32, device=x.device)
     d = library.DeferredNormArgs()
     d.mode = library.NORM_BRANCH
-    d.sums = sums.data_ptr()
+    d.sums, d.n_sums = sums.data_ptr(), units
     d.residual = sink.residual.data_ptr()
     d.w1, d.w1_dtype, d.off1 = sink.post.weight.data_ptr(), _dtype_code(sink.post.weight), float(sink.post.offset)
     d.w2, d.w2_dtype, d.off2 = sink.then.weight.data_ptr(), _dtype_code(sink.then.weight), float(sink.then.offset)
     d.branch, d.scaled = values.data_ptr(), sink.operand.data_ptr() + second_half_row(rows) * width * 2
-    library.check(library.load().rdl_gemm_skinny_norm(None, 0, _ptr(x), _ptr(weight), rows, width, x.shape[1], 0, 0, 0.0,
-                                                      ctypes.byref(d), _status(status), 0.0, _stream(x)))
+    if type(weight) is Mx4Weight:
+        library.check(library.load().rdl_mx_few_rows_norm(None, 0, _ptr(x), weight.handle, rows, 0, 0.0, 0.0, ctypes.byref(d), _status(status), _stream(x)))
+    else:
+        library.check(library.load().rdl_gemm_skinny_norm(None, 0, _ptr(x), _ptr(weight), rows, width, x.shape[1], 0, 0, 0.0,
+                                                          ctypes.byref(d), _status(status), 0.0, _stream(x)))
     return Branch(sink, values, sums)
 
 
-def _linear_deferred(x: DeferredRows, weight: torch.Tensor, n_out: int, out_dtype, gated: bool, activation: int, softcap, status, param: float = 0.0):
+def _linear_deferred(x: DeferredRows, weight, n_out: int, out_dtype, gated: bool, activation: int, softcap, status, param: float = 0.0):
     """The product after a deferred norm, or None if this weight cannot take it."""
     width = x.branch.shape[1]
+    if type(weight) is Mx4Weight:
+        if weight.columns != width or weight.gated is not gated or out_dtype not in _KINDS or not 0 < x.shape[0] <= DEFERRED_MAX_ROWS:
+            return None
+        out = torch.empty((x.shape[0], n_out), dtype=out_dtype, device=weight.device)
+        library.check(library.load().rdl_mx_few_rows_norm(_ptr(out), _KINDS[out_dtype], _ptr(x.branch.sink.operand), weight.handle, x.branch.shape[0],
+                                                          activation, float(param), float(softcap or 0.0), ctypes.byref(x._args()), _status(status),
+                                                          _stream(out)))
+        x.consumed = True
+        return out
     if not (weight.dtype is torch.bfloat16 and weight.is_contiguous() and weight.data_ptr() % 16 == 0 and weight.shape[1] == width):
         return None
     if n_out > DEFERRED_MAX_OUTPUTS:
@@ -564,7 +578,7 @@ def linear(x, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
 
     A 4-bit weight (`Mx4Weight`): `linear_mx4`.  Up to 16 rows of a tensor enter as they are, more bfloat16 rows are rounded to 8 bits
     first (`pack_mx8`); x may be rows that are in 8 bits already."""
-    if type(weight) is Mx4Weight:
+    if type(weight) is Mx4Weight and not isinstance(x, DeferredRows):
         return linear_mx4(_rows_for_mx4(x), weight, out_dtype, softcap, status, activation)
     _need(activation is None or (activation in UNARY_FORMS and softcap is None),
           f"linear: activation '{activation}' is not one of {sorted(UNARY_FORMS)} (and comes without a soft-cap)")
@@ -574,6 +588,8 @@ def linear(x, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
         if out is not None:
             return out
         x = x.materialise()
+        if type(weight) is Mx4Weight:
+            return linear_mx4(x, weight, out_dtype, softcap, status, activation)
     _need(x.dim() == 2 and weight.dim() == 2 and x.shape[1] == weight.shape[1],
           f"linear: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not fit")
     _need(x.dtype is weight.dtype, f"linear: input is {x.dtype}, weight is {weight.dtype}")
@@ -602,7 +618,7 @@ def linear_gated(x, weight_gate_up: torch.Tensor, activation: str, status: Optio
     `GATED_FORMS` (param: its parameter).
     In bfloat16 this is one kernel (the activation is the product's epilogue); otherwise a product
     and the gated activation kernel.  A 4-bit weight: as in `linear`; rows in 8 bits give a result in 8 bits, for the product behind."""
-    if type(weight_gate_up) is Mx4Weight:
+    if type(weight_gate_up) is Mx4Weight and not isinstance(x, DeferredRows):
         x = _rows_for_mx4(x)
         return linear_gated_mx4(x, weight_gate_up, activation, param, type(x) is Mx8Rows, status)
     _need(activation in GATED_FORMS, f"unknown activation '{activation}', known: {sorted(GATED_FORMS)}")
@@ -612,6 +628,8 @@ def linear_gated(x, weight_gate_up: torch.Tensor, activation: str, status: Optio
         if out is not None:
             return out
         x = x.materialise()
+        if type(weight_gate_up) is Mx4Weight:
+            return linear_gated_mx4(x, weight_gate_up, activation, param, False, status)
     if _own_bf16_kernel(x, weight_gate_up):
         return _gemm_bf16(x, weight_gate_up, weight_gate_up.shape[0] // 2, x.dtype, True, GATED_FORMS[activation], None, status, param)
     return gated_activation(linear(x, weight_gate_up), activation, param)
@@ -1835,6 +1853,7 @@ class Mx4Weight:
         self._host = ctypes.create_string_buffer(lib.rdl_mx4_matrix_bytes() + 64)
         self.handle = -(-ctypes.addressof(self._host) // 64) * 64
         library.check(lib.rdl_mx4_describe(self.handle, self.codes.data_ptr(), self._scales.data_ptr(), self.rows, self.columns, int(self.gated)), 0)
+        self.branch_units = lib.rdl_mx_branch_units(self.handle)     # of partial sums, as the last product of a branch (0: no such form)
 
     def first(self, rows: int) -> "Mx4Weight":
         """The weight's first rows as a weight of their own, on the same memory."""
@@ -2050,10 +2069,14 @@ def _product_mx4(x, weight: Mx4Weight, gated: bool, out_dtype, out_mx8: bool, ac
     return norm_mx8(out) if out_mx8 else out
 
 
+def _branch_ok_mx4(x, weight: Mx4Weight) -> bool:
+    """Whether a few-row product with a 4-bit weight can deliver a branch of the stream in the split form."""
+    return (weight.branch_units > 0 and type(x) is torch.Tensor and x.dim() == 2 and x.shape[1] == weight.columns and x.is_contiguous()
+            and x.device == weight.device)
+
+
 def _rows_for_mx4(x):
     """What `linear` hands a 4-bit weight: many bfloat16 rows in 8 bits, everything else as it is."""
-    if isinstance(x, DeferredRows):
-        x = x.materialise()
     if type(x) is not Mx8Rows and x.dtype is torch.bfloat16 and x.shape[0] > MX_FEW_ROWS:
         x = pack_mx8(x)
     return x

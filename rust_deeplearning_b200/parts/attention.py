@@ -42,7 +42,7 @@ with max(head_dim, value_dim) values, the padding made by zero rows of the produ
 W_o), so that scores and outputs are unchanged and no kernel needs to know.
 Optional offers for the split form of the norms around few-row products (`parts/norm.py`):
 `takes_deferred_rows` (x may be `ops.DeferredRows`) and `delivers_branch` (forward takes `sink`).  `use_mx4()`: the projections go to
-4 bits (`ops.Mx4Weight`); the mixer then says `takes_mx8_rows` (x may be `ops.Mx8Rows`) and gives up the split form.
+4 bits (`ops.Mx4Weight`); the mixer then says `takes_mx8_rows` (x may be `ops.Mx8Rows`).
 """
 from __future__ import annotations
 
@@ -298,7 +298,7 @@ class Attention:
         self.w_qkv, self.w_o = ops.pack_mx4(self.w_qkv), ops.pack_mx4(self.w_o)
         if not self.extended:
             self.w_q = self.w_qkv.first(self.q_width)
-        self.takes_deferred_rows = self.delivers_branch = False
+        self.delivers_branch = self.delivers_branch and self.w_o.branch_units > 0
         self.takes_mx8_rows = not self.extended
         return 2
 

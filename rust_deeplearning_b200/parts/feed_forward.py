@@ -10,7 +10,7 @@ independent of each other, so packing and batching never concern it.  Two option
 form of the norms around few-row products (`parts/norm.py`): `takes_deferred_rows` (x may be
 `ops.DeferredRows`; it goes into `ops.linear` / `ops.linear_gated` only) and `delivers_branch` (forward takes
 `sink` and ends in `ops.linear_branch`).  `use_mx4()`: the part's matrices go to 4 bits (`ops.Mx4Weight`); it then says
-`takes_mx8_rows` (x may be `ops.Mx8Rows`) and gives up the split form.
+`takes_mx8_rows` (x may be `ops.Mx8Rows`).
 """
 from __future__ import annotations
 
@@ -36,7 +36,7 @@ class GatedMLP:
     def use_mx4(self) -> int:
         """The matrices in 4 bits from now on; how many."""
         self.w_gate_up, self.w_down = ops.pack_mx4(self.w_gate_up, gated=True), ops.pack_mx4(self.w_down)
-        self.takes_deferred_rows = self.delivers_branch = False
+        self.delivers_branch = self.w_down.branch_units > 0
         self.takes_mx8_rows = True
         return 2
 
@@ -65,7 +65,7 @@ class PlainMLP:
 
     def use_mx4(self) -> int:
         self.w_up, self.w_down = ops.pack_mx4(self.w_up), ops.pack_mx4(self.w_down)
-        self.takes_deferred_rows = self.delivers_branch = False
+        self.delivers_branch = self.w_down.branch_units > 0
         self.takes_mx8_rows = True
         return 2
 

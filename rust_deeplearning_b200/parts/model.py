@@ -66,7 +66,6 @@ class LinearHead:
 
     def use_mx4(self) -> int:
         self.weight = ops.pack_mx4(self.weight)
-        self.takes_deferred_rows = False
         return 1
 
     def forward(self, n) -> torch.Tensor:

@@ -237,6 +237,118 @@ def test_more_rows_of_a_tensor(kind):
     check(ops.linear_mx4(x, w, out_dtype=torch.float32), x64 @ w64.T, sum_tolerance(x64, w64, kind), "rows")
 
 
+def norm64(v, p):
+    w = f64(p.weight) + p.offset
+    return v / np.sqrt((v ** 2).mean(-1, keepdims=True) + p.eps) * w
+
+
+@pytest.mark.parametrize("m", [1, 4, 8])
+@pytest.mark.parametrize("width,k_in,n_out", [(2304, 2048, 4096), (1000, 1101, 20003), (3584, 520, 600), (640, 4608, 131)])
+def test_deferred_norms(m, width, k_in, n_out):
+    """A branch's product and the product behind the two norms that follow it, without a kernel between, and each of the two with a
+    bfloat16 weight on the other side.
+
+    The tolerance follows the roundings to bfloat16, each 2^-8 of what is rounded: the branch times its column factors, both halves of the
+    operand, the row that goes into parts; the row factors move by what the branch's rounding adds to the stream's norm."""
+    x, x64 = rows_for(m, k_in, "bfloat16", 50)
+    if m > 2:
+        x[m // 2] = 1.0
+        x64 = f64(x)
+    w_p, w_c = ops.pack_mx4(rnd((width, k_in), torch.float32, 51, 0.2)), ops.pack_mx4(rnd((n_out, width), torch.float32, 52, 0.2))
+    w_gu = ops.pack_mx4(rnd((2 * 72, width), torch.float32, 53, 0.1), gated=True)
+    p64, c64, gu64 = (f64(ops.expand_mx4(w, torch.float32)) for w in (w_p, w_c, w_gu))
+    h = rnd((m, width), torch.float32, 54, 2.0)
+    post = ops.NormParams(rnd((width,), torch.bfloat16, 55, 0.5), 1e-5, 1.0)
+    then = ops.NormParams(rnd((width,), torch.float32, 56, 0.5), 1e-6, 0.0)
+    nxt = ops.NormParams(rnd((width,), torch.bfloat16, 57, 0.5), 1e-6, 1.0)
+    h64, g1, g2, g3 = f64(h), f64(post.weight) + 1.0, f64(then.weight), f64(nxt.weight) + 1.0
+    y = x64 @ p64.T
+    added = norm64(y, post)
+    new = h64 + added
+    rows = norm64(new, then)
+    z = rows @ c64.T
+    s1 = 1 / np.sqrt((y ** 2).mean(-1, keepdims=True) + post.eps)
+    s2 = 1 / np.sqrt((new ** 2).mean(-1, keepdims=True) + then.eps)
+    float_y = s1 * np.abs(g1) * sum_tolerance(x64, p64, "bfloat16")
+    h_tol = np.abs(added) * (2.0 ** -8 + 2.0 ** -18) + float_y + 2.0 ** -22 * (np.abs(h64) + np.abs(new))
+    moved = np.linalg.norm(h_tol, axis=-1, keepdims=True) / np.linalg.norm(new, axis=-1, keepdims=True) + 2.0 ** -16
+    x_tol = s2 * np.abs(g2) * (np.abs(h64) * 2.0 ** -8 + np.abs(added) * (2.0 ** -7 + 2.0 ** -15) + float_y) + np.abs(rows) * (2.0 ** -8 + moved) * (1 + 2.0 ** -7)
+    z_tol = x_tol @ np.abs(c64).T + sum_tolerance(rows, c64, "bfloat16")
+    bf16 = lambda want, tol: tol + (np.abs(want) + tol) * 2.0 ** -8
+
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    bf_p, bf_c = ops.expand_mx4(w_p), ops.expand_mx4(w_c)                # the same values: 4 bits and a power of two are exact in bfloat16
+    for wp, wc in ((w_p, w_c), (bf_p, w_c), (w_p, bf_c)):
+        if type(wp) is torch.Tensor and k_in % 8:
+            continue                                                     # the bfloat16 kernels' rule
+        operand = ops.scaled_rows(h, then)
+        branch = ops.linear_branch(x, wp, ops.BranchSink(h, post, then, operand), status=status)
+        assert isinstance(branch, ops.Branch)
+        h_out, next_operand = torch.empty_like(h), torch.empty_like(operand)
+        d = ops.DeferredRows(branch, h_out, nxt, next_operand)
+        check(ops.linear(d, wc, status=status), z, bf16(z, z_tol), "product")
+        assert d.consumed
+        check(h_out, new, h_tol, "stream")
+        check(next_operand[:m], new * g3, np.abs(g3) * h_tol + np.abs(new * g3) * (2.0 ** -8 + 2.0 ** -15), "next operand")
+        if wc is w_c:
+            check(ops.linear(d, w_c, out_dtype=torch.float32, softcap=3.0, status=status), 3.0 * np.tanh(z / 3.0), z_tol + 2.0 ** -18, "soft-cap")
+            v = rows @ gu64.T
+            g, u = np.split(np.abs(v), 2, axis=-1)
+            t = x_tol @ np.abs(gu64).T + sum_tolerance(rows, gu64, "bfloat16")
+            check(ops.linear_gated(d, w_gu, "silu", status=status), plain.gated(v, "silu", 0.0),
+                  2 * (g + u + 1 + t[:, :72] + t[:, 72:]) * (t[:, :72] + t[:, 72:]) + 2.0 ** -10 * np.maximum(g, 1) * (u + 1) + 2.0 ** -8 * g * u, "gated")
+            chosen = torch.tensor([m - 1, 0], dtype=torch.int32, device=DEV)
+            h_out2 = torch.empty_like(h)
+            d2 = ops.DeferredRows(branch, h_out2, row_index=chosen)
+            check(ops.linear(d2, w_c, status=status), z[[m - 1, 0]], bf16(z, z_tol)[[m - 1, 0]], "chosen rows")
+            assert torch.equal(h_out2, h_out)
+        d3 = ops.DeferredRows(branch, torch.empty_like(h), nxt, torch.empty_like(operand))
+        check(d3.materialise(), rows, x_tol, "materialised")
+    assert status.item() == 0
+
+
+def test_deferred_norms_keep_rows_apart():
+    """A row that is not finite reaches its own results only; the others have the same bits without it."""
+    m, width = 5, 512
+    x, h = rnd((m, 1024), torch.bfloat16, 60), rnd((m, width), torch.float32, 61)
+    w_p, w_c = ops.pack_mx4(rnd((width, 1024), torch.float32, 62)), ops.pack_mx4(rnd((300, width), torch.float32, 63))
+    norm = ops.NormParams(rnd((width,), torch.bfloat16, 64, 0.5), 1e-6, 1.0)
+
+    def run():
+        operand = ops.scaled_rows(h, norm)
+        branch = ops.linear_branch(x, w_p, ops.BranchSink(h, norm, norm, operand))
+        out = torch.empty_like(h)
+        return ops.linear(ops.DeferredRows(branch, out, norm, torch.empty_like(operand)), w_c, out_dtype=torch.float32), out
+
+    clean = run()
+    x[3, 5] = float("inf")
+    h[1, 7] = float("nan")
+    for got, want in zip(run(), clean):
+        assert torch.equal(got[[0, 2, 4]], want[[0, 2, 4]])
+    z, out = run()
+    assert z[1].isnan().all() and z[3].isnan().all() and out[1, 7].isnan()
+
+
+def test_no_split_form_of_a_branch():
+    """A matrix that no clusters share, and a gated one, say so; the plain result is delivered."""
+    w = ops.pack_mx4(rnd((64, 64), torch.float32, 65))
+    assert w.branch_units == 0 and ops.pack_mx4(rnd((512, 1024), torch.float32, 65), gated=True).branch_units == 0
+    h, norm = rnd((2, 64), torch.float32, 66), ops.NormParams(rnd((64,), torch.bfloat16, 67), 1e-6, 1.0)
+    x = rnd((2, 64), torch.bfloat16, 68)
+    got = ops.linear_branch(x, w, ops.BranchSink(h, norm, norm, ops.scaled_rows(h, norm)))
+    assert torch.equal(got, ops.linear_mx4(x, w))
+    lib, d = library.load(), library.DeferredNormArgs()
+    d.mode, d.sums, d.n_sums = library.NORM_DEFERRED, torch.zeros(64, device=DEV).data_ptr(), 2
+    for rows, cap, n_out, text in ((0, 0.0, 1, "1 to 8"), (9, 0.0, 1, "1 to 8"), (2, -1.0, 2, "soft-cap"), (2, 0.0, 9, "9 output rows"), (2, 0.0, 3, "3 output rows")):
+        d.n_out = n_out
+        with pytest.raises(library.KernelError, match=text):
+            library.check(lib.rdl_mx_few_rows_norm(h.data_ptr(), 0, x.data_ptr(), w.handle, rows, 0, 0.0, cap, d, None, None))
+    d.mode = library.NORM_BRANCH
+    d.residual = d.w1 = d.w2 = d.branch = d.scaled = h.data_ptr()
+    with pytest.raises(library.KernelError, match="units of sums"):
+        library.check(lib.rdl_mx_few_rows_norm(None, 0, x.data_ptr(), w.handle, 2, 0, 0.0, 0.0, d, None, None))
+
+
 @pytest.mark.parametrize("act", ["gelu_pytorch_tanh", "silu", "swish_limit"])
 @pytest.mark.parametrize("m,n,k,kind", [(1, 1, 32, "bfloat16"), (7, 37, 300, "bfloat16"), (16, 100, 5000, "float32"), (9, 64, 128, "mx8"), (17, 65, 128, "mx8"),
                                         (140, 190, 1003, "mx8"), (64, 33, 40, "mx8")])
