@@ -18,8 +18,9 @@
 // form's tile is 128 gate and 128 up rows of the same 128 outputs; its result may leave as 8-bit rows with scales: 32 outputs of a
 // row lie in one thread, which is a group.
 //
-// Measured: gate and up of the 2B shape, 2,048 rows to 8 bits, 62.1 us, 2.8 PFLOP/s; 8,192 rows x 36,864 x 4,608 outputs 895 us, 3.1 PFLOP/s.
-// The tensor cores bound it: what a block of columns takes is the same in both, and longer than at full clock, which the power limit takes away.
+// Measured: gate and up of the 2B shape, 2,048 rows to 8 bits, 58.2 us, 3.0 PFLOP/s; 8,192 rows x 36,864 x 4,608 outputs 884 us, 3.15 PFLOP/s.
+// The tensor cores bound it: 530 cycles a block of columns, of which the products take 513, at the clock that the power limit leaves; between
+// two tiles they wait 1,100 cycles, from their end until the accumulator is in registers.
 //
 // Every wait is bounded; a block that gives up sets `status` and every path ends in the common tear-down.
 #include "activations.cuh"
@@ -96,7 +97,9 @@ __device__ __forceinline__ uint32_t map_to_block(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+// Relaxed: what it orders, this warp's reads of tensor memory, has completed before (tcgen05.wait::ld), and no memory is handed over.  A
+// release at cluster scope cost 1,750 cycles from the last read to the next product, and this 250.
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory"); }
 // 16 accumulator columns of the warp's lanes, as bits; there after mx_tmem_wait_ld
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
