@@ -191,10 +191,10 @@ __device__ __forceinline__ int make_parts(const Chunk<PARTS>& d, uint2 (&bytes)[
 template <int PARTS, int R, int MODE>
 __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs a) {
     constexpr int NB = PARTS * R;                            // columns of the product: part p of row m is column p R + m
-    constexpr int PIECES = STEP * (R / 8);                   // of a group of STEP blocks: eight rows of a block each
     constexpr int X_BLOCK = NB * MX_BLOCK;                   // bytes of a block of 128 columns of the rows
     constexpr int TMEM_COLS = 2 * NB + SCALE_BUFS * 8 <= 128 ? 128 : 256;
-    constexpr int AHEAD = PARTS == 6 ? 2 : 4;                // chunks a lane asks for before it works on the first
+    constexpr int AHEAD = PARTS == 6 ? 2 : 4;                // chunks a lane asks for before it works on the first: two rows each
+    constexpr int PIECE_ROWS = 2 * AHEAD, PIECES = STEP * (R / PIECE_ROWS);              // pieces of a group of STEP blocks
     // behind a deferred norm four of the workers see to the sums and to the stream; the others make parts (of 18 blocks of 16 rows, three
     // pieces each, as sixteen would)
     constexpr int SIDE = MODE == RDL_NORM_DEFERRED ? 4 : 0, TAKERS = WORKERS / 32 - SIDE;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         const uint32_t my_scale = xs_s + (uint32_t)((lane >> 4) * 16 + ((lane & 15) >> 2));
         // behind a deferred norm the rows are the operand's: R / 2 of the stream, R / 2 of the branch, the first src_rows of each in use
         auto used_row = [&](int r) { return MODE != RDL_NORM_DEFERRED || (r & (R / 2 - 1)) < a.src_rows; };
-        // The rows of tile `turn` of this block: warps take pieces in turn, eight rows of a block of columns each, and hand them over; the
+        // The rows of tile `turn` of this block: warps take pieces in turn, PIECE_ROWS rows of a block of columns, and hand them over; the
         // products begin with the first STEP blocks.  Where the rows do not stay, a piece waits until its slot has been read.  The pieces
         // are counted on over the tiles, and there are no more warps at it than a round over the slots has pieces: so a warp's next piece
         // is at most one round on, and the phase of its slot's barrier before the one that it waits for is over.
@@ -327,17 +327,15 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             for (int p = before + ((warp - 2 - before % takers + takers) % takers); p < before + pieces; p += takers) {
                 const int nth = p / PIECES, piece = p - before, gi = piece / PIECES, round = nth / x_groups, gs = nth - round * x_groups;
                 if (round > 0 && !resident && !mx_bar_wait(mx_smem(&x_free[gs]), (round - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
-                const int j = piece % PIECES / (R / 8), first = piece % (R / 8) * 8, block = b0 + gi * STEP + j, slot = gs * STEP + j;
-                const int chunks = block < b1 ? min((MODE == RDL_NORM_DEFERRED ? R : a.M) - first, 8) * (MX_BLOCK / 8) : 0;
+                const int j = piece % PIECES / (R / PIECE_ROWS), first = piece % (R / PIECE_ROWS) * PIECE_ROWS, block = b0 + gi * STEP + j, slot = gs * STEP + j;
+                const int chunks = block < b1 ? min((MODE == RDL_NORM_DEFERRED ? R : a.M) - first, PIECE_ROWS) * (MX_BLOCK / 8) : 0;     // 16 a row
                 const uint32_t at = my_place + (uint32_t)(slot * X_BLOCK + first * 128), sc_at = my_scale + (uint32_t)(slot * MX_SCALE_BYTES + first * 16);
                 uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
-#pragma unroll
-                for (int c0 = 0; c0 < 8 * (MX_BLOCK / 8); c0 += 32 * AHEAD) {
-                    if (c0 >= chunks) break;
+                if (chunks > 0) {
                     Chunk<PARTS> d[AHEAD];
 #pragma unroll
                     for (int u = 0; u < AHEAD; ++u) {
-                        const int i = c0 + u * 32 + lane;                            // 16 chunks a row
+                        const int i = u * 32 + lane;
 #pragma unroll
                         for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
                         d[u].code = 0;
@@ -345,16 +343,16 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                     }
 #pragma unroll 1                                                                     // short code: see the head of the file
                     for (int u = 0; u < AHEAD; ++u) {
-                        const int m0 = c0 / 16 + u * 2;                              // this lane's row: m0 or m0 + 1
-                        if (c0 + u * 32 >= chunks) break;                            // none of this warp's
+                        const int m0 = u * 2;                                        // this lane's row of the piece: m0 or m0 + 1
+                        if (u * 32 >= chunks) break;                                 // none of this warp's
                         if (MODE == RDL_NORM_DEFERRED && !used_row(first + m0)) { shift(d); continue; }
                         uint2 bytes[PARTS];
                         uint32_t code[PARTS];
                         const int kind = make_parts<PARTS>(d[0], bytes, code);
                         shift(d);
-                        if (c0 + u * 32 + lane < chunks) {
-                            // swizzled by the row: rows m0 and m0 + 1 of eight flip the pieces by m0 & 6 beside what my_place has of the lane's own
-                            const uint32_t to = (at ^ (uint32_t)((m0 & 6) << 4)) + (uint32_t)((m0 >> 3) * 1024 + (m0 & 6) * 128);
+                        if (u * 32 + lane < chunks) {
+                            // swizzled by the row: rows r and r + 1, r even, flip the pieces by r & 6 beside what my_place has of the lane's own
+                            const uint32_t to = (at ^ (uint32_t)(((first + m0) & 6) << 4)) + (uint32_t)(m0 * 128);
 #pragma unroll
                             for (int part = 0; part < PARTS; ++part)
                                 asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (uint32_t)(part * R * 128)), "r"(bytes[part].x), "r"(bytes[part].y) : "memory");
