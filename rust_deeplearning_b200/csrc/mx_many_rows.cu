@@ -299,7 +299,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx_many_rows_kernel(const __grid_c
                     y[i] = __uint_as_float(v[r]);
                     u[i] = GATED ? __uint_as_float(v[(r + 16) & 63]) : 0.f;
                 }
-                finish<GATED>(a, y, u);
+                // rows that are not there are zeros, and zeros take the long way through a division: 64 rows of 128, 256,000 capped
+                // outputs took 159 us with their epilogue and take 90 without
+                if (m < a.M) finish<GATED>(a, y, u);
                 if (a.out_kind == RDL_MX8) {
                     if (m < a.M) store_group(a, m, n, y);
                     continue;
