@@ -455,6 +455,7 @@ int rdl_mx_few_rows(void* out, int out_dtype, const void* x, int x_kind, const v
 // The same with one side of a deferred norm (DeferredNormArgs; bfloat16 rows, 1 to 8 of them).  A branch's product (no epilogue; not a
 // gated matrix) writes rdl_mx_branch_units(weight) units of sums, the count of which norm->n_sums repeats; 0: this matrix has no such form.
 int rdl_mx_branch_units(const void* weight);
+int rdl_mx_deferred_rows(const void* weight);      // up to how many rows the product behind a deferred norm pays
 int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, const void* weight, int m, int activation, float act_param, float softcap,
                          const DeferredNormArgs* norm, int* status, void* stream);
 // the same for up to 128 rows of 8 bits

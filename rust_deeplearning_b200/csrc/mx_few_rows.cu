@@ -35,7 +35,7 @@
 namespace {
 
 // A stage of the ring is STEP blocks of columns: a stage costs the issuing thread a wait beside its products, about as long as those of a block.
-constexpr int WORKERS = 512, THREADS = 64 + WORKERS, MAX_STAGES = 8, STEP = 2, SCALE_BUFS = 4, MAX_SLOTS = 64;
+constexpr int WORKERS = 512, THREADS = 64 + WORKERS, MAX_STAGES = 8, STEP = 2, SCALE_BUFS = 4, MAX_SLOTS = 64, AHEAD_L2 = 4;
 
 struct FewArgs {
     const void* x; const uint8_t* row_scales;
@@ -59,6 +59,9 @@ __device__ __forceinline__ void tma_codes(uint32_t dst, const CUtensorMap* map, 
 __device__ __forceinline__ void bulk_scales(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, unsigned long long policy) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void ask_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
@@ -247,6 +250,23 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
             int s = 0, piece = first_tile * a.blocks + b0;   // place in the ring; block of columns over all tiles
             uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
+            // A short ring keeps too few bytes on their way: L2 is asked for what will be loaded up to AHEAD_L2 stages later (16 rows x 3,584,
+            // 28,672 gated outputs, two stages: 24.9 -> 21.8 us; with five stages it costs: 1 row x 2,304, 18,432 outputs 7.1 -> 8.1).
+            int ask_tile = a.stages < 4 ? first_tile : a.tiles, ask_kb = b0, asked = 0;
+            auto ask = [&]() {
+                if (ask_tile >= a.tiles || b0 >= b1) return;
+                const int n = min(STEP, b1 - ask_kb);
+                const long long at = (long long)ask_tile * a.blocks + ask_kb;
+                if (asked >= a.stages) {
+                    ask_l2(a.codes + at * (MX_ROWS * MX_BLOCK / 2), (uint32_t)n * (MX_ROWS * MX_BLOCK / 2));
+                    ask_l2(a.scales + at * MX_SCALE_BYTES, (uint32_t)n * MX_SCALE_BYTES);
+                }
+                ++asked;
+                ask_kb += n;
+                if (ask_kb >= b1) { ask_kb = b0; ask_tile += tile_step; }
+            };
+#pragma unroll 1
+            for (int i = 0; i < a.stages + AHEAD_L2; ++i) ask();
             for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, piece += (tile_step - 1) * a.blocks + (a.blocks - (b1 - b0))) {
                 for (int kb = b0; kb < b1;) {
                     const int n = min(STEP, b1 - kb);
@@ -258,6 +278,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                         if (j < n) tma_codes(at + (uint32_t)(j * MX_TILE_BYTES), &map_w, (piece + j) * MX_ROWS, full, policy);
                     bulk_scales(ws_s + (uint32_t)(s * STEP * MX_SCALE_BYTES), a.scales + (long long)piece * MX_SCALE_BYTES, (uint32_t)n * MX_SCALE_BYTES, full, policy);
                     extra = 0;
+                    ask();
                     kb += n;
                     piece += n;
                     if (++s == a.stages) { s = 0; parity ^= 1; }
@@ -604,14 +625,12 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
-template <int PARTS, int R, int MODE = 0>
-int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
+// How a product is divided and what shared memory holds; returns its bytes.
+template <int PARTS, int R, int MODE>
+int plan(FewArgs& a, const Mx4Matrix& w) {
     constexpr int NB = PARTS * R, PER_BLOCK = NB * MX_BLOCK + MX_SCALE_BYTES, PER_STAGE = STEP * (MX_TILE_BYTES + MX_SCALE_BYTES);
     const int sms = rdl_sm_count();
-    a.codes = w.codes; a.scales = w.scales;
-    a.N = w.gated ? w.rows / 2 : w.rows; a.K = w.columns;
     a.blocks = w.blocks; a.gated = w.gated;
-    a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_FEW); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_FEW);
     a.tiles = w.tiles;
     a.split = mx_split(a.tiles, a.blocks, sms);
     a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
@@ -628,7 +647,17 @@ int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
     const int turns = a.split > 1 ? 1 : (a.tiles + sms - 1) / sms;
     const int steps = (a.slice_blocks + STEP - 1) / STEP;
     if ((long long)a.stages > (long long)turns * steps) a.stages = turns * steps;
-    const int smem = 1024 + a.slots * PER_BLOCK + a.stages * PER_STAGE + sums;
+    return 1024 + a.slots * PER_BLOCK + a.stages * PER_STAGE + sums;
+}
+// the rows of a block are made ready once, not again for every tile
+bool once(const FewArgs& a) { return a.slots >= a.slice_blocks || a.split > 1 || a.tiles <= rdl_sm_count(); }
+
+template <int PARTS, int R, int MODE = 0>
+int launch(FewArgs a, const Mx4Matrix& w, cudaStream_t st) {
+    a.codes = w.codes; a.scales = w.scales;
+    a.N = w.gated ? w.rows / 2 : w.rows; a.K = w.columns;
+    a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_MX_FEW); a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_MX_FEW);
+    const int smem = plan<PARTS, R, MODE>(a, w), sms = rdl_sm_count();
     RDL_CUDA((rdl_allow_shared<mx_few_rows_kernel<PARTS, R, MODE>>(smem)), "mx_few_rows");
     const int grid = a.split > 1 ? a.tiles * a.split : (a.tiles < sms ? a.tiles : sms);
     RDL_CHECK_EX(rdl_launch_cluster(mx_few_rows_kernel<PARTS, R, MODE>, dim3(grid), dim3(THREADS), a.split, (size_t)smem, st, w.codes_map, a), "mx_few_rows");
@@ -667,6 +696,19 @@ extern "C" int rdl_mx_branch_units(const void* weight) {
     if (!w || !w->codes || w->gated) return 0;
     const int split = mx_split(w->tiles, w->blocks, rdl_sm_count());
     return split > 1 ? w->tiles * split : 0;
+}
+
+// Up to how many rows the product behind a deferred norm pays.  Above 4 rows its operand has 16; where those have to be made ready again for
+// every tile the norm is better off in a kernel of its own (8 rows x 4,608, 36,864 gated outputs: 63 us against 35 and 5 for the norm; 1 row
+// 34 against 33 and 5).
+extern "C" int rdl_mx_deferred_rows(const void* weight) {
+    const Mx4Matrix* w = (const Mx4Matrix*)weight;
+    if (!w || !w->codes) return 0;
+    FewArgs a{};
+    plan<2, 16, RDL_NORM_DEFERRED>(a, *w);
+    if (once(a)) return 8;
+    plan<2, 8, RDL_NORM_DEFERRED>(a, *w);
+    return once(a) ? 4 : 0;
 }
 
 extern "C" int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, const void* weight, int m, int activation, float act_param,

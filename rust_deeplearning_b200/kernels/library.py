@@ -439,6 +439,7 @@ _SIGNATURES = {
     "rdl_mx4_describe": [_P, _P, _P, _I, _I, _I],
     "rdl_mx_few_rows": [_P, _I, _P, _I, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_mx_branch_units": [_P],
+    "rdl_mx_deferred_rows": [_P],
     "rdl_mx_few_rows_norm": [_P, _I, _P, _P, _I, _I, _F, _F, ctypes.POINTER(DeferredNormArgs), _P, _P],
     "rdl_mx_some_rows": [_P, _I, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_mx_many_rows": [_P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P, _P],

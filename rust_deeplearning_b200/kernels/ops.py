@@ -532,7 +532,8 @@ def _linear_deferred(x: DeferredRows, weight, n_out: int, out_dtype, gated: bool
     """The product after a deferred norm, or None if this weight cannot take it."""
     width = x.branch.shape[1]
     if type(weight) is Mx4Weight:
-        if weight.columns != width or weight.gated is not gated or out_dtype not in _KINDS or not 0 < x.shape[0] <= DEFERRED_MAX_ROWS:
+        if (weight.columns != width or weight.gated is not gated or out_dtype not in _KINDS or not 0 < x.shape[0] <= DEFERRED_MAX_ROWS
+                or x.branch.shape[0] > weight.deferred_rows):
             return None
         out = torch.empty((x.shape[0], n_out), dtype=out_dtype, device=weight.device)
         library.check(library.load().rdl_mx_few_rows_norm(_ptr(out), _KINDS[out_dtype], _ptr(x.branch.sink.operand), weight.handle, x.branch.shape[0],
@@ -1854,6 +1855,7 @@ class Mx4Weight:
         self.handle = -(-ctypes.addressof(self._host) // 64) * 64
         library.check(lib.rdl_mx4_describe(self.handle, self.codes.data_ptr(), self._scales.data_ptr(), self.rows, self.columns, int(self.gated)), 0)
         self.branch_units = lib.rdl_mx_branch_units(self.handle)     # of partial sums, as the last product of a branch (0: no such form)
+        self.deferred_rows = lib.rdl_mx_deferred_rows(self.handle)   # up to how many rows it is worth taking behind a deferred norm
 
     def first(self, rows: int) -> "Mx4Weight":
         """The weight's first rows as a weight of their own, on the same memory."""

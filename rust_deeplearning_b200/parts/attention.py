@@ -299,6 +299,7 @@ class Attention:
         if not self.extended:
             self.w_q = self.w_qkv.first(self.q_width)
         self.delivers_branch = self.delivers_branch and self.w_o.branch_units > 0
+        self.deferred_rows = self.w_qkv.deferred_rows
         self.takes_mx8_rows = not self.extended
         return 2
 

@@ -7,7 +7,7 @@ row-concatenated matrices; the activation and the product with `up` run in float
 
 Interface of a feed-forward: `forward(x [rows, hidden] normed) -> [rows, hidden]`.  Rows are
 independent of each other, so packing and batching never concern it.  Two optional offers, for the split
-form of the norms around few-row products (`parts/norm.py`): `takes_deferred_rows` (x may be
+form of the norms around few-row products (`parts/norm.py`): `takes_deferred_rows` (up to `deferred_rows` rows, where a part names a number; x may be
 `ops.DeferredRows`; it goes into `ops.linear` / `ops.linear_gated` only) and `delivers_branch` (forward takes
 `sink` and ends in `ops.linear_branch`).  `use_mx4()`: the part's matrices go to 4 bits (`ops.Mx4Weight`); it then says
 `takes_mx8_rows` (x may be `ops.Mx8Rows`).
@@ -36,6 +36,7 @@ class GatedMLP:
     def use_mx4(self) -> int:
         """The matrices in 4 bits from now on; how many."""
         self.w_gate_up, self.w_down = ops.pack_mx4(self.w_gate_up, gated=True), ops.pack_mx4(self.w_down)
+        self.deferred_rows = self.w_gate_up.deferred_rows
         self.delivers_branch = self.w_down.branch_units > 0
         self.takes_mx8_rows = True
         return 2
@@ -65,6 +66,7 @@ class PlainMLP:
 
     def use_mx4(self) -> int:
         self.w_up, self.w_down = ops.pack_mx4(self.w_up), ops.pack_mx4(self.w_down)
+        self.deferred_rows = self.w_up.deferred_rows
         self.delivers_branch = self.w_down.branch_units > 0
         self.takes_mx8_rows = True
         return 2

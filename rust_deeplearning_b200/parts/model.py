@@ -309,6 +309,9 @@ class Model:
             packed += self.head.use_mx4() if hasattr(self.head, "use_mx4") else 0
         if weight_format is not None and packed == 0:
             raise ValueError(f"{spec.architecture}: none of its parts keeps its matrices in 4 bits")
+        # rows up to which the split form of the norms is used: as many as pay for every part
+        self.deferred_rows = min((getattr(p, "deferred_rows", ops.DEFERRED_MAX_ROWS) for b in self.layers
+                                  for p in (getattr(b, "mixer", None), getattr(b, "feed_forward", None))), default=ops.DEFERRED_MAX_ROWS)
         self.schedule = list(spec.schedule)
         # what joins the stream before a run: (whether the embedded rows do, a float32 vector or None)
         self.entries = {e: (s.enters.embedding, None if s.enters.vectors is None else
@@ -352,6 +355,7 @@ class Model:
         embedded = self.embedding.forward(batch.tokens, tok_pos=batch.tok_pos) if takes_positions else self.embedding.forward(batch.tokens)
         # rows that join the stream again later stay as they are: an entry before the first run forms its sum elsewhere
         stream = self.start_stream(embedded.clone() if self.keeps_embedding and 0 not in self.entries else embedded)
+        stream.deferred_rows = self.deferred_rows
         batch.deferred_writes.clear()
         lazy_head = getattr(self.head, "takes_deferred_rows", False)
         for run, entry in enumerate(self.schedule):

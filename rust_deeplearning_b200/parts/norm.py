@@ -85,8 +85,8 @@ class ResidualStream:
     the split form asks for `branch_sink(post, then)` and ends in `ops.linear_branch(..., sink)`; a part
     whose first product can take the split form is handed `normed(..., deferred_ok=True)`, which may then
     return `ops.DeferredRows` in place of a tensor.  Both are offers: where one side is missing, where
-    the rows are too many or where another norm is asked for than was announced, the stream falls back to
-    the kernels of its own, with the same result up to rounding."""
+    the rows are too many (`deferred_rows`: the model says up to how many it pays) or where another norm
+    is asked for than was announced, the stream falls back to the kernels of its own, with the same result up to rounding."""
 
     def __init__(self, x: torch.Tensor):
         if x.dtype is not torch.float32:
@@ -98,6 +98,7 @@ class ResidualStream:
         self._operand = None     # (bfloat16 [16, hidden] whose first rows are x times a norm's column factors, that norm)
         self._lent = None        # DeferredRows handed out; x is valid once they have been used
         self._rows = None        # x in the activations' dtype, as `renorm` left it (valid until x changes again)
+        self.deferred_rows = ops.DEFERRED_MAX_ROWS   # rows up to which the split form is begun
         self.norm_after_block = None     # a hint the model sets: the norm the stream is asked for first after the current block
 
     # ---- the split form ----
@@ -119,7 +120,8 @@ class ResidualStream:
     def _prepare(self, upcoming, act_dtype):
         """After x has changed: the first half of the operand for `upcoming`, by a kernel of its own."""
         self._operand = None
-        if upcoming is not None and _fusable(upcoming) and ops.deferred_ok(self.x.shape[0], self.x.shape[1], act_dtype):
+        if upcoming is not None and _fusable(upcoming) and self.x.shape[0] <= self.deferred_rows and ops.deferred_ok(
+                self.x.shape[0], self.x.shape[1], act_dtype):
             self._operand = (ops.scaled_rows(self.x, upcoming.fused_params()), upcoming)
 
     @staticmethod

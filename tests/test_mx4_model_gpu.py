@@ -175,3 +175,21 @@ def test_unknown_formats_and_the_command_line(tmp_path, capsys):
         assert cli.main(argv + extra) == 0
         outs.append(capsys.readouterr().out.split())
     assert all(len(o) <= 4 for o in outs)
+
+
+def test_rows_of_the_split_form():
+    """How many rows take the norms apart follows from the sizes: as many as every part's product can keep in shared memory."""
+    small = ops.pack_mx4(torch.zeros((2 * 64, 128), device=DEV), gated=True)
+    tall = ops.pack_mx4(torch.zeros((2 * 10000, 4608), device=DEV), gated=True)          # 157 tiles, 36 blocks of columns
+    taller = ops.pack_mx4(torch.zeros((20000, 8320), device=DEV))                        # 65 blocks
+    assert (small.deferred_rows, tall.deferred_rows, taller.deferred_rows) == (8, 4, 0)
+    model = load_model(mh.model_folder("A"), "bfloat16", DEV, weight_format="mx4")
+    assert model.deferred_rows == 8
+    h = torch.randn((5, 4608), device=DEV)
+    norm = ops.NormParams(torch.zeros(4608, device=DEV), 1e-6, 1.0)
+    w = ops.pack_mx4(torch.randn((4608, 2048), device=DEV))
+    operand = ops.scaled_rows(h, norm)
+    branch = ops.linear_branch(torch.randn((5, 2048), device=DEV).bfloat16(), w, ops.BranchSink(h, norm, norm, operand))
+    d = ops.DeferredRows(branch, torch.empty_like(h), norm, torch.empty_like(operand))
+    rows = ops.linear_gated(d, tall, "silu")             # five rows: made into a tensor first
+    assert d.consumed and torch.equal(rows, ops.linear_gated_mx4(d.materialise(), tall, "silu"))
