@@ -19,12 +19,11 @@
 // distributed shared memory to the one that adds up that part of the outputs, in rank order.  Every wait is bounded.
 //
 // Up to 8 bfloat16 rows can have a deferred norm on either side (the algebra: DeferredNormArgs in api.h).  The branch's product writes its
-// partial sums a block of the cluster at a time.  The product behind the norm takes both halves of the operand as its rows; four warps add
-// the partial sums up and see to the stream while it multiplies, and a row's two sums are joined on their way out of tensor memory.
-// (Joining the halves before the product, as x = s2 (ht + s1 at), makes parts of half as many rows, but only after the sums are there: it
-// took 2 us more than a plain product; this way 1 us with up to 4 rows, 1.1 to 2.5 us with 8.)  Output projection, gated product, down
-// projection and next projection of a layer of width 2,304, with the norms between: 1 row 27.0 us, 29.7 with kernels for the norms; 8
-// rows 32.8 and 34.0.
+// partial sums a block of the cluster at a time.  In the product behind the norm four warps add them up and see to the stream.  Up to 4
+// rows: both halves of the operand are rows of the product, and a row's two sums are joined on their way out of tensor memory, so
+// that nothing waits for the partial sums.  5 to 8 rows: that would be 16 rows to make parts of; the halves are joined first, x = s2 (ht + s1 at),
+// rounded to bfloat16.  Output projection, gated product, down projection and next projection of a layer with the norms between: width
+// 2,304 1 row 27.6 us (29.9 with kernels for the norms), 8 rows 32.0 (34.6); width 3,584 40.1 (46.5), 46.9 (52.0); 4,608 74.9 (82.0), 83.6 (89.6).
 #include <cuda_fp16.h>
 
 #include "activations.cuh"
@@ -140,6 +139,17 @@ __device__ __forceinline__ uint32_t raw_load(const void* p, long long i, int dty
 }
 __device__ __forceinline__ float raw_value(uint32_t bits, int dtype) { return __uint_as_float(dtype == RDL_BF16 ? bits << 16 : bits); }
 
+// The two halves of the operand behind a deferred norm joined: what the rows stand for, rounded to bfloat16 as a norm's result is
+__device__ __forceinline__ float join(float h, float b, float2 r) { return r.y * fmaf(r.x, b, h); }
+__device__ __forceinline__ uint32_t join_pair(uint32_t h, uint32_t b, float2 r) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(join(__uint_as_float(h << 16), __uint_as_float(b << 16), r),
+                                                   join(__uint_as_float(h & 0xffff0000u), __uint_as_float(b & 0xffff0000u), r));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// A kernel's MODE is 0, RDL_NORM_BRANCH, RDL_NORM_DEFERRED (both halves of the operand are rows of the product) or this (they are joined first).
+constexpr int NORM_JOINED = 3;
+__host__ __device__ constexpr bool behind_norm(int mode) { return mode == RDL_NORM_DEFERRED || mode == NORM_JOINED; }
+
 constexpr int ROW_FINE = 0, ROW_ZERO = 1, ROW_TINY = 2, ROW_BAD = 3;
 
 // The parts of a chunk as e4m3 bytes, and the scale codes of its group; the four lanes of a group come here together.  A part is the
@@ -190,17 +200,17 @@ __device__ __forceinline__ int make_parts(const Chunk<PARTS>& d, uint2 (&bytes)[
     }
 }
 
-// PARTS: 1 (8-bit rows), 2 (bfloat16), 6 (float32); R: rows the product has place for; MODE: 0, or the side of a deferred norm
+// PARTS: 1 (8-bit rows), 2 (bfloat16), 6 (float32); R: rows the product has place for; MODE: see above
 template <int PARTS, int R, int MODE>
 __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs a) {
     constexpr int NB = PARTS * R;                            // columns of the product: part p of row m is column p R + m
     constexpr int X_BLOCK = NB * MX_BLOCK;                   // bytes of a block of 128 columns of the rows
     constexpr int TMEM_COLS = 2 * NB + SCALE_BUFS * 8 <= 128 ? 128 : 256;
-    constexpr int AHEAD = PARTS == 6 ? 2 : 4;                // chunks a lane asks for before it works on the first: two rows each
+    constexpr int AHEAD = PARTS == 6 || MODE == NORM_JOINED ? 2 : 4;                // chunks a lane asks for before it works on the first: two rows each
     constexpr int PIECE_ROWS = 2 * AHEAD, PIECES = STEP * (R / PIECE_ROWS);              // pieces of a group of STEP blocks
     // behind a deferred norm four of the workers see to the sums and to the stream; the others make parts (of 18 blocks of 16 rows, three
     // pieces each, as sixteen would)
-    constexpr int SIDE = MODE == RDL_NORM_DEFERRED ? 4 : 0, TAKERS = WORKERS / 32 - SIDE;
+    constexpr int SIDE = behind_norm(MODE) ? 4 : 0, TAKERS = WORKERS / 32 - SIDE;
     static_assert(NB % 16 == 0 && 2 * NB + SCALE_BUFS * 8 <= TMEM_COLS, "the sums of two tiles and the scales share tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -342,6 +352,11 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
 #pragma unroll
             for (int i = 1; i < AHEAD; ++i) d[i - 1] = d[i];
         };
+        // the rows' numbers, for the warps that need them: the ones that take sums out, or the ones that join halves
+        constexpr int SCALED = (MODE == NORM_JOINED ? TAKERS : 8) * 32;
+        auto wait_scales = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(SIDE * 32 + SCALED) : "memory"); };
+        bool have_scales = false;
+        const int branch_row = a.src_rows <= 4 ? 4 : 8;      // where the operand's second half begins
         auto prepare = [&](int turn) {
             if (warp - 2 >= takers) return;
             const int before = turn * pieces;
@@ -349,24 +364,45 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                 const int nth = p / PIECES, piece = p - before, gi = piece / PIECES, round = nth / x_groups, gs = nth - round * x_groups;
                 if (round > 0 && !resident && !mx_bar_wait(mx_smem(&x_free[gs]), (round - 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
                 const int j = piece % PIECES / (R / PIECE_ROWS), first = piece % (R / PIECE_ROWS) * PIECE_ROWS, block = b0 + gi * STEP + j, slot = gs * STEP + j;
-                const int chunks = block < b1 ? min((MODE == RDL_NORM_DEFERRED ? R : a.M) - first, PIECE_ROWS) * (MX_BLOCK / 8) : 0;     // 16 a row
+                const int chunks = block < b1 ? min((MODE == RDL_NORM_DEFERRED ? R : a.src_rows) - first, PIECE_ROWS) * (MX_BLOCK / 8) : 0;     // 16 a row
                 const uint32_t at = my_place + (uint32_t)(slot * X_BLOCK + first * 128), sc_at = my_scale + (uint32_t)(slot * MX_SCALE_BYTES + first * 16);
                 uint32_t seen[4] = {0, 0, 0, 0};         // rows by kind
+                Chunk<PARTS> d[AHEAD];
+                uint4 branch[MODE == NORM_JOINED ? AHEAD : 1];
                 if (chunks > 0) {
-                    Chunk<PARTS> d[AHEAD];
 #pragma unroll
                     for (int u = 0; u < AHEAD; ++u) {
                         const int i = u * 32 + lane;
 #pragma unroll
                         for (int e = 0; e < (int)(sizeof(d[u].w) / 4); ++e) d[u].w[e] = 0;
                         d[u].code = 0;
-                        if (i < chunks && used_row(first + (i >> 4))) load_chunk<PARTS>(a, first + (i >> 4), block * MX_BLOCK + (lane & 15) * 8, d[u]);
+                        const int k = block * MX_BLOCK + (lane & 15) * 8;
+                        if (i < chunks && used_row(first + (i >> 4))) load_chunk<PARTS>(a, first + (i >> 4), k, d[u]);
+                        if constexpr (MODE == NORM_JOINED) {
+                            branch[u] = make_uint4(0, 0, 0, 0);
+                            if (i < chunks && k < a.K) branch[u] = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.x + (long long)(branch_row + first + (i >> 4)) * a.K + k);
+                        }
                     }
+                }
+                if (MODE == NORM_JOINED && !have_scales) {           // asked for before the rows' numbers are there
+                    wait_scales();
+                    have_scales = true;
+                }
+                if (chunks > 0) {
 #pragma unroll 1                                                                     // short code: see the head of the file
                     for (int u = 0; u < AHEAD; ++u) {
                         const int m0 = u * 2;                                        // this lane's row of the piece: m0 or m0 + 1
                         if (u * 32 >= chunks) break;                                 // none of this warp's
                         if (MODE == RDL_NORM_DEFERRED && !used_row(first + m0)) { shift(d); continue; }
+                        if constexpr (MODE == NORM_JOINED) {
+                            const float2 r = row_scale[(first + m0 + (lane >> 4)) & 7];
+                            d[0].w[0] = join_pair(d[0].w[0], branch[0].x, r);
+                            d[0].w[1] = join_pair(d[0].w[1], branch[0].y, r);
+                            d[0].w[2] = join_pair(d[0].w[2], branch[0].z, r);
+                            d[0].w[3] = join_pair(d[0].w[3], branch[0].w, r);
+#pragma unroll
+                            for (int i = 1; i < AHEAD; ++i) branch[i - 1] = branch[i];
+                        }
                         uint2 bytes[PARTS];
                         uint32_t code[PARTS];
                         const int kind = make_parts<PARTS>(d[0], bytes, code);
@@ -403,6 +439,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
         int lt = 0;
         // (a wait in vain ends no loop here: the blocks of a cluster meet again below)
         prepare(0);
+        if (MODE == NORM_JOINED && warp < 2 + TAKERS && !have_scales) wait_scales();     // (it had no rows: the barrier counts it)
         if (SIDE > 0 && warp >= 2 + TAKERS) {
             // a row's two numbers, lane & 7 the row, from the branch's partial sums in a fixed order
             const DeferredNormArgs& d = a.norm;
@@ -437,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             const float s2 = rsqrtf(fmaxf(t.y + 2.f * s1 * t.z + s1 * s1 * t.w, 0.f) / (float)a.K + d.eps2);     // of the squares of h + s1 a'
             if (me == 0 && lane < 8) row_scale[lane] = make_float2(s1, s2);
             __syncwarp();
-            asm volatile("bar.arrive 2, %0;" ::"n"(SIDE * 32 + 256) : "memory");         // for the warps that take the sums out
+            asm volatile("bar.arrive 2, %0;" ::"n"(SIDE * 32 + SCALED) : "memory");
             // this block's slice of the updated stream and of the operand after it
             if (d.residual_out || d.scaled_next) {
                 const long long total = (long long)a.src_rows * a.K, per = (total + gridDim.x - 1) / gridDim.x;
@@ -462,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             const int buf = lt & 1;
             if (!mx_bar_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
             mx_fence_after();
-            if (SIDE > 0 && lt == 0 && warp < 10) asm volatile("bar.sync 2, %0;" ::"n"(SIDE * 32 + 256) : "memory");
+            if (MODE == RDL_NORM_DEFERRED && lt == 0 && warp < 10) wait_scales();
             float* y = reinterpret_cast<float*>(smem + y_off);       // a cluster's sums (one tile each)
             if (warp < 10) {
                 // lane l of quarter q: weight row 32 q + l of the tile; this warp takes half of the rows
@@ -506,7 +543,10 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                             mx_from_e2m1(code & 15u, h);
                             const float w = __half2float(__ushort_as_half((unsigned short)(h[0] & 0xffffu)))
                                             * mx_scale(a.scales[mx_scale_at(wr, k, a.blocks)]);
-                            y = fmaf(rdl_load(a.x, (long long)m * a.K + k, PARTS == 2 ? RDL_BF16 : RDL_F32), w, y);
+                            float x = rdl_load(a.x, (long long)m * a.K + k, PARTS == 2 ? RDL_BF16 : RDL_F32);
+                            if constexpr (MODE == NORM_JOINED)
+                                x = __bfloat162float(__float2bfloat16_rn(join(x, rdl_load(a.x, (long long)(branch_row + m) * a.K + k, RDL_BF16), row_scale[m])));
+                            y = fmaf(x, w, y);
                         }
 #pragma unroll
                         for (int i = 0; i < MINE; ++i)
@@ -530,7 +570,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                         const float up = a.gated ? __shfl_down_sync(0xffffffffu, sum[0], 16) : 0.f;
                         if (n < a.N && (!a.gated || lane < 16)) {
                             const float y = finish(a, sum[0], up);
-                            if (MODE != RDL_NORM_DEFERRED || !a.norm.row_index) rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, y);
+                            if (!behind_norm(MODE) || !a.norm.row_index) rdl_store(a.out, (long long)m * a.N + n, a.out_dtype, y);
                             else
                                 for (int j = 0; j < a.M; ++j)
                                     if (a.norm.row_index[j] == m) rdl_store(a.out, (long long)j * a.N + n, a.out_dtype, y);
@@ -603,7 +643,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             const float* y = reinterpret_cast<const float*>(smem + y_off);
             for (int idx = tid; idx < a.M * a.share; idx += WORKERS) {
                 const int m = idx / a.share, o = idx - m * a.share, of_tile = rank * a.share + o, n = first_tile * per_tile + of_tile;
-                const int src = MODE == RDL_NORM_DEFERRED && a.norm.row_index ? a.norm.row_index[m] : m;
+                const int src = behind_norm(MODE) && a.norm.row_index ? a.norm.row_index[m] : m;
                 if (of_tile >= per_tile || n >= a.N || src < 0 || src >= a.src_rows) continue;
                 const float* ys = y + src * outs + (a.gated ? 2 * o : o);
                 float v[8], u[8];
@@ -635,7 +675,7 @@ int plan(FewArgs& a, const Mx4Matrix& w) {
     a.split = mx_split(a.tiles, a.blocks, sms);
     a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
     a.slice_blocks = (a.blocks + a.split - 1) / a.split;
-    const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - (MODE == RDL_NORM_DEFERRED ? 2048 : 1024) - sums;    // alignment, static shared memory
+    const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - (behind_norm(MODE) ? 2048 : 1024) - sums;    // alignment, static shared memory
     // The rows of all of a block's columns, if a ring of two stages fits beside them (float32, 8 rows x 2,304, 256,000 outputs: 71 us so and 94
     // with the rows brought anew for every tile; bfloat16, 16 x 3,584, 28,672 gated: 20.5 and 23.0); else as many as fit beside four.
     a.slots = (a.slice_blocks + STEP - 1) / STEP * STEP;
@@ -698,17 +738,13 @@ extern "C" int rdl_mx_branch_units(const void* weight) {
     return split > 1 ? w->tiles * split : 0;
 }
 
-// Up to how many rows the product behind a deferred norm pays.  Above 4 rows its operand has 16; where those have to be made ready again for
-// every tile the norm is better off in a kernel of its own (8 rows x 4,608, 36,864 gated outputs: 63 us against 35 and 5 for the norm; 1 row
-// 34 against 33 and 5).
+// Up to how many rows the product behind a deferred norm pays: none where its rows are made ready again for every tile
 extern "C" int rdl_mx_deferred_rows(const void* weight) {
     const Mx4Matrix* w = (const Mx4Matrix*)weight;
     if (!w || !w->codes) return 0;
     FewArgs a{};
-    plan<2, 16, RDL_NORM_DEFERRED>(a, *w);
-    if (once(a)) return 8;
-    plan<2, 8, RDL_NORM_DEFERRED>(a, *w);
-    return once(a) ? 4 : 0;
+    plan<2, 8, NORM_JOINED>(a, *w);
+    return once(a) ? 8 : 0;
 }
 
 extern "C" int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, const void* weight, int m, int activation, float act_param,
@@ -743,5 +779,6 @@ extern "C" int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, con
     RDL_REQUIRE(!norm->scaled_next || (norm->w_next && rdl_valid_dtype(norm->w_next_dtype)), "mx_few_rows_norm: the next operand needs the next norm's weight");
     a.out = out; a.out_dtype = out_dtype;
     a.M = norm->n_out;
-    return m <= 4 ? launch<2, 8, RDL_NORM_DEFERRED>(a, *w, (cudaStream_t)stream) : launch<2, 16, RDL_NORM_DEFERRED>(a, *w, (cudaStream_t)stream);
+    // 4 rows, 2,304 wide, gated 18,432 and 4,096 outputs: 8.7 and 6.8 us as halves, 9.9 and 6.9 joined; 8 rows: 11.1 and 7.1, 9.7 and 6.6
+    return m <= 4 ? launch<2, 8, RDL_NORM_DEFERRED>(a, *w, (cudaStream_t)stream) : launch<2, 8, NORM_JOINED>(a, *w, (cudaStream_t)stream);
 }

@@ -182,7 +182,7 @@ def test_rows_of_the_split_form():
     small = ops.pack_mx4(torch.zeros((2 * 64, 128), device=DEV), gated=True)
     tall = ops.pack_mx4(torch.zeros((2 * 10000, 4608), device=DEV), gated=True)          # 157 tiles, 36 blocks of columns
     taller = ops.pack_mx4(torch.zeros((20000, 8320), device=DEV))                        # 65 blocks
-    assert (small.deferred_rows, tall.deferred_rows, taller.deferred_rows) == (8, 4, 0)
+    assert (small.deferred_rows, tall.deferred_rows, taller.deferred_rows) == (8, 8, 0)
     model = load_model(mh.model_folder("A"), "bfloat16", DEV, weight_format="mx4")
     assert model.deferred_rows == 8
     h = torch.randn((5, 4608), device=DEV)
