@@ -442,6 +442,10 @@ int rdl_norm_mx8(const void* x, int x_dtype, const void* w1, int w1_dtype, float
 // A [rows, columns] matrix to 4 bits, in tiles of 128 x 128: codes of 8 KB a tile, scales of 512 bytes a tile and 16 bytes more.
 // gated: a [gate; up] matrix.  The padding becomes zeros.
 int rdl_pack_mx4(const void* w, int dtype, void* codes, void* scales, int rows, int columns, int gated, void* stream);
+// Codes [rows][stride bytes] and scales [rows][ceil(columns / 32)] that are there already, to the same layout.
+int rdl_lay_mx4(const void* from, long long stride, const void* from_scales, void* codes, void* scales, int rows, int columns, int gated, void* stream);
+// 8-bit rows [rows][stride bytes] with scales [rows][ceil(columns / 32)], to the layout rdl_norm_mx8 writes
+int rdl_lay_mx8(const void* from, long long stride, const void* from_scales, void* values, void* scales, int rows, int columns, void* stream);
 // the values of a 4-bit matrix, [rows, columns]
 int rdl_expand_mx4(const void* codes, const void* scales, void* out, int dtype, int rows, int columns, int gated, void* stream);
 // What the products take as `weight`: a block of host memory of rdl_mx4_matrix_bytes bytes on a 64-byte boundary, filled once by

@@ -11,6 +11,8 @@
 // Measured: 8,192 float32 rows of 4,608 (492 MB) 75.6 us, 6.5 TB/s; 2,048 bfloat16 rows of 2,304 with both norms (52 MB) 11.2 us; 17 rows 3.6 us.
 //
 // rdl_pack_mx4: a matrix to 4 bits, padding and all.  Memory bound: 36,864 x 4,608 bfloat16 (430 MB) 87 us, 4.9 TB/s.
+// rdl_lay_mx4, rdl_lay_mx8: a matrix or rows that came in these formats, to the products' layout: 36,864 x 4,608 codes
+// (175 MB) 52 us, 3.4 TB/s.
 // rdl_expand_mx4: the values the codes stand for; exact in bfloat16 for scales from 2^-125 up to 2^125.  The same matrix 71 us, 6.1 TB/s.
 #include <cuda_fp16.h>
 
@@ -310,6 +312,7 @@ __global__ void __launch_bounds__(256) expand_mx4_kernel(const __grid_constant__
     const int tile = blockIdx.x / a.blocks, block = blockIdx.x - tile * a.blocks, c = block * MX_BLOCK + (lane & 15) * 8;
     const uint8_t* codes = a.codes + (long long)blockIdx.x * (MX_ROWS * MX_BLOCK / 2);
     const uint8_t* scales = a.scales + (long long)blockIdx.x * (MX_ROWS * 4);
+    __shared__ float turned[VEC ? 1 : 8][2][VEC ? 4 : MX_BLOCK];
 #pragma unroll
     for (int r0 = 0; r0 < MX_ROWS; r0 += 16 * TILE_AHEAD) {
         uint32_t w[TILE_AHEAD], sc[TILE_AHEAD];
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(256) expand_mx4_kernel(const __grid_constant__
 #pragma unroll
         for (int i = 0; i < TILE_AHEAD; ++i) {
             const int row = mx_row_at(tile * MX_ROWS + r0 + i * 16 + warp * 2 + (lane >> 4), a.rows, a.half);
-            if (row < 0) continue;
+            if (VEC && row < 0) continue;
             uint32_t h[4];
             mx_from_e2m1(w[i], h);
             const float s = mx_scale(sc[i]);
@@ -347,12 +350,79 @@ __global__ void __launch_bounds__(256) expand_mx4_kernel(const __grid_constant__
                     *reinterpret_cast<float4*>((float*)a.out + base + 4) = make_float4(v[4], v[5], v[6], v[7]);
                 }
             } else {
+                // rows that begin anywhere: through shared memory, so that neighbouring lanes store neighbouring columns (777 x 1,003: 6.6 us
+                // and 10.1 with eight neighbouring columns a lane)
+                float* mine = &turned[warp][lane >> 4][(lane & 15) * 8];
+                *reinterpret_cast<float4*>(mine) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(mine + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                __syncwarp();
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (c + k < a.columns) rdl_store(a.out, base + k, a.dtype, v[k]);
+                for (int k = 0; k < 8; ++k) {
+                    const int to = __shfl_sync(0xffffffffu, row, (k >> 2) * 16), col = block * MX_BLOCK + (k & 3) * 32 + lane;
+                    if (to >= 0 && col < a.columns) rdl_store(a.out, (long long)to * a.columns + col, a.dtype, turned[warp][k >> 2][(k & 3) * 32 + lane]);
+                }
+                __syncwarp();
             }
         }
     }
+}
+
+// Codes and scales that are there already, to the products' layout; blocks as above.  What lies beyond the last column is cleared.
+struct LayArgs {
+    const uint8_t* from; long long stride; const uint8_t* from_scales;       // bytes from a row's codes (4 bits) or values (8 bits) to the next one's
+    uint8_t* to; uint8_t* to_scales;
+    int rows, columns, blocks, half;                        // 8 bits: half is the rows' padded count
+};
+
+// four bytes of a row from byte b on; zeros from byte `end` on
+template <bool VEC>
+__device__ __forceinline__ uint32_t four_bytes(const uint8_t* row, int b, int end) {
+    if (VEC && b + 4 <= end) return *reinterpret_cast<const uint32_t*>(row + b);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (b + i < end) w |= (uint32_t)row[b + i] << (8 * i);
+    return w;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(256) lay_mx4_kernel(const __grid_constant__ LayArgs a) {
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x / a.blocks, block = blockIdx.x - tile * a.blocks, c = block * MX_BLOCK + (lane & 15) * 8;
+    const int groups = (a.columns + MX_GROUP - 1) / MX_GROUP;
+    uint8_t* to = a.to + (long long)blockIdx.x * (MX_ROWS * MX_BLOCK / 2);
+    uint8_t* to_scales = a.to_scales + (long long)blockIdx.x * (MX_ROWS * 4);
+    constexpr int EACH = MX_ROWS / 16;
+    uint32_t w[EACH], sc[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {                         // all asked for before the first is stored
+        const int src = mx_row_at(tile * MX_ROWS + i * 16 + warp * 2 + (lane >> 4), a.rows, a.half), group = block * 4 + (lane & 15);
+        w[i] = src < 0 ? 0u : four_bytes<VEC>(a.from + src * a.stride, c / 2, (a.columns + 1) / 2);
+        sc[i] = src < 0 || (lane & 15) >= 4 || group >= groups ? 0u : a.from_scales[(long long)src * groups + group];
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int r = i * 16 + warp * 2 + (lane >> 4);
+        // of an odd row's last byte the upper half is padding, whatever it held
+        if (c < a.columns && c + 8 > a.columns) w[i] &= 0xffffffffu >> (4 * (c + 8 - a.columns));
+        *reinterpret_cast<uint32_t*>(to + r * (MX_BLOCK / 2) + (lane & 15) * 4) = w[i];
+        if ((lane & 15) < 4) to_scales[r % 32 * 16 + r / 32 * 4 + (lane & 15)] = (uint8_t)sc[i];
+    }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(256) lay_mx8_kernel(const __grid_constant__ LayArgs a) {
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const int m = blockIdx.x, groups = (a.columns + MX_GROUP - 1) / MX_GROUP;
+    const uint8_t* from = a.from + m * a.stride;
+    uint8_t* to = a.to + (long long)m * a.blocks * MX_BLOCK;
+#pragma unroll 4
+    for (int b = threadIdx.x * 4; b < a.blocks * MX_BLOCK; b += 1024) *reinterpret_cast<uint32_t*>(to + b) = four_bytes<VEC>(from, b, a.columns);
+    for (int block = threadIdx.x; block < a.blocks; block += 256)
+        *reinterpret_cast<uint32_t*>(a.to_scales + ((long long)block * a.half + m) * 4) = four_bytes<false>(a.from_scales + (long long)m * groups, block * 4, groups);
 }
 
 // tiles of 128 rows of a weight
@@ -431,6 +501,33 @@ extern "C" int rdl_expand_mx4(const void* codes, const void* scales, void* out, 
     const cudaError_t e = columns % 8 == 0 && aligned16(out) ? rdl_launch(expand_mx4_kernel<true>, dim3((unsigned)grid), dim3(256), 0, st, a)
                                                              : rdl_launch(expand_mx4_kernel<false>, dim3((unsigned)grid), dim3(256), 0, st, a);
     RDL_CHECK_EX(e, "expand_mx4");
+    return 0;
+}
+
+extern "C" int rdl_lay_mx4(const void* from, long long stride, const void* from_scales, void* codes, void* scales, int rows, int columns, int gated, void* stream) {
+    RDL_REQUIRE(from && from_scales && codes && scales, "lay_mx4: missing operand");
+    RDL_REQUIRE(rows > 0 && columns > 0 && stride >= (columns + 1) / 2 && (!gated || rows % 2 == 0), "lay_mx4: bad sizes rows=%d columns=%d", rows, columns);
+    RDL_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0, "lay_mx4: the results must start on 16-byte boundaries");
+    const LayArgs a{(const uint8_t*)from, stride, (const uint8_t*)from_scales, (uint8_t*)codes, (uint8_t*)scales, rows, columns, mx_blocks(columns), gated ? rows / 2 : 0};
+    const long long grid = (long long)weight_tiles(rows, gated) * a.blocks;
+    RDL_REQUIRE(grid <= 0x7fffffffLL, "lay_mx4: %d x %d is too large", rows, columns);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool vec = stride % 4 == 0 && (uintptr_t)from % 4 == 0;
+    RDL_CHECK_EX(vec ? rdl_launch(lay_mx4_kernel<true>, dim3((unsigned)grid), dim3(256), 0, st, a)
+                     : rdl_launch(lay_mx4_kernel<false>, dim3((unsigned)grid), dim3(256), 0, st, a), "lay_mx4");
+    RDL_CUDA(cudaMemsetAsync((uint8_t*)scales + grid * (MX_ROWS * 4), 0, 16, st), "lay_mx4");       // as after the packing
+    return 0;
+}
+
+extern "C" int rdl_lay_mx8(const void* from, long long stride, const void* from_scales, void* values, void* scales, int rows, int columns, void* stream) {
+    if (rows == 0) return 0;
+    RDL_REQUIRE(from && from_scales && values && scales, "lay_mx8: missing operand");
+    RDL_REQUIRE(rows > 0 && columns > 0 && stride >= 0, "lay_mx8: bad sizes rows=%d columns=%d", rows, columns);
+    RDL_REQUIRE((uintptr_t)values % 4 == 0 && (uintptr_t)scales % 4 == 0, "lay_mx8: the results must start on 4-byte boundaries");
+    const LayArgs a{(const uint8_t*)from, stride, (const uint8_t*)from_scales, (uint8_t*)values, (uint8_t*)scales, rows, columns, mx_blocks(columns), (rows + 3) / 4 * 4};
+    const bool vec = stride % 4 == 0 && (uintptr_t)from % 4 == 0;
+    RDL_CHECK_EX(vec ? rdl_launch(lay_mx8_kernel<true>, dim3((unsigned)rows), dim3(256), 0, (cudaStream_t)stream, a)
+                     : rdl_launch(lay_mx8_kernel<false>, dim3((unsigned)rows), dim3(256), 0, (cudaStream_t)stream, a), "lay_mx8");
     return 0;
 }
 

@@ -434,6 +434,8 @@ _SIGNATURES = {
     "rdl_gemm_tc": [_P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _F, _P],
     "rdl_norm_mx8": [_P, _I, _P, _I, _F, _F, _P, _P, _P, _I, _F, _F, _P, _P, _I, _I, _P],
     "rdl_pack_mx4": [_P, _I, _P, _P, _I, _I, _I, _P],
+    "rdl_lay_mx4": [_P, _LL, _P, _P, _P, _I, _I, _I, _P],
+    "rdl_lay_mx8": [_P, _LL, _P, _P, _P, _I, _I, _P],
     "rdl_expand_mx4": [_P, _P, _P, _I, _I, _I, _I, _P],
     "rdl_mx4_matrix_bytes": [],
     "rdl_mx4_describe": [_P, _P, _P, _I, _I, _I],

@@ -1854,8 +1854,6 @@ class Mx4Weight:
         self._host = ctypes.create_string_buffer(lib.rdl_mx4_matrix_bytes() + 64)
         self.handle = -(-ctypes.addressof(self._host) // 64) * 64
         library.check(lib.rdl_mx4_describe(self.handle, self.codes.data_ptr(), self._scales.data_ptr(), self.rows, self.columns, int(self.gated)), 0)
-        self.branch_units = lib.rdl_mx_branch_units(self.handle)     # of partial sums, as the last product of a branch (0: no such form)
-        self.deferred_rows = lib.rdl_mx_deferred_rows(self.handle)   # up to how many rows it is worth taking behind a deferred norm
 
     def first(self, rows: int) -> "Mx4Weight":
         """The weight's first rows as a weight of their own, on the same memory."""
@@ -1866,6 +1864,16 @@ class Mx4Weight:
         w.codes, w._scales, w.device, w._index = self.codes[:w.tiles], self._scales[:w.tiles * _blocks(self.columns) * MX_ROWS * 4 + 16], self.device, self._index
         w._describe()
         return w
+
+    @functools.cached_property
+    def branch_units(self) -> int:
+        """of partial sums, as the last product of a branch (0: it has no such form)"""
+        return library.load().rdl_mx_branch_units(self.handle)
+
+    @functools.cached_property
+    def deferred_rows(self) -> int:
+        """up to how many rows it is worth taking behind a deferred norm"""
+        return library.load().rdl_mx_deferred_rows(self.handle)
 
     @property
     def scales(self) -> torch.Tensor:
@@ -1940,22 +1948,9 @@ def mx4_weight(codes: torch.Tensor, scales: torch.Tensor, columns: int, gated: b
           f"mx4_weight: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit {columns} columns")
     _need(codes.device == scales.device, "mx4_weight: codes and scales lie on one device")
     w = Mx4Weight(rows, columns, gated, codes.device)
-    if columns % 2:          # the half byte behind an odd row's last column is padding, whatever it held
-        codes = codes.clone()
-        codes[:, used - 1] &= 15
-    blocks = _blocks(columns)
-
-    def laid_out(t, per_block):          # [rows, some] -> [tiles, blocks, 128, per_block]
-        if gated:                        # 16 gate rows, then their 16 up rows
-            halves = torch.zeros((2, -(-w.outputs // 16) * 16, t.shape[1]), dtype=torch.uint8, device=t.device)
-            halves[:, :w.outputs] = t.reshape(2, w.outputs, -1)
-            t = halves.view(2, -1, 16, t.shape[1]).transpose(0, 1).reshape(-1, t.shape[1])
-        wide = torch.zeros((w.tiles * MX_ROWS, blocks * per_block), dtype=torch.uint8, device=t.device)
-        wide[:t.shape[0], :t.shape[1]] = t
-        return wide.view(w.tiles, MX_ROWS, blocks, per_block).transpose(1, 2)
-
-    w.codes.copy_(laid_out(codes[:, :used], MX_BLOCK // 2))
-    w.scales.copy_(laid_out(scales, 4).reshape(w.tiles, blocks, 4, 32, 4).transpose(2, 3))
+    codes, scales = codes if codes.stride(1) == 1 and codes.stride(0) >= used else codes.contiguous(), scales.contiguous()
+    library.check(library.load().rdl_lay_mx4(codes.data_ptr(), codes.stride(0) if rows > 1 else used, scales.data_ptr(), w.codes.data_ptr(),
+                                             w._scales.data_ptr(), rows, columns, int(w.gated), _raw_stream(w._index)))
     return w
 
 
@@ -1975,12 +1970,9 @@ def mx8_rows(values: torch.Tensor, scales: torch.Tensor) -> Mx8Rows:
           "mx8_rows: float8_e4m3fn [rows, columns] and uint8 [rows, groups of 32 columns]")
     _need(values.is_cuda and values.device == scales.device, "mx8_rows: values and scales lie on one CUDA device")
     r = Mx8Rows(values.shape[0], values.shape[1], values)
-    if r.columns % MX_BLOCK:
-        r._data.view(torch.uint8).zero_()
-    r.values.copy_(values)
-    padded = torch.zeros((r.rows, _blocks(r.columns) * 4), dtype=torch.uint8, device=r.device)
-    padded[:, :scales.shape[1]] = scales
-    r.scales.copy_(padded.view(r.rows, -1, 4))
+    values, scales = values if values.stride(1) == 1 and values.stride(0) >= 0 else values.contiguous(), scales.contiguous()
+    library.check(library.load().rdl_lay_mx8(values.data_ptr(), values.stride(0), scales.data_ptr(), *r._addresses, r.rows, r.columns,
+                                             _raw_stream(values.get_device())))
     return r
 
 

@@ -112,6 +112,40 @@ def test_mx4_weight_from_codes_is_the_packed_one():
         assert np.array_equal(f64(ops.expand_mx4(given, torch.float32)), q)
 
 
+@pytest.mark.parametrize("rows,columns,gated", [(1, 1, False), (3, 33, False), (130, 257, False), (2, 31, True), (34, 300, True), (270, 1003, True)])
+def test_layout_of_given_codes_and_rows(rows, columns, gated):
+    """Any strides and starts: views of wider tensors, every second column, a start at an odd byte; whatever the padding held does not enter."""
+    groups, used = -(-columns // 32), -(-columns // 2)
+    g = torch.Generator().manual_seed(70)
+    codes = torch.randint(0, 256, (rows, used), generator=g, dtype=torch.uint8)          # an odd row's last half byte holds something
+    scales = torch.randint(100, 140, (rows, groups), generator=g, dtype=torch.uint8)
+    nib = torch.stack([codes & 15, codes >> 4], dim=-1).view(rows, -1)[:, :columns].numpy()
+    table = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6])
+    want = table[nib] * np.repeat(2.0 ** (scales.numpy().astype(np.float64) - 127), 32, axis=1)[:, :columns]
+    codes, scales = codes.to(DEV), scales.to(DEV)
+    wide = torch.full((rows, used + 5), 255, dtype=torch.uint8, device=DEV)
+    wide[:, 3:3 + used] = codes
+    apart = torch.full((rows, 2 * used), 255, dtype=torch.uint8, device=DEV)
+    apart[:, ::2] = codes
+    padded = torch.full((rows, groups * 16), 255, dtype=torch.uint8, device=DEV)
+    padded[:, :used] = codes
+    wide_scales = torch.cat([scales, scales], dim=1)[:, :groups]
+    first = None
+    for c, s in ((codes, scales), (wide[:, 3:3 + used], wide_scales), (apart[:, ::2], scales), (padded, scales), (codes[:1].expand(rows, used) if rows == 1 else codes, scales)):
+        w = ops.mx4_weight(c, s, columns, gated)
+        assert np.array_equal(f64(ops.expand_mx4(w, torch.float32)), want)
+        first = first or w
+        assert torch.equal(w.codes, first.codes) and torch.equal(w.scales, first.scales)
+    assert int((first.codes != 0).sum()) <= rows * used                  # nothing in the padding
+    values = torch.randint(0, 120, (rows, columns), generator=g, dtype=torch.uint8).to(DEV)
+    around = torch.full((rows, columns + 3), 120, dtype=torch.uint8, device=DEV)
+    around[:, 1:1 + columns] = values
+    for v in (values, around[:, 1:1 + columns]):
+        r = ops.mx8_rows(v.view(torch.float8_e4m3fn), scales)
+        assert torch.equal(r.values.view(torch.uint8), values) and torch.equal(r.scales.reshape(rows, -1)[:, :groups], scales)
+        assert not r._data.view(torch.uint8)[:rows, columns:].any() and not r.scales.reshape(rows, -1)[:, groups:].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,columns", [(1, 1), (5, 31), (3, 128), (7, 1003), (2, 8192), (2, 8197), (3, 20000)])
 def test_pack_mx8(rows, columns, dtype):
