@@ -1844,7 +1844,7 @@ class Mx4Weight:
         self.shape = (rows, columns)
         blocks = _blocks(columns)
         self.codes = torch.empty((self.tiles, blocks, MX_ROWS, MX_BLOCK // 2), dtype=torch.uint8, device=device)
-        self._scales = self.codes.new_empty((self.tiles * blocks * MX_ROWS * 4 + 16,))       # 16 bytes more, which the packing clears last
+        self._scales = self.codes.new_empty(self.tiles * blocks * MX_ROWS * 4 + 16)          # 16 bytes more, which the packing clears last
         self.device = self.codes.device
         self._index = self.device.index
         self._describe()
@@ -1899,7 +1899,7 @@ class Mx8Rows:
         # values [padded rows][padded columns], then scales [blocks][padded rows][4], a 32nd of that.  The padding rows hold whatever the
         # memory held: nothing reads a result that comes of them.
         self._layout = (padded, blocks)
-        self._data = like.new_empty((padded + (padded + 31) // 32, blocks * MX_BLOCK), dtype=torch.float8_e4m3fn)
+        self._data = like.new_empty(padded + (padded + 31) // 32, blocks * MX_BLOCK, dtype=torch.float8_e4m3fn)
         self.device = like.device
 
     @property
@@ -2030,28 +2030,28 @@ def _mx4_refuse(x, weight, gated: bool, who: str):
 
 
 def _product_mx4(x, weight: Mx4Weight, gated: bool, out_dtype, out_mx8: bool, activation: int, param: float, softcap: float, status, who: str):
-    packed = type(x) is Mx8Rows
-    if type(weight) is not Mx4Weight or weight.gated is not gated or len(x.shape) != 2 or x.shape[1] != weight.columns or x.device != weight.device or not (
-            packed or (x.dtype in _KINDS and x.is_contiguous())):
+    shape, packed = x.shape, type(x) is Mx8Rows
+    kind = _MX8 if packed else _KINDS.get(x.dtype)
+    if (type(weight) is not Mx4Weight or weight.gated is not gated or len(shape) != 2 or shape[1] != weight.columns or kind is None
+            or x.device != weight.device or not (packed or x.is_contiguous())):
         _mx4_refuse(x, weight, gated, who)
-    rows, n = x.shape[0], weight.outputs
-    status = status if status is not None else _step_status
-    status = status.data_ptr() if status is not None else None
+    rows, n = shape[0], weight.outputs
+    if status is None:
+        status = _step_status
+    if status is not None:
+        status = status.data_ptr()
     lib, stream = library.load(), _raw_stream(weight._index)
-    if packed:
-        (data, scales), kind = x._addresses, _MX8
-    else:
-        data, scales, kind = x.data_ptr(), None, _KINDS[x.dtype]
+    data, scales = x._addresses if packed else (x.data_ptr(), None)
     if packed and rows > MX_FEW_ROWS:
         if out_mx8:
             out = Mx8Rows(rows, n, weight.codes)
             (to, to_scales), out_kind = out._addresses, _MX8
         else:
-            out = weight.codes.new_empty((rows, n), dtype=out_dtype or torch.bfloat16)
+            out = weight.codes.new_empty(rows, n, dtype=out_dtype or torch.bfloat16)
             to, to_scales, out_kind = out.data_ptr(), None, _KINDS[out.dtype]
         library.check(lib.rdl_mx_many_rows(to, out_kind, to_scales, data, scales, weight.handle, rows, activation, param, softcap, status, stream))
         return out
-    out = weight.codes.new_empty((rows, n), dtype=torch.float32 if out_mx8 else out_dtype or (torch.bfloat16 if packed else x.dtype))
+    out = weight.codes.new_empty(rows, n, dtype=torch.float32 if out_mx8 else out_dtype or (torch.bfloat16 if packed else x.dtype))
     to, out_kind = out.data_ptr(), _KINDS[out.dtype]
     if 0 < rows <= MX_FEW_ROWS:
         library.check(lib.rdl_mx_few_rows(to, out_kind, data, kind, scales, weight.handle, rows, activation, param, softcap, status, stream))
