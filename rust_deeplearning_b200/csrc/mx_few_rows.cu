@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     static_assert(NB % 16 == 0 && 2 * NB + SCALE_BUFS * 8 <= TMEM_COLS, "the sums of two tiles and the scales share tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], x_ready[MAX_SLOTS / STEP], x_free[MAX_SLOTS / STEP];
+    __shared__ __align__(8) unsigned long long full_bar[MAX_STAGES], empty_bar[MAX_STAGES * STEP], acc_full[2], acc_empty[2], x_ready[MAX_SLOTS / STEP], x_free[MAX_SLOTS / STEP];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     // rows with an infinity or a NaN here; rows with a group too small for its last parts; rows with one that is not
@@ -235,7 +235,11 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     const bool resident = groups <= x_groups;
     {   // every barrier by a thread of its own
         const int t = threadIdx.x;
-        if (t < MAX_STAGES) { mx_bar_init(mx_smem(&full_bar[t]), 1); mx_bar_init(mx_smem(&empty_bar[t]), 1); }
+        if (t < MAX_STAGES) {
+            mx_bar_init(mx_smem(&full_bar[t]), STEP);
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) mx_bar_init(mx_smem(&empty_bar[t * STEP + j]), 1);
+        }
         else if (t < MAX_STAGES + 2) { mx_bar_init(mx_smem(&acc_full[t - MAX_STAGES]), 1); mx_bar_init(mx_smem(&acc_empty[t - MAX_STAGES]), 8); }
         else if (t == MAX_STAGES + 2) { gave_up = 0; bad_rows = tiny_rows = fine_rows = 0; }
         else if (t >= 64 && t < 64 + MAX_SLOTS / STEP) { mx_bar_init(mx_smem(&x_ready[t - 64]), PIECES); mx_bar_init(mx_smem(&x_free[t - 64]), 1); }
@@ -280,14 +284,17 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, piece += (tile_step - 1) * a.blocks + (a.blocks - (b1 - b0))) {
                 for (int kb = b0; kb < b1;) {
                     const int n = min(STEP, b1 - kb);
-                    if (!mx_bar_wait(mx_smem(&empty_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
-                    const uint32_t full = mx_smem(&full_bar[s]), at = ring_s + (uint32_t)(s * STEP * MX_TILE_BYTES);
-                    mx_bar_expect(full, (uint32_t)n * (MX_TILE_TX + MX_SCALE_BYTES) + extra);
+                    const uint32_t full = mx_smem(&full_bar[s]);
 #pragma unroll
-                    for (int j = 0; j < STEP; ++j)
-                        if (j < n) tma_codes(at + (uint32_t)(j * MX_TILE_BYTES), &map_w, (piece + j) * MX_ROWS, full, policy);
-                    bulk_scales(ws_s + (uint32_t)(s * STEP * MX_SCALE_BYTES), a.scales + (long long)piece * MX_SCALE_BYTES, (uint32_t)n * MX_SCALE_BYTES, full, policy);
-                    extra = 0;
+                    for (int j = 0; j < STEP; ++j) {         // a block's place is filled again as soon as its own products are done
+                        if (!mx_bar_wait(mx_smem(&empty_bar[s * STEP + j]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
+                        if (j >= n) { mx_bar_arrive(full); continue; }
+                        mx_bar_expect(full, MX_TILE_TX + MX_SCALE_BYTES + extra);
+                        extra = 0;
+                        tma_codes(ring_s + (uint32_t)((s * STEP + j) * MX_TILE_BYTES), &map_w, (piece + j) * MX_ROWS, full, policy);
+                        bulk_scales(ws_s + (uint32_t)((s * STEP + j) * MX_SCALE_BYTES), a.scales + (long long)(piece + j) * MX_SCALE_BYTES, MX_SCALE_BYTES, full, policy);
+                    }
+                    if (!ok) break;
                     ask();
                     kb += n;
                     piece += n;
@@ -313,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                     mx_fence_after();
 #pragma unroll
                     for (int j = 0; j < STEP; ++j) {
-                        if (j >= n) break;
+                        if (j >= n) { commit(mx_smem(&empty_bar[s * STEP + j])); break; }
                         const uint32_t sa = tmem + 2 * NB + (uint32_t)((scale_buf + j) & (SCALE_BUFS - 1)) * 8, sb = sa + 4;
                         copy_scales(sa, mx_scale_desc(ws_s + (uint32_t)((s * STEP + j) * MX_SCALE_BYTES)));
                         copy_scales(sb, mx_scale_desc(xs_s + (uint32_t)((g * STEP + j) * MX_SCALE_BYTES)));
@@ -321,8 +328,8 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             mma_mx(tmem + buf * NB, ad + (uint32_t)(k * 2), bd + (uint32_t)(k * 2), mx_idesc(MX_E2M1, MX_E4M3, MX_ROWS, NB, k), sa, sb, kb + j != b0 || k != 0);
+                        commit(mx_smem(&empty_bar[s * STEP + j]));
                     }
-                    commit(mx_smem(&empty_bar[s]));
                     if (!resident) commit(mx_smem(&x_free[g]));
                     scale_buf = (scale_buf + n) & (SCALE_BUFS - 1);
                     if (++s == a.stages) { s = 0; parity ^= 1; }
