@@ -1818,7 +1818,6 @@ MX_GROUP, MX_BLOCK, MX_ROWS = 32, 128, 128
 MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs, which also takes tensors; above, 8-bit rows only
 _MX8 = 2                 # rows of 8 bits, where a kernel's argument says of what kind its rows are
 _KINDS = {torch.float32: 0, torch.bfloat16: 1}
-MX8 = "mx8"              # in place of a dtype: rows wanted as `Mx8Rows`
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # what torch.cuda.current_stream(i).cuda_stream gives, in a thirtieth of the time
 
 
