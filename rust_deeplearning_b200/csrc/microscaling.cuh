@@ -77,3 +77,9 @@ __device__ __forceinline__ void mx_from_e2m1(uint32_t w, uint32_t (&h)[4]) {
         "cvt.rn.f16x2.e2m1x2 %0, a;\ncvt.rn.f16x2.e2m1x2 %1, b;\ncvt.rn.f16x2.e2m1x2 %2, c;\ncvt.rn.f16x2.e2m1x2 %3, d;\n}"
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
+// two e4m3 values (the low half of w)
+__device__ __forceinline__ float2 mx_from_e4m3(uint32_t w) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)w));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}

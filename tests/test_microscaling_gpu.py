@@ -430,6 +430,25 @@ def test_rows_of_any_size(kind):
         check(ops.linear_mx4(x, packed, out_dtype=torch.float32), f64(x) @ w64.T, sum_tolerance(f64(x), w64, kind) + 2.0 ** -149 * 128, str(factor))
 
 
+@pytest.mark.parametrize("spread", [2.0 ** 8, 2.0 ** 12, 2.0 ** 16, 2.0 ** 24])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_one_large_value_in_every_group(kind, spread):
+    """The others of its group stay: exact down to 2^-13 of the largest, off by 2^-21 (float32: 2^-37) of it below that.  The weights of the large
+    columns are zero, so that nothing hides what becomes of the small ones."""
+    m, n, k = 7, 40, 320
+    x = rnd((m, k), torch.float32, 80).to(getattr(torch, kind))
+    large = torch.arange(k, device=DEV) % 32 == 5
+    x[:, large] = spread * 1.1
+    w = rnd((n, k), torch.float32, 81)
+    w[:, large] = 0
+    w = ops.pack_mx4(w)
+    w64, x64 = f64(ops.expand_mx4(w, torch.float32)), f64(x)
+    small = np.where(large.cpu().numpy(), 0.0, x64)
+    top = spread * 1.1 * 1.01
+    lost = np.where(np.abs(small) < top * 2.0 ** -13, top * 2.0 ** (-21 if kind == "bfloat16" else -37), 0.0)
+    check(ops.linear_mx4(x, w, out_dtype=torch.float32), small @ w64.T, sum_tolerance(small, w64, kind) + lost @ np.abs(w64).T, kind)
+
+
 @pytest.mark.parametrize("m,kind", [(4, "bfloat16"), (4, "float32"), (4, "mx8"), (40, "mx8")])
 def test_infinities_and_nan(m, kind):
     """What is not finite reaches the outputs of its own row, and only those; a NaN scale of a weight reaches its own column."""
