@@ -513,7 +513,9 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             // the last turn saw to)
             if (!resident && tile + tile_step < a.tiles) prepare(lt + 1);
             const int buf = lt & 1;
-            if (!mx_bar_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
+            // Only the warps that take the sums out wait for them: the products of the tile after next need their arrival, so this barrier
+            // is never two phases ahead of them.  A warp without a say in that could come two tiles late and wait for a phase that is not to be.
+            if (warp < 10 && !mx_bar_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) ok = false;
             mx_fence_after();
             if (MODE == RDL_NORM_DEFERRED && lt == 0 && warp < 10) wait_scales();
             float* y = reinterpret_cast<float*>(smem + y_off);       // a cluster's sums (one tile each)

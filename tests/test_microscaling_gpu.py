@@ -341,6 +341,44 @@ def test_deferred_norms(m, width, k_in, n_out):
     assert status.item() == 0
 
 
+@pytest.mark.parametrize("m", [1, 4, 8])
+def test_deferred_norms_in_front_of_many_tiles(m):
+    """A block works on four tiles of weights or more, each of few products, while some of its warps still write the stream: no wait
+    is in vain, and every call gives the same bits.
+
+    The tolerance is that of test_deferred_norms."""
+    width, n_out = 256, 80000
+    x, _ = rows_for(m, 2048, "bfloat16", 70)
+    x[x.abs().amax(1) == 0] = 1.0
+    w_p, w_c = ops.pack_mx4(rnd((width, 2048), torch.float32, 71, 0.2)), ops.pack_mx4(rnd((n_out, width), torch.float32, 72, 0.2))
+    h, norm = rnd((m, width), torch.float32, 73, 2.0), ops.NormParams(rnd((width,), torch.bfloat16, 74, 0.5), 1e-6, 1.0)
+    x64, p64, c64 = f64(x), f64(ops.expand_mx4(w_p, torch.float32)), f64(ops.expand_mx4(w_c, torch.float32))
+    h64, g = f64(h), f64(norm.weight) + 1.0
+    y = x64 @ p64.T
+    added = norm64(y, norm)
+    new = h64 + added
+    rows = norm64(new, norm)
+    s1, s2 = (1 / np.sqrt((v ** 2).mean(-1, keepdims=True) + norm.eps) for v in (y, new))
+    float_y = s1 * np.abs(g) * sum_tolerance(x64, p64, "bfloat16")
+    h_tol = np.abs(added) * (2.0 ** -8 + 2.0 ** -18) + float_y + 2.0 ** -22 * (np.abs(h64) + np.abs(new))
+    moved = np.linalg.norm(h_tol, axis=-1, keepdims=True) / np.linalg.norm(new, axis=-1, keepdims=True) + 2.0 ** -16
+    x_tol = s2 * np.abs(g) * (np.abs(h64) * 2.0 ** -8 + np.abs(added) * (2.0 ** -7 + 2.0 ** -15) + float_y) + np.abs(rows) * (2.0 ** -8 + moved) * (1 + 2.0 ** -7)
+    z_tol = x_tol @ np.abs(c64).T + sum_tolerance(rows, c64, "bfloat16")
+
+    status, first = torch.zeros(1, dtype=torch.int32, device=DEV), None
+    for _ in range(50):
+        operand = ops.scaled_rows(h, norm)
+        branch = ops.linear_branch(x, w_p, ops.BranchSink(h, norm, norm, operand), status=status)
+        h_out, following = torch.empty_like(h), torch.empty_like(operand)
+        z = ops.linear(ops.DeferredRows(branch, h_out, norm, following), w_c, out_dtype=torch.float32, status=status)
+        got = (z, h_out, following[:m])
+        assert first is None or all(torch.equal(a, b) for a, b in zip(got, first))
+        first = first or got
+    assert status.item() == 0
+    check(first[0], rows @ c64.T, z_tol, "product")
+    check(first[1], new, h_tol, "stream")
+
+
 def test_deferred_norms_keep_rows_apart():
     """A row that is not finite reaches its own results only; the others have the same bits without it."""
     m, width = 5, 512
