@@ -789,7 +789,7 @@ extern "C" int rdl_mx_few_rows_norm(void* out, int out_dtype, const void* x, con
     RDL_REQUIRE(!w->gated || rdl_gated_known(activation), "mx_few_rows_norm: unknown activation %d", activation);
     RDL_REQUIRE(softcap >= 0.f, "mx_few_rows_norm: soft-cap must not be negative");
     RDL_REQUIRE(a.vec, "mx_few_rows_norm: the operand needs a multiple of 8 columns and a 16-byte boundary");
-    RDL_REQUIRE(norm->n_sums > 0 && norm->n_out > 0 && norm->n_out <= 8 && (norm->row_index || norm->n_out <= m), "mx_few_rows_norm: %d units of sums, %d output rows", norm->n_sums, norm->n_out);
+    RDL_REQUIRE(norm->n_sums > 0 && norm->n_out > 0 && norm->n_out <= 8 && (norm->row_index || norm->n_out == m), "mx_few_rows_norm: %d units of sums, %d output rows of %d", norm->n_sums, norm->n_out, m);
     const bool side = norm->residual_out || norm->scaled_next;
     RDL_REQUIRE(!side || (norm->branch_in && norm->residual_in), "mx_few_rows_norm: the stream's update needs the branch and the stream");
     // other blocks still read the old one

@@ -421,6 +421,21 @@ def test_no_split_form_of_a_branch():
         library.check(lib.rdl_mx_few_rows_norm(None, 0, x.data_ptr(), w.handle, 2, 0, 0.0, 0.0, d, None, None))
 
 
+def test_a_product_behind_a_deferred_norm_has_all_rows_or_chosen_ones():
+    """Without a list of rows the output has as many as the operand; any other number is refused, whether clusters share a tile or not."""
+    lib, d = library.load(), library.DeferredNormArgs()
+    h = rnd((16, 1024), torch.bfloat16, 69)
+    for w in (ops.pack_mx4(rnd((64, 64), torch.float32, 65)), ops.pack_mx4(rnd((512, 1024), torch.float32, 65))):
+        d.mode, d.sums, d.n_sums = library.NORM_DEFERRED, torch.zeros(64, device=DEV).data_ptr(), 2
+        for rows, n_out in ((2, 1), (8, 7), (8, 1), (5, 4), (1, 2)):
+            d.n_out = n_out
+            out = torch.full((rows, w.rows), 7.0, device=DEV)
+            with pytest.raises(library.KernelError, match=f"{n_out} output rows of {rows}"):
+                library.check(lib.rdl_mx_few_rows_norm(out.data_ptr(), 0, h.data_ptr(), w.handle, rows, 0, 0.0, 0.0, d, None, None))
+            torch.cuda.synchronize()
+            assert (out == 7.0).all()
+
+
 @pytest.mark.parametrize("act", ["gelu_pytorch_tanh", "silu", "swish_limit"])
 @pytest.mark.parametrize("m,n,k,kind", [(1, 1, 32, "bfloat16"), (7, 37, 300, "bfloat16"), (16, 100, 5000, "float32"), (9, 64, 128, "mx8"), (17, 65, 128, "mx8"),
                                         (140, 190, 1003, "mx8"), (64, 33, 40, "mx8")])
