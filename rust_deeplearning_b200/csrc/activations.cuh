@@ -14,6 +14,18 @@
 static inline bool rdl_activation_known(int act) { return act == RDL_ACT_GELU_TANH || act == RDL_ACT_SILU; }
 static inline bool rdl_gated_known(int act) { return rdl_activation_known(act) || act == RDL_ACT_SWISH_LIMIT; }
 
+// the smaller and the larger of two values; a NaN on either side stays (fminf and fmaxf would give the other one)
+__device__ __forceinline__ float rdl_min(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float rdl_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // exact form: library tanh and exp
 __device__ __forceinline__ float rdl_activation(float x, int act) {
     switch (act) {
@@ -39,16 +51,16 @@ __device__ __forceinline__ float rdl_activation_fast(float x, int act) {
 // RDL_ACT_SWISH_LIMIT; unused by the others).
 __device__ __forceinline__ float rdl_gated(float g, float u, int act, float param) {
     if (act == RDL_ACT_SWISH_LIMIT) {
-        g = fminf(g, param);
-        u = fminf(fmaxf(u, -param), param);
+        g = rdl_min(g, param);
+        u = rdl_min(rdl_max(u, -param), param);
         return g / (1.0f + expf(-1.702f * g)) * (u + 1.0f);
     }
     return rdl_activation(g, act) * u;
 }
 __device__ __forceinline__ float rdl_gated_fast(float g, float u, int act, float param) {
     if (act == RDL_ACT_SWISH_LIMIT) {
-        g = fminf(g, param);
-        u = fminf(fmaxf(u, -param), param);
+        g = rdl_min(g, param);
+        u = rdl_min(rdl_max(u, -param), param);
         return __fdividef(g, 1.0f + __expf(fminf(-1.702f * g, 80.0f))) * (u + 1.0f);
     }
     return rdl_activation_fast(g, act) * u;
@@ -61,8 +73,8 @@ __device__ __forceinline__ float rdl_gated_near(float g, float u, int act, float
     if (act == RDL_ACT_GELU_TANH) t = g * fmaf(-0.10294324f, g * g, -2.3022082f);       // -2 z log2(e)
     else if (act == RDL_ACT_SILU) t = -1.4426950f * g;
     else {                                                                              // RDL_ACT_SWISH_LIMIT
-        g = fminf(g, param);
-        u = fminf(fmaxf(u, -param), param) + 1.0f;
+        g = rdl_min(g, param);
+        u = rdl_min(rdl_max(u, -param), param) + 1.0f;
         t = -1.702f * 1.4426950f * g;
     }
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
@@ -74,10 +86,10 @@ __device__ __forceinline__ float rdl_gated_near(float g, float u, int act, float
 // gated forms' default code 0 stays plain): relu2(x) = max(x, 0)^2, silu.
 static inline bool rdl_unary_known(int act) { return act == RDL_UNARY_RELU2 || act == RDL_UNARY_SILU; }
 __device__ __forceinline__ float rdl_unary(float x, int act) {
-    if (act == RDL_UNARY_RELU2) { const float r = fmaxf(x, 0.f); return r * r; }
+    if (act == RDL_UNARY_RELU2) { const float r = rdl_max(x, 0.f); return r * r; }
     return x / (1.0f + expf(-x));
 }
 __device__ __forceinline__ float rdl_unary_fast(float x, int act) {
-    if (act == RDL_UNARY_RELU2) { const float r = fmaxf(x, 0.f); return r * r; }
+    if (act == RDL_UNARY_RELU2) { const float r = rdl_max(x, 0.f); return r * r; }
     return __fdividef(x, 1.0f + __expf(fminf(-x, 80.0f)));
 }

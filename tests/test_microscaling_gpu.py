@@ -522,6 +522,30 @@ def test_infinities_and_nan(m, kind):
     assert np.isnan(got[:, 7]).all() and np.isfinite(np.delete(got, 7, axis=1)).all()
 
 
+@pytest.mark.parametrize("m,kind", [(4, "bfloat16"), (4, "float32"), (13, "bfloat16"), (16, "mx8"), (40, "mx8"), (300, "mx8")])
+def test_nan_passes_every_epilogue(m, kind):
+    """A row with a NaN gives NaN whatever follows its sums; the other rows keep their bits."""
+    x = rnd((m, 320), torch.float32, 90)
+    x[1, 40] = float("nan")
+    clean = x.clone()
+    clean[1] = 1.0
+    if kind == "mx8":
+        x, clean = ops.pack_mx8(x), ops.pack_mx8(clean)
+    else:
+        x, clean = (t.to(getattr(torch, kind)) for t in (x, clean))
+    w, gu = ops.pack_mx4(rnd((200, 320), torch.float32, 91)), ops.pack_mx4(rnd((2 * 100, 320), torch.float32, 92), gated=True)
+    calls = {"silu_plain": lambda v: ops.linear_mx4(v, w, activation="silu_plain"), "relu2": lambda v: ops.linear_mx4(v, w, activation="relu2"),
+             "soft-cap": lambda v: ops.linear_mx4(v, w, out_dtype=torch.float32, softcap=3.0)}
+    for act, param in (("gelu_pytorch_tanh", 0.0), ("silu", 0.0), ("swish_limit", 2.0)):
+        calls[act] = lambda v, act=act, param=param: ops.linear_gated_mx4(v, gu, act, param)
+        calls[act + " in 8 bits"] = lambda v, act=act, param=param: ops.linear_gated_mx4(v, gu, act, param, out_mx8=True).dequantise()
+    others = [i for i in range(m) if i != 1]
+    for name, call in calls.items():
+        got, want = call(x), call(clean)
+        assert got[1].isnan().all(), name
+        assert torch.isfinite(want).all() and torch.equal(got[others], want[others]), name
+
+
 def test_a_row_does_not_depend_on_the_others():
     w = ops.pack_mx4(rnd((300, 1000), torch.float32, 16))
     x, _ = rows_for(16, 1000, "bfloat16", 17)
