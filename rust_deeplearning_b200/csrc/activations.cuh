@@ -67,7 +67,10 @@ __device__ __forceinline__ float rdl_gated_fast(float g, float u, int act, float
 }
 
 // For results that are rounded to bfloat16 or to 8 bits with a scale: 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z)), by the hardware's powers of two and
-// reciprocal, good to 2^-20.  (The hardware's tanh, at 2^-11, moves one 8-bit code in a thousand.)
+// reciprocal.  With t the power of two's exponent the result is off by at most 2^-20.5 + 2^-22 |t| of itself: what the hardware's two
+// functions and the products round, and what t was rounded by, which the power passes on.  From t = 126 on it is zero (g below -87, for GELU
+// -10, for the limited form -51).
+// (The hardware's tanh, at 2^-11, moves one 8-bit code in a thousand.)
 __device__ __forceinline__ float rdl_gated_near(float g, float u, int act, float param) {
     float t, e, r;
     if (act == RDL_ACT_GELU_TANH) t = g * fmaf(-0.10294324f, g * g, -2.3022082f);       // -2 z log2(e)

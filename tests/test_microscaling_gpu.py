@@ -460,6 +460,65 @@ def test_gated(m, n, k, kind, act):
     assert not rows._data.view(torch.uint8)[:m, n:].any() and not rows.scales.reshape(m, -1)[:, -(-n // 32):].any()
 
 
+@pytest.mark.parametrize("m,kind", [(3, "bfloat16"), (16, "bfloat16"), (16, "mx8"), (40, "mx8"), (300, "mx8")])
+def test_the_parts_of_a_row_are_the_row(m, kind):
+    """A matrix with a single one in every row hands the rows through: nothing but how they enter shows.  bfloat16 values above 2^-13 of the
+    largest of their group are exact, the others off by 2^-21 of it; 8-bit values are exact."""
+    k = 200
+    x = rnd((m, k), torch.float32, 100) * torch.exp2(torch.randint(-17, 1, (m, k), generator=torch.Generator().manual_seed(101)).float()).to(DEV)
+    _enters(x, kind, 2.0 ** -21)
+
+
+@pytest.mark.parametrize("m", [1, 8, 9, 16])
+def test_the_parts_of_a_float32_row_are_the_row(m):
+    """As above: float32 values above 2^-13 of the largest of their group are exact to the last bit, the others off by 2^-37 of it."""
+    x = rnd((m, 200), torch.float32, 102) * torch.exp2(torch.randint(-30, 1, (m, 200), generator=torch.Generator().manual_seed(103)).float()).to(DEV)
+    _enters(x, "float32", 2.0 ** -37)
+
+
+def _enters(x, kind, below):
+    m, k = x.shape
+    rows = ops.pack_mx8(x) if kind == "mx8" else x.to(getattr(torch, kind))
+    want = f64(rows.dequantise() if kind == "mx8" else rows)
+    got = f64(ops.linear_mx4(rows, ops.pack_mx4(torch.eye(k, device=DEV)), out_dtype=torch.float32))
+    top = np.repeat(np.abs(plain.groups_of(want)).max(-1), 32, axis=1)[:, :k]
+    exact = np.abs(want) >= top * (0.0 if kind == "mx8" else 2.0 ** -13)
+    assert np.array_equal(got[exact], want[exact])
+    assert (np.abs(got - want) <= below * top).all()
+
+
+@pytest.mark.parametrize("act,param", [("gelu_pytorch_tanh", 0.0), ("silu", 0.0), ("swish_limit", 3.0)])
+@pytest.mark.parametrize("m,kind", [(5, "bfloat16"), (16, "bfloat16"), (16, "mx8"), (40, "mx8"), (300, "mx8")])
+def test_the_gate_itself(m, kind, act, param):
+    """Matrices with a single one in every row: the gate's and the other half's sums are known exactly, and what is left is the
+    activation, in bfloat16 (2^-8) and in 8 bits, where a value takes the code of a value this near.
+
+    With t = -log2(e) times what the sigmoid is taken of: off by 2^-20.5 + 2^-22 |t| of the result, zero where that is below 2^-126; up to
+    16 rows whose result is in 8 bits take the library's functions in float32: 2^-22 |g u|."""
+    gen = torch.Generator().manual_seed(110)
+    g, u = (torch.rand((m, 64), generator=gen) - 0.5) * 19.0, (torch.rand((m, 64), generator=gen) + 0.25) * 2.0
+    g = torch.where(g.abs() < 0.01, torch.full_like(g, 0.25), g)
+    x = torch.cat([g, u], dim=1).to(DEV)
+    x = ops.pack_mx8(x) if kind == "mx8" else x.to(torch.bfloat16)
+    y = f64(x.dequantise() if kind == "mx8" else x)
+    w = ops.pack_mx4(torch.eye(128, device=DEV), gated=True)
+    g, u = np.split(y, 2, axis=-1)
+    # 0.5 (1 + tanh z) as 1 / (1 + exp(-2 z)): far below zero the sum with one would lose the result in 64 bits too
+    want = g * u / (1 + np.exp(-2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3))) if act == "gelu_pytorch_tanh" else plain.gated(y, act, param)
+    t = {"silu": g, "swish_limit": 1.702 * np.minimum(g, param)}.get(act, 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)) / np.log(2)
+    near = np.abs(want) * (2.0 ** -20.5 + 2.0 ** -22 * np.abs(t)) + np.abs(g) * (u + 1) * 2.0 ** -126
+    check(ops.linear_gated_mx4(x, w, act, param), want, near + (np.abs(want) + near) * 2.0 ** -8, act)
+    if m <= 16:
+        near = near + np.abs(g) * (u + 1) * 2.0 ** -22
+    rows = ops.linear_gated_mx4(x, w, act, param, out_mx8=True)
+    codes = plain.scale_codes(plain.groups_of(want), plain.E4M3[-1])
+    assert np.array_equal(rows.scales.reshape(m, -1)[:, :2].cpu().numpy(), codes)
+    scale = np.repeat(2.0 ** (codes - 127.0), 32, axis=1)                # a value this near must not move the group's scale
+    low, high = (np.sign(v) * plain.E4M3[plain.nearest(np.abs(v) / scale, plain.E4M3)] * scale for v in (want - near, want + near))
+    got = f64(rows.dequantise())
+    assert (got >= low).all() and (got <= high).all(), act + " in 8 bits"
+
+
 @pytest.mark.parametrize("m,kind", [(3, "bfloat16"), (12, "float32"), (16, "mx8"), (50, "mx8")])
 def test_epilogues(m, kind):
     w = ops.pack_mx4(rnd((90, 256), torch.float32, 11, 0.2))
