@@ -591,6 +591,7 @@ def linear(x, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
         x = x.materialise()
         if type(weight) is Mx4Weight:
             return linear_mx4(x, weight, out_dtype, softcap, status, activation)
+    _need(type(x) is not Mx8Rows, "linear: rows in 8 bits go with a 4-bit weight")
     _need(x.dim() == 2 and weight.dim() == 2 and x.shape[1] == weight.shape[1],
           f"linear: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not fit")
     _need(x.dtype is weight.dtype, f"linear: input is {x.dtype}, weight is {weight.dtype}")
@@ -622,6 +623,7 @@ def linear_gated(x, weight_gate_up: torch.Tensor, activation: str, status: Optio
     if type(weight_gate_up) is Mx4Weight and not isinstance(x, DeferredRows):
         x = _rows_for_mx4(x)
         return linear_gated_mx4(x, weight_gate_up, activation, param, type(x) is Mx8Rows, status)
+    _need(type(x) is not Mx8Rows, "linear_gated: rows in 8 bits go with a 4-bit weight")
     _need(activation in GATED_FORMS, f"unknown activation '{activation}', known: {sorted(GATED_FORMS)}")
     _need(weight_gate_up.shape[0] % 2 == 0, "linear_gated: the weight must hold gate rows and as many up rows")
     if isinstance(x, DeferredRows):

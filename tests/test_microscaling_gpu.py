@@ -735,3 +735,10 @@ def test_refusals():
             call()
     assert ops.linear_mx4(x[:0], w).shape == (0, 32) and ops.linear_mx4(ops.pack_mx8(x[:0]), w).shape == (0, 32)
     assert ops.linear_gated_mx4(x[:0], g, "silu", out_mx8=True).shape == (0, 16)
+
+
+def test_rows_in_8_bits_go_with_a_4_bit_weight():
+    x, w = ops.pack_mx8(rnd((20, 64), torch.bfloat16, 28)), rnd((32, 64), torch.bfloat16, 29)
+    for call in (lambda: ops.linear(x, w), lambda: ops.linear_gated(x, w, "silu"), lambda: ops.linear_branch(x, w, None)):
+        with pytest.raises(library.KernelError, match="4-bit weight"):
+            call()
