@@ -1820,7 +1820,8 @@ MX_GROUP, MX_BLOCK, MX_ROWS = 32, 128, 128
 MX_FEW_ROWS = 16         # up to this many rows the few-row kernel runs, which also takes tensors; above, 8-bit rows only
 _MX8 = 2                 # rows of 8 bits, where a kernel's argument says of what kind its rows are
 _KINDS = {torch.float32: 0, torch.bfloat16: 1}
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # what torch.cuda.current_stream(i).cuda_stream gives, in a thirtieth of the time
+# what torch.cuda.current_stream(i).cuda_stream gives, in a thirtieth of the time, where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _blocks(columns: int) -> int:

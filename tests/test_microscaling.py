@@ -46,3 +46,15 @@ def test_the_smallest_scale_that_cuts_nothing_off():
 
 def test_weight_formats_are_named():
     assert WEIGHT_FORMATS == ("mx4", "mx4+head")
+
+
+def test_the_stream_without_torchs_short_cut(monkeypatch):
+    """torch builds that lack the raw-stream function: the stream's number comes the long way."""
+    import importlib.util
+    import types
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    spec = importlib.util.spec_from_file_location("rust_deeplearning_b200.kernels.ops_again", ops.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index: types.SimpleNamespace(cuda_stream=100 + index))
+    assert again._raw_stream(3) == 103
