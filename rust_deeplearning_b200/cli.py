@@ -47,7 +47,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16",
                    help="bfloat16: the serving kernels; float32: everything in true 32-bit.")
     p.add_argument("--weights", choices=["as-stored", "mx4", "mx4+head"], default="as-stored",
-                   help="mx4: the projections in 4 bits with a scale a group of 32 (mx4+head: the output head too).")
+                   help="mx4: the attention's and the dense feed-forwards' matrices in 4 bits with a scale a group of 32; other parts keep "
+                        "theirs (mx4+head: the output head too).  In bfloat16, steps of more than 16 rows (prompts, batches of more than 16 "
+                        "sequences) round what enters these matrices to 8 bits, smaller ones nothing.")
     p.add_argument("--stop-ids", default=None, help="Stop token ids (default: the model's end-of-sequence ids).")
     p.add_argument("--max-context", type=int, default=None, help="Longest sequence the cache is sized for.")
     p.add_argument("--timings", action="store_true", help="Print the device time of every step (CUDA events) to stderr.")

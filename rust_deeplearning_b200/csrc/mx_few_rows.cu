@@ -23,15 +23,15 @@
 // rows: both halves of the operand are rows of the product, and a row's two sums are joined on their way out of tensor memory, so
 // that nothing waits for the partial sums.  5 to 8 rows: that would be 16 rows to make parts of; the halves are joined first, x = s2 (ht + s1 at),
 // rounded to bfloat16.  Output projection, gated product, down projection and next projection of a layer with the norms between: width
-// 2,304 1 row 27.6 us (29.9 with kernels for the norms), 8 rows 32.0 (34.6); width 3,584 40.1 (46.5), 46.9 (52.0); 4,608 74.9 (82.0), 83.6 (89.6).
+// 2,304 1 row 28.5 us (29.9 with kernels for the norms), 8 rows 32.7 (34.7); width 3,584 40.9 (45.1), 47.2 (51.3); 4,608 74.7 (79.3), 83.4 (87.6).
 //
 // The loops that make parts and write results are not unrolled.  In a step this kernel's forms alternate with one another and with other
 // kernels, and each starts with instructions that are not at hand: with the loops unrolled a pair of forms took 0.5 to 2.2 us more than
 // each of them alone, and now 0 to 0.4.
 //
-// Measured on the device, one bfloat16 row: 256,000 outputs of 2,304 columns (313 MB) 52.4 us, 6.0 TB/s; 28,672 of 3,584, gated, 14.0 us,
-// 3.9 TB/s; 4,096 of 2,304 (5 MB) 5.5 us: there what bounds it is the chain of a launch, the first copy, the products of a block's columns
-// and the exchange in the cluster.  16 rows: 59.1, 19.1 and 6.9 us (in 8 bits already: 57.1, 16.2 and 6.0).
+// Measured on the device, one bfloat16 row: 256,000 outputs of 2,304 columns (313 MB) 52.1 us, 6.0 TB/s; 28,672 of 3,584, gated, 14.0 us,
+// 3.9 TB/s; 4,096 of 2,304 (5 MB) 5.4 us: there what bounds it is the chain of a launch, the first copy, the products of a block's columns
+// and the exchange in the cluster.  16 rows: 58.6, 20.2 and 6.9 us (in 8 bits already: 56.7, 16.2 and 6.0; float32: 172, 39.7 and 8.1).
 #include <cuda_fp16.h>
 
 #include "activations.cuh"
@@ -165,7 +165,7 @@ constexpr int ROW_FINE = 0, ROW_ZERO = 1, ROW_TINY = 2, ROW_BAD = 3;
 // The parts of a chunk as e4m3 bytes, and the scale codes of its group; the four lanes of a group come here together.  A part is what the
 // parts before it leave, rounded to four bits, which leaves at most a 2^-4 of the largest: so the next one's scale is 2^4 smaller.
 // (Cut off instead of rounded, and not converted back, values below 2^-13 lost up to 2^-17 of the largest; 8 rows x 2,304, 18,432 gated
-// outputs took 8.65 us and take 8.9.)
+// outputs took 8.65 us, and 8.7 to 8.9 so.)
 template <int PARTS>
 __device__ __forceinline__ int make_parts(const Chunk<PARTS>& d, uint2 (&bytes)[PARTS], uint32_t (&code)[PARTS]) {
     if constexpr (PARTS == 1) {
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             int s = 0, piece = first_tile * a.blocks + b0;   // place in the ring; block of columns over all tiles
             uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
             // A short ring keeps too few bytes on their way: L2 is asked for what will be loaded up to AHEAD_L2 stages later (16 rows x 3,584,
-            // 28,672 gated outputs, two stages: 24.9 -> 21.8 us; with five stages it costs: 1 row x 2,304, 18,432 outputs 7.1 -> 8.1).
+            // 28,672 gated outputs, two stages: 24.9 -> 21.8 us in the form of that time; with five stages it costs: 1 row x 2,304, 18,432 outputs 7.1 -> 8.1).
             int ask_tile = a.stages < 4 ? first_tile : a.tiles, ask_kb = b0, asked = 0;
             auto ask = [&]() {
                 if (ask_tile >= a.tiles || b0 >= b1) return;
@@ -694,8 +694,8 @@ int plan(FewArgs& a, const Mx4Matrix& w) {
     a.share = ((a.gated ? MX_ROWS / 2 : MX_ROWS) + a.split - 1) / a.split;
     a.slice_blocks = (a.blocks + a.split - 1) / a.split;
     const int sums = a.split > 1 ? R * (MX_ROWS + 16) * 4 : 0, most = 226 * 1024 - 1024 - (behind_norm(MODE) ? 2048 : 1024) - sums;    // alignment, static shared memory
-    // The rows of all of a block's columns, if a ring of two stages fits beside them (float32, 8 rows x 2,304, 256,000 outputs: 71 us so and 94
-    // with the rows brought anew for every tile; bfloat16, 16 x 3,584, 28,672 gated: 20.5 and 23.0); else as many as fit beside four.
+    // The rows of all of a block's columns, if a ring of two stages fits beside them (in the form of that time float32, 8 rows x 2,304, 256,000 outputs: 71 us so
+    // and 94 with the rows brought anew for every tile; bfloat16, 16 x 3,584, 28,672 gated: 20.5 and 23.0; now 62.7 and 20.2); else as many as fit beside four.
     a.slots = (a.slice_blocks + STEP - 1) / STEP * STEP;
     if (a.slots * PER_BLOCK + 2 * PER_STAGE > most) a.slots = (most - 4 * PER_STAGE) / PER_BLOCK / STEP * STEP;
     if (a.slots > MAX_SLOTS) a.slots = MAX_SLOTS;

@@ -18,7 +18,8 @@
 // form's tile is 128 gate and 128 up rows of the same 128 outputs; its result may leave as 8-bit rows with scales: 32 outputs of a
 // row lie in one thread, which is a group.
 //
-// Measured: gate and up of the 2B shape, 2,048 rows to 8 bits, 56.8 us, 3.1 PFLOP/s; 8,192 rows x 36,864 x 4,608 outputs 868 us, 3.2 PFLOP/s.
+// Measured: gate and up of the 2B shape, 2,048 rows to 8 bits, 56.5 us, 3.1 PFLOP/s; 8,192 rows x 36,864 x 4,608 outputs 865 us, 3.2 PFLOP/s
+// (1,020 to 1,050 us, 2.7 PFLOP/s, when such calls go on for seconds and the power limit lowers the clock).
 // The tensor cores bound it: 530 cycles a block of columns, of which the products take 513, at the clock that the power limit leaves; between
 // two tiles they wait 1,100 cycles, from their end until the accumulator is in registers.
 //

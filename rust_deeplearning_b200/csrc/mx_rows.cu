@@ -8,11 +8,11 @@
 // a group is eight lanes of a warp and a block of 128 columns one warp: the largest magnitude is three shuffles away and the four
 // scale codes of a block leave as one word.  The threads a row gets depend on its width alone, so its result does
 // not depend on how many rows a step has.
-// Measured: 8,192 float32 rows of 4,608 (492 MB) 75.6 us, 6.5 TB/s; 2,048 bfloat16 rows of 2,304 with both norms (52 MB) 11.2 us; 17 rows 3.6 us.
+// Measured: 8,192 float32 rows of 4,608 (492 MB) 75.6 us, 6.5 TB/s; 2,048 bfloat16 rows of 2,304 with both norms (52 MB) 11.2 us; 17 rows 3.5 us.
 //
-// rdl_pack_mx4: a matrix to 4 bits, padding and all.  Memory bound: 36,864 x 4,608 bfloat16 (430 MB) 87 us, 4.9 TB/s.
+// rdl_pack_mx4: a matrix to 4 bits, padding and all.  Memory bound: 36,864 x 4,608 bfloat16 (430 MB) 76 us, 5.7 TB/s.
 // rdl_lay_mx4, rdl_lay_mx8: a matrix or rows that came in these formats, to the products' layout: 36,864 x 4,608 codes
-// (175 MB) 52 us, 3.4 TB/s.
+// (180 MB) 52 us, 3.5 TB/s; 8,192 rows of 4,608 in 8 bits (78 MB) 15.6 us, 5.0 TB/s.
 // rdl_expand_mx4: the values the codes stand for; exact in bfloat16 for scales from 2^-125 up to 2^125.  The same matrix 71 us, 6.1 TB/s.
 #include <cuda_fp16.h>
 

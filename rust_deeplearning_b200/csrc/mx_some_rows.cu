@@ -13,7 +13,7 @@
 // columns; when all are done they send their sums through distributed shared memory, over what was the ring, to the block that adds
 // up that part of the outputs, in rank order.  Every wait is bounded.
 //
-// Measured: 64 rows x 2,304 x 4,096 outputs 7.5 us, x 14,336 x 3,584 12.8 us (27 MB of weights, 2.2 TB/s); 128 rows 10.8 and 15.8 us.
+// Measured: 64 rows x 2,304 x 4,096 outputs 7.6 us, x 14,336 x 3,584 12.7 us (27 MB of weights, 2.2 TB/s); 128 rows 10.5 and 15.7 us.
 #include <atomic>
 
 #include "activations.cuh"

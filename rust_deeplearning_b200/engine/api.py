@@ -32,8 +32,10 @@ def load_model(folder: str, dtype: Union[str, torch.dtype] = "bfloat16", device=
     """A model folder (config.json + model.safetensors) -> a model on the device.  The model class
     is chosen by config.json.  dtype "bfloat16": the serving kernels; "float32": everything in
     true 32-bit.  strict False: tensors the model does not read are skipped with a warning instead
-    of being an error.  weight_format: "mx4" rounds the projections to 4 bits with a scale a group of 32 as they are loaded, "mx4+head"
-    the output head too (None: as they are; see `Model`)."""
+    of being an error.  weight_format: "mx4" rounds the matrices of the parts that offer it (plain attention, dense feed-forwards) to 4
+    bits with a scale a group of 32 as they are loaded, "mx4+head" the output head's too; other parts keep theirs (None: all do; see
+    `Model`).  With it a bfloat16 step of more than 16 rows rounds what enters these matrices to 8 bits, a smaller one does not, so a
+    sequence's logits depend on which of the two its step is."""
     dev = _require_cuda(device)
     dtype = parse_dtype(dtype)
     raw = read_config_json(folder)

@@ -619,7 +619,8 @@ def linear_gated(x, weight_gate_up: torch.Tensor, activation: str, status: Optio
     """act(x Wg^T) * (x Wu^T) for the row-concatenated matrix [Wg; Wu] ([2I, in]) -> [rows, I]; or another form of
     `GATED_FORMS` (param: its parameter).
     In bfloat16 this is one kernel (the activation is the product's epilogue); otherwise a product
-    and the gated activation kernel.  A 4-bit weight: as in `linear`; rows in 8 bits give a result in 8 bits, for the product behind."""
+    and the gated activation kernel.  A 4-bit weight: as in `linear`; rows in 8 bits give a result in 8 bits (`Mx8Rows`), for
+    the product behind, and so do more than 16 bfloat16 rows, which are rounded to 8 bits first (`linear_gated_mx4` leaves them as they are)."""
     if type(weight_gate_up) is Mx4Weight and not isinstance(x, DeferredRows):
         x = _rows_for_mx4(x)
         return linear_gated_mx4(x, weight_gate_up, activation, param, type(x) is Mx8Rows, status)
