@@ -26,7 +26,10 @@ namespace {
 constexpr int THREADS = 320, EPI = 256, MAX_STAGES = 6, SCALE_BUFS = 4, ROWS = 128;
 constexpr int STAGE_BYTES = 2 * MX_TILE_BYTES + 2 * MX_SCALE_BYTES;                   // codes | rows | scales of both
 constexpr int STAGE_TX = MX_TILE_TX + MX_TILE_BYTES + 2 * MX_SCALE_BYTES;
-constexpr int TMEM_COLS = 512, SCALES_AT = 2 * ROWS;                                  // two accumulators of 128 columns, then scales
+// Tensor memory: two accumulators of 128 columns, then scales; in a cluster, where a block has one tile, one accumulator (the reason stands in mx_tensor.cuh)
+constexpr int TMEM_COLS = 512, CLUSTER_TMEM_COLS = 256, CLUSTER_STAGES = 3;
+static_assert(2 * ROWS + SCALE_BUFS * 8 <= TMEM_COLS && ROWS + SCALE_BUFS * 8 <= CLUSTER_TMEM_COLS && 2 * CLUSTER_TMEM_COLS <= 512, "columns of tensor memory");
+static_assert(3 * (CLUSTER_STAGES * STAGE_BYTES + 1024) > 228 * 1024, "no three blocks of clusters on a multiprocessor");
 constexpr int OUTS_MOST = MX_ROWS + 16;                                               // weight rows of a tile over all blocks of a cluster, rounded up
 // floats from a weight row's sums to the next one's: 16 bytes beyond whole lines, so that neighbouring lanes use different banks
 __host__ __device__ constexpr int sums_pitch(int m) { return (m + 31) / 32 * 32 + 4; }
@@ -81,6 +84,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_some_rows_kernel(const __grid_c
     const int rank = a.split > 1 ? (int)(blockIdx.x % a.split) : 0;
     const int first_tile = blockIdx.x / a.split, tile_step = gridDim.x / a.split;
     const int b0 = min(rank * a.slice_blocks, a.blocks), b1 = min(b0 + a.slice_blocks, a.blocks);
+    const uint32_t tmem_cols = a.split > 1 ? CLUSTER_TMEM_COLS : TMEM_COLS, scales_at = a.split > 1 ? ROWS : 2 * ROWS;
     // shared memory: of each stage codes and rows | of each stage the scales of both
     const uint32_t ring_s = mx_smem(smem), scales_s = ring_s + (uint32_t)(a.stages * 2 * MX_TILE_BYTES);
     {
@@ -91,7 +95,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_some_rows_kernel(const __grid_c
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mx_smem(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mx_smem(&tmem_slot)), "r"(tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     mx_fence_before();
@@ -147,7 +151,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_some_rows_kernel(const __grid_c
                 if (!mx_warp_wait(mx_smem(&full_bar[s]), parity, a.wait_cycles, gave_up_v)) { ok = false; break; }
                 mx_fence_after();
                 if (mx_elect()) {
-                    const uint32_t sa = tmem + SCALES_AT + (uint32_t)scale_buf * 8, sb = sa + 4, at = ring_s + (uint32_t)(s * 2 * MX_TILE_BYTES);
+                    const uint32_t sa = tmem + scales_at + (uint32_t)scale_buf * 8, sb = sa + 4, at = ring_s + (uint32_t)(s * 2 * MX_TILE_BYTES);
                     const uint64_t sc = mx_scale_desc(scales_s + (uint32_t)(s * 2 * MX_SCALE_BYTES));
                     copy_scales(sa, sc);
                     copy_scales(sb, sc + (MX_SCALE_BYTES >> 4));
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_some_rows_kernel(const __grid_c
     if (*gave_up_v && threadIdx.x == 0) mx_drain();
     mx_fence_before();
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
 }
 
 }  // namespace
@@ -288,6 +292,7 @@ extern "C" int rdl_mx_some_rows(void* out, int out_dtype, const void* x, const v
     const int turns = a.split > 1 ? 1 : (a.tiles + sms - 1) / sms, sums = a.split > 1 ? OUTS_MOST * sums_pitch(m) * 4 : 0;
     a.stages = (long long)turns * a.slice_blocks < MAX_STAGES ? turns * a.slice_blocks : MAX_STAGES;
     if (a.stages * STAGE_BYTES < sums) a.stages = (sums + STAGE_BYTES - 1) / STAGE_BYTES;
+    if (a.split > 1 && a.stages < CLUSTER_STAGES) a.stages = CLUSTER_STAGES;
     const int smem = 1024 + a.stages * STAGE_BYTES;
     cudaStream_t st = (cudaStream_t)stream;
     RDL_CUDA(rdl_allow_shared<mx_some_rows_kernel>(smem), "mx_some_rows");

@@ -14,6 +14,14 @@
 #include "common.cuh"
 #include "microscaling.cuh"
 
+// Tensor memory.  A block whose columns are taken waits in tcgen05.alloc until a block that has them ends, for as long as that takes.  Blocks of
+// a cluster wait for one another, so two clusters on the same multiprocessors, each with the columns the other one's block waits for,
+// would never end.  So: what blocks of clusters can be on one multiprocessor together never wants more than its 512 columns.  Few rows: 128
+// columns, at most three blocks by their threads (16 float32 rows: 256, one block by its registers).  Up to 128 rows, shared by a
+// cluster: 256 columns, and shared memory of three stages, so that there is room for two of them, or for one beside blocks of few rows, of which
+// registers allow one.  Pairs of many rows: 512, and no room in shared memory beside them.  Blocks without a cluster may take what
+// they want: they wait for nobody once they have it.
+
 // A 4-bit weight on the host's side: made once, when the weight is laid out.
 struct alignas(64) Mx4Matrix {
     CUtensorMap codes_map;                       // [tile x block x row][128 codes], a box is a tile

@@ -646,6 +646,28 @@ def test_another_stream_and_a_graph():
     assert gw.gated
 
 
+def test_clusters_of_several_streams():
+    """Products whose tiles are shared by clusters, on streams of their own at the same time: blocks of different ones meet on a multiprocessor, every
+    call ends and has the bits it has alone."""
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    calls = []
+    for i, (m, n, k, gated) in enumerate([(40, 2304, 2304, False), (128, 700, 1100, False), (17, 2048, 600, True), (64, 300, 9000, False), (5, 1200, 2304, False), (16, 400, 700, False)]):
+        w = ops.pack_mx4(rnd((n, k), torch.float32, 120 + i, 0.1), gated=gated)
+        x = ops.pack_mx8(rnd((m, k), torch.bfloat16, 130 + i)) if m > 16 else rnd((m, k), torch.bfloat16, 130 + i)
+        call = (lambda x=x, w=w: ops.linear_gated_mx4(x, w, "silu", status=status)) if gated else (lambda x=x, w=w: ops.linear_mx4(x, w, status=status))
+        calls.append((torch.cuda.Stream(), call, call()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        results = [[] for _ in calls]
+        for _ in range(10):
+            for (stream, call, _), out in zip(calls, results):
+                with torch.cuda.stream(stream):
+                    out.append(call())
+        torch.cuda.synchronize()
+        assert all(torch.equal(r, want) for (_, _, want), out in zip(calls, results) for r in out)
+    assert status.item() == 0
+
+
 def test_a_product_right_behind_the_packing():
     """The weights are read before the kernel ahead has ended: the packing keeps that safe by itself."""
     x = rnd((8, 2304), torch.bfloat16, 24)
