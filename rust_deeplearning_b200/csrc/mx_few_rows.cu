@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             unsigned long long policy;                       // read once a step: first to leave L2
             asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
             int s = 0, piece = first_tile * a.blocks + b0;   // place in the ring; block of columns over all tiles
+            bool behind = false;                             // the kernel ahead has ended
             uint32_t parity = 1, extra = (uint32_t)a.test_extra_tx;      // the first round finds every place free
             // A short ring keeps too few bytes on their way: L2 is asked for what will be loaded up to AHEAD_L2 stages later (16 rows x 3,584,
             // 28,672 gated outputs, two stages: 24.9 -> 21.8 us in the form of that time; with five stages it costs: 1 row x 2,304, 18,432 outputs 7.1 -> 8.1).
@@ -307,7 +308,12 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
                     ask();
                     kb += n;
                     piece += n;
-                    if (++s == a.stages) { s = 0; parity ^= 1; }
+                    if (++s == a.stages) {
+                        // the ring is full: waits from here on are for products, which wait for the kernel ahead, and its time is not to count
+                        if (!behind) { rdl_grid_wait(); behind = true; }
+                        s = 0;
+                        parity ^= 1;
+                    }
                 }
             }
         }
@@ -315,6 +321,7 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
     } else if (warp == 1) {
         // ---- scales to tensor memory, and the products ----
         if (mx_elect()) {
+            rdl_grid_wait();                                 // as the rows do: the waits here count from then on
             int s = 0, lt = 0, scale_buf = 0, g = 0;         // g: the rows' group
             uint32_t parity = 0, x_parity = 0;
             for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++lt) {

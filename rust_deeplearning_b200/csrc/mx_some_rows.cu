@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx_some_rows_kernel(const __grid_c
         }
     } else if (warp == 1) {
         // ---- scales to tensor memory, and the products ----
+        rdl_grid_wait();                                     // as the rows do: the waits here count from then on
         int s = 0, lt = 0, scale_buf = 0;
         uint32_t parity = 0;
         for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++lt) {

@@ -698,6 +698,27 @@ def test_a_wait_that_runs_out(m, k, code, name):
     assert status.item() == 0
 
 
+@pytest.mark.parametrize("m,n,k,code", [(8, 300, 9000, 8), (3, 19001, 1300, 8), (16, 19001, 4700, 8), (40, 300, 4096, 10), (100, 19001, 512, 10), (17, 19001, 300, 10)])
+def test_a_long_kernel_ahead_is_no_wait_in_vain(m, n, k, code):
+    """A product begins while the kernel ahead of it still runs; however long that takes, none of its waits counts it.  The kernel ahead: one tile of a
+    million columns, over 2 ms, twenty times what the waits are given here."""
+    lib, status = library.load(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    ahead, rows = ops.pack_mx4(torch.ones((256, 1 << 20), device=DEV)), ops.pack_mx8(torch.ones((200, 1 << 20), dtype=torch.bfloat16, device=DEV))
+    w = ops.pack_mx4(rnd((n, k), torch.float32, 140, 0.1))
+    x = rnd((m, k), torch.bfloat16, 141)
+    x = ops.pack_mx8(x) if m > 16 else x
+    want = ops.linear_mx4(x, w)
+    for _ in range(3):
+        try:
+            lib.rdl_set_wait_test(code, 200_000, 0)
+            first = ops.linear_mx4(rows, ahead, out_dtype=torch.float32)
+            got = ops.linear_mx4(x, w, status=status)
+            torch.cuda.synchronize()
+        finally:
+            lib.rdl_set_wait_test(0, 0, 0)
+        assert status.item() == 0 and torch.equal(got, want) and (first == float(1 << 20)).all()
+
+
 def test_tensors_that_start_anywhere():
     """Contiguous rows at an odd place of their memory: the same results as aligned ones."""
     w = rnd((70, 200), torch.float32, 33, 0.05)
