@@ -193,7 +193,11 @@ __global__ void __launch_bounds__(ST_THREADS, 2) gemm_stream_kernel(const __grid
                     __syncwarp(0xffffu);
                     if (row_ok) st_bulk_load(tiles_s + (uint32_t)(s * ST_TILE_BYTES + lane * ST_PITCH), a.w + row * K + k0, bytes, full_s + 8 * s, policy);
                     first_copy = false;
-                    if (++s == stages) { s = 0; ++round; }
+                    if (++s == stages) {
+                        s = 0;
+                        // the ring is full: waits from here on are for the readers, which wait for the kernel ahead, and its time is not to count
+                        if (round++ == 0) rdl_grid_wait();
+                    }
                 }
                 if (*gave_up_v) break;
             }

@@ -147,3 +147,23 @@ def test_engine_names_the_kernel_that_gave_up():
     for t in range(30, 40):
         mh.assert_logits(eng.step([slot], [[ids[t]]], "last"), want[t:t + 1], "bfloat16", f"position {t} after the fault")
     eng.check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 304, 9000), (3, 19001, 1304), (16, 19001, 4704), (1, 40000, 2304)])
+def test_a_long_kernel_ahead_of_the_streaming_product_is_no_wait_in_vain(m, n, k):
+    """The product begins while the kernel ahead of it still runs; however long that takes, its copying warp's waits do not count it.  The kernel
+    ahead: one tile of a million columns, over 2 ms, twenty times what the waits are given here."""
+    lib, status = library.load(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    ahead, rows = ops.pack_mx4(torch.ones((256, 1 << 20), device=DEV)), ops.pack_mx8(torch.ones((200, 1 << 20), dtype=torch.bfloat16, device=DEV))
+    g = torch.Generator().manual_seed(150)
+    w, x = (torch.randn(shape, generator=g).to(torch.bfloat16).to(DEV) for shape in ((n, k), (m, k)))
+    want = ops.linear(x, w)
+    for _ in range(3):
+        try:
+            lib.rdl_set_wait_test(7, SHORT_WAIT, 0)
+            ops.linear_mx4(rows, ahead)
+            got = ops.linear(x, w, status=status)
+            torch.cuda.synchronize()
+        finally:
+            lib.rdl_set_wait_test(0, 0, 0)
+        assert status.item() == 0 and torch.equal(got, want)
