@@ -331,8 +331,7 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) moe_gate_up_kernel(T* __restr
     const float in_w = sel_w ? sel_w[p] : 1.0f;
     if (activation >= 16) {
         const float u = warp_sum(lane_dot<T>(w + ((long long)e * ff + j) * width, row, width, lane)) * in_w;
-        const float r = fmaxf(u, 0.f);
-        if (lane == 0) mid[(long long)p * ff + j] = from_float<T>(activation == RDL_UNARY_RELU2 ? r * r : u / (1.0f + expf(-u)));
+        if (lane == 0) mid[(long long)p * ff + j] = from_float<T>(rdl_unary(u, activation));
         return;
     }
     const T* wg = w + ((long long)e * 2 * ff + j) * width;

@@ -781,3 +781,21 @@ def test_sampling_writes_pinned_host_memory_and_upload_takes_fed_tokens():
     want[tokens_at:tokens_at + n_fed] = torch.tensor([500, 100, 300], dtype=torch.int32)
     want[n - 64:] = -7
     assert torch.equal(dst.cpu(), want)
+
+
+@pytest.mark.parametrize("form,param", [("relu2", 0.0), ("silu_plain", 0.0), ("silu", 0.0), ("swish_limit", 2.0)])
+@pytest.mark.parametrize("rows,dtype", [(3, torch.float32), (3, torch.bfloat16), (200, torch.bfloat16)])
+def test_nan_passes_the_experts(rows, dtype, form, param):
+    """A row with a NaN gives NaN, however few or many rows there are; the other rows keep their bits."""
+    experts, width, ff = 4, 128, 128
+    gen = torch.Generator().manual_seed(160)
+    x, w_up, w_down = (torch.randn(s, generator=gen).to(dtype).to(DEV)
+                       for s in ((rows, width), (experts, ff * (1 if form in ops.UNARY_FORMS else 2), width), (experts, width, ff)))
+    sel = (torch.arange(2 * rows, device=DEV, dtype=torch.int32) % experts).view(rows, 2).contiguous()
+    sel_w = torch.full((rows, 2), 0.5, device=DEV)
+    run = ops.moe_experts_few if rows < 100 else ops.moe_experts_grouped
+    want = run(x, sel, sel_w, w_up, w_down, experts, form, param)
+    x[1, 7] = math.nan
+    got = run(x, sel, sel_w, w_up, w_down, experts, form, param)
+    others = [i for i in range(rows) if i != 1]
+    assert got[1].isnan().all() and torch.equal(got[others], want[others]) and torch.isfinite(want).all()
