@@ -11,7 +11,7 @@ extern "C" {
 #define RDL_ACT_SILU 1
 #define RDL_ACT_SWISH_LIMIT 2   // min(g, L) sigmoid(1.702 min(g, L)) (clamp(u, -L, L) + 1), L a parameter
 
-#define RDL_ABI_VERSION 27
+#define RDL_ABI_VERSION 28
 
 const char* rdl_last_error(void);
 int rdl_abi_version(void);
@@ -31,6 +31,7 @@ void rdl_set_programmatic_launch(int on);
 #define RDL_FAULT_MX_FEW 8             // mx_few_rows: a weight copy or a product did not complete
 #define RDL_FAULT_MX_MANY 9            // mx_many_rows: a stage or an accumulator was not handed over
 #define RDL_FAULT_MX_SOME 10           // mx_some_rows: as 9
+#define RDL_FAULT_TARGET_ID 11         // token_logprobs, linear_logprobs: a token id outside the vocabulary (its log probability is NaN)
 
 // For tests of the bounded waits: the kernel whose fault code is `code` gives up a wait after `cycles`
 // clock cycles instead of about a second, and announces `extra_tx_bytes` more bytes to the barrier of
@@ -571,6 +572,23 @@ typedef struct {
 int rdl_sample(int* out_tokens, int* host_tokens, const float* logits, int n_rows, int vocab, const SamplingArgs* params,
                const unsigned long long* row_stream, const int* row_step,
                const int* history, const int* history_start, float* work, void* stream);
+// Of every row of logits [rows][vocab] (consecutive columns, rows row_stride elements apart): its entropy, the log probability of the
+// token targets[row] (targets may be NULL; a negative id asks for none and gets 0), and its `top` (0 to 32) largest logits as ids [rows][top] and
+// log probabilities, equal logits in the order of their ids and NaN behind everything (csrc/logprobs.cuh).  In nats.
+int rdl_token_logprobs(const void* logits, int dtype, long long row_stride, int rows, int vocab, const int* targets, int top, float* logprobs,
+                       float* entropy, float* top_logprobs, int* top_ids, int* status, void* stream);
+
+// Rows copied within tensors: row dst of every set becomes row src, for each tensor's list of pairs: list + 2 first_pair holds
+// `pairs` sources, then as many destinations; tensors may share a list.  Strides in bytes, tensors and list in host memory (read before the call returns).  No destination may be a source or
+// another pair's destination, and tensors may not overlap; row numbers are the caller's to check.
+#define RDL_COPY_ROWS_MAX_TENSORS 64
+typedef struct {
+    void* base;
+    long long set_stride, row_stride, row_bytes;
+    int sets, first_pair, pairs;
+} CopyRowsTensor;
+int rdl_copy_rows(const CopyRowsTensor* tensors, int n_tensors, const int* list, void* stream);
+
 // the uniform number in [0, 1) that rdl_sample draws with for (seed, stream id, step); host function
 float rdl_sampling_uniform(unsigned long long seed, unsigned long long stream, unsigned long long step);
 

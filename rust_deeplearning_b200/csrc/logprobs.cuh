@@ -1,0 +1,120 @@
+// What the kernels that turn logits into log probabilities share: the running statistics of a row, and the list of its
+// largest logits.
+//
+// Of logits z with largest value m:  s = sum exp(z - m),  t = sum (z - m) exp(z - m);  the log probability of token i is
+// z_i - m - ln s and the entropy ln s - t / s (every term relative to m, so that nothing cancels).  Two parts of a row with statistics of
+// their own join by moving both to the larger m:  exp(z - M) = exp(z - m) exp(m - M),  (z - M) = (z - m) + (m - M).
+// A logit of minus infinity (a forbidden token) adds nothing; a NaN or plus infinity makes s NaN, and a row of nothing but minus
+// infinities has s = 0 and gives NaN as well: there is no distribution.  m starts at the lowest finite value, so that a row
+// masked with that value is uniform.
+//
+// A logit and its id are one 64-bit key whose order is the order of the alternatives: larger logits first, of equal logits the lowest id
+// first, NaN behind everything.  Keys of a row are distinct; 0 is no key.
+#pragma once
+
+#include <float.h>
+
+#include "common.cuh"
+
+#define RDL_LOGPROBS_MAX_TOP 32       // alternatives: a key a lane
+
+namespace {
+
+constexpr float LP_LOG2E = 1.4426950408889634f;
+
+struct LpStats { float m, s, t; };
+
+__device__ __forceinline__ LpStats lp_empty() { return {-FLT_MAX, 0.f, 0.f}; }
+
+// 2^x: two units in the last place (the hardware's), 0 for minus infinity
+__device__ __forceinline__ float lp_exp2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// the statistics seen from a larger maximum; the lower bound keeps 0 * infinity out (what it cuts off is multiplied by 2^-huge = 0)
+__device__ __forceinline__ void lp_move(LpStats& a, float m) {
+    const float d = fmaxf(a.m - m, -1e30f), c = lp_exp2(d * LP_LOG2E);
+    a.t = c * fmaf(a.s, d, a.t);
+    a.s *= c;
+    a.m = m;
+}
+
+__device__ __forceinline__ void lp_join(LpStats& a, LpStats b) {
+    const float m = fmaxf(a.m, b.m);
+    lp_move(a, m);
+    lp_move(b, m);
+    a.s += b.s;
+    a.t += b.t;
+}
+
+// N logits more; m is not below any of them
+template <int N>
+__device__ __forceinline__ void lp_add(LpStats& a, const float (&z)[N]) {
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = z[i] - a.m, e = lp_exp2(d * LP_LOG2E);
+        s += e;
+        t = fmaf(e, fmaxf(d, -1e30f), t);
+    }
+    a.s += s;
+    a.t += t;
+}
+
+__device__ __forceinline__ LpStats lp_warp_join(LpStats a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const LpStats b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)};
+        lp_join(a, b);
+    }
+    return a;
+}
+
+typedef unsigned long long LpKey;
+
+__device__ __forceinline__ LpKey lp_key(float z, unsigned id) {
+    const unsigned u = __float_as_uint(z + 0.0f);               // -0 and +0 are one value
+    const unsigned o = z != z ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+    return (LpKey)o << 32 | (unsigned)~id;
+}
+// the logit of a key (minus infinity for no key and for a NaN's)
+__device__ __forceinline__ float lp_key_logit(LpKey k) {
+    const unsigned o = (unsigned)(k >> 32);
+    return o == 0 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ unsigned lp_key_id(LpKey k) { return ~(unsigned)k; }
+
+// A warp's list: 32 keys, a lane each, largest in lane 0.
+
+// descending order over the lanes of a sequence that first falls and then rises, or the other way round (bitonic)
+__device__ __forceinline__ LpKey lp_bitonic(LpKey k, int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const LpKey other = __shfl_xor_sync(0xffffffffu, k, o);
+        const bool first = (lane & o) == 0;                     // the place that gets the larger one
+        k = (k > other) == first ? k : other;
+    }
+    return k;
+}
+// any 32 keys, 0 for none; keys may not repeat but for 0
+__device__ __forceinline__ LpKey lp_sort(LpKey k, int lane) {
+#pragma unroll
+    for (int n = 2; n <= 32; n <<= 1) {
+#pragma unroll
+        for (int o = n >> 1; o > 0; o >>= 1) {
+            const LpKey other = __shfl_xor_sync(0xffffffffu, k, o);
+            const bool larger = ((lane & o) == 0) == ((lane & n) == 0 || n == 32);
+            k = (k > other) == larger ? k : other;
+        }
+    }
+    return k;
+}
+// the 32 largest of two sorted lists
+__device__ __forceinline__ LpKey lp_merge(LpKey a, LpKey b, int lane) {
+    const LpKey r = __shfl_sync(0xffffffffu, b, 31 - lane);
+    return lp_bitonic(a > r ? a : r, lane);
+}
+
+}  // namespace

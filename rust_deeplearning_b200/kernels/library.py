@@ -23,7 +23,7 @@ from concurrent.futures import ThreadPoolExecutor
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(_PKG, "csrc")
 LIB_NAME = "librdl_b200_kernels.so"
-ABI_VERSION = 27
+ABI_VERSION = 28
 
 # fast math is never enabled: the 32-bit path relies on exact tanhf/expf/sqrtf and plain FMA
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -191,6 +191,7 @@ FAULTS = {
     8: "mx_few_rows: a weight copy or a product did not complete",
     9: "mx_many_rows: a stage or an accumulator was not handed over",
     10: "mx_some_rows: a stage or an accumulator was not handed over",
+    11: "token_logprobs: a token id outside the vocabulary (its log probability is NaN)",
 }
 
 
@@ -392,6 +393,15 @@ class SamplingArgs(ctypes.Structure):
                 ("repetition_penalty", ctypes.c_float), ("seed", ctypes.c_ulonglong)]
 
 
+COPY_ROWS_MAX_TENSORS = 64
+
+
+class CopyRowsTensor(ctypes.Structure):
+    """A tensor whose rows are copied, and its part of the list of pairs (`csrc/api.h`)."""
+    _fields_ = [("base", ctypes.c_void_p), ("set_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong), ("row_bytes", ctypes.c_longlong),
+                ("sets", ctypes.c_int), ("first_pair", ctypes.c_int), ("pairs", ctypes.c_int)]
+
+
 _P, _I, _F, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 _SIGNATURES = {
     "rdl_attention_plain": [ctypes.POINTER(AttentionArgs), _P],
@@ -447,6 +457,8 @@ _SIGNATURES = {
     "rdl_mx_many_rows": [_P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P, _P],
     "rdl_random_normal": [_P, _I, _LL, ctypes.c_ulonglong, ctypes.c_double, _P],
     "rdl_sample": [_P, _P, _P, _I, _I, ctypes.POINTER(SamplingArgs), _P, _P, _P, _P, _P, _P],
+    "rdl_token_logprobs": [_P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
+    "rdl_copy_rows": [ctypes.POINTER(CopyRowsTensor), _I, _P, _P],
     "rdl_upload_batch": [_P, _P, _I, _P, _I, _I, _I, _P],
     "rdl_latent_prepare": [ctypes.POINTER(LatentPrepareArgs), _P],
     "rdl_latent_write": [ctypes.POINTER(LatentPrepareArgs), _P],

@@ -7,6 +7,8 @@ raise.  Parts call them as `ops.<name>` (attribute lookup at call time).
 """
 from __future__ import annotations
 
+import array
+import contextlib
 import ctypes
 import functools
 import os
@@ -77,6 +79,14 @@ def _need(cond, msg):
 def _dense(t, name):
     _need(t.is_contiguous(), f"{name} must be contiguous")
     return t
+
+
+_AS_IT_IS = contextlib.nullcontext()
+
+
+def _on_device(device: torch.device):
+    """A launch goes to the current device; this makes it the tensors' own where it is another."""
+    return _AS_IT_IS if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _int32(t, name, n=None):
@@ -1158,6 +1168,154 @@ def sample(logits: torch.Tensor, *, temperature: float, top_k: Optional[int] = N
                                             ctypes.byref(prm), _ptr(row_stream),
                                             _ptr(row_step), _ptr(history), _ptr(history_start), _ptr(work), _stream(logits)))
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# how probable tokens are
+# ------------------------------------------------------------------------------------------
+
+LOGPROBS_MAX_TOP = 32    # alternatives a row can be asked for
+# float32 logits that `linear_logprobs` holds at a time where the product has a kernel of its own
+LOGPROBS_PIECE = 1 << 26
+
+
+class TokenLogprobs(NamedTuple):
+    """Of every row: the log probability of its token (None without tokens) and the entropy of its distribution, in nats, float32 [rows];
+    its most probable tokens, int32 [rows, top] (equal logits: the lowest id first), and their log probabilities, float32 [rows, top]."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def _logprobs_result(like: torch.Tensor, rows: int, top: int, with_targets: bool) -> TokenLogprobs:
+    f32 = dict(dtype=torch.float32, device=like.device)
+    return TokenLogprobs(torch.empty(rows, **f32) if with_targets else None, torch.empty(rows, **f32),
+                         torch.empty((rows, top), dtype=torch.int32, device=like.device), torch.empty((rows, top), **f32))
+
+
+def _logprobs_check(who: str, rows: int, vocab: int, device, targets: Optional[torch.Tensor], top: int):
+    _need(vocab > 0, f"{who}: rows of no logits")
+    _need(isinstance(top, int) and not isinstance(top, bool) and 0 <= top <= min(LOGPROBS_MAX_TOP, vocab),
+          f"{who}: {top} alternatives of {vocab} tokens (a whole number, {LOGPROBS_MAX_TOP} at most)")
+    if targets is not None:
+        _need(targets.dtype is torch.int32 and targets.dim() == 1 and targets.numel() == rows and targets.is_contiguous() and targets.device == device,
+              f"{who}: targets must be contiguous int32 [{rows}] on {device}")
+
+
+def _token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], out: TokenLogprobs, first: int, top: int, status):
+    """Rows of logits into rows `first` and on of the result."""
+    rows, vocab = logits.shape
+    at = lambda t, width: ctypes.c_void_p(t.data_ptr() + 4 * first * width) if t is not None and width else None
+    with _on_device(logits.device):
+        library.check(library.load().rdl_token_logprobs(
+            _ptr(logits), _dtype_code(logits), logits.stride(0), rows, vocab, at(targets, 1), top, at(out.logprobs, 1), at(out.entropy, 1),
+            at(out.top_logprobs, top), at(out.top_ids, top), _status(status), _stream(logits)))
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0,
+                   status: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """How probable tokens are by rows of logits (float32 or bfloat16 [rows, vocab], rows may lie apart): the log softmax at
+    targets[row] (int32), the entropy, and the `top` most probable tokens; one pass over the logits, everything in float32.
+
+    A negative target asks for none and gets 0; one outside the vocabulary gets NaN and is reported to `status`.  Logits of minus infinity
+    are tokens of probability 0.  A row with a NaN or plus infinity, or of minus infinities alone, has no distribution: NaN (its
+    alternatives are still those of its largest logits, a NaN counting as the smallest)."""
+    _need(logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1) and logits.stride(0) >= 0, "token_logprobs: logits [rows, vocab], a row's consecutive")
+    _dtype_code(logits)
+    rows, vocab = logits.shape
+    _logprobs_check("token_logprobs", rows, vocab, logits.device, targets, top)
+    _stream(logits)
+    out = _logprobs_result(logits, rows, top, targets is not None)
+    if rows:
+        _token_logprobs(logits, targets, out, 0, top, status)
+    return out
+
+
+def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = None, top: int = 0, softcap: Optional[float] = None,
+                    scale: float = 1.0, status: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """`token_logprobs` of the logits scale * softcap(x W^T) of rows x [rows, in] behind an output head [vocab, in] (a tensor of x's type, or
+    `Mx4Weight`), without keeping the logits."""
+    _need(x.dim() == 2 and len(weight.shape) == 2 and x.shape[1] == weight.shape[1] and x.shape[1] > 0,
+          f"linear_logprobs: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not fit")
+    _need(type(weight) is Mx4Weight or x.dtype is weight.dtype, "linear_logprobs: rows and weight of one type")
+    _need(x.device == weight.device, f"linear_logprobs: rows on {x.device}, weight on {weight.device}")
+    _need(softcap is None or softcap > 0, "linear_logprobs: the soft-cap must be positive")
+    _dtype_code(x)
+    _dense(x, "x")
+    _need(type(weight) is Mx4Weight or weight.is_contiguous(), "linear_logprobs: the weight must be contiguous")
+    rows, vocab = x.shape[0], weight.shape[0]
+    _logprobs_check("linear_logprobs", rows, vocab, x.device, targets, top)
+    _stream(x)
+    out = _logprobs_result(x, rows, top, targets is not None)
+    piece = max(1, LOGPROBS_PIECE // vocab)
+    for r in range(0, rows, piece):
+        z = linear(x[r:r + piece], weight, torch.float32, softcap, status)
+        if scale != 1.0:
+            scale_(z, scale)
+        _token_logprobs(z, targets, out, r, top, status)
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# copies inside a cache
+# ------------------------------------------------------------------------------------------
+
+def _extent(t: torch.Tensor):
+    """First and last byte of a tensor of at least one element."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def copy_rows(moves):
+    """Rows copied inside tensors, in one kernel: for every (tensor, src, dst) of `moves`, tensor[:, dst[i]] = tensor[:, src[i]].
+
+    Tensors are [sets, rows, ...] (the pages of a cache, or its states, of all layer runs) of any type, on one device; a row's own
+    elements are contiguous, sets and rows may lie apart.  src and dst are lists of row numbers on the host, read before the call returns.  No
+    row may be the destination of two copies, or source of one and destination of another, and the tensors may not overlap."""
+    moves = list(moves)
+    _need(len(moves) <= library.COPY_ROWS_MAX_TENSORS, f"copy_rows: {len(moves)} tensors, {library.COPY_ROWS_MAX_TENSORS} at most")
+    if not moves:
+        return
+    device = moves[0][0].device
+    args = (library.CopyRowsTensor * len(moves))()
+    pairs, used, extents, lists = array.array("i"), 0, [], {}
+    for a, (t, src, dst) in zip(args, moves):
+        _need(t.device == device, "copy_rows: tensors on one device")
+        _need(t.dim() >= 2, "copy_rows: tensors are [sets, rows, ...]")
+        sets, rows = t.shape[0], t.shape[1]
+        inner = 1
+        for n, s in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+            _need(n <= 1 or s == inner, "copy_rows: a row's own elements must be contiguous")
+            inner *= n
+        s0, s1 = t.stride(0), t.stride(1)
+        if sets * rows > 1 and inner > 0:
+            # either sets of rows or rows of sets, with or without gaps
+            near, far, n_near, n_far = (s1, s0, rows, sets) if (s1 <= s0 and rows > 1) or sets == 1 else (s0, s1, sets, rows)
+            _need((n_near == 1 or near >= inner) and (n_far == 1 or far >= (near * (n_near - 1) if n_near > 1 else 0) + inner), "copy_rows: rows that overlap")
+        key = (id(src), id(dst), rows)
+        if key not in lists:                     # keys and values share their lists
+            n = len(src)
+            _need(len(dst) == n, f"copy_rows: {n} sources and {len(dst)} destinations")
+            to, touched = set(dst), set(src)
+            _need(len(to) == n and to.isdisjoint(touched), "copy_rows: a row that is the destination of two copies, or source of one and destination of another")
+            _need(n == 0 or (min(min(to), min(touched)) >= 0 and max(max(to), max(touched)) < rows), f"copy_rows: a row outside {rows}")
+            lists[key] = (used, n)
+            pairs.extend(src)
+            pairs.extend(dst)
+            used += n
+        first, n = lists[key]
+        esz = t.element_size()
+        a.base, a.set_stride, a.row_stride, a.row_bytes, a.sets, a.first_pair, a.pairs = t.data_ptr(), s0 * esz, s1 * esz, inner * esz, sets, first, n
+        if sets * rows * inner:
+            extents.append(_extent(t))
+    extents.sort()
+    _need(all(a[1] <= b[0] for a, b in zip(extents, extents[1:])), "copy_rows: tensors that overlap")
+    stream = _stream(moves[0][0])
+    if not used:
+        return
+    with _on_device(device):
+        library.check(library.load().rdl_copy_rows(args, len(moves), pairs.buffer_info()[0], stream))
 
 
 def upload_batch(dst: torch.Tensor, src_pinned: torch.Tensor, n_ints: int, fed: Optional[Tuple[torch.Tensor, int, int, int]] = None):
