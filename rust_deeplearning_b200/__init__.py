@@ -10,7 +10,7 @@ from .config import dokulorn as _dokulorn, gasetar as _gasetar, gemma2 as _gemma
 from .config import ligirax as _ligirax, paditar as _paditar, revepel as _revepel
 from .config.base import ConfigError, load_config, register_architecture, registered_architectures
 from .engine.api import Generator, load_model, random_model
-from .engine.generate import GenerationResult, generate
+from .engine.generate import GenerationResult, ScoredText, generate, score
 from .engine.step import Engine, StepError
 from .cache.cache import Cache, CacheError
 from .sampling.sampler import SamplingParams
@@ -19,6 +19,6 @@ from .weights.random_init import write_random_model
 
 __all__ = [
     "ConfigError", "load_config", "register_architecture", "registered_architectures",
-    "Generator", "load_model", "random_model", "GenerationResult", "generate", "Engine", "StepError",
+    "Generator", "load_model", "random_model", "GenerationResult", "ScoredText", "generate", "score", "Engine", "StepError",
     "Cache", "CacheError", "SamplingParams", "WeightError", "write_random_model",
 ]

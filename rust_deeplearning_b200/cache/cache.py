@@ -17,6 +17,10 @@ Here
 * state of fixed size lives beside it, [runs in group][slot][*shape], zeroed when a slot
   is handed out.
 
+A slot can be *forked*: its copies share its pages, each page counting its holders, and get copies of its state.  A page is copied
+only when one of several holders is about to write into it behind positions of its own (`reserve`), in one kernel for all layers; a page
+whose old rows the writer no longer sees is replaced without a copy.
+
 Freed slots and pages are reused; what a sequence reads is bounded by its length, so stale rows
 of an earlier occupant never contribute and nothing is cleared on free.  (Kernels that copy whole
 pages may touch such rows, but give them the weight zero; storage starts zero-filled so that
@@ -30,6 +34,7 @@ from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple, Union
 import numpy as np
 import torch
 
+from ..kernels import ops
 
 DEFAULT_PAGE_SIZE = 64   # positions a page holds unless an engine is built with another size
 
@@ -73,12 +78,12 @@ def _state_list(state) -> Tuple[StateRequirement, ...]:
 
 
 class PagePool:
-    """Free list of page ids.  Host only."""
+    """Free list of page ids, and how many slots hold each page.  Host only."""
 
     def __init__(self, n_pages: int):
         self.n_pages = n_pages
         self._free = list(range(n_pages - 1, -1, -1))
-        self._held = [False] * n_pages
+        self._held = [0] * n_pages
 
     @property
     def n_free(self):
@@ -89,15 +94,27 @@ class PagePool:
             raise CacheError(f"cache is full: {n} pages needed, {len(self._free)} of {self.n_pages} free")
         out = [self._free.pop() for _ in range(n)]
         for p in out:
-            self._held[p] = True
+            self._held[p] = 1
         return out
 
+    def holders(self, page: int) -> int:
+        return self._held[page]
+
+    def share(self, pages: Sequence[int], times: int = 1):
+        """`times` more holders of each page."""
+        for p in pages:
+            if not (0 <= p < self.n_pages) or not self._held[p]:
+                raise CacheError(f"page {p} is shared but not held")
+            self._held[p] += times
+
     def give_back(self, pages: Sequence[int]):
+        """One holder less of each page; a page without holders is free."""
         for p in pages:
             if not (0 <= p < self.n_pages) or not self._held[p]:
                 raise CacheError(f"page {p} is given back but not held")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
 
 
 def ring_pages_for(window: int, page_size: int) -> int:
@@ -146,6 +163,38 @@ class KVGroup:
 
     def release(self, slot: int):
         self.pool.give_back(self.pages.pop(slot, []))
+
+    def fork(self, slot: int, copies: Sequence[int]):
+        """Slots `copies` hold the same pages as `slot`."""
+        held = self.pages.get(slot, [])
+        self.pool.share(held, len(copies))
+        for c in copies:
+            self.pages[c] = list(held)
+
+    def shared_and_written(self, slots: Sequence[int], past: Sequence[int], totals: Sequence[int]):
+        """What the next positions of each slot fall on that other slots hold too: (slot, entry of its page list, whether a query of these
+        positions still sees one of the page's).  The last of a page's holders keeps it.
+
+        A step's queries read earlier positions before its own are written, so a page of a window group counts as long as the first of
+        them sees its last position."""
+        window, size, ring = self.requirement.window, self.page_size, self.ring_pages
+        holders: Dict[int, int] = {}
+        out = []
+        for s, first, total in zip(slots, past, totals):
+            held = self.pages.get(s, ())
+            lo, hi = first // size, (total - 1) // size
+            for k in range(lo, min(hi, lo + ring - 1) + 1):
+                e = k % ring
+                if e >= len(held):
+                    continue
+                n = holders.get(held[e], self.pool.holders(held[e]))
+                if n > 1:
+                    holders[held[e]] = n - 1
+                    newest = (first - 1) // size
+                    page = newest - (newest - e) % ring              # which of the sequence's pages lies there now (negative: none yet)
+                    last = min(page * size + size - 1, first - 1)
+                    out.append((s, e, page >= 0 and (window is None or last > first - window)))
+        return out
 
     def table_rows(self, slots: Sequence[int], n_rows: Optional[int] = None) -> np.ndarray:
         out = np.zeros((n_rows or len(slots), self.table_width), dtype=np.int32)
@@ -245,6 +294,26 @@ class Cache:
                 g.data[:, s].zero_()
         return s
 
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """`n` more slots that go on from where `slot` is: they share its pages and get its state (one kernel copies the state of all
+        runs).  All or nothing."""
+        self._check(slot)
+        if n < 0:
+            raise CacheError(f"slot {slot} cannot be forked into {n}")
+        if n > len(self._free_slots):
+            raise CacheError(f"no free slot: {n} needed, {len(self._free_slots)} of {self.max_seqs} free")
+        copies = [self._free_slots[-1 - i] for i in range(n)]
+        states = [(g.data, [slot] * n, copies) for g in self.state_groups if g.data is not None]
+        if n and states:
+            ops.copy_rows(states)
+        for s in copies:
+            self._free_slots.pop()
+            self._live[s] = True
+            self.lengths[s] = self.lengths[slot]
+        for g in self.kv_groups:
+            g.fork(slot, copies)
+        return copies
+
     def _check(self, slot: int):
         if not (0 <= slot < self.max_seqs) or not self._live[slot]:
             raise CacheError(f"slot {slot} is not in use")
@@ -263,7 +332,8 @@ class Cache:
 
     # ---- growth ----
     def reserve(self, slots: Sequence[int], new_tokens: Sequence[int]):
-        """Make room for `new_tokens[i]` more positions of `slots[i]`; all or nothing."""
+        """Make room for `new_tokens[i]` more positions of `slots[i]`; all or nothing.  Shared pages that these positions fall on become the
+        slots' own (copied on the current stream, where the slot still needs what they hold)."""
         if len(set(slots)) != len(slots):
             raise CacheError("a slot is named twice in one step")
         totals = []
@@ -275,14 +345,42 @@ class Cache:
             if total > self.max_context:
                 raise CacheError(f"slot {s}: {total} positions exceed the cache's longest context of {self.max_context}")
             totals.append(total)
-        for g in self.kv_groups:
-            need = sum(g.pages_needed(s, t) for s, t in zip(slots, totals))
+        past = [self.lengths[s] for s in slots]
+        own = [g.shared_and_written(slots, past, totals) for g in self.kv_groups]
+        for g, shared in zip(self.kv_groups, own):
+            need = sum(g.pages_needed(s, t) for s, t in zip(slots, totals)) + len(shared)
             if need > g.pool.n_free:
                 raise CacheError(f"cache is full: the step needs {need} more pages of {g.page_size} positions, "
                                  f"{g.pool.n_free} of {g.pool.n_pages} are free (window={g.requirement.window})")
+        if any(own):
+            self._unshare(own)
         for g in self.kv_groups:
             for s, t in zip(slots, totals):
                 g.grow(s, t)
+
+    def _unshare(self, own):
+        """Pages of their own for the slots and entries of `KVGroup.shared_and_written`, group by group."""
+        taken, moves = [], []
+        for g, shared in zip(self.kv_groups, own):
+            pages = g.pool.take(len(shared))
+            taken.append(pages)
+            copied = [(g.pages[s][e], p) for (s, e, used), p in zip(shared, pages) if used]
+            if copied and g.k is not None:
+                src, dst = [a for a, _ in copied], [b for _, b in copied]
+                moves.append((g.k, src, dst))
+                if not g.shares_values:
+                    moves.append((g.v, src, dst))
+        try:
+            if moves:
+                ops.copy_rows(moves)
+        except Exception:
+            for g, pages in zip(self.kv_groups, taken):
+                g.pool.give_back(pages)
+            raise
+        for g, shared, pages in zip(self.kv_groups, own, taken):
+            for (s, e, _), p in zip(shared, pages):
+                g.pool.give_back([g.pages[s][e]])
+                g.pages[s][e] = p
 
     def advance(self, slots: Sequence[int], new_tokens: Sequence[int]):
         for s, n in zip(slots, new_tokens):

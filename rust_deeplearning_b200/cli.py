@@ -10,6 +10,9 @@ UTF-8 bytes to ids, as the reference's byte tokenizer does (`rustml/tokenizer/ma
 error, generated ids to standard output (`infer.rs:71-119, 145-158`); among them the model's
 sizes (`infer.rs:86-89`) and, after the run, prompt and decode rates in the wording of
 `rustml/nlp/examples/gemma3_gguf.rs:43-46, :73`.  `--timings` adds the device time of every step.
+
+Beyond the reference: `--samples N` prints N continuations of every prompt (which runs once), `--logprobs N` a line per new token with its
+log probability, the entropy and N alternatives, and `--score` the same lines for the tokens of the prompts themselves, without generating.
 """
 from __future__ import annotations
 
@@ -52,6 +55,9 @@ def build_parser() -> argparse.ArgumentParser:
                         "sequences) round what enters these matrices to 8 bits, smaller ones nothing.")
     p.add_argument("--stop-ids", default=None, help="Stop token ids (default: the model's end-of-sequence ids).")
     p.add_argument("--max-context", type=int, default=None, help="Longest sequence the cache is sized for.")
+    p.add_argument("--samples", type=int, default=1, help="Continuations of every prompt (one after another in the output); a prompt runs once.")
+    p.add_argument("--logprobs", type=int, default=None, metavar="N", help="Print a line for every new token: id, log probability, entropy, N alternatives as id:log-probability.")
+    p.add_argument("--score", action="store_true", help="Generate nothing: print such a line for every token of the prompts from the second on (alternatives as --logprobs says).")
     p.add_argument("--timings", action="store_true", help="Print the device time of every step (CUDA events) to stderr.")
     return p
 
@@ -82,11 +88,21 @@ def read_prompts(args, stdin) -> List[List[int]]:
     return prompts
 
 
+def _write_logprobs(out, tokens, r):
+    """One line a token: id, log probability, entropy, alternatives."""
+    for t, lp, h, top in zip(tokens, r.logprobs, r.entropy, r.top):
+        out.write("\t".join([str(t), f"{lp:.6f}", f"{h:.6f}"] + [f"{i}:{v:.6f}" for i, v in top]) + "\n")
+
+
 def main(argv: Optional[List[str]] = None, stdin=None, stdout=None) -> int:
     args = build_parser().parse_args(argv)
     stdin, stdout = stdin or sys.stdin, stdout or sys.stdout
     if (args.model_dir is None) == (args.random_config is None):
         raise SystemExit("error: give either MODEL_DIR or --random-config FILE.json")
+    if args.stream and (args.logprobs is not None or args.score):
+        raise SystemExit("error: --stream prints tokens alone; leave out --logprobs and --score")
+    if args.score and args.samples != 1:
+        raise SystemExit("error: --score generates nothing; leave out --samples")
     prompts = read_prompts(args, stdin)
 
     from .config.base import ConfigError
@@ -120,7 +136,7 @@ def main(argv: Optional[List[str]] = None, stdin=None, stdout=None) -> int:
     from .engine.step import StepError
 
     def on_token(request, token):
-        stdout.write(f"{request}\t{token}\n" if len(prompts) > 1 else f"{token}\n")
+        stdout.write(f"{request}\t{token}\n" if len(prompts) * args.samples > 1 else f"{token}\n")
         stdout.flush()
 
     stats = GenerationStats()
@@ -129,23 +145,35 @@ def main(argv: Optional[List[str]] = None, stdin=None, stdout=None) -> int:
         # sampling option outside its range) comes back as the library's own errors: one line, no traceback
         if args.max_context is not None and args.max_context < 1:
             raise ValueError("--max-context must be at least 1")
-        longest = max(len(p) for p in prompts) + max(args.max_tokens, 0)
-        gen = Generator(model, max_batch=min(len(prompts), 64), max_context=args.max_context or min(longest, model.max_positions),
+        if args.samples < 1:
+            raise ValueError("--samples must be at least 1")
+        longest = max(len(p) for p in prompts) + (0 if args.score else max(args.max_tokens, 0))
+        gen = Generator(model, max_batch=max(min(len(prompts) * args.samples, 64), args.samples), max_context=args.max_context or min(longest, model.max_positions),
                         time_steps=args.timings)
         gen.with_temperature(args.temperature).with_top_k(args.top_k).with_top_p(args.top_p)
         gen.with_repetition_penalty(args.repetition_penalty).with_seed(args.seed)
         if args.stop_ids is not None:
             gen.with_stop_tokens(_parse_ids(args.stop_ids))
+        if args.score:
+            print(f"Scoring {len(prompts)} prompt(s)...", file=sys.stderr)
+            for i, (p, r) in enumerate(zip(prompts, gen.score(prompts, args.logprobs or 0))):
+                _write_logprobs(stdout, p[1:], r)
+                print(f"prompt {i}: {len(p)} tokens, perplexity {r.perplexity:.4f}", file=sys.stderr)
+            return 0
+        gen.with_logprobs(args.logprobs)
         print(f"Generating up to {args.max_tokens} tokens for {len(prompts)} prompt(s)...", file=sys.stderr)
-        results = gen.generate_batch_results(prompts, args.max_tokens, stream=on_token if args.stream else None, stats=stats)
+        results = gen.generate_batch_results(prompts, args.max_tokens, stream=on_token if args.stream else None, stats=stats,
+                                              samples=args.samples)
     except (StepError, CacheError, ValueError) as e:
         print(f"error: {e}", file=sys.stderr)
         return 1
     if not args.stream:
         for r in results:
             stdout.write(" ".join(str(t) for t in r.tokens) + "\n")
+            if args.logprobs is not None:
+                _write_logprobs(stdout, r.tokens, r)
     for i, r in enumerate(results):
-        print(f"prompt {i}: {len(r.tokens)} tokens, finished by {r.finish_reason}", file=sys.stderr)
+        print(f"prompt {i // args.samples}{f', continuation {i % args.samples}' if args.samples > 1 else ''}: {len(r.tokens)} tokens, finished by {r.finish_reason}", file=sys.stderr)
     print(f"  Prefill: {stats.prefill_tokens} tokens in {stats.prefill_seconds:.2f}s ({stats.prefill_rate():.1f} tok/s)", file=sys.stderr)
     print(f"  Decode: {stats.decode_tokens} tokens in {stats.decode_seconds:.2f}s ({stats.decode_rate():.1f} tok/s)", file=sys.stderr)
     if args.timings:

@@ -14,7 +14,7 @@ from ..parts.model import Model
 from ..sampling.sampler import SamplingParams
 from ..weights.loader import load_weights, random_weights
 from ..weights.random_init import parse_dtype
-from .generate import GenerationResult, GenerationStats, generate
+from .generate import GenerationResult, GenerationStats, ScoredText, generate, score
 from .step import Engine
 
 
@@ -74,6 +74,7 @@ class Generator:
         self._stop: Optional[frozenset] = None
         self._include_stop = False
         self._bos: Optional[int] = None
+        self._logprobs: Optional[int] = None
 
     # ---- options (generator.rs:96-128) ----
     def with_temperature(self, temperature: float):
@@ -110,6 +111,12 @@ class Generator:
         self._bos = token_id
         return self
 
+    def with_logprobs(self, top: Optional[int] = 0):
+        """Results say how probable every new token was, with the entropy of that choice and the `top` most probable tokens
+        (`GenerationResult.logprobs`, `.entropy`, `.top`), by the model's own distribution.  None: they do not."""
+        self._logprobs = top
+        return self
+
     def _params(self) -> SamplingParams:
         return SamplingParams(self._temperature, self._top_k, self._top_p, self._repetition_penalty, self._seed)
 
@@ -122,9 +129,11 @@ class Generator:
     # ---- generation ----
     def generate_batch_results(self, prompts: Sequence[Sequence[int]], max_tokens: int = 256,
                                stream: Optional[Callable[[int, int], Optional[bool]]] = None,
-                               stats: Optional[GenerationStats] = None) -> List[GenerationResult]:
+                               stats: Optional[GenerationStats] = None, samples: int = 1) -> List[GenerationResult]:
+        """samples: so many continuations of every prompt, one after another in the results; a prompt runs once."""
         return generate(self.engine, self._prompts(prompts), max_new_tokens=max_tokens, sampling=self._params(),
-                        stop_token_ids=self._stop, include_stop=self._include_stop, stream=stream, stats=stats)
+                        stop_token_ids=self._stop, include_stop=self._include_stop, stream=stream, stats=stats,
+                        samples=samples, logprobs=self._logprobs)
 
     def generate(self, prompt: Sequence[int], max_tokens: int = 256) -> List[int]:
         """Prompt plus generated tokens, as the reference returns prompt plus completion (generator.rs:272)."""
@@ -142,3 +151,13 @@ class Generator:
         generator.rs:402-411)."""
         ps = self._prompts(prompts)
         return [p + r.tokens for p, r in zip(ps, self.generate_batch_results(prompts, max_tokens))]
+
+    def generate_several(self, prompt: Sequence[int], n: int, max_tokens: int = 256) -> List[List[int]]:
+        """`n` continuations of one prompt, each with the prompt in front; the prompt runs once."""
+        p = self._prompts([prompt])[0]
+        return [p + r.tokens for r in self.generate_batch_results([prompt], max_tokens, samples=n)]
+
+    # ---- scoring ----
+    def score(self, texts: Sequence[Sequence[int]], top: int = 0) -> List[ScoredText]:
+        """How probable the tokens of given texts are: all texts together, in as many steps as the cache asks for."""
+        return score(self.engine, self._prompts(texts), top)

@@ -16,16 +16,22 @@ last token turns out to be a stop token has then been part of one step too many;
 for it is dropped.  With a repetition penalty the sampler needs every token on the host first, and
 the loop waits for each step.
 
+Several continuations of one prompt (`samples`) run the prompt once: its sequence is forked behind it (`Engine.fork`), and each
+continuation draws its own tokens from there.  With `logprobs` every new token comes with how probable it was (`ops.token_logprobs`
+on the logits it was sampled from); these stay on the device until the batch has ended.
+
 `plan_batches` and `SequenceState` hold the loop's decisions and need no device.
 """
 from __future__ import annotations
 
+import math
 import time
 from dataclasses import dataclass, field
-from typing import Callable, Iterable, List, Optional, Sequence
+from typing import Callable, Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..kernels import ops
 from ..sampling.sampler import Sampler, SamplingParams
 
 
@@ -33,6 +39,23 @@ from ..sampling.sampler import Sampler, SamplingParams
 class GenerationResult:
     tokens: List[int]          # the new tokens (a stop token is left out unless asked for)
     finish_reason: str         # "stop" | "length" | "context"
+    # asked for with `logprobs`: of every token of `tokens`, by the model's own logits (before penalty, temperature and the rest), in nats
+    logprobs: Optional[List[float]] = None                       # its log probability
+    entropy: Optional[List[float]] = None                        # of the distribution it was taken from
+    top: Optional[List[List[Tuple[int, float]]]] = None          # the most probable tokens there, with their log probabilities
+
+
+@dataclass
+class ScoredText:
+    """Of every token of a text from its second one on, in nats."""
+    logprobs: List[float]                            # its log probability behind the tokens before it
+    entropy: List[float]                             # of the distribution there
+    top: List[List[Tuple[int, float]]]               # the most probable tokens there, with their log probabilities
+
+    @property
+    def perplexity(self) -> float:
+        """exp of the mean of -logprobs (1 for a text of one token)"""
+        return math.exp(-sum(self.logprobs) / len(self.logprobs)) if self.logprobs else 1.0
 
 
 @dataclass
@@ -99,10 +122,12 @@ class SequenceState:
 
 
 def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, *, max_seqs: int, max_tokens: int,
-                 page_size: int, max_context: int) -> List[List[int]]:
+                 page_size: int, max_context: int, samples: int = 1, prompt_shared: bool = False) -> List[List[int]]:
     """Split requests, in order, into batches that fit the cache: at most `max_seqs` sequences and
     at most `max_tokens` positions, counting every sequence at the longest it can get, rounded up
-    to the page size."""
+    to the page size.  samples: sequences per request; prompt_shared: they share the whole pages of its prompt for good."""
+    if samples > max_seqs:
+        raise ValueError(f"{samples} continuations of a prompt, the cache holds {max_seqs} sequences")
     batches, cur, used = [], [], 0
     for i, n in enumerate(prompt_lens):
         if n < 1:
@@ -110,10 +135,11 @@ def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, *, max_seqs: i
         if n > max_context:
             raise ValueError(f"request {i}: prompt of {n} tokens exceeds the context of {max_context}")
         longest = min(n + max(max_new_tokens - 1, 0), max_context)
-        cost = -(-longest // page_size) * page_size
+        shared = n // page_size * page_size if prompt_shared else 0
+        cost = shared + samples * (-(-longest // page_size) * page_size - shared)
         if cost > max_tokens:
             raise ValueError(f"request {i}: needs {cost} cache positions, the cache holds {max_tokens}")
-        if cur and (len(cur) >= max_seqs or used + cost > max_tokens):
+        if cur and ((len(cur) + 1) * samples > max_seqs or used + cost > max_tokens):
             batches.append(cur)
             cur, used = [], 0
         cur.append(i)
@@ -146,8 +172,11 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
              sampling: Optional[SamplingParams] = None, stop_token_ids: Optional[Iterable[int]] = None,
              include_stop: bool = False, stream: Optional[Callable[[int, int], Optional[bool]]] = None,
              max_batch: Optional[int] = None, run_ahead: bool = True,
-             stats: Optional[GenerationStats] = None) -> List[GenerationResult]:
+             stats: Optional[GenerationStats] = None, samples: int = 1, logprobs: Optional[int] = None) -> List[GenerationResult]:
     """Generate for every prompt (lists of token ids).
+
+    samples: so many continuations of every prompt, which runs once; the results (and the stream's request indexes) of prompt i are
+    [i * samples, (i + 1) * samples).  logprobs: how probable every new token was, with its entropy and so many alternatives (0: none).
 
     stop_token_ids: default, the model's end-of-sequence ids.  stream(request index, token) is
     called for every kept token; returning False ends that request (as the reference's streaming
@@ -159,19 +188,29 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
     stops = frozenset(model.spec.stop_token_ids if stop_token_ids is None else stop_token_ids)
     sampler = Sampler(sampling, engine.device)
     prompts = [list(map(int, p)) for p in prompts]
+    if isinstance(samples, bool) or not isinstance(samples, int) or samples < 1:
+        raise ValueError("samples must be a whole number, at least 1")
+    most = min(ops.LOGPROBS_MAX_TOP, model.vocab_size)
+    if logprobs is not None and (isinstance(logprobs, bool) or not isinstance(logprobs, int) or not 0 <= logprobs <= most):
+        raise ValueError(f"logprobs must be a whole number of alternatives from 0 to {most}")
     if max_new_tokens < 1:
-        return [GenerationResult([], "length") for _ in prompts]
+        nothing = dict(logprobs=[], entropy=[], top=[]) if logprobs is not None else {}
+        return [GenerationResult([], "length", **nothing) for _ in range(len(prompts) * samples)]
     max_context = min(cache.max_context, model.max_positions)
     batches = plan_batches([len(p) for p in prompts], max_new_tokens,
                            max_seqs=min(cache.max_seqs, max_batch or cache.max_seqs),
-                           max_tokens=cache.max_tokens, page_size=cache.page_size, max_context=max_context)
-    results: List[Optional[GenerationResult]] = [None] * len(prompts)
+                           max_tokens=cache.max_tokens, page_size=cache.page_size, max_context=max_context, samples=samples,
+                           prompt_shared=samples > 1 and not any(g.is_ring for g in cache.kv_groups))
+    results: List[Optional[GenerationResult]] = [None] * (len(prompts) * samples)
     need_history = sampling.repetition_penalty is not None and not sampling.greedy
 
     for members in batches:
-        seqs = [SequenceState(i, prompts[i], max_new_tokens, max_context, stops, include_stop) for i in members]
-        slots = [engine.new_sequence() for _ in seqs]
+        seqs = [SequenceState(i * samples + k, prompts[i], max_new_tokens, max_context, stops, include_stop) for i in members for k in range(samples)]
+        slots: List[Optional[int]] = []
+        scored: List[tuple] = []                # (rows, how probable their tokens were), sampling by sampling
         try:
+            for _ in members:
+                slots.append(engine.new_sequence())
             issued = [0] * len(seqs)            # samplings queued per sequence (keys its random stream)
             pinned = None
             if engine.device.type == "cuda":    # two buffers: one being read on the host, one being written by the device
@@ -185,11 +224,19 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
                                       [seqs[j].history() for j in rows] if need_history else None, host_out=host)
                 for j in rows:
                     issued[j] += 1
+                if logprobs is not None:
+                    scored.append((rows, ops.token_logprobs(logits, toks, logprobs)))
                 return _Readback(toks, host)
 
             rows = list(range(len(seqs)))       # the sequences whose tokens `sampled` holds, row by row
             t_start = time.perf_counter()
-            sampled = sample(rows, engine.step([slots[j] for j in rows], [s.prompt for s in seqs], "last"))
+            logits = engine.step(slots, [prompts[i] for i in members], "last")
+            if samples > 1:
+                for at in range(0, len(seqs), samples):
+                    slots[at + 1:at + 1] = engine.fork(slots[at], samples - 1)
+                each = torch.arange(len(members), dtype=torch.int32).repeat_interleave(samples).to(engine.device, non_blocking=True)
+                logits = ops.convert_rows(logits, torch.float32, each)
+            sampled = sample(rows, logits)
             ahead = run_ahead and not need_history
             first = True
             while rows:
@@ -207,7 +254,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
                 if first and stats is not None:
                     # the first tokens are on the host: the prompts' step is over
                     now = time.perf_counter()
-                    stats.prefill_tokens += sum(len(s.prompt) for s in seqs)
+                    stats.prefill_tokens += sum(len(prompts[i]) for i in members)
                     stats.prefill_seconds += now - t_start
                     t_start = now
                 first = False
@@ -242,4 +289,47 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
             stats.decode_seconds += time.perf_counter() - t_start
         for s in seqs:
             results[s.request] = GenerationResult(s.new_tokens, s.finish_reason)
+        if logprobs is not None:
+            _attach_logprobs([results[s.request] for s in seqs], scored)
+    return results
+
+
+def _attach_logprobs(results: Sequence[GenerationResult], scored: Sequence[tuple]):
+    """Hand every sequence of a batch its tokens' log probabilities.  scored: for each sampling, the sequences of its rows.  A sequence
+    keeps the first of its sampled tokens; those behind the one that ended it have no place."""
+    for r in results:
+        r.logprobs, r.entropy, r.top = [], [], []
+    lp, entropy, ids, top = (torch.cat(t).tolist() for t in zip(*(s for _, s in scored)))
+    for at, j in enumerate(j for rows, _ in scored for j in rows):
+        r = results[j]
+        if len(r.logprobs) < len(r.tokens):
+            r.logprobs.append(lp[at])
+            r.entropy.append(entropy[at])
+            r.top.append(list(zip(ids[at], top[at])))
+
+
+def score(engine, texts: Sequence[Sequence[int]], top: int = 0) -> List[ScoredText]:
+    """How probable each token of every text is behind the tokens before it.  Texts go through the model as prompts do, as many in a step
+    as the cache holds; no logits are kept."""
+    texts = [list(map(int, t)) for t in texts]
+    cache = engine.cache
+    batches = plan_batches([len(t) for t in texts], 0, max_seqs=cache.max_seqs, max_tokens=cache.max_tokens, page_size=cache.page_size,
+                           max_context=min(cache.max_context, engine.model.max_positions))
+    results: List[Optional[ScoredText]] = [None] * len(texts)
+    for members in batches:
+        slots: List[int] = []
+        try:
+            for _ in members:
+                slots.append(engine.new_sequence())
+            r = engine.score(slots, [texts[i] for i in members], top=top)
+            lp, entropy, ids, best = (t.tolist() for t in r)
+            engine.check_status()
+        finally:
+            for s in slots:
+                engine.release(s)
+        at = 0
+        for i in members:
+            n = len(texts[i]) - 1
+            results[i] = ScoredText(lp[at:at + n], entropy[at:at + n], [list(zip(a, b)) for a, b in zip(ids[at:at + n], best[at:at + n])])
+            at += n
     return results

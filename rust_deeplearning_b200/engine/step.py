@@ -75,6 +75,11 @@ class Engine:
     def new_sequence(self) -> int:
         return self.cache.alloc_slot()
 
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """`n` more sequences that go on from where `slot` is, without running its tokens again: they share its pages of keys and values
+        (a page is copied when one of them comes to write into it) and get its state."""
+        return self.cache.fork(slot, n)
+
     def release(self, slot: int):
         self.cache.free_slot(slot)
 
@@ -103,6 +108,33 @@ class Engine:
         are wanted.  Returns float32 logits [wanted places, vocab] on the device, in the order of
         the sequences and of their wanted places.  When it comes from a graph the tensor is
         reused by the next step of the same shape: consume it before stepping again."""
+        return self._step(slots, tokens, want, fed, None)
+
+    def score(self, slots: Sequence[int], tokens: Sequence[Sequence[int]], following: Optional[Sequence[int]] = None,
+              top: int = 0) -> ops.TokenLogprobs:
+        """Run `tokens[i]` as the next tokens of sequence `slots[i]`, as `step` does, and say how probable each was by what came before it, with the
+        entropy of that choice and its `top` most probable tokens, in nats, for the sequences one after another: len(tokens[i]) - 1
+        rows each, the first for tokens[i][1].  following: for each sequence the token behind its new ones, which gets a row too.
+        The logits are not kept (`ops.linear_logprobs`), so long texts need no memory for them.
+
+        A sequence's first token is scored by `step(..., "last")` of what is before it, or by giving it as `following` of that step.  A step
+        without any row (one token a sequence, nothing following) runs all the same."""
+        lens = [len(t) for t in tokens]
+        if following is None:
+            want, targets = [list(range(l - 1)) for l in lens], [list(t)[1:] for t in tokens]
+        else:
+            if len(following) != len(tokens):
+                raise StepError("`following` must name a token for every sequence")
+            want, targets = "all", [list(t)[1:] + [f] for t, f in zip(tokens, following)]
+        targets = np.asarray([t for ts in targets for t in ts])
+        if targets.size and (targets.dtype.kind not in "iu" or targets.min() < 0 or targets.max() >= self.model.vocab_size):
+            raise StepError(f"token ids must be whole numbers inside the vocabulary of {self.model.vocab_size}")
+        most = min(ops.LOGPROBS_MAX_TOP, self.model.vocab_size)
+        if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= most:
+            raise StepError(f"top must be a whole number from 0 to {most}")
+        return self._step(slots, tokens, want, None, (targets.astype(np.int32), top))
+
+    def _step(self, slots, tokens, want, fed, scored):
         n = len(slots)
         if fed is not None:
             prev, src = fed
@@ -146,7 +178,7 @@ class Engine:
         widths = [g.table_width for g in self.cache.kv_groups]
         is_decode = max(lens) == 1
 
-        if is_decode and self.use_graphs:
+        if is_decode and self.use_graphs and scored is None:
             logits = self._graph_step(slots, tokens, past, want, tables, widths, max(totals), fed)
         else:
             n_want = sum(len(w) for w in want)
@@ -163,6 +195,11 @@ class Engine:
             batch.status = self.status
             batch.has_past = max(past) > 0
             batch.longest_new = max(lens)
+            if scored is not None:
+                targets = torch.from_numpy(scored[0])
+                if self.device.type == "cuda":
+                    targets = targets.pin_memory().to(self.device, non_blocking=True)
+                batch.scored = (targets, scored[1])
             logits = self._forward(batch)
             self.eager_steps += 1
         self.cache.advance(slots, lens)

@@ -72,6 +72,10 @@ class LinearHead:
         z = ops.linear(n, self.weight, out_dtype=torch.float32, softcap=self.softcap)
         return ops.scale_(z, self.scale) if self.scale != 1.0 else z
 
+    def logprobs(self, n, targets: torch.Tensor, top: int) -> "ops.TokenLogprobs":
+        """How probable the tokens `targets` are by the logits of rows n, without keeping the logits."""
+        return ops.linear_logprobs(n, self.weight, targets, top, self.softcap, self.scale)
+
 
 register_part("head", "linear_head",
               lambda spec, ctx: LinearHead(ctx.tensor(spec.tensors["weight"]), spec.params.get("softcap"),
@@ -347,7 +351,8 @@ class Model:
         return out
 
     def forward(self, batch, cache) -> torch.Tensor:
-        """Runs the batch's tokens through the schedule; float32 logits [wanted rows, vocab]."""
+        """Runs the batch's tokens through the schedule; float32 logits [wanted rows, vocab], or, where `batch.scored` gives each wanted row a
+        token (and how many alternatives to name), how probable those are (`ops.TokenLogprobs`)."""
         batch.cache_owner_of, batch.shared_runs = self.cache_owner_of, self.shared_runs
         batch.new_kv.clear()
         batch.carried.clear()
@@ -357,7 +362,7 @@ class Model:
         stream = self.start_stream(embedded.clone() if self.keeps_embedding and 0 not in self.entries else embedded)
         stream.deferred_rows = self.deferred_rows
         batch.deferred_writes.clear()
-        lazy_head = getattr(self.head, "takes_deferred_rows", False)
+        lazy_head = getattr(self.head, "takes_deferred_rows", False) and batch.scored is None
         for run, entry in enumerate(self.schedule):
             # what the stream will be asked for after this block, where the asker's first product takes the split form
             if run in self.entries:
@@ -380,9 +385,15 @@ class Model:
         batch.carried.clear()
         if batch.n_want == 0:
             stream.value()
-            return torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
+            none = torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
+            return none if batch.scored is None else ops.token_logprobs(none, *batch.scored)
         n = stream.normed_rows(self.final_norm, batch.want_rows, self.dtype, deferred_ok=lazy_head)
-        return self.head.forward(n)
+        if batch.scored is None:
+            return self.head.forward(n)
+        targets, top = batch.scored
+        if hasattr(self.head, "logprobs"):
+            return self.head.logprobs(n, targets, top)
+        return ops.token_logprobs(self.head.forward(n), targets, top)
 
 
 def build_block(layer: LayerSpec, ctx: BuildContext):
