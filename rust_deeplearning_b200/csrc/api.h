@@ -11,7 +11,7 @@ extern "C" {
 #define RDL_ACT_SILU 1
 #define RDL_ACT_SWISH_LIMIT 2   // min(g, L) sigmoid(1.702 min(g, L)) (clamp(u, -L, L) + 1), L a parameter
 
-#define RDL_ABI_VERSION 28
+#define RDL_ABI_VERSION 29
 
 const char* rdl_last_error(void);
 int rdl_abi_version(void);
@@ -31,13 +31,15 @@ void rdl_set_programmatic_launch(int on);
 #define RDL_FAULT_MX_FEW 8             // mx_few_rows: a weight copy or a product did not complete
 #define RDL_FAULT_MX_MANY 9            // mx_many_rows: a stage or an accumulator was not handed over
 #define RDL_FAULT_MX_SOME 10           // mx_some_rows: as 9
+#define RDL_FAULT_LOGPROBS_HEAD 12     // linear_logprobs: a stage or an accumulator was not handed over
 #define RDL_FAULT_TARGET_ID 11         // token_logprobs, linear_logprobs: a token id outside the vocabulary (its log probability is NaN)
 
 // For tests of the bounded waits: the kernel whose fault code is `code` gives up a wait after `cycles`
 // clock cycles instead of about a second, and announces `extra_tx_bytes` more bytes to the barrier of
 // its first copy than that copy delivers, so that this one wait cannot complete.  The block then
 // records its code and returns normally.  code 0 switches the test off.  Kernels with the codes
-// RDL_FAULT_ATTENTION_DECODE, RDL_FAULT_GEMM_STREAM, RDL_FAULT_MX_FEW, RDL_FAULT_MX_MANY and RDL_FAULT_MX_SOME honour it.
+// RDL_FAULT_ATTENTION_DECODE, RDL_FAULT_GEMM_STREAM, RDL_FAULT_MX_FEW, RDL_FAULT_MX_MANY, RDL_FAULT_MX_SOME and RDL_FAULT_LOGPROBS_HEAD
+// honour it.
 void rdl_set_wait_test(int code, long long cycles, int extra_tx_bytes);
 
 // One attention call over a batch of sequences: the new tokens of this step are the queries,
@@ -577,6 +579,12 @@ int rdl_sample(int* out_tokens, int* host_tokens, const float* logits, int n_row
 // log probabilities, equal logits in the order of their ids and NaN behind everything (csrc/logprobs.cuh).  In nats.
 int rdl_token_logprobs(const void* logits, int dtype, long long row_stride, int rows, int vocab, const int* targets, int top, float* logprobs,
                        float* entropy, float* top_logprobs, int* top_ids, int* status, void* stream);
+
+// The same of the logits scale * softcap(x w^T) of bfloat16 rows x [rows][k] behind an output head w [vocab][k], which are not kept (softcap 0:
+// none).  k is a multiple of 8.  work: rdl_linear_logprobs_work_bytes of device memory, which only this call uses until it has ended.
+int rdl_linear_logprobs(const void* x, const void* w, int rows, int vocab, int k, const int* targets, int top, float softcap, float scale,
+                        float* logprobs, float* entropy, float* top_logprobs, int* top_ids, void* work, long long work_bytes, int* status, void* stream);
+long long rdl_linear_logprobs_work_bytes(int rows, int vocab, int top);
 
 // Rows copied within tensors: row dst of every set becomes row src, for each tensor's list of pairs: list + 2 first_pair holds
 // `pairs` sources, then as many destinations; tensors may share a list.  Strides in bytes, tensors and list in host memory (read before the call returns).  No destination may be a source or

@@ -23,7 +23,7 @@ from concurrent.futures import ThreadPoolExecutor
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(_PKG, "csrc")
 LIB_NAME = "librdl_b200_kernels.so"
-ABI_VERSION = 28
+ABI_VERSION = 29
 
 # fast math is never enabled: the 32-bit path relies on exact tanhf/expf/sqrtf and plain FMA
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -192,6 +192,7 @@ FAULTS = {
     9: "mx_many_rows: a stage or an accumulator was not handed over",
     10: "mx_some_rows: a stage or an accumulator was not handed over",
     11: "token_logprobs: a token id outside the vocabulary (its log probability is NaN)",
+    12: "linear_logprobs: a stage or an accumulator was not handed over",
 }
 
 
@@ -458,6 +459,7 @@ _SIGNATURES = {
     "rdl_random_normal": [_P, _I, _LL, ctypes.c_ulonglong, ctypes.c_double, _P],
     "rdl_sample": [_P, _P, _P, _I, _I, ctypes.POINTER(SamplingArgs), _P, _P, _P, _P, _P, _P],
     "rdl_token_logprobs": [_P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
+    "rdl_linear_logprobs": [_P, _P, _I, _I, _I, _P, _I, _F, _F, _P, _P, _P, _P, _P, _LL, _P, _P],
     "rdl_copy_rows": [ctypes.POINTER(CopyRowsTensor), _I, _P, _P],
     "rdl_upload_batch": [_P, _P, _I, _P, _I, _I, _I, _P],
     "rdl_latent_prepare": [ctypes.POINTER(LatentPrepareArgs), _P],
@@ -517,6 +519,8 @@ def load():
         lib.rdl_delta_rule_chunked_work_bytes.restype = _LL
         lib.rdl_matrix_memory_chunked_work_bytes.argtypes = [_I, _I, _I, _I, _I]
         lib.rdl_matrix_memory_chunked_work_bytes.restype = _LL
+        lib.rdl_linear_logprobs_work_bytes.argtypes = [_I, _I, _I]
+        lib.rdl_linear_logprobs_work_bytes.restype = _LL
         lib.rdl_latent_decode_scratch_bytes.argtypes = [_I, _I, _I, _I]
         lib.rdl_latent_decode_scratch_bytes.restype = _LL
         lib.rdl_sampling_uniform.argtypes = [ctypes.c_ulonglong] * 3

@@ -1248,6 +1248,14 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
     _logprobs_check("linear_logprobs", rows, vocab, x.device, targets, top)
     _stream(x)
     out = _logprobs_result(x, rows, top, targets is not None)
+    if rows > SKINNY_MAX_ROWS and type(weight) is not Mx4Weight and _bf16_ok(x, weight):
+        lib = library.load()
+        with _on_device(x.device):
+            work = torch.empty(lib.rdl_linear_logprobs_work_bytes(rows, vocab, top), dtype=torch.uint8, device=x.device)
+            library.check(lib.rdl_linear_logprobs(_ptr(x), _ptr(weight), rows, vocab, x.shape[1], _ptr(targets), top, float(softcap or 0.0), float(scale),
+                                                  _ptr(out.logprobs), _ptr(out.entropy), _ptr(out.top_logprobs), _ptr(out.top_ids), _ptr(work),
+                                                  work.numel(), _status(status), _stream(x)))
+        return out
     piece = max(1, LOGPROBS_PIECE // vocab)
     for r in range(0, rows, piece):
         z = linear(x[r:r + piece], weight, torch.float32, softcap, status)
