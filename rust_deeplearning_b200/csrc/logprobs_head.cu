@@ -26,20 +26,23 @@
 namespace {
 
 constexpr int BM = 128, BN = 256, BK = 64, EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, THREADS = 64 + EPI_THREADS;
-constexpr int ASIDE = 8, AT_ONCE = 4;                     // logits a thread puts aside; that are looked at between two looks at how full that is
-constexpr int TMEM_COLS = 2 * BN, MOST_STAGES = 6;
+constexpr int AT_ONCE = 8;                                // logits of a row that are looked at together
+constexpr int TMEM_COLS = 2 * BN;
 constexpr int SMEM_BYTES = 232448 - 1024;                 // a block's limit less the static variables
 __host__ __device__ constexpr int stage_bytes(int ctas) { return BM * BK * 2 + BN / ctas * BK * 2; }
+__host__ __device__ constexpr int stages(int ctas) { return (SMEM_BYTES - 1024) / stage_bytes(ctas); }      // 7 of a pair, 4
 
 struct HeadArgs {
     int M, N, kblocks;
     int row_blocks, tiles_n;                              // of 128 CTAS rows, of 256 tokens
     int groups, slices, main_tiles;                       // slices share the first main_tiles tiles of every row block
-    int stages, top;
+    int top, places;                                      // alternatives; logits a thread can put aside
     float cap, inv_cap, scale;
     const int* targets; float* target_logit;              // [M]
-    float4* stats;                                        // [slot][column half][row of the block]: m, s, t
-    LpKey* keys;                                          // [slot][column half][top][row of the block]
+    float4* stats;                                        // [slot][column half][row of the block]: m, s, t, how many are put aside
+    float2* aside;                                        // [slot][column half][row of the block][places]: a logit and its token
+    LpKey* keys;                                          // [slot][column half][top][row of the block]: lists, where there are any
+    unsigned* seen;                                       // [32][M]: what groups of a row's columns were seen to hold at most (order-preserving bits)
     long long wait_cycles; int test_extra_tx;
     int* status;
 };
@@ -135,39 +138,156 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// A thread's `n` logits put aside, into its sorted list of `top` places (both in shared memory, a thread's keys EPI_THREADS apart).  Returns
-// what a logit must exceed to enter: NaN while anything does.
-__device__ __noinline__ float put_away(LpKey* list, const LpKey* aside, int n, int top) {
-    LpKey last = list[(top - 1) * EPI_THREADS];
-    for (int i = 0; i < n; ++i) {
-        const LpKey k = aside[i * EPI_THREADS];
-        if (k <= last) continue;
-        int p = top - 1;
-        for (; p > 0; --p) {
-            const LpKey above = list[(p - 1) * EPI_THREADS];
-            if (above > k) break;
-            list[p * EPI_THREADS] = above;
+// ---- the list of a row, kept by one thread ----
+//
+// All lanes of a warp work on their own rows at once and without exchanges.
+
+__device__ __forceinline__ void exchange(LpKey& a, LpKey& b) {      // the larger one first
+    const LpKey x = a, y = b;
+    a = x > y ? x : y;
+    b = x > y ? y : x;
+}
+// 16 keys into descending order, from a sequence that falls and then rises
+__device__ __forceinline__ void fall16(LpKey (&k)[16]) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((i & o) == 0) exchange(k[i], k[i + o]);
+}
+
+// Logits that may be among a row's largest are put aside in memory with their tokens, and the second kernel looks among them.  Should a thread
+// have put aside as many as there is place for (its logits rise along the vocabulary, say), it makes them a sorted list there: `n` of them at
+// `aside`, into `top` places `stride` keys apart, which `empty` says hold nothing yet.  Called, not inlined, and in loops: it is hardly ever
+// needed, and what lies between the instructions that are makes those wait for theirs.
+__device__ __noinline__ void put_away(LpKey* list, long long stride, const float2* aside, int n, int top, bool empty) {
+#pragma unroll 1
+    for (int done = 0; done < n; done += 16) {
+        LpKey fresh[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) fresh[i] = done + i < n ? lp_key(aside[done + i].x, __float_as_uint(aside[done + i].y)) : 0;
+#pragma unroll 1
+        for (int r = 0; r < 8; ++r) {                      // neighbours against each other, 16 rounds in all
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) exchange(fresh[i], fresh[i + 1]);
+#pragma unroll
+            for (int i = 1; i < 15; i += 2) exchange(fresh[i], fresh[i + 1]);
         }
-        list[p * EPI_THREADS] = k;
-        last = list[(top - 1) * EPI_THREADS];
+#pragma unroll 1
+        for (int first = 0; first < top; first += 16) {    // 16 places at a time: they keep the largest, the rest goes on
+            LpKey held[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) held[i] = first + i < top && !(empty && done == 0) ? list[(first + i) * stride] : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const LpKey a = held[i], b = fresh[15 - i];
+                held[i] = a > b ? a : b;
+                fresh[15 - i] = a > b ? b : a;
+            }
+            fall16(held);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (first + i < top) list[(first + i) * stride] = held[i];
+            if (first + 16 < top) fall16(fresh);
+        }
     }
-    return (last >> 32) == 0 ? NAN : lp_key_logit(last);
+}
+
+// A logit that is not below or equal to `least` (a NaN on either side passes), and its token, to `at`, which moves on; one lane as the
+// other without a branch
+__device__ __forceinline__ void put_aside(float2*& at, float v, float least, int token) {
+    asm volatile("{\n.reg .pred p;\nsetp.gtu.f32 p, %1, %2;\n@p st.global.v2.b32 [%0], {%1, %3};\n@p add.s64 %0, %0, 8;\n}"
+                 : "+l"(at) : "f"(v), "f"(least), "r"(token) : "memory");
+}
+
+// What a logit must exceed.  A row's columns form 32 groups (by column mod 32), and `seen` holds the largest logit that any block has seen of each
+// so far.  At least `top` logits are not below the top-th of these 32, so that a logit below it is none of the row's `top` largest,
+// whatever else comes.  When another block's numbers arrive does not change a result, only what is put aside.
+//
+// A thread keeps the maxima of what it has seen in registers, puts them in and takes the bound of all after its first tile (which it goes
+// through a second time for what exceeds that) and after every doubling of its tiles.  Of N logits in no order about 1.5 top / N of the next
+// exceed the bound.  Measured instead, 2,048 rows and 20 alternatives: a sorted list a thread in shared memory (a call that merges 16 logits
+// waits 10,000 cycles for its instructions) 1.8 ms, its logits alone in registers (2,000 instructions a piece of 32 columns) 4.1 ms.
+//
+__device__ __forceinline__ unsigned ordered(float z) {
+    const unsigned u = __float_as_uint(z);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(unsigned o) { return o == 0 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+
+// What a row's logit must exceed, NaN where nothing is known; the number under the top-th value keeps logits that equal it.
+// `least` rises to `now` where that is known and higher
+__device__ __forceinline__ void begin_with(float& least, float now) {
+    if (!(now < least) && now == now) least = now;
+}
+template <int N>
+__device__ __forceinline__ float bound_among(float (&v)[N], int top) {
+#pragma unroll 1
+    for (int r = 0; r < N / 2; ++r) {                      // neighbours against each other, N rounds in all
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float hi = fmaxf(v[i], v[i + 1]);
+            v[i + 1] = fminf(v[i], v[i + 1]);
+            v[i] = hi;
+        }
+#pragma unroll
+        for (int i = 1; i < N - 1; i += 2) {
+            const float hi = fmaxf(v[i], v[i + 1]);
+            v[i + 1] = fminf(v[i], v[i + 1]);
+            v[i] = hi;
+        }
+    }
+    float b = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) b = top - 1 == i ? v[i] : b;
+    if (b == -INFINITY) return NAN;
+    if (b == 0.f) return -__uint_as_float(1);
+    return __uint_as_float(b > 0.f ? __float_as_uint(b) - 1 : __float_as_uint(b) + 1);
+}
+__device__ __noinline__ float bound_of(const unsigned* seen, int rows, int top) {
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = from_ordered(__ldcg(seen + (long long)i * rows));
+    if (top > 8) return bound_among(v, top);
+    float w[16];                                           // few alternatives: 16 groups tell as much
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = fmaxf(v[i], v[i + 16]);
+    return bound_among(w, top);
+}
+
+// Logits from their sums of products.  cap tanh(y) = cap - 2 cap / (e^(2 y) + 1), from the hardware's power and reciprocal (2^-22 and 2^-23 of
+// themselves): off by at most 2^-22 of the cap wherever it lies, which is less than float32 sums of a few hundred products are off by; tanhf
+// would take five times the instructions, and the tile's statistics longer than its products.
+__device__ __forceinline__ void logits_of(const HeadArgs& a, float (&v)[32]) {
+    if (a.cap > 0.f) {
+        const float f = a.inv_cap * (2.f * LP_LOG2E), c2 = -2.f * a.cap;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            float r;
+            asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(lp_exp2(v[i] * f) + 1.f));
+            v[i] = fmaf(c2, r, a.cap);
+        }
+    }
+    if (a.scale != 1.f) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= a.scale;
+    }
 }
 
 template <int CTAS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ HeadArgs a) {
-    constexpr int STAGE = stage_bytes(CTAS), A_BYTES = BM * BK * 2, ROWS = BM * CTAS;
+    constexpr int STAGE = stage_bytes(CTAS), STAGES = stages(CTAS), A_BYTES = BM * BK * 2, ROWS = BM * CTAS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long full_bar[MOST_STAGES], empty_bar[MOST_STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1), group = blockIdx.x / CTAS;
     if (threadIdx.x == 0) {
         gave_up = 0;
-        for (int s = 0; s < MOST_STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mx_bar_init(mx_smem(&full_bar[s]), 1);
             mx_bar_init(mx_smem(&empty_bar[s]), 1);
         }
@@ -216,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
                     }
                     __syncwarp();
                     extra = 0;
-                    if (++s == a.stages) { s = 0; parity ^= 1; }
+                    if (++s == STAGES) { s = 0; parity ^= 1; }
                 }
             }
         }
@@ -240,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
                         commit<CTAS>(mx_smem(&empty_bar[s]));
                     }
                     __syncwarp();
-                    if (++s == a.stages) { s = 0; parity ^= 1; }
+                    if (++s == STAGES) { s = 0; parity ^= 1; }
                 }
                 if (ok && mx_elect()) commit<CTAS>(mx_smem(&acc_full[buf]));
                 __syncwarp();
@@ -248,9 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
         }
     } else {
         // ---- statistics and lists: warp q of four has the lanes of rows 32 q + lane, and of two such warps each has half of the columns ----
-        const int q = warp & 3, half = (warp - 2) >> 2, own_row = rank * BM + q * 32 + lane, id = (int)threadIdx.x - 64;
-        LpKey* list = reinterpret_cast<LpKey*>(smem + (size_t)a.stages * STAGE) + id;
-        LpKey* aside = list + (TOP ? a.top : 0) * EPI_THREADS;
+        const int q = warp & 3, half = (warp - 2) >> 2, own_row = rank * BM + q * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
         const uint32_t to_issuer = CTAS == 1 ? mx_smem(&acc_empty[0]) : map_to_block(mx_smem(&acc_empty[0]), 0);
         int lt = 0;
@@ -261,33 +379,45 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
             LpStats st = lp_empty();
             float s_low = 0.f, t_low = 0.f;               // what the sums have lost to rounding: thousands of tiles may come
             float least = mine ? NAN : INFINITY;          // what a logit must exceed to enter the list (NaN: nothing)
-            int n_aside = 0;
+            const long long place = 2LL * slot + half;
+            float2* const aside = a.aside + (TOP ? (place * ROWS + own_row) * a.places : 0);
+            float2* at = aside;                           // where the next logit is put aside
+            bool listed = false;                          // whether some have been put into a list
+            float groups[TOP ? 32 : 1];                   // the largest of every group
             if (TOP)
-                for (int i = 0; i < a.top; ++i) list[i * EPI_THREADS] = 0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) groups[j] = -INFINITY;
+            auto put_in = [&] {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) atomicMax(a.seen + (long long)j * a.M + row, ordered(groups[j]));
+            };
             for (int t = t0; t < t1; ++t, ++lt) {
                 const int buf = lt & 1;
                 if (!mx_warp_wait(mx_smem(&acc_full[buf]), (lt >> 1) & 1, a.wait_cycles, gave_up_v)) { ok = false; break; }
                 mx_fence_after();
                 const int n0 = t * BN + half * (BN / 2);
+                const int since = t - t0;
+                const bool two = TOP && since == 0 && t1 - t0 > 1;
+                if (TOP && since > 0 && (since & (since - 1)) == 0 && mine) {
+                    if (since > 1) put_in();
+                    begin_with(least, bound_of(a.seen + row, a.M, a.top));
+                }
 #pragma unroll 1
-                for (int c = 0; c < BN / 2; c += 32) {
-                    const int n = n0 + c, there = a.N - n;                 // columns from here on
+                for (int i = two ? -4 : 0; i < 4; ++i) {
+                    const int c = (i & 3) * 32, n = n0 + c, there = a.N - n;                 // columns from here on
+                    if (two && i == 0 && mine) {
+                        put_in();
+                        begin_with(least, bound_of(a.seen + row, a.M, a.top));
+                    }
                     float v[32];
                     if (any_row && there > 0) tmem_ld32(lanes + (uint32_t)(buf * BN + c), v);
-                    if (c == BN / 2 - 32) {                                // the last columns are in registers: the accumulator is free
+                    if (i == 3) {                                // the last columns are in registers: the accumulator is free
                         mx_fence_before();
                         __syncwarp();
                         if (lane == 0) arrive_at(to_issuer + (uint32_t)(buf * 8));
                     }
                     if (!any_row || there <= 0) continue;
-                    if (a.cap > 0.f && mine) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = a.cap * tanhf(v[i] * a.inv_cap);
-                    }
-                    if (a.scale != 1.f) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= a.scale;
-                    }
+                    if (mine) logits_of(a, v);
                     if (there < 32) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = i < there ? v[i] : -INFINITY;
@@ -298,48 +428,56 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
                         for (int i = 1; i < 32; ++i) z = target - n == i ? v[i] : z;
                         if (target < a.N) a.target_logit[row] = z;
                     }
-                    float most = v[0];
+                    float of[32 / AT_ONCE], most = -INFINITY;             // the largest of every few
 #pragma unroll
-                    for (int i = 1; i < 32; ++i) most = fmaxf(most, v[i]);
-                    if (most > st.m) {
-                        const float d = fmaxf(st.m - most, -1e30f), f = lp_exp2(d * LP_LOG2E);
-                        t_low = f * fmaf(s_low, d, t_low);
-                        s_low *= f;
-                        lp_move(st, most);
+                    for (int g = 0; g < 32 / AT_ONCE; ++g) {
+                        of[g] = v[g * AT_ONCE];
+#pragma unroll
+                        for (int i = 1; i < AT_ONCE; ++i) of[g] = fmaxf(of[g], v[g * AT_ONCE + i]);
+                        most = fmaxf(most, of[g]);
                     }
-                    LpStats more = {st.m, 0.f, 0.f};
-                    lp_add(more, v);
-                    const float ys = more.s + s_low, ns = st.s + ys, yt = more.t + t_low, nt = st.t + yt;
-                    s_low = ys - (ns - st.s);
-                    t_low = yt - (nt - st.t);
-                    st.s = ns;
-                    st.t = nt;
-                    if (TOP && __any_sync(0xffffffffu, !(most <= least))) {
+                    if (!two || i < 0) {
+                        if (most > st.m) {
+                            const float d = fmaxf(st.m - most, -1e30f), f = lp_exp2(d * LP_LOG2E);
+                            t_low = f * fmaf(s_low, d, t_low);
+                            s_low *= f;
+                            lp_move(st, most);
+                        }
+                        LpStats more = {st.m, 0.f, 0.f};
+                        lp_add(more, v);
+                        const float ys = more.s + s_low, ns = st.s + ys, yt = more.t + t_low, nt = st.t + yt;
+                        s_low = ys - (ns - st.s);
+                        t_low = yt - (nt - st.t);
+                        st.s = ns;
+                        st.t = nt;
+                        if (TOP)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) groups[j] = fmaxf(groups[j], v[j]);
+                    }
+                    if (TOP && i >= 0 && __any_sync(0xffffffffu, !(most <= least))) {
 #pragma unroll
                         for (int g = 0; g < 32; g += AT_ONCE) {
-                            if (__any_sync(0xffffffffu, n_aside > ASIDE - AT_ONCE)) {
-                                if (mine) least = put_away(list, aside, n_aside, a.top);
-                                n_aside = 0;
+                            if (!__any_sync(0xffffffffu, !(of[g / AT_ONCE] <= least))) continue;
+                            if (__any_sync(0xffffffffu, at > aside + (a.places - AT_ONCE))) {
+                                if (mine) put_away(a.keys + place * a.top * ROWS + own_row, ROWS, aside, (int)(at - aside), a.top, !listed);
+                                at = aside;
+                                listed = true;
                             }
+                            if (there >= 32) {
 #pragma unroll
-                            for (int i = g; i < g + AT_ONCE; ++i)
-                                if (!(v[i] <= least) && i < there) {
-                                    aside[n_aside * EPI_THREADS] = lp_key(v[i], (unsigned)(n + i));
-                                    ++n_aside;
-                                }
+                                for (int j = g; j < g + AT_ONCE; ++j) put_aside(at, v[j], least, n + j);
+                            } else {
+#pragma unroll
+                                for (int j = g; j < g + AT_ONCE; ++j)
+                                    if (j < there) put_aside(at, v[j], least, n + j);
+                            }
                         }
                     }
                 }
             }
             if (!ok) break;
-            if (mine) {
-                const long long place = 2LL * slot + half;
-                a.stats[place * ROWS + own_row] = make_float4(st.m, st.s + s_low, st.t + t_low, 0.f);
-                if (TOP) {
-                    put_away(list, aside, n_aside, a.top);
-                    for (int i = 0; i < a.top; ++i) a.keys[(place * a.top + i) * ROWS + own_row] = list[i * EPI_THREADS];
-                }
-            }
+            // with the statistics: how many logits have been put aside, one's complement where there is a list as well
+            if (mine) a.stats[place * ROWS + own_row] = make_float4(st.m, st.s + s_low, st.t + t_low, __int_as_float(listed ? ~(int)(at - aside) : (int)(at - aside)));
         }
     }
     if (!ok && a.status) atomicExch(a.status, RDL_FAULT_LOGPROBS_HEAD);
@@ -356,10 +494,19 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
     }
 }
 
+// Nothing has been seen yet.
+__global__ void __launch_bounds__(256) head_clear_kernel(unsigned* seen, long long n) {
+    rdl_grid_wait();
+    rdl_grid_launch_dependents();
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
+    if (i < n) seen[i] = 0;
+}
+
 // ---- the partial results of a row, joined: a block a row ----
 
 struct JoinOut { float* logprobs; float* entropy; float* top_logprobs; int* top_ids; };
 
+// Partial results are shared out to the warps, a lane one.  What they have put aside is looked at 32 logits at a time, no matter whose they are.
 template <int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) head_join_kernel(const __grid_constant__ HeadArgs a, int rows_a_block, JoinOut o) {
     __shared__ LpStats part[WARPS];
@@ -378,27 +525,65 @@ __global__ void __launch_bounds__(WARPS * 32) head_join_kernel(const __grid_cons
     rdl_grid_wait();
     rdl_grid_launch_dependents();
     LpStats st = lp_empty();
-    LpKey keys = 0;
-    const int n = a.slices + x1 - x0;
-    for (int p = warp; p < 2 * n; p += WARPS) {
-        const int i = p >> 1;
-        if (i >= a.slices && total * (x0 + i - a.slices) / extras == total * (x0 + i - a.slices + 1) / extras) continue;
-        const long long place = 2LL * (i < a.slices ? block * a.slices + i : mains + (x0 + i - a.slices) + block) + (p & 1);
-        const float4 s = a.stats[place * rows_a_block + own_row];
-        lp_join(st, LpStats{s.x, s.y, s.z});
-        if (a.top > 0) {
-            const LpKey k = lane < a.top ? a.keys[(place * a.top + lane) * rows_a_block + own_row] : 0;
-            keys = lp_merge(keys, k, lane);
+    LpKey keys = 0, least = 0;
+    const int n = 2 * (a.slices + x1 - x0);
+    auto offer = [&](LpKey key) {                          // a key a lane, or 0
+        if (!__any_sync(0xffffffffu, key > least)) return;
+        keys = lp_merge(keys, lp_sort(key, lane), lane);
+        least = __shfl_sync(0xffffffffu, keys, a.top - 1);
+    };
+    for (int first = warp * 32; first < n; first += WARPS * 32) {
+        const int p = first + lane, i = p >> 1, x = x0 + i - a.slices;
+        const bool there = p < n && (i < a.slices || total * x / extras != total * (x + 1) / extras);
+        const long long place = (2LL * (i < a.slices ? block * a.slices + i : mains + x + block) + (p & 1)) * rows_a_block + own_row;
+        int count = 0;
+        if (there) {
+            const float4 s = a.stats[place];
+            lp_join(st, LpStats{s.x, s.y, s.z});
+            count = __float_as_int(s.w);
+        }
+        if (a.top == 0) continue;
+        const bool listed = count < 0;
+        if (listed) count = ~count;
+        int upto = count;                                  // logits put aside by this lane's and the lanes before
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        const int all = __shfl_sync(0xffffffffu, upto, 31);
+        for (int e = 0; e < all; e += 32) {
+            // whose is number e + lane: the first lane whose count reaches beyond it
+            const int mine = e + lane;
+            int owner = 0;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) owner += __shfl_sync(0xffffffffu, upto, owner + d - 1) <= mine ? d : 0;
+            const long long at = __shfl_sync(0xffffffffu, place, owner & 31);
+            const int before = __shfl_sync(0xffffffffu, upto - count, owner & 31);
+            LpKey key = 0;
+            if (mine < all) {
+                const float2 v = a.aside[at * a.places + (mine - before)];
+                key = lp_key(v.x, __float_as_uint(v.y));
+            }
+            offer(key);
+        }
+        if (__any_sync(0xffffffffu, listed)) {
+            const long long list = place - own_row;        // rows of the places before
+            for (int k = 0; k < a.top; ++k) offer(listed ? a.keys[list * a.top + (long long)k * rows_a_block + own_row] : 0);
         }
     }
+    st = lp_warp_join(st);
     if (lane == 0) part[warp] = st;
     lists[warp][lane] = keys;
     __syncthreads();
-    if (warp != 0) return;
-    for (int w = 1; w < WARPS; ++w) {
-        lp_join(st, part[w]);
-        if (a.top > 0) keys = lp_merge(keys, lists[w][lane], lane);
+#pragma unroll 1
+    for (int w = WARPS / 2; w > 0; w >>= 1) {
+        if (warp < w && a.top > 0) lists[warp][lane] = lp_merge(lists[warp][lane], lists[warp + w][lane], lane);
+        if (WARPS > 1) __syncthreads();
     }
+    if (warp != 0) return;
+    keys = lists[0][lane];
+    st = lp_warp_join(lane < WARPS ? part[lane] : lp_empty());
     const float log_s = logf(st.s);
     if (lane == 0) {
         o.entropy[row] = log_s - st.t / st.s;
@@ -435,14 +620,18 @@ int rows_a_launch(int rows, int ctas) {
     const long long most = rows_at_once(ctas), launches = (rows + most - 1) / most, blocks = ((long long)rows + BM * ctas - 1) / (BM * ctas);
     return launches <= 1 ? rows : (int)((blocks + launches - 1) / launches * BM * ctas);
 }
-struct Work { long long stats, keys, targets, bytes; };
+// About 1.5 top ln(tiles) are put aside where logits come in no order.
+int places_for(int top) { return top ? 16 + 12 * top : 0; }
+struct Work { long long stats, keys, aside, targets, seen, bytes; };
 Work work_of(const HeadArgs& a, int ctas, int top) {
     const long long slots = (long long)a.groups + a.row_blocks, places = slots * 2 * BM * ctas;
     Work w;
     w.stats = 0;
     w.keys = w.stats + places * (long long)sizeof(float4);
-    w.targets = w.keys + places * top * (long long)sizeof(LpKey);
-    w.bytes = w.targets + ((long long)a.M * 4 + 15) / 16 * 16;
+    w.aside = w.keys + places * top * (long long)sizeof(LpKey);
+    w.targets = w.aside + places * places_for(top) * (long long)sizeof(float2);
+    w.seen = w.targets + ((long long)a.M * 4 + 15) / 16 * 16;
+    w.bytes = w.seen + (top ? 32LL * a.M * 4 : 0);
     return w;
 }
 
@@ -489,8 +678,7 @@ extern "C" int rdl_linear_logprobs(const void* x, const void* w, int rows, int v
         const Work space = work_of(a, ctas, top);
         a.kblocks = (k + BK - 1) / BK;
         a.top = top;
-        const int lists = top ? (top + ASIDE) * EPI_THREADS * (int)sizeof(LpKey) : 0, fit = (SMEM_BYTES - 1024 - lists) / stage_bytes(ctas);
-        a.stages = fit < MOST_STAGES ? fit : MOST_STAGES;
+        a.places = places_for(top);
         a.cap = softcap;
         a.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
         a.scale = scale;
@@ -498,17 +686,21 @@ extern "C" int rdl_linear_logprobs(const void* x, const void* w, int rows, int v
         a.stats = (float4*)((char*)work + space.stats);
         a.keys = (LpKey*)((char*)work + space.keys);
         a.target_logit = (float*)((char*)work + space.targets);
+        a.aside = (float2*)((char*)work + space.aside);
+        a.seen = (unsigned*)((char*)work + space.seen);
         a.wait_cycles = rdl_wait_cycles_for(RDL_FAULT_LOGPROBS_HEAD);
         a.test_extra_tx = rdl_test_extra_tx_for(RDL_FAULT_LOGPROBS_HEAD);
         a.status = status;
         CUtensorMap mx;
         if (int e = bf16_map(&mx, (const char*)x + r * k * 2, a.M, k, BM, "the rows")) return e;
+        if (top) RDL_CHECK_EX(rdl_launch(head_clear_kernel, dim3((unsigned)((32LL * a.M + 255) / 256)), dim3(256), 0, st, a.seen, 32LL * a.M), "linear_logprobs");
         const int e = ctas == 1 ? (top ? run<1, true>(mx, mw, a, st) : run<1, false>(mx, mw, a, st)) : (top ? run<2, true>(mx, mw, a, st) : run<2, false>(mx, mw, a, st));
         if (e) return e;
         const JoinOut o{targets ? logprobs + r : nullptr, entropy + r, top ? top_logprobs + r * top : nullptr, top ? top_ids + r * top : nullptr};
         // a row has few partial results where there are many rows, and the other way round
-        auto join = a.slices >= 16 ? head_join_kernel<16> : (a.slices >= 4 ? head_join_kernel<4> : head_join_kernel<1>);
-        RDL_CHECK_EX(rdl_launch(join, dim3((unsigned)a.M), dim3(a.slices >= 16 ? 512u : a.slices >= 4 ? 128u : 32u), 0, st, a, BM * ctas, o), "linear_logprobs");
+        const int warps = a.slices > 64 ? 16 : a.slices > 16 ? 4 : 1;
+        auto join = warps == 16 ? head_join_kernel<16> : warps == 4 ? head_join_kernel<4> : head_join_kernel<1>;
+        RDL_CHECK_EX(rdl_launch(join, dim3((unsigned)a.M), dim3(warps * 32u), 0, st, a, BM * ctas, o), "linear_logprobs");
     }
     return 0;
 }
