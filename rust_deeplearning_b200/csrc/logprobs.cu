@@ -1,11 +1,18 @@
 // Log probabilities of given tokens, entropy and the largest logits of rows of logits, in one pass over the row.
+//
+// Memory bounds many rows (2,048 rows of 256,000 float32 logits: 2.1 GB), latency few of them.  A row belongs to a block, or to a cluster of 2, 4
+// or 8 where there are fewer rows than the device has room for blocks.  A thread copies what it looks at into shared memory of its own,
+// LP_RING batches ahead (cp.async), so that memory is kept busy while lists are sorted, and no thread waits for another's copy.
 #include "api.h"
 #include "launch.cuh"
 #include "logprobs.cuh"
 
 namespace {
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_BATCH = 4;      // vectors a thread asks for before it uses the first
+constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_BATCH = 4, LP_RING = 3;                             // 16-byte vectors of a thread in a batch; batches on their way or looked at
+constexpr int LP_RING_BYTES = LP_RING * LP_BATCH * LP_THREADS * 16;
+constexpr int LP_MAX_CLUSTER = 8;
 
 struct LpArgs {
     const void* z;
@@ -17,12 +24,10 @@ struct LpArgs {
 };
 
 // 16 bytes of a row as floats
-__device__ __forceinline__ void lp_load16(const float* p, float (&f)[4]) {
-    const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+__device__ __forceinline__ void lp_widen(const uint4 v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
 }
-__device__ __forceinline__ void lp_load16(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void lp_widen(const uint4 v, float (&f)[8]) {
     const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -30,6 +35,12 @@ __device__ __forceinline__ void lp_load16(const __nv_bfloat16* p, float (&f)[8])
         f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
+__device__ __forceinline__ void lp_copy16(unsigned to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void lp_copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void lp_copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // A warp's list of largest logits while a row passes by.  Logits not below `least` are put aside in shared memory; when there are 32
 // of them they are sorted and merged into the list, whose last wanted place raises `least`: for itself, and through `shared_least` for
@@ -68,32 +79,111 @@ struct LpList {
         aside += __popc(mask);
         if (aside >= 32) take(32);
     }
+    // The first logits of a warp: of what its lanes hold at most, a logit below the top-th is none of the row's largest (32 logits here are
+    // not below that).
+    __device__ __forceinline__ void begin(float most) {
+        const LpKey k = lp_sort(lp_key(most, lane), lane);
+        const float bound = lp_key_logit(__shfl_sync(0xffffffffu, k, top - 1));
+        if (lane == 0) atomicMax(shared_least, (unsigned)(lp_key(bound, 0) >> 32));
+        least = fmaxf(least, bound);
+    }
     __device__ __forceinline__ void look() {                      // what the block's other warps have found
         least = fmaxf(least, lp_key_logit((LpKey)(*(volatile unsigned*)shared_least) << 32));
     }
 };
 
+__device__ __forceinline__ unsigned lp_cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned lp_cluster_size() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void lp_cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory"); }
+// a 32-bit word of the shared memory of the cluster's block `rank`
+__device__ __forceinline__ unsigned lp_remote(const void* p, unsigned rank) {
+    unsigned a, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
+    extern __shared__ uint4 ring[];                                  // [LP_RING][LP_BATCH][thread]
     __shared__ LpStats part[LP_WARPS];
     __shared__ LpKey lists[TOP ? LP_WARPS : 1][TOP ? 64 : 1];
     __shared__ unsigned shared_least;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long row = blockIdx.x;
+    const unsigned rank = lp_cluster_rank(), size = lp_cluster_size();
+    const long long row = blockIdx.x / size;
     if (threadIdx.x == 0) shared_least = 0;
     rdl_grid_wait();
     rdl_grid_launch_dependents();
     __syncthreads();
     const T* z = (const T*)a.z + row * a.row_stride;
-    // columns before the first 16-byte boundary, whole vectors, columns behind the last
+    // columns before the first 16-byte boundary, whole vectors, columns behind the last; a block of a cluster has its part of the vectors
     const int head = min(a.vocab, (int)(((16 - ((uintptr_t)z & 15)) & 15) / sizeof(T)));
-    const int vectors = (a.vocab - head) / V, tail = head + vectors * V;
+    const int all = (a.vocab - head) / V, tail = head + all * V;
+    const int from = (int)((long long)all * rank / size), vectors = (int)((long long)all * (rank + 1) / size) - from;
+    const T* body = z + head + (long long)from * V;
+    const int body_id = head + from * V;
+
+    const unsigned own = (unsigned)__cvta_generic_to_shared(ring + threadIdx.x);
+    constexpr int STEP = LP_THREADS * LP_BATCH;
+    auto ask = [&](int first, int place) {
+#pragma unroll
+        for (int j = 0; j < LP_BATCH; ++j) {
+            const int at = first + j * LP_THREADS + (int)threadIdx.x;
+            if (at < vectors) lp_copy16(own + (unsigned)((place * LP_BATCH + j) * LP_THREADS * 16), body + (long long)at * V);
+        }
+        lp_copies_end();
+    };
+#pragma unroll
+    for (int r = 0; r < LP_RING - 1; ++r) ask(r * STEP, r);
 
     LpStats st = lp_empty();
     LpList list;
     if (TOP) list = {0, -INFINITY, 0, lists[warp], &shared_least, a.top, lane};
-    if (warp == 0) {                                                 // fewer than 8 columns at either end
+    int place = 0;
+    for (int first = 0; first < vectors; first += STEP) {
+        ask(first + (LP_RING - 1) * STEP, place == 0 ? LP_RING - 1 : place - 1);
+        lp_copies_wait<LP_RING - 1>();
+        float v[LP_BATCH][V];
+        float most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < LP_BATCH; ++j) {
+            if (first + j * LP_THREADS + (int)threadIdx.x < vectors) {
+                lp_widen(ring[(place * LP_BATCH + j) * LP_THREADS + threadIdx.x], v[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[j][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) most = fmaxf(most, v[j][i]);
+        }
+        if (++place == LP_RING) place = 0;
+        if (most > st.m) lp_move(st, most);
+#pragma unroll
+        for (int j = 0; j < LP_BATCH; ++j) lp_add(st, v[j]);
+        if (TOP) {
+            if (first == 0) list.begin(most);
+            list.look();
+            if (__any_sync(0xffffffffu, !(most < list.least))) {
+#pragma unroll
+                for (int j = 0; j < LP_BATCH; ++j) {
+                    const int at = first + j * LP_THREADS + (int)threadIdx.x;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) list.offer(v[j][i], body_id + at * V + i, at < vectors);
+                }
+            }
+        }
+    }
+    if (warp == 0 && rank == 0) {                                    // fewer than 8 columns at either end
         const int i = lane < 16 ? lane : tail + lane - 16;
         const bool valid = lane < 16 ? lane < head : i < a.vocab;
         const float v = valid ? to_float<T>(z[i]) : -INFINITY;
@@ -101,38 +191,6 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
         const float one[1] = {v};
         if (valid) lp_add(st, one);
         if (TOP) list.offer(v, i, valid);
-    }
-    for (int first = 0; first < vectors; first += LP_THREADS * LP_BATCH) {
-        float v[LP_BATCH][V];
-#pragma unroll
-        for (int j = 0; j < LP_BATCH; ++j) {
-            const int at = first + j * LP_THREADS + (int)threadIdx.x;
-            if (at < vectors) {
-                lp_load16(z + head + (long long)at * V, v[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[j][i] = -INFINITY;
-            }
-        }
-        float most = v[0][0];
-#pragma unroll
-        for (int j = 0; j < LP_BATCH; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) most = fmaxf(most, v[j][i]);
-        if (most > st.m) lp_move(st, most);
-#pragma unroll
-        for (int j = 0; j < LP_BATCH; ++j) lp_add(st, v[j]);
-        if (TOP) {
-            list.look();
-            if (__any_sync(0xffffffffu, !(most < list.least))) {
-#pragma unroll
-                for (int j = 0; j < LP_BATCH; ++j) {
-                    const int at = first + j * LP_THREADS + (int)threadIdx.x;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) list.offer(v[j][i], head + at * V + i, at < vectors);
-                }
-            }
-        }
     }
     if (TOP) {
         if (list.aside > 0) list.take(list.aside);
@@ -149,8 +207,32 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
             __syncthreads();
         }
     }
+    if (warp == 0) {
+        st = lp_warp_join(lane < LP_WARPS ? part[lane] : lp_empty());
+        if (lane == 0) part[0] = st;
+    }
+    if (size > 1) {                                                  // the cluster's blocks, a warp of the first for each
+        lp_cluster_sync();
+        if (rank == 0 && warp > 0 && warp < (int)size) {
+            if (TOP) {
+                const LpKey lo = lp_remote((const unsigned*)&lists[0][lane], warp), hi = lp_remote((const unsigned*)&lists[0][lane] + 1, warp);
+                lists[warp][lane] = hi << 32 | lo;
+            }
+            if (lane < 3) ((unsigned*)&part[warp])[lane] = lp_remote((const unsigned*)&part[0] + lane, warp);
+        }
+        __syncthreads();
+        if (TOP && rank == 0) {
+#pragma unroll 1
+            for (int n = (int)size / 2; n > 0; n >>= 1) {
+                if (warp < n) lists[warp][lane] = lp_merge(lists[warp][lane], lists[warp + n][lane], lane);
+                __syncthreads();
+            }
+        }
+        lp_cluster_sync();                                           // no block leaves while its memory may be read
+        if (rank != 0) return;
+        if (warp == 0) st = lp_warp_join(lane < (int)size ? part[lane] : lp_empty());
+    }
     if (warp != 0) return;
-    st = lp_warp_join(lane < LP_WARPS ? part[lane] : lp_empty());
     const float log_s = logf(st.s);
     if (lane == 0) {
         a.entropy[row] = log_s - st.t / st.s;
@@ -168,6 +250,14 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
     }
 }
 
+template <typename T, bool TOP>
+int lp_run(const LpArgs& a, int cluster, cudaStream_t st) {
+    RDL_CUDA((rdl_allow_shared<token_logprobs_kernel<T, TOP>>(LP_RING_BYTES)), "token_logprobs");
+    RDL_CHECK_EX(rdl_launch_cluster(token_logprobs_kernel<T, TOP>, dim3((unsigned)a.rows * cluster), dim3(LP_THREADS), cluster, (size_t)LP_RING_BYTES, st, a),
+                 "token_logprobs");
+    return 0;
+}
+
 }  // namespace
 
 extern "C" int rdl_token_logprobs(const void* logits, int dtype, long long row_stride, int rows, int vocab, const int* targets, int top, float* logprobs,
@@ -179,8 +269,10 @@ extern "C" int rdl_token_logprobs(const void* logits, int dtype, long long row_s
     RDL_REQUIRE(logits && entropy && (!targets || logprobs) && (top == 0 || (top_logprobs && top_ids)), "token_logprobs: missing operand");
     RDL_REQUIRE((uintptr_t)logits % rdl_dtype_size(dtype) == 0, "token_logprobs: logits that are not on an element's boundary");
     const LpArgs a{logits, row_stride, rows, vocab, top, targets, logprobs, entropy, top_logprobs, top_ids, status};
-    auto kernel = dtype == RDL_BF16 ? (top ? token_logprobs_kernel<__nv_bfloat16, true> : token_logprobs_kernel<__nv_bfloat16, false>)
-                                    : (top ? token_logprobs_kernel<float, true> : token_logprobs_kernel<float, false>);
-    RDL_CHECK_EX(rdl_launch(kernel, dim3((unsigned)rows), dim3(LP_THREADS), 0, (cudaStream_t)stream, a), "token_logprobs");
-    return 0;
+    // blocks that share a row: as many as there is room for at once (two on a multiprocessor), each with a batch of its threads or more
+    int cluster = 1;
+    while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= 2 * rdl_sm_count() && (long long)vocab * (int)rdl_dtype_size(dtype) >= cluster * 2LL * LP_THREADS * 16) cluster *= 2;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == RDL_BF16) return top ? lp_run<__nv_bfloat16, true>(a, cluster, st) : lp_run<__nv_bfloat16, false>(a, cluster, st);
+    return top ? lp_run<float, true>(a, cluster, st) : lp_run<float, false>(a, cluster, st);
 }

@@ -397,12 +397,6 @@ class SamplingArgs(ctypes.Structure):
 COPY_ROWS_MAX_TENSORS = 64
 
 
-class CopyRowsTensor(ctypes.Structure):
-    """A tensor whose rows are copied, and its part of the list of pairs (`csrc/api.h`)."""
-    _fields_ = [("base", ctypes.c_void_p), ("set_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong), ("row_bytes", ctypes.c_longlong),
-                ("sets", ctypes.c_int), ("first_pair", ctypes.c_int), ("pairs", ctypes.c_int)]
-
-
 _P, _I, _F, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 _SIGNATURES = {
     "rdl_attention_plain": [ctypes.POINTER(AttentionArgs), _P],
@@ -460,7 +454,7 @@ _SIGNATURES = {
     "rdl_sample": [_P, _P, _P, _I, _I, ctypes.POINTER(SamplingArgs), _P, _P, _P, _P, _P, _P],
     "rdl_token_logprobs": [_P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P],
     "rdl_linear_logprobs": [_P, _P, _I, _I, _I, _P, _I, _F, _F, _P, _P, _P, _P, _P, _LL, _P, _P],
-    "rdl_copy_rows": [ctypes.POINTER(CopyRowsTensor), _I, _P, _P],
+    "rdl_copy_rows": [ctypes.c_char_p, _I, _P, _P],
     "rdl_upload_batch": [_P, _P, _I, _P, _I, _I, _I, _P],
     "rdl_latent_prepare": [ctypes.POINTER(LatentPrepareArgs), _P],
     "rdl_latent_write": [ctypes.POINTER(LatentPrepareArgs), _P],

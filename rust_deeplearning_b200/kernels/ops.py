@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 import functools
 import os
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -84,9 +85,9 @@ def _dense(t, name):
 _AS_IT_IS = contextlib.nullcontext()
 
 
-def _on_device(device: torch.device):
+def _on_device(index: int):
     """A launch goes to the current device; this makes it the tensors' own where it is another."""
-    return _AS_IT_IS if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _AS_IT_IS if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _int32(t, name, n=None):
@@ -1188,29 +1189,33 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
-def _logprobs_result(like: torch.Tensor, rows: int, top: int, with_targets: bool) -> TokenLogprobs:
-    f32 = dict(dtype=torch.float32, device=like.device)
-    return TokenLogprobs(torch.empty(rows, **f32) if with_targets else None, torch.empty(rows, **f32),
-                         torch.empty((rows, top), dtype=torch.int32, device=like.device), torch.empty((rows, top), **f32))
+def _logprobs_result(device, rows: int, top: int, with_targets: bool) -> TokenLogprobs:
+    f32 = torch.float32
+    return TokenLogprobs(torch.empty(rows, dtype=f32, device=device) if with_targets else None, torch.empty(rows, dtype=f32, device=device),
+                         torch.empty((rows, top), dtype=torch.int32, device=device), torch.empty((rows, top), dtype=f32, device=device))
 
 
 def _logprobs_check(who: str, rows: int, vocab: int, device, targets: Optional[torch.Tensor], top: int):
-    _need(vocab > 0, f"{who}: rows of no logits")
-    _need(isinstance(top, int) and not isinstance(top, bool) and 0 <= top <= min(LOGPROBS_MAX_TOP, vocab),
-          f"{who}: {top} alternatives of {vocab} tokens (a whole number, {LOGPROBS_MAX_TOP} at most)")
-    if targets is not None:
-        _need(targets.dtype is torch.int32 and targets.dim() == 1 and targets.numel() == rows and targets.is_contiguous() and targets.device == device,
-              f"{who}: targets must be contiguous int32 [{rows}] on {device}")
+    if vocab <= 0:
+        _refuse(f"{who}: rows of no logits")
+    if type(top) is not int or not 0 <= top <= LOGPROBS_MAX_TOP or top > vocab:
+        _refuse(f"{who}: {top} alternatives of {vocab} tokens (a whole number, {LOGPROBS_MAX_TOP} at most)")
+    if targets is not None and (targets.dtype is not torch.int32 or targets.shape != (rows,) or not targets.is_contiguous() or targets.device != device):
+        _refuse(f"{who}: targets must be contiguous int32 [{rows}] on {device}")
 
 
 def _token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor], out: TokenLogprobs, first: int, top: int, status):
     """Rows of logits into rows `first` and on of the result."""
-    rows, vocab = logits.shape
-    at = lambda t, width: ctypes.c_void_p(t.data_ptr() + 4 * first * width) if t is not None and width else None
-    with _on_device(logits.device):
+    lp, entropy, ids, best = out
+    index = logits.get_device()
+    if status is None:
+        status = _step_status
+    with _on_device(index):
         library.check(library.load().rdl_token_logprobs(
-            _ptr(logits), _dtype_code(logits), logits.stride(0), rows, vocab, at(targets, 1), top, at(out.logprobs, 1), at(out.entropy, 1),
-            at(out.top_logprobs, top), at(out.top_ids, top), _status(status), _stream(logits)))
+            logits.data_ptr(), _KINDS[logits.dtype], logits.stride(0), logits.shape[0], logits.shape[1],
+            targets.data_ptr() + 4 * first if targets is not None else None, top, lp.data_ptr() + 4 * first if lp is not None else None,
+            entropy.data_ptr() + 4 * first, best.data_ptr() + 4 * first * top, ids.data_ptr() + 4 * first * top,
+            status.data_ptr() if status is not None else None, _raw_stream(index)))
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0,
@@ -1221,12 +1226,15 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     A negative target asks for none and gets 0; one outside the vocabulary gets NaN and is reported to `status`.  Logits of minus infinity
     are tokens of probability 0.  A row with a NaN or plus infinity, or of minus infinities alone, has no distribution: NaN (its
     alternatives are still those of its largest logits, a NaN counting as the smallest)."""
-    _need(logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1) and logits.stride(0) >= 0, "token_logprobs: logits [rows, vocab], a row's consecutive")
-    _dtype_code(logits)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.stride(0) < 0:
+        _refuse("token_logprobs: logits [rows, vocab], a row's consecutive")
+    if logits.dtype not in _KINDS:
+        _dtype_code(logits)
     rows, vocab = logits.shape
     _logprobs_check("token_logprobs", rows, vocab, logits.device, targets, top)
-    _stream(logits)
-    out = _logprobs_result(logits, rows, top, targets is not None)
+    if not logits.is_cuda:
+        _refuse("kernels run on CUDA tensors only; there is no CPU path")
+    out = _logprobs_result(logits.device, rows, top, targets is not None)
     if rows:
         _token_logprobs(logits, targets, out, 0, top, status)
     return out
@@ -1247,10 +1255,10 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
     rows, vocab = x.shape[0], weight.shape[0]
     _logprobs_check("linear_logprobs", rows, vocab, x.device, targets, top)
     _stream(x)
-    out = _logprobs_result(x, rows, top, targets is not None)
+    out = _logprobs_result(x.device, rows, top, targets is not None)
     if rows > SKINNY_MAX_ROWS and type(weight) is not Mx4Weight and _bf16_ok(x, weight):
         lib = library.load()
-        with _on_device(x.device):
+        with _on_device(x.device.index):
             work = torch.empty(lib.rdl_linear_logprobs_work_bytes(rows, vocab, top), dtype=torch.uint8, device=x.device)
             library.check(lib.rdl_linear_logprobs(_ptr(x), _ptr(weight), rows, vocab, x.shape[1], _ptr(targets), top, float(softcap or 0.0), float(scale),
                                                   _ptr(out.logprobs), _ptr(out.entropy), _ptr(out.top_logprobs), _ptr(out.top_ids), _ptr(work),
@@ -1269,10 +1277,28 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
 # copies inside a cache
 # ------------------------------------------------------------------------------------------
 
-def _extent(t: torch.Tensor):
-    """First and last byte of a tensor of at least one element."""
-    first = t.data_ptr()
-    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+def _rows_of(t: torch.Tensor):
+    """Of a tensor [sets, rows, ...]: sets, rows, bytes of a row, bytes from set to set and from row to row, its first byte and the one behind its last."""
+    sets, rows = t.shape[:2]
+    first, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        total = t.numel() * size
+        row = total // (sets * rows) if sets * rows else 0
+        return sets, rows, row, rows * row, row, first, first + total
+    inner = 1
+    for n, s in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+        _need(n <= 1 or s == inner, "copy_rows: a row's own elements must be contiguous")
+        inner *= n
+    s0, s1 = t.stride(0), t.stride(1)
+    if not sets * rows * inner:
+        return sets, rows, 0, 0, 0, first, first
+    # either sets of rows or rows of sets, with or without gaps
+    near, far, n_near, n_far = (s1, s0, rows, sets) if (s1 <= s0 and rows > 1) or sets == 1 else (s0, s1, sets, rows)
+    _need((n_near == 1 or near >= inner) and (n_far == 1 or far >= (near * (n_near - 1) if n_near > 1 else 0) + inner), "copy_rows: rows that overlap")
+    return sets, rows, inner * size, s0 * size, s1 * size, first, first + ((sets - 1) * s0 + (rows - 1) * s1 + inner) * size
+
+
+_copy_tensor = struct.Struct("@Pqqqiiii").pack          # library.CopyRowsTensor, with its padding
 
 
 def copy_rows(moves):
@@ -1282,48 +1308,39 @@ def copy_rows(moves):
     elements are contiguous, sets and rows may lie apart.  src and dst are lists of row numbers on the host, read before the call returns.  No
     row may be the destination of two copies, or source of one and destination of another, and the tensors may not overlap."""
     moves = list(moves)
-    _need(len(moves) <= library.COPY_ROWS_MAX_TENSORS, f"copy_rows: {len(moves)} tensors, {library.COPY_ROWS_MAX_TENSORS} at most")
     if not moves:
         return
+    _need(len(moves) <= library.COPY_ROWS_MAX_TENSORS, "copy_rows: more tensors than one call takes (64)")
     device = moves[0][0].device
-    args = (library.CopyRowsTensor * len(moves))()
-    pairs, used, extents, lists = array.array("i"), 0, [], {}
-    for a, (t, src, dst) in zip(args, moves):
-        _need(t.device == device, "copy_rows: tensors on one device")
-        _need(t.dim() >= 2, "copy_rows: tensors are [sets, rows, ...]")
-        sets, rows = t.shape[0], t.shape[1]
-        inner = 1
-        for n, s in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
-            _need(n <= 1 or s == inner, "copy_rows: a row's own elements must be contiguous")
-            inner *= n
-        s0, s1 = t.stride(0), t.stride(1)
-        if sets * rows > 1 and inner > 0:
-            # either sets of rows or rows of sets, with or without gaps
-            near, far, n_near, n_far = (s1, s0, rows, sets) if (s1 <= s0 and rows > 1) or sets == 1 else (s0, s1, sets, rows)
-            _need((n_near == 1 or near >= inner) and (n_far == 1 or far >= (near * (n_near - 1) if n_near > 1 else 0) + inner), "copy_rows: rows that overlap")
+    args, pairs, used, extents, lists = [], array.array("i"), 0, [], {}
+    for t, src, dst in moves:
+        _need(t.device == device and t.dim() >= 2, "copy_rows: tensors are [sets, rows, ...] on one device")
+        sets, rows, row, set_stride, row_stride, first, end = _rows_of(t)
         key = (id(src), id(dst), rows)
         if key not in lists:                     # keys and values share their lists
             n = len(src)
-            _need(len(dst) == n, f"copy_rows: {n} sources and {len(dst)} destinations")
-            to, touched = set(dst), set(src)
-            _need(len(to) == n and to.isdisjoint(touched), "copy_rows: a row that is the destination of two copies, or source of one and destination of another")
-            _need(n == 0 or (min(min(to), min(touched)) >= 0 and max(max(to), max(touched)) < rows), f"copy_rows: a row outside {rows}")
+            _need(len(dst) == n, "copy_rows: as many sources as destinations")
+            if n:
+                to, touched = set(dst), set(src)
+                _need(len(to) == n and to.isdisjoint(touched), "copy_rows: a row that is the destination of two copies, or source of one and destination of another")
+                _need(min(to) >= 0 and min(touched) >= 0 and max(to) < rows and max(touched) < rows, "copy_rows: a row that the tensor does not have")
+                pairs.extend(src)
+                pairs.extend(dst)
             lists[key] = (used, n)
-            pairs.extend(src)
-            pairs.extend(dst)
             used += n
-        first, n = lists[key]
-        esz = t.element_size()
-        a.base, a.set_stride, a.row_stride, a.row_bytes, a.sets, a.first_pair, a.pairs = t.data_ptr(), s0 * esz, s1 * esz, inner * esz, sets, first, n
-        if sets * rows * inner:
-            extents.append(_extent(t))
-    extents.sort()
-    _need(all(a[1] <= b[0] for a, b in zip(extents, extents[1:])), "copy_rows: tensors that overlap")
-    stream = _stream(moves[0][0])
+        at, n = lists[key]
+        args.append(_copy_tensor(first, set_stride, row_stride, row, sets, at, n, 0))
+        if end > first:
+            extents.append((first, end))
+    if len(extents) > 1:
+        extents.sort()
+        _need(all(a[1] <= b[0] for a, b in zip(extents, extents[1:])), "copy_rows: tensors that overlap")
+    if device.type != "cuda":
+        _refuse("kernels run on CUDA tensors only; there is no CPU path")
     if not used:
         return
-    with _on_device(device):
-        library.check(library.load().rdl_copy_rows(args, len(moves), pairs.buffer_info()[0], stream))
+    with _on_device(device.index):
+        library.check(library.load().rdl_copy_rows(b"".join(args), len(moves), pairs.buffer_info()[0], _raw_stream(device.index)))
 
 
 def upload_batch(dst: torch.Tensor, src_pinned: torch.Tensor, n_ints: int, fed: Optional[Tuple[torch.Tensor, int, int, int]] = None):
