@@ -9,9 +9,9 @@
 
 namespace {
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_MAX_THREADS = 512, LP_MAX_WARPS = LP_MAX_THREADS / 32;
 constexpr int LP_BATCH = 4, LP_RING = 3;                             // 16-byte vectors of a thread in a batch; batches on their way or looked at
-constexpr int LP_RING_BYTES = LP_RING * LP_BATCH * LP_THREADS * 16;
+constexpr int LP_THREAD_BYTES = LP_RING * LP_BATCH * 16;             // of the ring
 constexpr int LP_MAX_CLUSTER = 8;
 
 struct LpArgs {
@@ -42,9 +42,12 @@ __device__ __forceinline__ void lp_copies_end() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void lp_copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A warp's list of largest logits while a row passes by.  Logits not below `least` are put aside in shared memory; when there are 32
-// of them they are sorted and merged into the list, whose last wanted place raises `least`: for itself, and through `shared_least` for
-// the block's other warps, whose lists cannot hold less than that either.
+// What a warp takes of its logits for the list of largest ones.  A row's logits form 32 groups, by the lane that sees them; `seen` holds the largest
+// one of each that the block's warps have put in.  At least `top` logits are not below the top-th of these, so that one below it is none of
+// the row's largest.  A warp puts in what its lanes hold and takes the bound of all after its first batch and after every doubling of
+// them; what is not below it is put aside, and one warp looks among it in the end.  (Bounds that rose only with a warp's own sorted list let
+// one or two logits of every 512 through: 21 instructions a logit instead of 11.)  Where a warp has put 32 aside it merges them into a list
+// of its own.
 // (called, not inlined: its 20 exchanges between lanes stand once in the kernel and not behind every logit of a batch)
 __device__ __noinline__ LpKey lp_take(LpKey keys, LpKey* buffer, int n, int aside, int lane) {
     __syncwarp();
@@ -60,15 +63,15 @@ struct LpList {
     float least;
     int aside;                     // how many are put aside
     LpKey* buffer;                 // 64
-    unsigned* shared_least;        // order-preserving bits
+    unsigned* seen;                // 32, order-preserving bits
     int top, lane;
+    bool listed;                   // `keys` holds some
 
     __device__ __forceinline__ void take(int n) {
         keys = lp_take(keys, buffer, n, aside, lane);
         aside -= n;
-        const LpKey last = __shfl_sync(0xffffffffu, keys, top - 1);
-        if (lane == 0) atomicMax(shared_least, (unsigned)(last >> 32));
-        least = fmaxf(least, lp_key_logit(last));
+        listed = true;
+        least = fmaxf(least, lp_key_logit(__shfl_sync(0xffffffffu, keys, top - 1)));
     }
     // one logit a lane (or none)
     __device__ __forceinline__ void offer(float z, unsigned id, bool valid) {
@@ -79,16 +82,19 @@ struct LpList {
         aside += __popc(mask);
         if (aside >= 32) take(32);
     }
-    // The first logits of a warp: of what its lanes hold at most, a logit below the top-th is none of the row's largest (32 logits here are
-    // not below that).
-    __device__ __forceinline__ void begin(float most) {
-        const LpKey k = lp_sort(lp_key(most, lane), lane);
-        const float bound = lp_key_logit(__shfl_sync(0xffffffffu, k, top - 1));
-        if (lane == 0) atomicMax(shared_least, (unsigned)(lp_key(bound, 0) >> 32));
-        least = fmaxf(least, bound);
-    }
-    __device__ __forceinline__ void look() {                      // what the block's other warps have found
-        least = fmaxf(least, lp_key_logit((LpKey)(*(volatile unsigned*)shared_least) << 32));
+    // most: the largest logit that the lane has seen
+    __device__ __forceinline__ void look(float most) {
+        atomicMax(seen + lane, (unsigned)(lp_key(most, 0) >> 32));
+        __syncwarp();
+        float v = lp_key_logit((LpKey)(*(volatile unsigned*)(seen + lane)) << 32);
+#pragma unroll 1
+        for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll 1
+            for (int o = n >> 1; o > 0; o >>= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, v, o);
+                v = (((lane & o) == 0) == ((lane & n) == 0 || n == 32)) ? fmaxf(v, other) : fminf(v, other);
+            }
+        least = fmaxf(least, __shfl_sync(0xffffffffu, v, top - 1));
     }
 };
 
@@ -112,16 +118,17 @@ __device__ __forceinline__ unsigned lp_remote(const void* p, unsigned rank) {
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a) {
+__global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
     extern __shared__ uint4 ring[];                                  // [LP_RING][LP_BATCH][thread]
-    __shared__ LpStats part[LP_WARPS];
-    __shared__ LpKey lists[TOP ? LP_WARPS : 1][TOP ? 64 : 1];
-    __shared__ unsigned shared_least;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ LpStats part[LP_MAX_WARPS];
+    __shared__ LpKey lists[TOP ? LP_MAX_WARPS : 1][TOP ? 64 : 1];
+    __shared__ unsigned seen[32];
+    __shared__ int counts[LP_MAX_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = threads >> 5;
     const unsigned rank = lp_cluster_rank(), size = lp_cluster_size();
     const long long row = blockIdx.x / size;
-    if (threadIdx.x == 0) shared_least = 0;
+    if (threadIdx.x < 32) seen[threadIdx.x] = 0;
     rdl_grid_wait();
     rdl_grid_launch_dependents();
     __syncthreads();
@@ -134,31 +141,31 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
     const int body_id = head + from * V;
 
     const unsigned own = (unsigned)__cvta_generic_to_shared(ring + threadIdx.x);
-    constexpr int STEP = LP_THREADS * LP_BATCH;
+    const int step = threads * LP_BATCH;
     auto ask = [&](int first, int place) {
 #pragma unroll
         for (int j = 0; j < LP_BATCH; ++j) {
-            const int at = first + j * LP_THREADS + (int)threadIdx.x;
-            if (at < vectors) lp_copy16(own + (unsigned)((place * LP_BATCH + j) * LP_THREADS * 16), body + (long long)at * V);
+            const int at = first + j * threads + (int)threadIdx.x;
+            if (at < vectors) lp_copy16(own + (unsigned)((place * LP_BATCH + j) * threads * 16), body + (long long)at * V);
         }
         lp_copies_end();
     };
 #pragma unroll
-    for (int r = 0; r < LP_RING - 1; ++r) ask(r * STEP, r);
+    for (int r = 0; r < LP_RING - 1; ++r) ask(r * step, r);
 
     LpStats st = lp_empty();
     LpList list;
-    if (TOP) list = {0, -INFINITY, 0, lists[warp], &shared_least, a.top, lane};
-    int place = 0;
-    for (int first = 0; first < vectors; first += STEP) {
-        ask(first + (LP_RING - 1) * STEP, place == 0 ? LP_RING - 1 : place - 1);
+    if (TOP) list = {0, -INFINITY, 0, lists[warp], seen, a.top, lane, false};
+    int place = 0, batches = 0;
+    for (int first = 0; first < vectors; first += step) {
+        ask(first + (LP_RING - 1) * step, place == 0 ? LP_RING - 1 : place - 1);
         lp_copies_wait<LP_RING - 1>();
         float v[LP_BATCH][V];
         float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < LP_BATCH; ++j) {
-            if (first + j * LP_THREADS + (int)threadIdx.x < vectors) {
-                lp_widen(ring[(place * LP_BATCH + j) * LP_THREADS + threadIdx.x], v[j]);
+            if (first + j * threads + (int)threadIdx.x < vectors) {
+                lp_widen(ring[(place * LP_BATCH + j) * threads + threadIdx.x], v[j]);
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[j][i] = -INFINITY;
@@ -171,12 +178,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
 #pragma unroll
         for (int j = 0; j < LP_BATCH; ++j) lp_add(st, v[j]);
         if (TOP) {
-            if (first == 0) list.begin(most);
-            list.look();
+            if ((batches & (batches - 1)) == 0) list.look(st.m > -FLT_MAX ? st.m : -INFINITY);
+            ++batches;
             if (__any_sync(0xffffffffu, !(most < list.least))) {
 #pragma unroll
                 for (int j = 0; j < LP_BATCH; ++j) {
-                    const int at = first + j * LP_THREADS + (int)threadIdx.x;
+                    const int at = first + j * threads + (int)threadIdx.x;
 #pragma unroll
                     for (int i = 0; i < V; ++i) list.offer(v[j][i], body_id + at * V + i, at < vectors);
                 }
@@ -193,23 +200,47 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
         if (TOP) list.offer(v, i, valid);
     }
     if (TOP) {
-        if (list.aside > 0) list.take(list.aside);
-        __syncwarp();
-        lists[warp][lane] = list.keys;
+        if (list.listed) {
+            if (list.aside > 0) list.take(list.aside);
+            __syncwarp();
+            lists[warp][lane] = list.keys;
+            list.aside = 32;
+        }
+        if (lane == 0) counts[warp] = list.aside;
     }
     st = lp_warp_join(st);
     if (lane == 0) part[warp] = st;
     __syncthreads();
-    if (TOP) {
-#pragma unroll 1
-        for (int n = LP_WARPS / 2; n > 0; n >>= 1) {
-            if (warp < n) lists[warp][lane] = lp_merge(lists[warp][lane], lists[warp + n][lane], lane);
-            __syncthreads();
-        }
-    }
     if (warp == 0) {
-        st = lp_warp_join(lane < LP_WARPS ? part[lane] : lp_empty());
+        st = lp_warp_join(lane < warps ? part[lane] : lp_empty());
         if (lane == 0) part[0] = st;
+        if (TOP) {
+            // what the warps have put aside, 32 keys at a time, no matter whose they are
+            int upto = lane < warps ? counts[lane] : 0;
+            const int count = upto;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += v;
+            }
+            const int all_keys = __shfl_sync(0xffffffffu, upto, 31);
+            LpKey keys = 0, least = 0;
+#pragma unroll 1
+            for (int e = 0; e < all_keys; e += 32) {
+                const int mine = e + lane;
+                int owner = 0;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) owner += __shfl_sync(0xffffffffu, upto, owner + d - 1) <= mine ? d : 0;
+                const int before = __shfl_sync(0xffffffffu, upto - count, owner & 31);
+                const LpKey key = mine < all_keys ? lists[owner][mine - before] : 0;
+                if (!__any_sync(0xffffffffu, key > least)) continue;
+                keys = lp_merge(keys, lp_sort(key, lane), lane);
+                least = __shfl_sync(0xffffffffu, keys, a.top - 1);
+            }
+            __syncwarp();
+            lists[0][lane] = keys;
+            __syncwarp();
+        }
     }
     if (size > 1) {                                                  // the cluster's blocks, a warp of the first for each
         lp_cluster_sync();
@@ -251,9 +282,9 @@ __global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(LpArgs a)
 }
 
 template <typename T, bool TOP>
-int lp_run(const LpArgs& a, int cluster, cudaStream_t st) {
-    RDL_CUDA((rdl_allow_shared<token_logprobs_kernel<T, TOP>>(LP_RING_BYTES)), "token_logprobs");
-    RDL_CHECK_EX(rdl_launch_cluster(token_logprobs_kernel<T, TOP>, dim3((unsigned)a.rows * cluster), dim3(LP_THREADS), cluster, (size_t)LP_RING_BYTES, st, a),
+int lp_run(const LpArgs& a, int cluster, int threads, cudaStream_t st) {
+    RDL_CUDA((rdl_allow_shared<token_logprobs_kernel<T, TOP>>(LP_MAX_THREADS * LP_THREAD_BYTES)), "token_logprobs");
+    RDL_CHECK_EX(rdl_launch_cluster(token_logprobs_kernel<T, TOP>, dim3((unsigned)a.rows * cluster), dim3(threads), cluster, (size_t)threads * LP_THREAD_BYTES, st, a),
                  "token_logprobs");
     return 0;
 }
@@ -269,10 +300,14 @@ extern "C" int rdl_token_logprobs(const void* logits, int dtype, long long row_s
     RDL_REQUIRE(logits && entropy && (!targets || logprobs) && (top == 0 || (top_logprobs && top_ids)), "token_logprobs: missing operand");
     RDL_REQUIRE((uintptr_t)logits % rdl_dtype_size(dtype) == 0, "token_logprobs: logits that are not on an element's boundary");
     const LpArgs a{logits, row_stride, rows, vocab, top, targets, logprobs, entropy, top_logprobs, top_ids, status};
-    // blocks that share a row: as many as there is room for at once (two on a multiprocessor), each with a batch of its threads or more
-    int cluster = 1;
-    while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= 2 * rdl_sm_count() && (long long)vocab * (int)rdl_dtype_size(dtype) >= cluster * 2LL * LP_THREADS * 16) cluster *= 2;
+    // Few rows: as many blocks share a row as there is room for at once (two on a multiprocessor), each thread with a batch where the row has
+    // one.  Many: a thread has four batches, since what a warp does once for a row takes as long as one or two of them.
+    const long long vectors = (long long)vocab * (long long)rdl_dtype_size(dtype) / 16;
+    const bool few = rows <= 2 * rdl_sm_count();
+    int threads = 32, cluster = 1;
+    while (threads < LP_MAX_THREADS && vectors >= threads * 2LL * LP_BATCH * (few ? 1 : 4)) threads *= 2;
+    while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= 2 * rdl_sm_count() && vectors >= cluster * 2LL * LP_MAX_THREADS) cluster *= 2;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == RDL_BF16) return top ? lp_run<__nv_bfloat16, true>(a, cluster, st) : lp_run<__nv_bfloat16, false>(a, cluster, st);
-    return top ? lp_run<float, true>(a, cluster, st) : lp_run<float, false>(a, cluster, st);
+    if (dtype == RDL_BF16) return top ? lp_run<__nv_bfloat16, true>(a, cluster, threads, st) : lp_run<__nv_bfloat16, false>(a, cluster, threads, st);
+    return top ? lp_run<float, true>(a, cluster, threads, st) : lp_run<float, false>(a, cluster, threads, st);
 }
