@@ -49,18 +49,49 @@ __device__ __forceinline__ void lp_join(LpStats& a, LpStats b) {
     a.t += b.t;
 }
 
-// N logits more; m is not below any of them
+// two floats in a register pair, and arithmetic on both at once
+__device__ __forceinline__ unsigned long long lp_pair(float a, float b) {
+    unsigned long long p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void lp_unpair(unsigned long long p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ unsigned long long lp_add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long lp_mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long lp_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// N logits more, an even number of them; m is not below any
 template <int N>
 __device__ __forceinline__ void lp_add(LpStats& a, const float (&z)[N]) {
-    float s = 0.f, t = 0.f;
+    const unsigned long long less = lp_pair(-a.m, -a.m), log2e = lp_pair(LP_LOG2E, LP_LOG2E);
+    unsigned long long s = 0, t = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = z[i] - a.m, e = lp_exp2(d * LP_LOG2E);
-        s += e;
-        t = fmaf(e, fmaxf(d, -1e30f), t);
+    for (int i = 0; i < N; i += 2) {
+        const unsigned long long d = lp_add2(lp_pair(z[i], z[i + 1]), less);
+        float d0, d1, x0, x1;
+        lp_unpair(d, d0, d1);
+        lp_unpair(lp_mul2(d, log2e), x0, x1);
+        const unsigned long long e = lp_pair(lp_exp2(x0), lp_exp2(x1));
+        s = lp_add2(s, e);
+        t = lp_fma2(e, lp_pair(fmaxf(d0, -1e30f), fmaxf(d1, -1e30f)), t);
     }
-    a.s += s;
-    a.t += t;
+    float s0, s1, t0, t1;
+    lp_unpair(s, s0, s1);
+    lp_unpair(t, t0, t1);
+    a.s += s0 + s1;
+    a.t += t0 + t1;
 }
 
 __device__ __forceinline__ LpStats lp_warp_join(LpStats a) {
