@@ -2,9 +2,9 @@
 // [vocab, k], without logits in memory: the product runs on the fifth-generation tensor cores, and what takes a tile of it out
 // of tensor memory keeps each row's statistics and list (logprobs.cuh) instead of storing it.
 //
-// A tile is 128 CTAS rows x 256 tokens.  CTAS 2 (more than 128 rows): a pair of blocks on two multiprocessors (cta_group::2); each holds 128 of
+// A tile is 128 CTAS rows x 256 tokens.  CTAS 2 (many rows): a pair of blocks on two multiprocessors (cta_group::2); each holds 128 of
 // the rows and 128 of the tile's weight rows, and the products, issued by a thread of block 0, read both halves.  CTAS 1: up to 128
-// rows, where reading the weights is what takes the time.  Two accumulators: the products of a tile run while the tile before it is
+// rows, where reading the weights is what takes the time, and where pairs would leave too much of their tiles empty.  Two accumulators: the products of a tile run while the tile before it is
 // taken out.
 //
 // Persistent: a group (a pair, or a block) walks along the vocabulary for one block of rows, so that a row's statistics stay in one
@@ -614,7 +614,9 @@ void plan(HeadArgs& a, int rows, int vocab, int ctas) {
     a.main_tiles = mains == a.groups ? a.tiles_n : (int)((long long)a.tiles_n * mains / a.groups);
 }
 int rows_at_once(int ctas) { return (rdl_sm_count() / ctas > 0 ? rdl_sm_count() / ctas : 1) * BM * ctas; }
-int ctas_for(int rows) { return rows <= BM ? 1 : 2; }
+// Pairs from 129 rows on, but for three blocks of 128: as two of 256 a quarter of the products are for nobody (384 rows, 20 alternatives: 490 us
+// by pairs, 430 without; 300 rows 480 and 420).  Blocks without a partner fetch half as much again (2,048 rows: 1.8 ms by pairs, 2.0 without).
+int ctas_for(int rows) { return rows <= BM || (rows > 2 * BM && rows <= 3 * BM) ? 1 : 2; }
 // the rows of a launch: all, or equal parts where there are more row blocks than groups
 int rows_a_launch(int rows, int ctas) {
     const long long most = rows_at_once(ctas), launches = (rows + most - 1) / most, blocks = ((long long)rows + BM * ctas - 1) / (BM * ctas);

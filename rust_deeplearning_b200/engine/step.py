@@ -71,6 +71,16 @@ class Engine:
         if self.device.type == "cuda":
             self.status = self.status.pin_memory()
 
+    def __del__(self):
+        # The kernels that upload a step's description read the pinned buffers, of which the allocator of pinned memory knows nothing: an
+        # engine that is dropped with steps in flight waits until they have been read, or the next engine's description would lie there.
+        for event in getattr(self, "_pinned_event", ()):
+            if event is not None:
+                try:
+                    event.synchronize()
+                except Exception:      # the context is gone, or has failed: nothing reads them any more
+                    pass
+
     # ---- sequences ----
     def new_sequence(self) -> int:
         return self.cache.alloc_slot()

@@ -57,6 +57,7 @@ def test_forked_sequences_equal_separate_ones(module, name, dtype):
             eng.step([fourth], [tails[0][5:25]], "last")
         for t in range(25, 40):                                          # the fourth one's logits are compared where its past came in the same steps
             out.append(eng.step(slots, [[x[t]] for x in tails], "last")[:3].clone())
+        torch.cuda.synchronize()
         eng.check_status()
         for s in slots:
             eng.release(s)
@@ -64,6 +65,30 @@ def test_forked_sequences_equal_separate_ones(module, name, dtype):
         got.append(out)
     for i, (x, y) in enumerate(zip(*got)):
         assert torch.isfinite(x).all() and torch.equal(x, y), f"step {i}"
+
+
+def test_an_engine_dropped_with_steps_in_flight():
+    """The next engine's pinned buffers are the last one's: its first description must not reach a kernel of the last one's steps."""
+    cfg, seed = tiny_configs.config("A")
+    model = random_model(cfg, seed, "float32")
+    ids = ids_of(60, 40, model.vocab_size)
+
+    def steps(n):
+        eng = Engine(model, max_tokens=512, max_seqs=2, max_context=128)
+        a, b = eng.new_sequence(), eng.new_sequence()
+        eng.step([a, b], [ids[:9], ids[9:13]], "last")
+        out = [eng.step([a, b], [[ids[t]], [ids[-t]]], "last").clone() for t in range(1, n)]
+        return out                                           # the engine is gone, its steps may not be
+
+    want = steps(30)
+    torch.cuda.synchronize()
+    want = [w.clone() for w in want]
+    for _ in range(5):
+        torch.cuda._sleep(20_000_000)                        # ten milliseconds: the host is ahead by all of the steps
+        runs = [steps(30), steps(7)]
+        torch.cuda.synchronize()
+        for got in runs:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
 def log_p(z):

@@ -325,6 +325,23 @@ def test_batches_of_requests_with_several_continuations():
         plan_batches([5], 8, samples=7, **kw)
 
 
+def test_a_dropped_engine_waits_for_its_uploads(tmp_path, monkeypatch):
+    engine, cfg, w = build(tmp_path, "A", monkeypatch)
+    waited = []
+
+    class Event:
+        def __init__(self, fails=False):
+            self.fails = fails
+
+        def synchronize(self):
+            waited.append(self)
+            if self.fails:
+                raise RuntimeError("the context is gone")
+    engine._pinned_event = [Event(True), Event()]
+    del engine
+    assert len(waited) == 2
+
+
 # ---- refusals that need no device ----
 
 def test_refused_copies():
