@@ -84,6 +84,7 @@ class PagePool:
         self.n_pages = n_pages
         self._free = list(range(n_pages - 1, -1, -1))
         self._held = [0] * n_pages
+        self.n_shared = 0            # pages with more than one holder
 
     @property
     def n_free(self):
@@ -105,6 +106,8 @@ class PagePool:
         for p in pages:
             if not (0 <= p < self.n_pages) or not self._held[p]:
                 raise CacheError(f"page {p} is shared but not held")
+        for p in pages if times else ():
+            self.n_shared += self._held[p] == 1
             self._held[p] += times
 
     def give_back(self, pages: Sequence[int]):
@@ -113,6 +116,7 @@ class PagePool:
             if not (0 <= p < self.n_pages) or not self._held[p]:
                 raise CacheError(f"page {p} is given back but not held")
             self._held[p] -= 1
+            self.n_shared -= self._held[p] == 1
             if not self._held[p]:
                 self._free.append(p)
 
@@ -177,9 +181,11 @@ class KVGroup:
 
         A step's queries read earlier positions before its own are written, so a page of a window group counts as long as the first of
         them sees its last position."""
+        out = []
+        if not self.pool.n_shared:
+            return out
         window, size, ring = self.requirement.window, self.page_size, self.ring_pages
         holders: Dict[int, int] = {}
-        out = []
         for s, first, total in zip(slots, past, totals):
             held = self.pages.get(s, ())
             lo, hi = first // size, (total - 1) // size

@@ -1,11 +1,11 @@
 // Log probabilities, entropy and alternatives by the logits  z = scale * cap tanh(x W^T / cap)  of bfloat16 rows x behind an output head W
 // [vocab, k], without logits in memory: the product runs on the fifth-generation tensor cores, and what takes a tile of it out
-// of tensor memory keeps each row's statistics and list (logprobs.cuh) instead of storing it.
+// of tensor memory keeps each row's statistics (logprobs.cuh) instead of storing it.
 //
 // A tile is 128 CTAS rows x 256 tokens.  CTAS 2 (many rows): a pair of blocks on two multiprocessors (cta_group::2); each holds 128 of
 // the rows and 128 of the tile's weight rows, and the products, issued by a thread of block 0, read both halves.  CTAS 1: up to 128
-// rows, where reading the weights is what takes the time, and where pairs would leave too much of their tiles empty.  Two accumulators: the products of a tile run while the tile before it is
-// taken out.
+// rows, where reading the weights is what takes the time, and where pairs would leave too much of their tiles empty.  Two accumulators:
+// the products of a tile run while the tile before it is taken out.
 //
 // Persistent: a group (a pair, or a block) walks along the vocabulary for one block of rows, so that a row's statistics stay in one
 // thread's registers.  Groups of all row blocks walk side by side over the same part of it (a slice), and their weight tiles come from
@@ -13,8 +13,13 @@
 // turn, so that every group has as many tiles.  Each (row block, range) leaves partial results, which a second kernel joins.
 //
 // Warp 0 loads (TMA, a ring of stages of 64 k), warp 1 issues the products, eight warps take the accumulator out: two a quarter of
-// tensor memory, half of the columns each, a row a thread.  A row's logits beyond its list's last place are put aside in shared memory, and put
-// into the list when some lane has five of them: all lanes of a warp then do so together, which a logit by itself would not.
+// tensor memory, half of the columns each, a row a thread.  Logits that may be among a row's largest are put aside in memory (`seen` below
+// says which), and the second kernel looks among them.
+//
+// Measured, 256,000 tokens, k 2,304, soft-cap: 8,192 rows and five alternatives 6.5 ms, 1.48 PFLOP/s; 2,048 rows, none, 1.56 ms, 1.54 PFLOP/s: a
+// tile's products take 18,432 cycles and a tile 18,450 to 19,500, at the clock that the power limit leaves (1.25 to 1.4 GHz).  What
+// is done with a tile takes 5,000 cycles (9,000 with a soft-cap, up to 15,000 with alternatives) beside them.  64 rows: 190 us, 208 with
+// alternatives (a kernel more, a longer second kernel), 6.2 and 5.7 TB/s of weights.
 //
 // Every wait is bounded; a block that gives up sets `status` and every path ends in the common tear-down.  A block takes all of a
 // multiprocessor's shared memory (see "Tensor memory" in mx_tensor.cuh: nothing that holds tensor memory fits beside it).
@@ -138,9 +143,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// ---- the list of a row, kept by one thread ----
-//
-// All lanes of a warp work on their own rows at once and without exchanges.
+// ---- a row's largest logits, as one thread sees them ----
 
 __device__ __forceinline__ void exchange(LpKey& a, LpKey& b) {      // the larger one first
     const LpKey x = a, y = b;
@@ -200,22 +203,12 @@ __device__ __forceinline__ void put_aside(float2*& at, float v, float least, int
                  : "+l"(at) : "f"(v), "f"(least), "r"(token) : "memory");
 }
 
-// What a logit must exceed.  A row's columns form 32 groups (by column mod 32), and `seen` holds the largest logit that any block has seen of each
-// so far.  At least `top` logits are not below the top-th of these 32, so that a logit below it is none of the row's `top` largest,
-// whatever else comes.  When another block's numbers arrive does not change a result, only what is put aside.
-//
-// A thread keeps the maxima of what it has seen in registers, puts them in and takes the bound of all after its first tile (which it goes
-// through a second time for what exceeds that) and after every doubling of its tiles.  Of N logits in no order about 1.5 top / N of the next
-// exceed the bound.  Measured instead, 2,048 rows and 20 alternatives: a sorted list a thread in shared memory (a call that merges 16 logits
-// waits 10,000 cycles for its instructions) 1.8 ms, its logits alone in registers (2,000 instructions a piece of 32 columns) 4.1 ms.
-//
 __device__ __forceinline__ unsigned ordered(float z) {
     const unsigned u = __float_as_uint(z);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float from_ordered(unsigned o) { return o == 0 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-// What a row's logit must exceed, NaN where nothing is known; the number under the top-th value keeps logits that equal it.
 // `least` rises to `now` where that is known and higher
 __device__ __forceinline__ void begin_with(float& least, float now) {
     if (!(now < least) && now == now) least = now;
@@ -244,6 +237,16 @@ __device__ __forceinline__ float bound_among(float (&v)[N], int top) {
     if (b == 0.f) return -__uint_as_float(1);
     return __uint_as_float(b > 0.f ? __float_as_uint(b) - 1 : __float_as_uint(b) + 1);
 }
+// What a logit must exceed.  A row's columns form 32 groups (by column mod 32), and `seen` holds the largest logit that any block has seen of each
+// so far.  At least `top` logits are not below the top-th of these 32, so that a logit below it is none of the row's `top` largest,
+// whatever else comes.  When another block's numbers arrive does not change a result, only what is put aside.
+//
+// A thread keeps the maxima of what it has seen in registers, puts them in and takes the bound of all after its first tile (which it goes
+// through a second time for what exceeds that) and after every doubling of its tiles.  Of N logits in no order about 1.5 top / N of the next
+// exceed the bound.  Measured instead, 2,048 rows and 20 alternatives: a sorted list a thread in shared memory (a call that merges 16 logits
+// waits 10,000 cycles for its instructions) 1.8 ms, its logits alone in registers (2,000 instructions a piece of 32 columns) 4.1 ms.
+//
+// NaN where nothing is known; the number under the top-th value keeps logits that equal it.
 __device__ __noinline__ float bound_of(const unsigned* seen, int rows, int top) {
     float v[32];
 #pragma unroll
@@ -256,8 +259,8 @@ __device__ __noinline__ float bound_of(const unsigned* seen, int rows, int top) 
 }
 
 // Logits from their sums of products.  cap tanh(y) = cap - 2 cap / (e^(2 y) + 1), from the hardware's power and reciprocal (2^-22 and 2^-23 of
-// themselves): off by at most 2^-22 of the cap wherever it lies, which is less than float32 sums of a few hundred products are off by; tanhf
-// would take five times the instructions, and the tile's statistics longer than its products.
+// themselves): off by at most 2^-21 of the cap wherever it lies, which is what float32 sums of a few hundred products are off by.  tanhf
+// takes five times the instructions: 10,000 instead of 6,000 cycles a tile, 512 rows with 20 alternatives 796 instead of 658 us.
 __device__ __forceinline__ void logits_of(const HeadArgs& a, float (&v)[32]) {
     if (a.cap > 0.f) {
         const float f = a.inv_cap * (2.f * LP_LOG2E), c2 = -2.f * a.cap;
@@ -459,9 +462,11 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
                         for (int g = 0; g < 32; g += AT_ONCE) {
                             if (!__any_sync(0xffffffffu, !(of[g / AT_ONCE] <= least))) continue;
                             if (__any_sync(0xffffffffu, at > aside + (a.places - AT_ONCE))) {
-                                if (mine) put_away(a.keys + place * a.top * ROWS + own_row, ROWS, aside, (int)(at - aside), a.top, !listed);
+                                if (mine && at > aside) {                  // a lane that has put nothing aside has no list either
+                                    put_away(a.keys + place * a.top * ROWS + own_row, ROWS, aside, (int)(at - aside), a.top, !listed);
+                                    listed = true;
+                                }
                                 at = aside;
-                                listed = true;
                             }
                             if (there >= 32) {
 #pragma unroll
@@ -545,6 +550,7 @@ __global__ void __launch_bounds__(WARPS * 32) head_join_kernel(const __grid_cons
         if (a.top == 0) continue;
         const bool listed = count < 0;
         if (listed) count = ~count;
+        count = min(count, a.places);                      // of a block that gave up there is anything here
         int upto = count;                                  // logits put aside by this lane's and the lanes before
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {

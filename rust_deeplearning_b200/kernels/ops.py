@@ -1243,7 +1243,11 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = None, top: int = 0, softcap: Optional[float] = None,
                     scale: float = 1.0, status: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """`token_logprobs` of the logits scale * softcap(x W^T) of rows x [rows, in] behind an output head [vocab, in] (a tensor of x's type, or
-    `Mx4Weight`), without keeping the logits."""
+    `Mx4Weight`), without keeping the logits.
+
+    More than 16 bfloat16 rows that meet `linear`'s alignment rules run in one kernel that forms the statistics as it takes the products out of
+    tensor memory (its work space: a few MB, up to 250 MB for 32 alternatives); others form pieces of the logits by `linear`, 256 MB
+    at a time.  softcap: cap * tanh(. / cap) of the products, before scale.  The weight is a constant, as `linear` has it."""
     _need(x.dim() == 2 and len(weight.shape) == 2 and x.shape[1] == weight.shape[1] and x.shape[1] > 0,
           f"linear_logprobs: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not fit")
     _need(type(weight) is Mx4Weight or x.dtype is weight.dtype, "linear_logprobs: rows and weight of one type")
@@ -1265,11 +1269,12 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
                                                   work.numel(), _status(status), _stream(x)))
         return out
     piece = max(1, LOGPROBS_PIECE // vocab)
-    for r in range(0, rows, piece):
-        z = linear(x[r:r + piece], weight, torch.float32, softcap, status)
-        if scale != 1.0:
-            scale_(z, scale)
-        _token_logprobs(z, targets, out, r, top, status)
+    with _on_device(x.device.index):
+        for r in range(0, rows, piece):
+            z = linear(x[r:r + piece], weight, torch.float32, softcap, status)
+            if scale != 1.0:
+                scale_(z, scale)
+            _token_logprobs(z, targets, out, r, top, status)
     return out
 
 

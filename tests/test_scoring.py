@@ -27,9 +27,12 @@ def test_a_page_is_free_when_its_last_holder_gives_it_back():
     p = PagePool(3)
     a, b = p.take(2)
     p.share([a], 2)
-    assert p.holders(a) == 3 and p.holders(b) == 1
-    p.give_back([a, b]); p.give_back([a])
-    assert p.n_free == 2 and p.holders(a) == 1
+    assert p.holders(a) == 3 and p.holders(b) == 1 and p.n_shared == 1
+    p.share([b], 0); p.share([])
+    p.give_back([a, b])
+    assert p.n_shared == 1
+    p.give_back([a])
+    assert p.n_free == 2 and p.holders(a) == 1 and p.n_shared == 0
     p.give_back([a])
     assert p.n_free == 3
     with pytest.raises(CacheError):
@@ -38,6 +41,10 @@ def test_a_page_is_free_when_its_last_holder_gives_it_back():
         p.share([b])
     with pytest.raises(CacheError):
         p.share([7])
+    c, = p.take(1)
+    with pytest.raises(CacheError):
+        p.share([c, 7])
+    assert p.holders(c) == 1 and p.n_shared == 0
 
 
 class Model:
@@ -132,9 +139,11 @@ def test_forked_slots_read_what_they_would_read_alone(monkeypatch, seed):
         for s in cache.live_slots():
             sees(s, len(text[s]), len(text[s]))
     assert copies[0] > 5
+    for g in cache.kv_groups:
+        assert g.pool.n_shared == sum(g.pool.holders(p) > 1 for p in range(g.pool.n_pages))
     for s in cache.live_slots():
         cache.free_slot(s)
-    assert all(g.pool.n_free == g.pool.n_pages for g in cache.kv_groups)
+    assert all(g.pool.n_free == g.pool.n_pages and g.pool.n_shared == 0 for g in cache.kv_groups)
 
 
 def test_only_what_a_slot_still_sees_is_copied(monkeypatch):

@@ -228,6 +228,109 @@ def test_infinities_and_nan_behind_a_head(rows):
     assert torch.isnan(r.logprobs[1:3]).all() and torch.isnan(r.entropy[1:3]).all()
 
 
+@pytest.mark.parametrize("rows,vocab", [(20, 20001), (300, 20001), (17, 300), (140, 5000)])
+@pytest.mark.parametrize("top", [1, 5, 20, 32])
+@pytest.mark.parametrize("falling", [False, True])
+def test_logits_that_rise_or_fall_along_the_vocabulary(rows, vocab, top, falling):
+    """Rising logits all exceed what came before: more than a thread can put aside.  id = 256 a + b with exact numbers a, b; some equal ones."""
+    ids = torch.arange(vocab - 1, -1, -1) if falling else torch.arange(vocab)
+    ids = ids // 3 * 3
+    w = torch.zeros((vocab, 64))
+    w[:, 0], w[:, 1] = (ids // 256).float(), (ids % 256).float() / 256
+    x = torch.zeros((rows, 64))
+    x[:, :2] = 0.25
+    x[1, :2] = 2.0                                       # steep
+    x[2, :2] = -0.25
+    x, w = x.to(torch.bfloat16).to(DEV), w.to(torch.bfloat16).to(DEV)
+    t = targets_of(rows, vocab, 11)
+    ref.check(ops.linear_logprobs(x, w, t, top), f64(x) @ f64(w).T, t.cpu().numpy(), top, "rising logits")
+
+
+def test_rows_without_a_distribution_name_the_lowest_ids():
+    x, w = head_case(40, 64, 5000, torch.bfloat16, 14)
+    x[3] = float("nan")                                  # every logit
+    w[:, 0] = 0
+    w[7:5000:9, 0] = float("nan")                        # some logits of every row
+    x[:, 0] = 1.0
+    r = ops.linear_logprobs(x, w, None, 32)
+    assert torch.isnan(r.entropy).all() and r.top_ids[3].tolist() == list(range(32))
+    z = f64(x) @ f64(w).T
+    for i in (0, 39):
+        assert not np.isnan(z[i, r.top_ids[i].cpu().numpy()]).any()
+    w[:, 1:] = 0
+    w[:, 0] = -float("inf")
+    r = ops.linear_logprobs(x[:2].repeat(20, 1), w, None, 5)
+    assert torch.isnan(r.entropy).all() and (r.top_ids == torch.arange(5, device=DEV)).all()
+    w[4000:, 0] = 1.0                                    # behind many tokens of no probability
+    r = ops.linear_logprobs(x[:2].repeat(20, 1), w, None, 5)
+    assert (r.top_ids == torch.arange(4000, 4005, device=DEV)).all() and torch.allclose(r.entropy, torch.tensor(float(np.log(1000)), device=DEV))
+
+
+@pytest.mark.parametrize("rows,vocab", [(19000, 300), (20000, 70)])
+def test_more_rows_than_one_launch_has_blocks_for(rows, vocab):
+    g = torch.Generator().manual_seed(15)
+    x = torch.randint(-3, 4, (rows, 64), generator=g).to(torch.bfloat16).to(DEV)
+    w = (torch.randint(-2, 3, (vocab, 64), generator=g) / 16).to(torch.bfloat16).to(DEV)
+    t = targets_of(rows, vocab, 12)
+    r = ops.linear_logprobs(x, w, t, 3)
+    some = list(range(0, rows, 997)) + [rows - 1]
+    part = ops.TokenLogprobs(*(v[some] for v in r))
+    ref.check(part, f64(x[some]) @ f64(w).T, t.cpu().numpy()[some], 3, "many rows")
+    want = ops.token_logprobs(ops.linear(x, w, torch.float32), t, 3)
+    assert torch.equal(r.top_ids, want.top_ids) and torch.allclose(r.logprobs, want.logprobs, atol=1e-5) and torch.allclose(r.entropy, want.entropy, atol=1e-5)
+
+
+@pytest.mark.parametrize("rows", [40, 300, 200])
+def test_a_token_outside_the_vocabulary_behind_a_head(rows):
+    x, w = head_case(rows, 64, 300, torch.bfloat16, 16)
+    t = torch.full((rows,), 5, dtype=torch.int32, device=DEV)
+    t[1], t[2], t[3], t[rows - 1] = 300, -1, 2 ** 31 - 1, 299
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    r = ops.linear_logprobs(x, w, t, 2, status=status)
+    assert status.item() == 11 and torch.isnan(r.logprobs).nonzero().flatten().tolist() == [1, 3] and r.logprobs[2].item() == 0.0
+    want = ops.token_logprobs(ops.linear(x, w, torch.float32), t, 2)
+    assert torch.allclose(r.logprobs, want.logprobs, atol=1e-4, equal_nan=True)
+
+
+SHORT_WAIT = 200_000       # clock cycles, about a tenth of a millisecond
+
+
+@pytest.mark.parametrize("rows", [40, 200, 300])
+@pytest.mark.parametrize("top", [0, 5])
+def test_a_wait_that_runs_out(rows, top):
+    lib = library.load()
+    x, w = head_case(rows, 256, 3000, torch.bfloat16, 17)
+    t = targets_of(rows, 3000, 13)
+    want = ops.linear_logprobs(x, w, t, top)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    try:
+        lib.rdl_set_wait_test(12, SHORT_WAIT, 64)
+        ops.linear_logprobs(x, w, t, top, status=status)
+        torch.cuda.synchronize()                         # the kernels returned by themselves
+    finally:
+        lib.rdl_set_wait_test(0, 0, 0)
+    assert "linear_logprobs" in library.FAULTS[status.item()]
+    status.zero_()
+    got = ops.linear_logprobs(x, w, t, top, status=status)
+    assert status.item() == 0 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_long_kernel_ahead_is_no_wait_in_vain():
+    lib, status = library.load(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    x, w = head_case(200, 256, 3000, torch.bfloat16, 18)
+    want = ops.linear_logprobs(x, w, None, 3)
+    a = torch.ones((4096, 4096), device=DEV)
+    try:
+        lib.rdl_set_wait_test(12, SHORT_WAIT, 0)
+        for _ in range(3):
+            ops.linear(a, a)                             # 2 ms
+            got = ops.linear_logprobs(x, w, None, 3, status=status)
+        torch.cuda.synchronize()
+    finally:
+        lib.rdl_set_wait_test(0, 0, 0)
+    assert status.item() == 0 and all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+
+
 @pytest.mark.parametrize("rows", [1, 16, 17, 130])
 @pytest.mark.parametrize("kind", ["bfloat16", "float32"])
 def test_a_4_bit_head(rows, kind):
