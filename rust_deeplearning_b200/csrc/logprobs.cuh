@@ -26,10 +26,11 @@ struct LpStats { float m, s, t; };
 
 __device__ __forceinline__ LpStats lp_empty() { return {-FLT_MAX, 0.f, 0.f}; }
 
-// 2^x: two units in the last place (the hardware's), 0 for minus infinity
+// 2^x: two units in the last place (the hardware's), 0 below 2^-126 (numbers that are not normal would take four instructions instead of one,
+// and none of them counts beside the 1 of a row's largest logit)
 __device__ __forceinline__ float lp_exp2(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 

@@ -267,7 +267,7 @@ __device__ __forceinline__ void logits_of(const HeadArgs& a, float (&v)[32]) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             float r;
-            asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(lp_exp2(v[i] * f) + 1.f));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(lp_exp2(v[i] * f) + 1.f));
             v[i] = fmaf(c2, r, a.cap);
         }
     }
