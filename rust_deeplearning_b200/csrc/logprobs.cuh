@@ -73,6 +73,13 @@ __device__ __forceinline__ unsigned long long lp_fma2(unsigned long long a, unsi
     return r;
 }
 
+// the largest of three (a NaN is passed over, as by fmaxf)
+__device__ __forceinline__ float lp_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // N logits more, an even number of them; m is not below any
 template <int N>
 __device__ __forceinline__ void lp_add(LpStats& a, const float (&z)[N]) {

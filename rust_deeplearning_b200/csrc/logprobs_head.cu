@@ -434,9 +434,9 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
                     float of[32 / AT_ONCE], most = -INFINITY;             // the largest of every few
 #pragma unroll
                     for (int g = 0; g < 32 / AT_ONCE; ++g) {
-                        of[g] = v[g * AT_ONCE];
+                        of[g] = fmaxf(v[g * AT_ONCE], v[g * AT_ONCE + 1]);
 #pragma unroll
-                        for (int i = 1; i < AT_ONCE; ++i) of[g] = fmaxf(of[g], v[g * AT_ONCE + i]);
+                        for (int i = 2; i < AT_ONCE; i += 2) of[g] = lp_max3(of[g], v[g * AT_ONCE + i], v[g * AT_ONCE + i + 1]);
                         most = fmaxf(most, of[g]);
                     }
                     if (!two || i < 0) {
