@@ -237,7 +237,7 @@ __device__ __forceinline__ float bound_among(float (&v)[N], int top) {
     if (b == 0.f) return -__uint_as_float(1);
     return __uint_as_float(b > 0.f ? __float_as_uint(b) - 1 : __float_as_uint(b) + 1);
 }
-// What a logit must exceed.  A row's columns form 32 groups (by column mod 32), and `seen` holds the largest logit that any block has seen of each
+// What a logit must exceed.  A row's columns form 32 groups (by column mod 16, and by the half of the tile they lie in), and `seen` holds the largest logit that any block has seen of each
 // so far.  At least `top` logits are not below the top-th of these 32, so that a logit below it is none of the row's `top` largest,
 // whatever else comes.  When another block's numbers arrive does not change a result, only what is put aside.
 //
@@ -386,13 +386,13 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
             float2* const aside = a.aside + (TOP ? (place * ROWS + own_row) * a.places : 0);
             float2* at = aside;                           // where the next logit is put aside
             bool listed = false;                          // whether some have been put into a list
-            float groups[TOP ? 32 : 1];                   // the largest of every group
+            float groups[TOP ? 16 : 1];                   // the largest of every group of this column half
             if (TOP)
 #pragma unroll
-                for (int j = 0; j < 32; ++j) groups[j] = -INFINITY;
+                for (int j = 0; j < 16; ++j) groups[j] = -INFINITY;
             auto put_in = [&] {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) atomicMax(a.seen + (long long)j * a.M + row, ordered(groups[j]));
+                for (int j = 0; j < 16; ++j) atomicMax(a.seen + (long long)(half * 16 + j) * a.M + row, ordered(groups[j]));
             };
             for (int t = t0; t < t1; ++t, ++lt) {
                 const int buf = lt & 1;
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
                         st.t = nt;
                         if (TOP)
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) groups[j] = fmaxf(groups[j], v[j]);
+                            for (int j = 0; j < 16; ++j) groups[j] = lp_max3(groups[j], v[j], v[j + 16]);
                     }
                     if (TOP && i >= 0 && __any_sync(0xffffffffu, !(most <= least))) {
 #pragma unroll
