@@ -1189,10 +1189,11 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
-def _logprobs_result(device, rows: int, top: int, with_targets: bool) -> TokenLogprobs:
-    f32 = torch.float32
-    return TokenLogprobs(torch.empty(rows, dtype=f32, device=device) if with_targets else None, torch.empty(rows, dtype=f32, device=device),
-                         torch.empty((rows, top), dtype=torch.int32, device=device), torch.empty((rows, top), dtype=f32, device=device))
+def _logprobs_result(device, rows: int, top: int, targets: Optional[torch.Tensor]) -> TokenLogprobs:
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    # new_empty takes the host half as long as torch.empty with a shape, a type and a device
+    ids = targets.new_empty(rows, top) if targets is not None else torch.empty((rows, top), dtype=torch.int32, device=device)
+    return TokenLogprobs(entropy.new_empty(rows) if targets is not None else None, entropy, ids, entropy.new_empty(rows, top))
 
 
 def _logprobs_check(who: str, rows: int, vocab: int, device, targets: Optional[torch.Tensor], top: int):
@@ -1226,15 +1227,16 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     A negative target asks for none and gets 0; one outside the vocabulary gets NaN and is reported to `status`.  Logits of minus infinity
     are tokens of probability 0.  A row with a NaN or plus infinity, or of minus infinities alone, has no distribution: NaN (its
     alternatives are still those of its largest logits, a NaN counting as the smallest)."""
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.stride(0) < 0:
+    shape, device = logits.shape, logits.device
+    if len(shape) != 2 or not (logits.is_contiguous() or ((shape[1] <= 1 or logits.stride(1) == 1) and logits.stride(0) >= 0)):
         _refuse("token_logprobs: logits [rows, vocab], a row's consecutive")
     if logits.dtype not in _KINDS:
         _dtype_code(logits)
-    rows, vocab = logits.shape
-    _logprobs_check("token_logprobs", rows, vocab, logits.device, targets, top)
+    rows, vocab = shape
+    _logprobs_check("token_logprobs", rows, vocab, device, targets, top)
     if not logits.is_cuda:
         _refuse("kernels run on CUDA tensors only; there is no CPU path")
-    out = _logprobs_result(logits.device, rows, top, targets is not None)
+    out = _logprobs_result(device, rows, top, targets)
     if rows:
         _token_logprobs(logits, targets, out, 0, top, status)
     return out
@@ -1259,7 +1261,7 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
     rows, vocab = x.shape[0], weight.shape[0]
     _logprobs_check("linear_logprobs", rows, vocab, x.device, targets, top)
     _stream(x)
-    out = _logprobs_result(x.device, rows, top, targets is not None)
+    out = _logprobs_result(x.device, rows, top, targets)
     if rows > SKINNY_MAX_ROWS and type(weight) is not Mx4Weight and _bf16_ok(x, weight):
         lib = library.load()
         with _on_device(x.device.index):
