@@ -259,10 +259,15 @@ __device__ __noinline__ float bound_of(const unsigned* seen, int rows, int top) 
 }
 
 // Logits from their sums of products.  cap tanh(y) = cap - 2 cap / (e^(2 y) + 1), from the hardware's power and reciprocal (2^-22 and 2^-23 of
-// themselves): off by at most 2^-21 of the cap wherever it lies, which is what float32 sums of a few hundred products are off by.  tanhf
-// takes five times the instructions: 10,000 instead of 6,000 cycles a tile, 512 rows with 20 alternatives 796 instead of 658 us.
+// themselves): off by at most 2^-21 of the cap wherever it lies, which up to a cap of 64 (3e-5) is what float32 sums of a few hundred products
+// are off by.  tanhf takes five times the instructions: 10,000 instead of 6,000 cycles a tile, 512 rows with 20 alternatives 796 instead of 658 us.
+// A larger cap would lose small logits that way and takes it.
+constexpr float FAST_CAP = 64.f;
 __device__ __forceinline__ void logits_of(const HeadArgs& a, float (&v)[32]) {
-    if (a.cap > 0.f) {
+    if (a.cap > FAST_CAP) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = a.cap * tanhf(v[i] / a.cap);
+    } else if (a.cap > 0.f) {
         const float f = a.inv_cap * (2.f * LP_LOG2E), c2 = -2.f * a.cap;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {

@@ -129,14 +129,15 @@ class Engine:
 
         A sequence's first token is scored by `step(..., "last")` of what is before it, or by giving it as `following` of that step.  A step
         without any row (one token a sequence, nothing following) runs all the same."""
-        lens = [len(t) for t in tokens]
+        tokens = [np.asarray(t).reshape(-1) for t in tokens]
         if following is None:
-            want, targets = [list(range(l - 1)) for l in lens], [list(t)[1:] for t in tokens]
+            want, targets = [list(range(len(t) - 1)) for t in tokens], [t[1:] for t in tokens]
         else:
-            if len(following) != len(tokens):
+            following = [np.asarray(f).reshape(-1) for f in following]
+            if len(following) != len(tokens) or any(f.size != 1 for f in following):
                 raise StepError("`following` must name a token for every sequence")
-            want, targets = "all", [list(t)[1:] + [f] for t, f in zip(tokens, following)]
-        targets = np.asarray([t for ts in targets for t in ts])
+            want, targets = "all", [a for t, f in zip(tokens, following) for a in (t[1:], f)]
+        targets = np.concatenate([t for t in targets if t.size] or [np.zeros(0, np.int64)])
         if targets.size and (targets.dtype.kind not in "iu" or targets.min() < 0 or targets.max() >= self.model.vocab_size):
             raise StepError(f"token ids must be whole numbers inside the vocabulary of {self.model.vocab_size}")
         most = min(ops.LOGPROBS_MAX_TOP, self.model.vocab_size)

@@ -1270,10 +1270,11 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
                                                   _ptr(out.logprobs), _ptr(out.entropy), _ptr(out.top_logprobs), _ptr(out.top_ids), _ptr(work),
                                                   work.numel(), _status(status), _stream(x)))
         return out
-    piece = max(1, LOGPROBS_PIECE // vocab)
+    # equal pieces, none of them few rows where the whole is not: a 4-bit weight takes few rows as they are and rounds many
+    pieces = -(-rows // max(4 * MX_FEW_ROWS, LOGPROBS_PIECE // vocab))
     with _on_device(x.device.index):
-        for r in range(0, rows, piece):
-            z = linear(x[r:r + piece], weight, torch.float32, softcap, status)
+        for r, end in ((rows * i // pieces, rows * (i + 1) // pieces) for i in range(pieces)):
+            z = linear(x[r:end], weight, torch.float32, softcap, status)
             if scale != 1.0:
                 scale_(z, scale)
             _token_logprobs(z, targets, out, r, top, status)

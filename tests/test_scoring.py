@@ -253,7 +253,7 @@ def test_scored_texts_equal_plain(tmp_path, monkeypatch):
     ids = texts[0]
     slot = engine.new_sequence()
     a = engine.score([slot], [ids[:10]], following=[ids[10]])
-    b = engine.score([slot], [ids[10:]])
+    b = engine.score([slot], [np.array(ids[10:])])
     got = torch.cat([a.logprobs, b.logprobs]).numpy()
     assert np.abs(got - [log_p(cfg, w, ids)[i, t] for i, t in enumerate(ids[1:])]).max() < 1e-4
     engine.release(slot)
@@ -265,7 +265,7 @@ def test_scoring_refusals(tmp_path, monkeypatch):
     s = engine.new_sequence()
     for kw in (dict(tokens=[[1, 2]], following=[1, 2]), dict(tokens=[[1, 2]], following=[cfg["vocab_size"]]), dict(tokens=[[1, -2]]),
                dict(tokens=[[1, 2]], top=33), dict(tokens=[[1, 2]], top=-1), dict(tokens=[[1, 2]], top=True), dict(tokens=[[1, 2.5]]),
-               dict(tokens=[[]]), dict(tokens=[[1], [2]])):
+               dict(tokens=[[]]), dict(tokens=[[1], [2]]), dict(tokens=[[1, 2]], following=[2.5]), dict(tokens=[[1, 2]], following=[[2, 3]])):
         with pytest.raises(StepError):
             engine.score([s], **kw)
     assert engine.length(s) == 0

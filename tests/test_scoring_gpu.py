@@ -164,13 +164,13 @@ def head_case(rows, width, vocab, dtype, seed, scale=0.1):
 
 def head_logits(x, w, softcap, scale):
     """float64 logits, and what 32 bits may make of them: K products and sums of up to sum |x w|, 2^-24 each (2^-23 where tensor cores round
-    towards zero), the soft-cap's argument, tanh (2^-22 of the cap) and product, the scale."""
+    towards zero), the soft-cap's argument, tanh and product (2^-21 of the cap up to 64, of the result above), the scale."""
     x, w = f64(x), f64(w)
     z = x @ w.T
     off = (np.abs(x) @ np.abs(w).T).max() * (x.shape[1] + 2) * 2.0 ** -23
     if softcap:
         z = softcap * np.tanh(z / softcap)
-        off += softcap * 2.0 ** -20
+        off += (softcap if softcap <= 64 else np.abs(z).max()) * 2.0 ** -20
     return z * scale, (off + np.abs(z).max() * 2.0 ** -22) * abs(scale)
 
 
@@ -181,7 +181,7 @@ HEADS = [(1, 64, 100, "bfloat16"), (1, 2304, 5000, "bfloat16"), (16, 256, 777, "
 
 
 @pytest.mark.parametrize("rows,width,vocab,kind", HEADS)
-@pytest.mark.parametrize("softcap,scale", [(None, 1.0), (8.0, 1.0), (None, 0.25), (5.0, -1.5)])
+@pytest.mark.parametrize("softcap,scale", [(None, 1.0), (8.0, 1.0), (None, 0.25), (5.0, -1.5), (64.0, 1.0), (1e4, 1.0), (1e30, 2.0), (1e-3, 1.0)])
 def test_behind_an_output_head(rows, width, vocab, kind, softcap, scale):
     x, w = head_case(rows, width, vocab, getattr(torch, kind), rows + width)
     t = targets_of(rows, vocab, 5)
@@ -329,6 +329,17 @@ def test_a_long_kernel_ahead_is_no_wait_in_vain():
     finally:
         lib.rdl_set_wait_test(0, 0, 0)
     assert status.item() == 0 and all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+
+
+def test_a_4_bit_head_in_pieces(monkeypatch):
+    """The last rows of many are taken as the others are."""
+    x, w = head_case(150, 320, 1000, torch.bfloat16, 21)
+    packed = ops.pack_mx4(w)
+    want = ops.token_logprobs(ops.linear(x, packed, torch.float32), None, 6)
+    monkeypatch.setattr(ops, "LOGPROBS_PIECE", 1000 * 70)
+    got = ops.linear_logprobs(x, packed, None, 6)
+    # 8-bit rows are multiplied by another kernel where they are fewer than 129: the order of 320 products' sums
+    assert torch.allclose(got.entropy, want.entropy, atol=1e-3) and torch.allclose(got.top_logprobs, want.top_logprobs, atol=1e-3)
 
 
 @pytest.mark.parametrize("rows", [1, 16, 17, 130])
