@@ -8,6 +8,8 @@
 #include "common.cuh"
 #include "launch.cuh"
 
+static_assert(sizeof(CopyRowsTensor) == 48, "kernels/ops.py packs 48 bytes");
+
 namespace {
 
 constexpr int CR_THREADS = 256, CR_DEPTH = 8;                       // 16-byte vectors a thread has on their way
