@@ -55,7 +55,8 @@ class ScoredText:
     @property
     def perplexity(self) -> float:
         """exp of the mean of -logprobs (1 for a text of one token)"""
-        return math.exp(-sum(self.logprobs) / len(self.logprobs)) if self.logprobs else 1.0
+        mean = -sum(self.logprobs) / len(self.logprobs) if self.logprobs else 0.0
+        return math.inf if mean > 700.0 else math.exp(mean)
 
 
 @dataclass

@@ -351,6 +351,13 @@ def test_a_dropped_engine_waits_for_its_uploads(tmp_path, monkeypatch):
     assert len(waited) == 2
 
 
+def test_perplexity():
+    from rust_deeplearning_b200 import ScoredText
+    inf = float("inf")
+    assert ScoredText([], [], []).perplexity == 1.0 and abs(ScoredText([-1.0, -3.0], [], []).perplexity - np.exp(2)) < 1e-9
+    assert ScoredText([-inf, -1.0], [], []).perplexity == inf and ScoredText([-1e4], [], []).perplexity == inf
+
+
 # ---- refusals that need no device ----
 
 def test_refused_copies():

@@ -153,6 +153,42 @@ def test_captured_replayed_and_on_other_streams(form):
         assert all(torch.equal(u, v) for u, v in zip(r, b))
 
 
+def test_calls_of_several_threads_at_once():
+    import threading
+    g = torch.Generator().manual_seed(30)
+    x = torch.randn((200, 256), generator=g).to(torch.bfloat16).to(DEV)
+    w = (torch.randn((5000, 256), generator=g) * 0.1).to(torch.bfloat16).to(DEV)
+    z, t = logits_of(50, 30000, torch.float32, 31), targets_of(50, 30000, 32)
+    k = torch.randn((3, 20, 1000), device=DEV)
+    want_head, want_rows = ops.linear_logprobs(x, w, None, 7, softcap=20.0), ops.token_logprobs(z, t, 7)
+    moved_k = moved(k, [0, 1], [5, 6])
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(form):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                own = k.clone()
+                for _ in range(30):
+                    if form == 0:
+                        ok = all(torch.equal(a, b) for a, b in zip(ops.linear_logprobs(x, w, None, 7, softcap=20.0)[1:], want_head[1:]))
+                    elif form == 1:
+                        ok = all(torch.equal(a, b) for a, b in zip(ops.token_logprobs(z, t, 7), want_rows))
+                    else:
+                        ops.copy_rows([(own, [0, 1], [5, 6])])
+                        ok = torch.equal(own, moved_k)
+                    if not ok:
+                        wrong.append(form)
+        except Exception as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i % 3,)) for i in range(6)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
 # ---- behind an output head ----
 
 def head_case(rows, width, vocab, dtype, seed, scale=0.1):
