@@ -4,9 +4,10 @@
 // or 8 where there are fewer rows than the device has room for blocks.  A thread copies what it looks at into shared memory of its own,
 // LP_RING batches ahead (cp.async), so that memory is kept busy while lists are sorted, and no thread waits for another's copy.
 //
-// Measured in a row of calls on the device: 2,048 rows of 256,000, float32 304 us without alternatives (6.9 TB/s), 312 with five, 349 with 20 (a logit
-// takes 12 to 16 instructions, so that the multiprocessors are busy four fifths of the time); bfloat16 248 and 275, bound by those instructions.
-// 8,192 rows of 1,000 28 us.  One row of 32,000 6.3 us, eight of 256,000 6.2 us, with 20 alternatives 14.7: latency, of the lists at last.
+// Measured in a row of calls on the device: 2,048 rows of 256,000, float32 299 us without alternatives (7.0 TB/s), 300 with five, 328 with 20 (a logit
+// takes 12 to 16 instructions, so that the multiprocessors are busy four fifths of the time); bfloat16 195 and 238, bound by those instructions;
+// seconds of it at 1,000 W, float32 355 with five.  8,192 rows of 32,000, float32 151 us, 183 and 231; of 1,000 9, 20 and 31 us.  One row of 32,000
+// 6.1 us; eight of 256,000 6.2 us, with 20 alternatives 11.4: latency, of the lists at last.
 #include "api.h"
 #include "launch.cuh"
 #include "logprobs.cuh"
@@ -16,6 +17,7 @@ namespace {
 constexpr int LP_MAX_THREADS = 512, LP_MAX_WARPS = LP_MAX_THREADS / 32;
 constexpr int LP_BATCH = 4, LP_RING = 3;                             // 16-byte vectors of a thread in a batch; batches on their way or looked at
 constexpr int LP_THREAD_BYTES = LP_RING * LP_BATCH * 16;             // of the ring
+constexpr int LP_LIST_BYTES = 64 / 32 * 8;                           // of its warp's list
 constexpr int LP_MAX_CLUSTER = 8;
 
 struct LpArgs {
@@ -51,18 +53,9 @@ __device__ __forceinline__ void lp_copies_wait() { asm volatile("cp.async.wait_g
 // What a warp takes of its logits for the list.  A row's logits form 32 groups, by the lane that sees them; `seen` holds the largest
 // one of each that the block's warps have put in.  At least `top` logits are not below the top-th of these, so that one below it is none of
 // the row's largest.  A warp puts in what its lanes hold and takes the bound of all after its first batch and after every doubling of
-// them; what is not below it is put aside, and one warp looks among it in the end.  (Bounds that rose only with a warp's own sorted list let
-// one or two logits of every 512 through, each of which costs its warp 200 instructions: 393 us for five alternatives.)  Where a warp has put 32 aside it merges them into a list
-// of its own (called, not inlined: the 20 exchanges between lanes stand once in the kernel and not behind every logit of a batch).
-__device__ __noinline__ LpKey lp_take(LpKey keys, LpKey* buffer, int n, int aside, int lane) {
-    __syncwarp();
-    const LpKey k = lane < n ? buffer[lane] : 0;
-    const LpKey rest = lane < aside - n ? buffer[n + lane] : 0;
-    __syncwarp();
-    if (lane < aside - n) buffer[lane] = rest;
-    return lp_merge(keys, lp_sort(k, lane), lane);
-}
-
+// them; what is not below it is put aside, and one warp looks among it in the end.
+// (Bounds that rose only with a warp's own sorted list let one or two logits of every 512 through, each of which costs its warp 200
+// instructions: 393 us for five alternatives.)  Where a warp has put 32 aside it merges them into a list of its own.
 struct LpList {
     LpKey keys;                    // lane: its place's key
     float least;
@@ -91,15 +84,8 @@ struct LpList {
     __device__ __forceinline__ void look(float most) {
         atomicMax(seen + lane, (unsigned)(lp_key(most, 0) >> 32));
         __syncwarp();
-        float v = lp_key_logit((LpKey)(*(volatile unsigned*)(seen + lane)) << 32);
-#pragma unroll 1
-        for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll 1
-            for (int o = n >> 1; o > 0; o >>= 1) {
-                const float other = __shfl_xor_sync(0xffffffffu, v, o);
-                v = (((lane & o) == 0) == ((lane & n) == 0 || n == 32)) ? fmaxf(v, other) : fminf(v, other);
-            }
-        least = fmaxf(least, __shfl_sync(0xffffffffu, v, top - 1));
+        const unsigned own = *(volatile unsigned*)(seen + lane);
+        least = fmaxf(least, lp_key_logit((LpKey)lp_bound(seen, own, top) << 32));
     }
 };
 
@@ -125,14 +111,15 @@ __device__ __forceinline__ unsigned lp_remote(const void* p, unsigned rank) {
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArgs a) {
     constexpr int V = 16 / (int)sizeof(T);
-    extern __shared__ uint4 ring[];                                  // [LP_RING][LP_BATCH][thread]
+    // [LP_RING][LP_BATCH][thread], then lists [warp][64]: no more than the block's warps need, since it bounds how many small blocks there are at once
+    extern __shared__ uint4 ring[];
     __shared__ LpStats part[LP_MAX_WARPS];
-    __shared__ LpKey lists[TOP ? LP_MAX_WARPS : 1][TOP ? 64 : 1];
-    __shared__ unsigned seen[32];
+    __shared__ __align__(16) unsigned seen[32];
     __shared__ int counts[LP_MAX_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = threads >> 5;
     const unsigned rank = lp_cluster_rank(), size = lp_cluster_size();
     const long long row = blockIdx.x / size;
+    LpKey (*lists)[64] = (LpKey (*)[64])(ring + threads * LP_RING * LP_BATCH);
     if (threadIdx.x < 32) seen[threadIdx.x] = 0;
     rdl_grid_wait();
     rdl_grid_launch_dependents();
@@ -146,11 +133,13 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
     const int body_id = head + from * V;
 
     const unsigned own = (unsigned)__cvta_generic_to_shared(ring + threadIdx.x);
-    const int step = threads * LP_BATCH;
+    // a warp's vectors of a batch lie side by side (2 KB; with a block's threads side by side and a warp's vectors 8 KB apart 2,048 rows of 256,000
+    // bfloat16 logits took 204 us, not 195)
+    const int step = threads * LP_BATCH, mine = warp * 32 * LP_BATCH + lane;
     auto ask = [&](int first, int place) {
 #pragma unroll
         for (int j = 0; j < LP_BATCH; ++j) {
-            const int at = first + j * threads + (int)threadIdx.x;
+            const int at = first + j * 32 + mine;
             if (at < vectors) lp_copy16(own + (unsigned)((place * LP_BATCH + j) * threads * 16), body + (long long)at * V);
         }
         lp_copies_end();
@@ -169,7 +158,7 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
         float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < LP_BATCH; ++j) {
-            if (first + j * threads + (int)threadIdx.x < vectors) {
+            if (first + j * 32 + mine < vectors) {
                 lp_widen(ring[(place * LP_BATCH + j) * threads + threadIdx.x], v[j]);
             } else {
 #pragma unroll
@@ -188,7 +177,11 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
             if (__any_sync(0xffffffffu, !(most < list.least))) {
 #pragma unroll
                 for (int j = 0; j < LP_BATCH; ++j) {
-                    const int at = first + j * threads + (int)threadIdx.x;
+                    float of_vector = -INFINITY;             // few vectors of a batch have one (8,192 rows of 32,000 in bfloat16: 236 -> 214 us)
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) of_vector = lp_max3(of_vector, v[j][i], v[j][i + 1]);
+                    if (!__any_sync(0xffffffffu, !(of_vector < list.least))) continue;
+                    const int at = first + j * 32 + mine;
 #pragma unroll
                     for (int i = 0; i < V; ++i) list.offer(v[j][i], body_id + at * V + i, at < vectors);
                 }
@@ -288,8 +281,9 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
 
 template <typename T, bool TOP>
 int lp_run(const LpArgs& a, int cluster, int threads, cudaStream_t st) {
-    RDL_CUDA((rdl_allow_shared<token_logprobs_kernel<T, TOP>>(LP_MAX_THREADS * LP_THREAD_BYTES)), "token_logprobs");
-    RDL_CHECK_EX(rdl_launch_cluster(token_logprobs_kernel<T, TOP>, dim3((unsigned)a.rows * cluster), dim3(threads), cluster, (size_t)threads * LP_THREAD_BYTES, st, a),
+    constexpr int BYTES = LP_THREAD_BYTES + (TOP ? LP_LIST_BYTES : 0);
+    RDL_CUDA((rdl_allow_shared<token_logprobs_kernel<T, TOP>>(LP_MAX_THREADS * BYTES)), "token_logprobs");
+    RDL_CHECK_EX(rdl_launch_cluster(token_logprobs_kernel<T, TOP>, dim3((unsigned)a.rows * cluster), dim3(threads), cluster, (size_t)threads * BYTES, st, a),
                  "token_logprobs");
     return 0;
 }
@@ -305,13 +299,15 @@ extern "C" int rdl_token_logprobs(const void* logits, int dtype, long long row_s
     RDL_REQUIRE(logits && entropy && (!targets || logprobs) && (top == 0 || (top_logprobs && top_ids)), "token_logprobs: missing operand");
     RDL_REQUIRE((uintptr_t)logits % rdl_dtype_size(dtype) == 0, "token_logprobs: logits that are not on an element's boundary");
     const LpArgs a{logits, row_stride, rows, vocab, top, targets, logprobs, entropy, top_logprobs, top_ids, status};
-    // Few rows: as many blocks share a row as there is room for at once (two on a multiprocessor), each thread with a batch where the row has
-    // one.  Many: a thread has eight batches or more where the row has them, since what
-    // a warp does once for a row takes as long as one or two of them (8,192 rows of 32,000, five alternatives: 226 us, with two to four 312 to 269).
+    // Few rows: as many blocks share a row as there is room for at once (two on a multiprocessor), each thread with a batch where the row has one.
+    // More: as many threads a row as keep the device about full, or as leave each 16 batches (8 without alternatives), since what a warp
+    // does once for a row takes as long as one or two of them (five alternatives: 600 rows of 32,000 22 us with 256 threads, 25 with 64, 35 with 32;
+    // 4,000 rows 94 us with 64, 104 with 256).
     const long long vectors = (long long)vocab * (long long)rdl_dtype_size(dtype) / 16;
-    const bool few = rows <= 2 * rdl_sm_count();
+    const long long room = (long long)rdl_sm_count() * 2 * LP_MAX_THREADS;
     int threads = 32, cluster = 1;
-    while (threads < LP_MAX_THREADS && vectors >= threads * 2LL * LP_BATCH * (few ? 1 : 8)) threads *= 2;
+    while (threads < LP_MAX_THREADS && vectors >= threads * 2LL * LP_BATCH
+           && (3LL * rows * threads <= 2 * room || vectors >= threads * 2LL * LP_BATCH * (top ? 16 : 8))) threads *= 2;
     while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= 2 * rdl_sm_count() && vectors >= cluster * 2LL * LP_MAX_THREADS) cluster *= 2;
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == RDL_BF16) return top ? lp_run<__nv_bfloat16, true>(a, cluster, threads, st) : lp_run<__nv_bfloat16, false>(a, cluster, threads, st);

@@ -156,4 +156,34 @@ __device__ __forceinline__ LpKey lp_merge(LpKey a, LpKey b, int lane) {
     return lp_bitonic(a > r ? a : r, lane);
 }
 
+// Keys put aside, the first n <= 32 of them, into a warp's list; what is left of `aside` < 64 moves to the front.  (Called, not inlined: the 20
+// exchanges between lanes stand once in a kernel and not behind every place that puts something aside.)
+__device__ __noinline__ LpKey lp_take(LpKey keys, LpKey* buffer, int n, int aside, int lane) {
+    __syncwarp();
+    const LpKey k = lane < n ? buffer[lane] : 0;
+    const LpKey rest = lane < aside - n ? buffer[n + lane] : 0;
+    __syncwarp();
+    if (lane < aside - n) buffer[lane] = rest;
+    return lp_merge(keys, lp_sort(k, lane), lane);
+}
+
+// The largest of 32 values (16-byte aligned in shared memory, order-preserving bits, own: the lane's) that at least `top` of them are not below,
+// by counting: 8 reads and 32 comparisons a lane, where a sort of them is 15 exchanges, one after another.
+__device__ __forceinline__ unsigned lp_bound(const unsigned* seen, unsigned own, int top) {
+    const unsigned at = (unsigned)__cvta_generic_to_shared(seen);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        unsigned v[4];
+        asm volatile("ld.volatile.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at + 16 * i) : "memory");
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n += v[j] >= own;
+    }
+    return __reduce_max_sync(0xffffffffu, n >= top ? own : 0u);
+}
+// the key that the largest ones of 32 groups with that bound are above
+__device__ __forceinline__ LpKey lp_floor(unsigned bound) {
+    return bound > (unsigned)(lp_key(-INFINITY, 0) >> 32) ? ((LpKey)bound << 32) - 1 : 0;
+}
+
 }  // namespace
