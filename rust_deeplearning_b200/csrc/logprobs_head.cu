@@ -520,7 +520,8 @@ struct JoinOut { float* logprobs; float* entropy; float* top_logprobs; int* top_
 template <int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) head_join_kernel(const __grid_constant__ HeadArgs a, int rows_a_block, JoinOut o) {
     __shared__ LpStats part[WARPS];
-    __shared__ LpKey lists[WARPS][32];
+    __shared__ LpKey lists[WARPS][32], buffer[WARPS][64];
+    __shared__ __align__(16) unsigned seen[WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x, block = row / rows_a_block, own_row = row - block * rows_a_block;
     // groups that share the vocabulary's end: those whose range meets this row block's
@@ -538,19 +539,25 @@ __global__ void __launch_bounds__(WARPS * 32) head_join_kernel(const __grid_cons
     LpKey keys = 0, least = 0;
     const int n = 2 * (a.slices + x1 - x0);
     if (a.top > 0) {
-        // what the 32 groups held in the end: the top-th of them, by counting
-        const unsigned v = a.seen[(long long)lane * a.M + row];
-        unsigned t = 0;
-#pragma unroll
-        for (int b = 31; b >= 0; --b)
-            if (__popc(__ballot_sync(0xffffffffu, v >= (t | 1u << b))) >= a.top) t |= 1u << b;
-        if (t > ordered(-INFINITY)) least = ((LpKey)t << 32) - 1;      // a logit that equals it is above this
+        const unsigned own = a.seen[(long long)lane * a.M + row];      // what the 32 groups held in the end
+        seen[warp][lane] = own;
+        __syncwarp();
+        least = lp_floor(lp_bound(seen[warp], own, a.top));
     }
-    auto offer = [&](LpKey key) {                          // a key a lane, or 0
-        if (!__any_sync(0xffffffffu, key > least)) return;
-        keys = lp_merge(keys, lp_sort(key > least ? key : 0, lane), lane);
+    int aside = 0;                                         // keys above the bound that are not in the list yet
+    auto take = [&](int count) {
+        keys = lp_take(keys, buffer[warp], count, aside, lane);
+        aside -= count;
         const LpKey last = __shfl_sync(0xffffffffu, keys, a.top - 1);
         least = last > least ? last : least;
+    };
+    auto offer = [&](LpKey key) {                          // a key a lane, or 0
+        const bool in = key > least;
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        if (mask == 0) return;
+        if (in) buffer[warp][aside + __popc(mask & ((1u << lane) - 1))] = key;
+        aside += __popc(mask);
+        if (aside >= 32) take(32);
     };
     for (int first = warp * 32; first < n; first += WARPS * 32) {
         const int p = first + lane, i = p >> 1, x = x0 + i - a.slices;
@@ -593,6 +600,7 @@ __global__ void __launch_bounds__(WARPS * 32) head_join_kernel(const __grid_cons
             for (int k = 0; k < a.top; ++k) offer(listed ? a.keys[list * a.top + (long long)k * rows_a_block + own_row] : 0);
         }
     }
+    if (aside > 0) take(aside);
     st = lp_warp_join(st);
     if (lane == 0) part[warp] = st;
     lists[warp][lane] = keys;
