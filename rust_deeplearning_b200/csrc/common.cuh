@@ -55,6 +55,12 @@ static inline long long rdl_wait_cycles_for(int code) {
 }
 static inline int rdl_test_extra_tx_for(int code) { return g_rdl_wait_test_code == code ? g_rdl_wait_test_extra : 0; }
 
+// Copies that are on their way when a block gives up still write to its shared memory: they get the time to arrive.  Called when nothing in the
+// block asks for more of them.
+__device__ __forceinline__ void rdl_drain_copies() {
+    for (const long long t0 = clock64(); clock64() - t0 < RDL_COPY_DRAIN_CYCLES;) {}
+}
+
 // Multiprocessors of the current device (asked once per device; 1 if the question fails).
 int rdl_sm_count();
 

@@ -491,10 +491,13 @@ __global__ void __launch_bounds__(THREADS, 1) head_logprobs_kernel(const __grid_
         }
     }
     if (!ok && a.status) atomicExch(a.status, RDL_FAULT_LOGPROBS_HEAD);
-    if (*gave_up_v && threadIdx.x == 0) mx_drain();
     // ---- tear-down, reached by every thread ----
     mx_fence_before();
     __syncthreads();
+    if (*gave_up_v) {                    // behind the barrier: whichever warp gave up, the loader has asked for its last copies by now
+        rdl_drain_copies();
+        __syncwarp();
+    }
     if (CTAS == 2) cluster_sync();       // neither block leaves while the other may still read its shared memory or report to its barriers
     if (warp == 1) {
         if constexpr (CTAS == 1)

@@ -684,9 +684,12 @@ __global__ void __launch_bounds__(THREADS, PARTS == 6 ? 1 : 2) mx_few_rows_kerne
             }
         }
     }
-    if (*gave_up_v && threadIdx.x == 0) mx_drain();
     mx_fence_before();
     __syncthreads();
+    if (*gave_up_v) {                    // behind the barrier: whichever warp gave up, the loader has asked for its last copies by now
+        rdl_drain_copies();
+        __syncwarp();
+    }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 

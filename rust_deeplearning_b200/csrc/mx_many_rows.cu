@@ -367,10 +367,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx_many_rows_kernel(const __grid_c
         }
     }
     if (!ok && a.status) atomicExch(a.status, RDL_FAULT_MX_MANY);
-    if (*gave_up_v && threadIdx.x == 0) mx_drain();
     // ---- tear-down, reached by every thread ----
     mx_fence_before();
     __syncthreads();
+    if (*gave_up_v) {                    // behind the barrier: whichever warp gave up, the loader has asked for its last copies by now
+        rdl_drain_copies();
+        __syncwarp();
+    }
     if (CTAS == 2) cluster_sync();       // neither block leaves while the other may still read its shared memory or report to its barriers
     if (warp == 1)
         MX_CTA_GROUP(CTAS, asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory"),

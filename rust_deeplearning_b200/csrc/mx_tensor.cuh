@@ -82,10 +82,6 @@ __device__ __forceinline__ bool mx_bar_wait_both(uint32_t bar0, uint32_t parity0
                  "and.pred p, p, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1) : "memory");
     return ok != 0 || (mx_bar_wait(bar0, parity0, limit, gave_up) && mx_bar_wait(bar1, parity1, limit, gave_up));
 }
-// copies that are on their way when a block gives up still write to its shared memory: they get the time to arrive
-__device__ __forceinline__ void mx_drain() {
-    for (const long long t0 = clock64(); clock64() - t0 < RDL_COPY_DRAIN_CYCLES;) {}
-}
 __device__ __forceinline__ void mx_tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
