@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2) gemm_stream_kernel(const __grid
         if (lane < ROWS) {
             int s = 0;                                   // place in the ring, and how often it has been gone round
             uint32_t round = 0;
-            bool first_copy = true;
+            bool first_copy = true, ok = true;           // ok: nobody has given up, the same in all 16 lanes
             // The weights are read once a step: they pass through L2 marked to be evicted first, so that what the step
             // reads again and again - the rows of activations, the residual stream - stays there.
             const unsigned long long policy = l2_evict_first_policy();
@@ -183,7 +183,10 @@ __global__ void __launch_bounds__(ST_THREADS, 2) gemm_stream_kernel(const __grid
                 const int n_ok = __popc(__ballot_sync(0xffffu, row_ok));
                 for (int tk = 0; tk < tiles_per_unit; ++tk) {
                     // the tile that lay here must have been read by all eight warps
-                    if (round > 0 && !st_wait(empty_s + 8 * s, (round & 1) ^ 1, a.wait_cycles, gave_up_v)) break;
+                    // (After a give-up the readers go through the tiles without waiting and free places whose last copy may not have come.
+                    // A barrier must not be told of another copy then, so the flag is looked at behind the wait too, which orders it.)
+                    if (round > 0) ok = __all_sync(0xffffu, st_wait(empty_s + 8 * s, (round & 1) ^ 1, a.wait_cycles, gave_up_v) && !*gave_up_v);
+                    if (!ok) break;
                     const int k0 = tk * ST_KT;
                     const uint32_t bytes = (uint32_t)((K - k0 < ST_KT ? K - k0 : ST_KT) * 2);
                     if (lane == 0) {
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2) gemm_stream_kernel(const __grid
                         if (round++ == 0) rdl_grid_wait();
                     }
                 }
-                if (*gave_up_v) break;
+                if (!ok) break;
             }
         }
     } else {

@@ -167,3 +167,21 @@ def test_a_long_kernel_ahead_of_the_streaming_product_is_no_wait_in_vain(m, n, k
         finally:
             lib.rdl_set_wait_test(0, 0, 0)
         assert status.item() == 0 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(16, 300, 9000), (1, 300, 9000), (8, 6000, 2304), (3, 19001, 1304)])
+def test_weight_streaming_product_gives_up_with_more_tiles_than_places(m, n, k):
+    """The readers that gave up free the places of the ring; the copying warp must not announce another copy to a barrier whose last one has not come."""
+    lib = library.load()
+    x, w = rnd((m, k), torch.bfloat16, 84), rnd((n, k), torch.bfloat16, 85, 0.2)
+    want = ops.linear(x, w)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    try:
+        lib.rdl_set_wait_test(7, SHORT_WAIT, 64)
+        ops.linear(x, w, status=status)
+        torch.cuda.synchronize()
+    finally:
+        lib.rdl_set_wait_test(0, 0, 0)
+    assert status.item() == 7
+    status.zero_()
+    assert torch.equal(ops.linear(x, w, status=status), want) and status.item() == 0
