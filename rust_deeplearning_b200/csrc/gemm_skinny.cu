@@ -423,7 +423,11 @@ __global__ void __launch_bounds__(ST_THREADS, 2) gemm_stream_kernel(const __grid
             asm volatile("bar.sync 1, %0;" ::"n"(ST_WARPS * 32) : "memory");      // the partial sums are free again
         }
     }
-    if (*gave_up_v && status && lane == 0) atomicExch(status, RDL_FAULT_GEMM_STREAM);
+    if (*gave_up_v) {
+        // Every warp for itself, there is no barrier at the end: the one that gave up covers what was asked for before, the copying warp what it still asked for.
+        if (status && lane == 0) atomicExch(status, RDL_FAULT_GEMM_STREAM);
+        rdl_drain_copies();
+    }
 }
 
 template <int NT, bool GATED, int KU, int MODE>

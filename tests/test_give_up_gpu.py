@@ -36,7 +36,8 @@ def product(rows, k):
 
 CALLS = [(12, "linear_logprobs", lambda: head(40, 0)), (12, "linear_logprobs", lambda: head(40, 5)), (12, "linear_logprobs", lambda: head(200, 0)),
          (12, "linear_logprobs", lambda: head(300, 5)), (9, "mx_many_rows", lambda: product_mx4(140, 512)), (9, "mx_many_rows", lambda: product_mx4(400, 512)),
-         (10, "mx_some_rows", lambda: product_mx4(40, 4096)), (8, "mx_few_rows", lambda: product_mx4(8, 512))]
+         (10, "mx_some_rows", lambda: product_mx4(40, 4096)), (8, "mx_few_rows", lambda: product_mx4(8, 512)),
+         (7, "gemm_skinny", lambda: product(8, 512)), (7, "gemm_skinny", lambda: product(16, 9000))]
 
 
 @pytest.mark.parametrize("case", range(len(CALLS)))
