@@ -11,6 +11,7 @@ import array
 import contextlib
 import ctypes
 import functools
+import math
 import os
 import struct
 from typing import NamedTuple, Optional, Tuple
@@ -1175,6 +1176,7 @@ def sample(logits: torch.Tensor, *, temperature: float, top_k: Optional[int] = N
 # how probable tokens are
 # ------------------------------------------------------------------------------------------
 
+_F32 = torch.finfo(torch.float32)
 LOGPROBS_MAX_TOP = 32    # alternatives a row can be asked for
 # float32 logits that `linear_logprobs` holds at a time where the product has a kernel of its own
 LOGPROBS_PIECE = 1 << 26
@@ -1249,12 +1251,13 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
 
     More than 16 bfloat16 rows that meet `linear`'s alignment rules run in one kernel that forms the statistics as it takes the products out of
     tensor memory (its work space: a few MB, up to 250 MB for 32 alternatives); others form pieces of the logits by `linear`, 256 MB
-    at a time.  softcap: cap * tanh(. / cap) of the products, before scale.  The weight is a constant, as `linear` has it."""
+    at a time.  softcap: cap * tanh(. / cap) of the products, before scale (both numbers that float32 holds).  The weight is a constant, as `linear` has it."""
     _need(x.dim() == 2 and len(weight.shape) == 2 and x.shape[1] == weight.shape[1] and x.shape[1] > 0,
           f"linear_logprobs: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not fit")
     _need(type(weight) is Mx4Weight or x.dtype is weight.dtype, "linear_logprobs: rows and weight of one type")
     _need(x.device == weight.device, f"linear_logprobs: rows on {x.device}, weight on {weight.device}")
-    _need(softcap is None or softcap > 0, "linear_logprobs: the soft-cap must be positive")
+    _need(softcap is None or _F32.tiny <= softcap <= _F32.max, "linear_logprobs: the soft-cap must be positive and a normal float32 number")
+    _need(math.isfinite(scale) and abs(scale) <= _F32.max, "linear_logprobs: the scale must be a finite float32 number")
     _dtype_code(x)
     _dense(x, "x")
     _need(type(weight) is Mx4Weight or weight.is_contiguous(), "linear_logprobs: the weight must be contiguous")

@@ -396,6 +396,13 @@ def test_refused_scoring_calls():
             call()
 
 
+@pytest.mark.parametrize("kw", [dict(softcap=float("inf")), dict(softcap=float("nan")), dict(softcap=1e39), dict(softcap=1e-40), dict(softcap=-30.0),
+                                dict(scale=float("inf")), dict(scale=float("nan")), dict(scale=1e39)])
+def test_numbers_that_float32_does_not_hold_are_refused(kw):
+    with pytest.raises(KernelError, match="float32"):
+        ops.linear_logprobs(torch.zeros((3, 10)), torch.zeros((5, 10)), None, 2, **kw)
+
+
 def test_command_line_refusals():
     from rust_deeplearning_b200.cli import main
     for more in (["--stream", "--logprobs", "1"], ["--stream", "--score"], ["--score", "--samples", "2"]):
