@@ -55,22 +55,26 @@ __device__ __forceinline__ void lp_copies_wait() { asm volatile("cp.async.wait_g
 // the row's largest.  A warp puts in what its lanes hold and takes the bound of all after its first batch and after every doubling of
 // them; what is not below it is put aside, and one warp looks among it in the end.
 // (Bounds that rose only with a warp's own sorted list let one or two logits of every 512 through, each of which costs its warp 200
-// instructions: 393 us for five alternatives.)  Where a warp has put 32 aside it merges them into a list of its own.
+// instructions: 393 us for five alternatives.)  Where a warp has put 32 aside it merges them into a list of its own.  A warp comes to larger
+// and larger tokens, so that behind such a list equal logits are of no use either: rows of few allowed tokens, or of one value, would put every
+// logit aside (2,048 rows of 256,000 with 10 allowed tokens 4,140 us, not 330).  What the list says is looked at once a vector: the lanes'
+// tokens interleave within one, and after each of its logits it took longer (1,024 rows of 256,000 in bfloat16, 20 alternatives 184 us, not 166).
 struct LpList {
     LpKey keys;                    // lane: its place's key
-    float least;
+    float least;                   // what a logit must reach
     int aside;                     // how many are put aside
     LpKey* buffer;                 // 64
     unsigned* seen;                // 32, order-preserving bits
     int top, lane;
-    bool listed;                   // `keys` holds some
+    int listed;                    // how often 32 have been merged into `keys`
 
     __device__ __forceinline__ void take(int n) {
         keys = lp_take(keys, buffer, n, aside, lane);
         aside -= n;
-        listed = true;
-        least = fmaxf(least, lp_key_logit(__shfl_sync(0xffffffffu, keys, top - 1)));
+        ++listed;
     }
+    // what follows are larger tokens than the list's
+    __device__ __forceinline__ void beyond() { least = fmaxf(least, lp_key_beyond(__shfl_sync(0xffffffffu, keys, top - 1))); }
     // one logit a lane (or none)
     __device__ __forceinline__ void offer(float z, unsigned id, bool valid) {
         const bool in = valid && !(z < least);
@@ -149,7 +153,7 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
 
     LpStats st = lp_empty();
     LpList list;
-    if (TOP) list = {0, -INFINITY, 0, lists[warp], seen, a.top, lane, false};
+    if (TOP) list = {0, -INFINITY, 0, lists[warp], seen, a.top, lane, 0};
     int place = 0, batches = 0;
     for (int first = 0; first < vectors; first += step) {
         ask(first + (LP_RING - 1) * step, place == 0 ? LP_RING - 1 : place - 1);
@@ -182,8 +186,10 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
                     for (int i = 0; i < V; i += 2) of_vector = lp_max3(of_vector, v[j][i], v[j][i + 1]);
                     if (!__any_sync(0xffffffffu, !(of_vector < list.least))) continue;
                     const int at = first + j * 32 + mine;
+                    const int listed = list.listed;
 #pragma unroll
                     for (int i = 0; i < V; ++i) list.offer(v[j][i], body_id + at * V + i, at < vectors);
+                    if (list.listed != listed) list.beyond();
                 }
             }
         }
@@ -195,7 +201,10 @@ __global__ void __launch_bounds__(LP_MAX_THREADS, 2) token_logprobs_kernel(LpArg
         if (v > st.m) lp_move(st, v);
         const float one[2] = {v, -INFINITY};
         if (valid) lp_add(st, one);
-        if (TOP) list.offer(v, i, valid);
+        if (TOP) {
+            if (list.listed) list.least = -INFINITY;                 // smaller tokens than the list's among them
+            list.offer(v, i, valid);
+        }
     }
     if (TOP) {
         if (list.listed) {

@@ -124,6 +124,11 @@ __device__ __forceinline__ float lp_key_logit(LpKey k) {
     return o == 0 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ unsigned lp_key_id(LpKey k) { return ~(unsigned)k; }
+// the least logit that comes before a key's at any larger id (minus infinity for no key and for a NaN's: every number does)
+__device__ __forceinline__ float lp_key_beyond(LpKey k) {
+    const unsigned o = (unsigned)(k >> 32);
+    return o == 0 ? -INFINITY : o >= 0xff800000u ? INFINITY : lp_key_logit(k + (1ull << 32));
+}
 
 // A warp's list: 32 keys, a lane each, largest in lane 0.
 
