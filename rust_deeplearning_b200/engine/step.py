@@ -31,6 +31,15 @@ def _next_pow2(n: int) -> int:
     return 1 << max(0, (n - 1).bit_length())
 
 
+# Status words of engines that were dropped, each with an event behind the engine's last step: a kernel of it that is still to run may write its
+# word, and the allocator of pinned memory, which knows nothing of that, must not hand it to anybody else.
+_retired: List[tuple] = []
+
+
+def _release_retired():
+    _retired[:] = [r for r in _retired if r[1] is None or not r[1].query()]
+
+
 class _Graph:
     def __init__(self):
         self.graph = None
@@ -58,6 +67,7 @@ class Engine:
         self._graphs: Dict[tuple, _Graph] = {}
         self._pinned: List[Optional[torch.Tensor]] = [None, None]
         self._pinned_event: List[Optional[torch.cuda.Event]] = [None, None]
+        self._last_stream: Optional[torch.cuda.Stream] = None      # of the last step
         self._flip = 0
         self._scratch: Dict[str, torch.Tensor] = {}
         self.graph_replays = 0
@@ -69,6 +79,7 @@ class Engine:
         # reads it without a device call (after any synchronising read of a step's result)
         self.status = torch.zeros(1, dtype=torch.int32)
         if self.device.type == "cuda":
+            _release_retired()
             self.status = self.status.pin_memory()
 
     def __del__(self):
@@ -80,6 +91,13 @@ class Engine:
                     event.synchronize()
                 except Exception:      # the context is gone, or has failed: nothing reads them any more
                     pass
+        if getattr(self, "_last_stream", None) is not None:
+            try:
+                event = torch.cuda.Event()
+                event.record(self._last_stream)
+            except Exception:
+                event = None           # kept for good
+            _retired.append((self.status, event))
 
     # ---- sequences ----
     def new_sequence(self) -> int:
@@ -257,7 +275,8 @@ class Engine:
         ops.upload_batch(dev, host, layout.size, fed)
         if self.device.type == "cuda":
             ev = torch.cuda.Event()
-            ev.record()
+            self._last_stream = torch.cuda.current_stream(self.device)
+            ev.record(self._last_stream)
             self._pinned_event[self._flip] = ev
 
     def _graph_step(self, slots, tokens, past, want, tables, widths, max_total, fed=None):

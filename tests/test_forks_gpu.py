@@ -91,6 +91,31 @@ def test_an_engine_dropped_with_steps_in_flight():
             assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_the_status_word_of_a_dropped_engine_is_nobody_elses():
+    """Kernels that are still to run may report to it: it stays out of the allocator's hands until the engine's last step is over."""
+    from rust_deeplearning_b200.engine import step
+    cfg, seed = tiny_configs.config("A")
+    model = random_model(cfg, seed, "float32")
+    ids = ids_of(61, 9, model.vocab_size)
+    Engine(model, max_tokens=64)                             # whatever earlier engines left is released
+    for side in (False, True):
+        stream = torch.cuda.Stream() if side else torch.cuda.current_stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            eng = Engine(model, max_tokens=64)
+            eng.step([eng.new_sequence()], [ids], "last")
+            word = eng.status.data_ptr()
+            torch.cuda._sleep(200_000_000)                   # stands for what is left of the step: a tenth of a second
+        del eng
+        held = [torch.zeros(1, dtype=torch.int32).pin_memory() for _ in range(20)]
+        assert all(t.data_ptr() != word for t in held) and any(r[0].data_ptr() == word for r in step._retired)
+        torch.cuda.synchronize()
+        del held
+        other = Engine(model, max_tokens=64)
+        assert not any(r[0].data_ptr() == word for r in step._retired)
+        other.check_status()
+
+
 def log_p(z):
     z = z.double().cpu().numpy()
     z = z - z.max(axis=1, keepdims=True)
