@@ -123,28 +123,36 @@ class SequenceState:
 
 
 def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, *, max_seqs: int, max_tokens: int,
-                 page_size: int, max_context: int, samples: int = 1, prompt_shared: bool = False) -> List[List[int]]:
+                 page_size: int, max_context: int, samples: int = 1, prompt_shared: bool = False,
+                 rings: Sequence[Tuple[int, int]] = ()) -> List[List[int]]:
     """Split requests, in order, into batches that fit the cache: at most `max_seqs` sequences and
     at most `max_tokens` positions, counting every sequence at the longest it can get, rounded up
-    to the page size.  samples: sequences per request; prompt_shared: they share the whole pages of its prompt for good."""
+    to the page size.  samples: sequences per request; prompt_shared: they share the whole pages of its prompt for good, but for
+    `rings`, the parts of the cache that keep a window, where every sequence comes round to pages of its own: (positions a sequence
+    holds there at most, positions there are) of each."""
     if samples > max_seqs:
         raise ValueError(f"{samples} continuations of a prompt, the cache holds {max_seqs} sequences")
-    batches, cur, used = [], [], 0
+    batches, cur, used, ring_used = [], [], 0, [0] * len(rings)
     for i, n in enumerate(prompt_lens):
         if n < 1:
             raise ValueError(f"request {i}: empty prompt")
         if n > max_context:
             raise ValueError(f"request {i}: prompt of {n} tokens exceeds the context of {max_context}")
         longest = min(n + max(max_new_tokens - 1, 0), max_context)
+        whole = -(-longest // page_size) * page_size
         shared = n // page_size * page_size if prompt_shared else 0
-        cost = shared + samples * (-(-longest // page_size) * page_size - shared)
-        if cost > max_tokens:
-            raise ValueError(f"request {i}: needs {cost} cache positions, the cache holds {max_tokens}")
-        if cur and ((len(cur) + 1) * samples > max_seqs or used + cost > max_tokens):
+        cost = shared + samples * (whole - shared)
+        ring_cost = [samples * min(whole, most) for most, _ in rings]
+        for need, room in [(cost, max_tokens)] + [(c, r) for c, (_, r) in zip(ring_cost, rings)]:
+            if need > room:
+                raise ValueError(f"request {i}: needs {need} cache positions, the cache holds {room}")
+        full = used + cost > max_tokens or any(u + c > room for u, c, (_, room) in zip(ring_used, ring_cost, rings))
+        if cur and ((len(cur) + 1) * samples > max_seqs or full):
             batches.append(cur)
-            cur, used = [], 0
+            cur, used, ring_used = [], 0, [0] * len(rings)
         cur.append(i)
         used += cost
+        ring_used = [u + c for u, c in zip(ring_used, ring_cost)]
     if cur:
         batches.append(cur)
     return batches
@@ -201,7 +209,7 @@ def generate(engine, prompts: Sequence[Sequence[int]], *, max_new_tokens: int = 
     batches = plan_batches([len(p) for p in prompts], max_new_tokens,
                            max_seqs=min(cache.max_seqs, max_batch or cache.max_seqs),
                            max_tokens=cache.max_tokens, page_size=cache.page_size, max_context=max_context, samples=samples,
-                           prompt_shared=samples > 1 and not any(g.is_ring for g in cache.kv_groups))
+                           prompt_shared=samples > 1, rings=[(g.ring_pages * g.page_size, g.pool.n_pages * g.page_size) for g in cache.kv_groups if g.is_ring])
     results: List[Optional[GenerationResult]] = [None] * (len(prompts) * samples)
     need_history = sampling.repetition_penalty is not None and not sampling.greedy
 

@@ -334,6 +334,32 @@ def test_batches_of_requests_with_several_continuations():
         plan_batches([5], 8, samples=7, **kw)
 
 
+def test_batches_of_continuations_where_some_layers_keep_a_window():
+    kw = dict(max_seqs=8, max_tokens=640, page_size=64, max_context=512, samples=4, prompt_shared=True)
+    assert plan_batches([400, 400], 40, rings=[(128, 1024)], **kw) == [[0], [1]]                        # 384 + 4 * 64 fill the pages that are shared
+    assert plan_batches([130, 130], 20, rings=[(128, 1024)], **kw) == [[0], [1]]                        # 2 * (128 + 4 * 64) do not fit
+    assert plan_batches([30, 30], 20, rings=[(128, 1024)], **kw) == [[0, 1]]
+    assert plan_batches([30, 30], 20, rings=[(128, 1024), (64, 448)], **kw) == [[0], [1]]               # 2 * 4 * 64 of 448
+    with pytest.raises(ValueError):
+        plan_batches([400], 40, rings=[(128, 511)], **kw)
+
+
+@pytest.mark.parametrize("name,n,samples", [("A", 40, 5), ("B", 40, 5)])
+def test_continuations_that_fit_only_as_they_share_a_prompt(tmp_path, monkeypatch, name, n, samples):
+    """A cache with room for the prompt once and a page or two of each continuation, and for every continuation's window."""
+    engine, cfg, w = build(tmp_path, name, monkeypatch, page_size=8, max_tokens=(n // 8 * 8) + samples * 16, max_seqs=samples)
+    scoring_refs.install(monkeypatch)
+    assert any(g.is_ring for g in engine.cache.kv_groups)
+    ids = prompt(np.random.default_rng(15), n, cfg["vocab_size"])
+    sampling = SamplingParams(temperature=0.9, seed=5)
+    got = generate(engine, [ids], max_new_tokens=14, sampling=sampling, stop_token_ids=[], samples=samples)
+    roomy, _, _ = build(tmp_path, name, monkeypatch, page_size=8, max_tokens=1024, max_seqs=samples)
+    scoring_refs.install(monkeypatch)
+    want = generate(roomy, [ids] * samples, max_new_tokens=14, sampling=sampling, stop_token_ids=[])
+    assert [r.tokens for r in got] == [r.tokens for r in want]
+    assert all(g.pool.n_free == g.pool.n_pages for g in engine.cache.kv_groups)
+
+
 def test_a_dropped_engine_waits_for_its_uploads(tmp_path, monkeypatch):
     engine, cfg, w = build(tmp_path, "A", monkeypatch)
     waited = []
