@@ -32,6 +32,8 @@ struct CrArgs {
     int2 pair[PAIRS];                               // source row, destination row
 };
 constexpr int CR_FEW = 64, CR_MANY = 2048;
+constexpr long long CR_MAX_BLOCKS = 0x7fffffff;     // of a launch
+__host__ inline long long cr_pieces(const CopyRowsTensor& t) { return (t.row_bytes + CR_PIECE - 1) / CR_PIECE; }
 
 template <typename U>
 __device__ __forceinline__ void cr_copy(char* to, const char* from, int bytes) {
@@ -93,11 +95,13 @@ int cr_run(const CopyRowsTensor* tensors, int n_tensors, const int* pairs, cudaS
             const bool there = done == 0 && i > 0 && last && last_whole == i - 1 && tensors[i - 1].first_pair == t.first_pair && tensors[i - 1].pairs == t.pairs;
             const int room = PAIRS - used;
             if (!there && room == 0) break;
-            const int take = there || t.pairs - done < room ? t.pairs - done : room, fresh = there ? 0 : take, at = there ? last->first_pair : used;
-            const long long pieces = (t.row_bytes + CR_PIECE - 1) / CR_PIECE;
-            const long long need = pieces * t.sets * take;
-            if (need == 0) { done = t.pairs; continue; }
-            RDL_REQUIRE(pieces <= 0x7fffffffLL && need + blocks <= 0x7fffffffLL, "copy_rows: more than one launch can copy");
+            const long long pieces = cr_pieces(t), of_row = pieces * t.sets;
+            if (of_row == 0 || t.pairs == 0) { done = t.pairs; continue; }
+            const long long fit = (CR_MAX_BLOCKS - blocks) / of_row;                 // rows that this launch has blocks for
+            if (fit == 0) break;
+            int take = there || t.pairs - done < room ? t.pairs - done : room;
+            if (take > fit) take = (int)fit;
+            const int fresh = there ? 0 : take, at = there ? last->first_pair : used;
             const uintptr_t all = (uintptr_t)t.base | (uintptr_t)t.set_stride | (uintptr_t)t.row_stride | (uintptr_t)t.row_bytes;
             CrTensor& c = a.tensor[a.n_tensors++];
             c = {(char*)t.base, t.set_stride, t.row_stride, t.row_bytes, (int)pieces, at, take, blocks, all & 15 ? (int)(all & (~all + 1)) : 16};
@@ -105,7 +109,7 @@ int cr_run(const CopyRowsTensor* tensors, int n_tensors, const int* pairs, cudaS
             for (int k = 0; k < fresh; ++k) a.pair[at + k] = make_int2(src[k], dst[k]);
             if (take == t.pairs) last_whole = i;
             used += fresh;
-            blocks += (unsigned)need;
+            blocks += (unsigned)(of_row * take);
             done += take;
         }
         if (blocks) RDL_CHECK_EX(rdl_launch(copy_rows_kernel<PAIRS>, dim3(blocks), dim3(CR_THREADS), 0, st, a), "copy_rows");
@@ -121,6 +125,7 @@ extern "C" int rdl_copy_rows(const CopyRowsTensor* tensors, int n_tensors, const
     for (int i = 0; i < n_tensors; ++i) {
         const CopyRowsTensor& t = tensors[i];
         RDL_REQUIRE(t.sets >= 0 && t.pairs >= 0 && t.row_bytes >= 0 && (t.base || !t.row_bytes || !t.pairs || !t.sets), "copy_rows: bad tensor %d", i);
+        RDL_REQUIRE(cr_pieces(t) == 0 || t.sets <= CR_MAX_BLOCKS / cr_pieces(t), "copy_rows: tensor %d has rows that a launch has no blocks for", i);
         total += t.pairs;
     }
     RDL_REQUIRE(total == 0 || pairs, "copy_rows: missing list");

@@ -403,6 +403,17 @@ def test_refused_copies():
     assert not t.any()
 
 
+def test_rows_that_no_launch_has_blocks_for_are_refused_before_anything_is_copied():
+    import ctypes
+    from rust_deeplearning_b200.kernels import library
+    pack = ops._copy_tensor
+    fine, large = pack(256, 64, 64, 64, 1, 0, 1, 0), pack(4096, 1 << 20, 1 << 20, 65536, 2 ** 31 - 1, 0, 1, 0)
+    pairs = (ctypes.c_int * 2)(0, 1)
+    for tensors in ([large], [fine, large]):
+        with pytest.raises(KernelError, match="no blocks"):
+            library.check(library.load().rdl_copy_rows(b"".join(tensors), len(tensors), ctypes.addressof(pairs), None))
+
+
 def test_refused_scoring_calls():
     z = torch.zeros((3, 10))
     ids = torch.zeros(3, dtype=torch.int32)

@@ -461,3 +461,16 @@ def test_copies_beyond_32_bits_and_in_a_graph():
     assert int(t[:, 0].max()) == 0
     g.replay()
     assert torch.equal(t[:, 0], t[:, 2]) and int(t[0, 0, -1]) == 7 and int(t[:, 1].max()) == 0
+
+
+def test_more_rows_than_a_launch_has_blocks_for():
+    """2^31 and more blocks of a byte each: the list is divided where the blocks end, and the tensor behind it, which shares the list, goes on."""
+    sets, pairs = 1 << 20, 2100
+    t = torch.zeros((sets, 2 * pairs), dtype=torch.uint8, device=DEV)        # 4.4 GB
+    t[:, :pairs] = (torch.arange(pairs, device=DEV) % 251 + 1).to(torch.uint8)
+    t[:, :pairs] += (torch.arange(sets, device=DEV) % 5).to(torch.uint8)[:, None]
+    small = torch.randn((2, 2 * pairs, 5), device=DEV)
+    src, dst = list(range(pairs)), list(range(pairs, 2 * pairs))
+    want = moved(small, src, dst)
+    ops.copy_rows([(t, src, dst), (small, src, dst)])
+    assert torch.equal(t[:, pairs:], t[:, :pairs]) and torch.equal(small, want)
