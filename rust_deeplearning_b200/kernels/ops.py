@@ -1178,6 +1178,10 @@ def sample(logits: torch.Tensor, *, temperature: float, top_k: Optional[int] = N
 
 _F32 = torch.finfo(torch.float32)
 LOGPROBS_MAX_TOP = 32    # alternatives a row can be asked for
+# Rows of an odd width up to which `linear_logprobs` leaves the product to `linear`, which takes it to the library; above, both operands are copied to whole
+# 16 bytes a row for the kernel.  Widths of 2,300: 129 rows, 32,000 tokens 145 us by `linear`, 245 copied; 257 rows 246 and 263; 257 x 1,003 x 256,000 1,508 and
+# 852; 2,048 rows, 256,000 tokens 10,332 and 3,110 (of which the copy 1,500).
+LOGPROBS_ODD_ROWS = 256
 # float32 logits that `linear_logprobs` holds at a time where the product has a kernel of its own
 LOGPROBS_PIECE = 1 << 26
 
@@ -1244,12 +1248,20 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     return out
 
 
+def _wide_rows(t: torch.Tensor) -> torch.Tensor:
+    """A bfloat16 matrix as the tensor-core kernels take it: rows of whole 16 bytes from a 16-byte boundary on (else a copy, zeros behind its columns)."""
+    short = -t.shape[1] % 8
+    if short:
+        return torch.nn.functional.pad(t, (0, short))
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = None, top: int = 0, softcap: Optional[float] = None,
                     scale: float = 1.0, status: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """`token_logprobs` of the logits scale * softcap(x W^T) of rows x [rows, in] behind an output head [vocab, in] (a tensor of x's type, or
     `Mx4Weight`), without keeping the logits.
 
-    More than 16 bfloat16 rows that meet `linear`'s alignment rules run in one kernel that forms the statistics as it takes the products out of
+    More than 16 bfloat16 rows that meet `linear`'s alignment rules, and more than 256 that do not (by way of copies that do), run in one kernel that forms the statistics as it takes the products out of
     tensor memory (its work space: a few MB, up to 250 MB for 32 alternatives); others form pieces of the logits by `linear`, 256 MB
     at a time.  softcap: cap * tanh(. / cap) of the products, before scale (both numbers that float32 holds).  The weight is a constant, as `linear` has it."""
     _need(x.dim() == 2 and len(weight.shape) == 2 and x.shape[1] == weight.shape[1] and x.shape[1] > 0,
@@ -1265,9 +1277,10 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
     _logprobs_check("linear_logprobs", rows, vocab, x.device, targets, top)
     _stream(x)
     out = _logprobs_result(x.device, rows, top, targets)
-    if rows > SKINNY_MAX_ROWS and type(weight) is not Mx4Weight and _bf16_ok(x, weight):
+    if type(weight) is not Mx4Weight and x.dtype is torch.bfloat16 and rows > (SKINNY_MAX_ROWS if _bf16_ok(x, weight) else LOGPROBS_ODD_ROWS):
         lib = library.load()
         with _on_device(x.device.index):
+            x, weight = _wide_rows(x), _wide_rows(weight)
             work = torch.empty(lib.rdl_linear_logprobs_work_bytes(rows, vocab, top), dtype=torch.uint8, device=x.device)
             library.check(lib.rdl_linear_logprobs(_ptr(x), _ptr(weight), rows, vocab, x.shape[1], _ptr(targets), top, float(softcap or 0.0), float(scale),
                                                   _ptr(out.logprobs), _ptr(out.entropy), _ptr(out.top_logprobs), _ptr(out.top_ids), _ptr(work),

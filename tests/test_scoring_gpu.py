@@ -474,3 +474,19 @@ def test_more_rows_than_a_launch_has_blocks_for():
     want = moved(small, src, dst)
     ops.copy_rows([(t, src, dst), (small, src, dst)])
     assert torch.equal(t[:, pairs:], t[:, :pairs]) and torch.equal(small, want)
+
+
+@pytest.mark.parametrize("rows,width,vocab,shift", [(300, 63, 900, 0), (257, 1003, 50, 0), (300, 64, 900, 1), (600, 7, 2000, 0)])
+def test_many_rows_of_odd_widths_take_the_kernel(monkeypatch, rows, width, vocab, shift):
+    """Widths that are no multiple of 8, and operands that start anywhere: sums that are exact, and no library product."""
+    g = torch.Generator().manual_seed(rows + width)
+    x, w = torch.empty(rows * width + shift, dtype=torch.bfloat16, device=DEV)[shift:], torch.empty(vocab * width + shift, dtype=torch.bfloat16, device=DEV)[shift:]
+    x, w = x.view(rows, width), w.view(vocab, width)
+    x.copy_(torch.randint(-3, 4, (rows, width), generator=g))
+    w.copy_(torch.randint(-2, 3, (vocab, width), generator=g) / 16)
+
+    def refuse(*args, **kw):
+        raise AssertionError("a library product")
+    monkeypatch.setattr(torch, "mm", refuse)
+    t = targets_of(rows, vocab, 6)
+    ref.check(ops.linear_logprobs(x, w, t, 7), f64(x) @ f64(w).T, t.cpu().numpy(), 7, "an odd width")
