@@ -155,13 +155,15 @@ class Engine:
             if len(following) != len(tokens) or any(f.size != 1 for f in following):
                 raise StepError("`following` must name a token for every sequence")
             want, targets = "all", [a for t, f in zip(tokens, following) for a in (t[1:], f)]
-        targets = np.concatenate([t for t in targets if t.size] or [np.zeros(0, np.int64)])
-        if targets.size and (targets.dtype.kind not in "iu" or targets.min() < 0 or targets.max() >= self.model.vocab_size):
+        targets = [t for t in targets if t.size]
+        # each by itself: together, arrays of int64 and uint64 would become float64
+        if any(t.dtype.kind not in "iu" or t.min() < 0 or t.max() >= self.model.vocab_size for t in targets):
             raise StepError(f"token ids must be whole numbers inside the vocabulary of {self.model.vocab_size}")
+        targets = np.concatenate([t.astype(np.int32) for t in targets] or [np.zeros(0, np.int32)])
         most = min(ops.LOGPROBS_MAX_TOP, self.model.vocab_size)
         if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= most:
             raise StepError(f"top must be a whole number from 0 to {most}")
-        return self._step(slots, tokens, want, None, (targets.astype(np.int32), top))
+        return self._step(slots, tokens, want, None, (targets, top))
 
     def _step(self, slots, tokens, want, fed, scored):
         n = len(slots)

@@ -274,6 +274,16 @@ def test_scoring_refusals(tmp_path, monkeypatch):
     assert score(engine, []) == []
 
 
+def test_ids_of_different_whole_types(tmp_path, monkeypatch):
+    engine, cfg, w = build(tmp_path, "A", monkeypatch)
+    scoring_refs.install(monkeypatch)
+    a, b = engine.new_sequence(), engine.new_sequence()
+    got = engine.score([a, b], [np.array([5, 6, 7], dtype=np.uint64), np.array([8, 9], dtype=np.int8)], following=[3, np.uint64(4)])
+    c, d = engine.new_sequence(), engine.new_sequence()
+    want = engine.score([c, d], [[5, 6, 7], [8, 9]], following=[3, 4])
+    assert got.logprobs.shape == (5,) and torch.equal(got.logprobs, want.logprobs)
+
+
 @pytest.mark.parametrize("name", ["A", "B"])
 def test_several_continuations_equal_as_many_requests(tmp_path, monkeypatch, name):
     engine, cfg, w = build(tmp_path, name, monkeypatch, max_tokens=512, max_seqs=6)
