@@ -661,8 +661,10 @@ void plan(HeadArgs& a, int rows, int vocab, int ctas) {
     a.main_tiles = mains == a.groups ? a.tiles_n : (int)((long long)a.tiles_n * mains / a.groups);
 }
 int rows_at_once(int ctas) { return (rdl_sm_count() / ctas > 0 ? rdl_sm_count() / ctas : 1) * BM * ctas; }
-// Pairs from 129 rows on, but for three blocks of 128: as two of 256 a quarter of the products are for nobody (384 rows, 20 alternatives: 490 us
-// by pairs, 430 without; 300 rows 480 and 420).  Blocks without a partner fetch half as much again (2,048 rows: 1.8 ms by pairs, 2.0 without).
+// Pairs from 129 rows on, but for three blocks of 128: as two of 256 a quarter of the products are for nobody (300 rows by pairs and without, 2,304 x
+// 256,000: 382 and 342 us, 2,304 x 32,000 55 and 53, 256 x 30,000 20 and 18, 256 x 3,000 10.5 and 8.9; 384 rows within 0.3 us of each other at the
+// smallest).  Blocks without a partner fetch half as much again (129 rows, 2,304 x 256,000: 218 us by pairs, 245 without; 200 rows, 256 x 30,000 with 20
+// alternatives, where products are the least of it, 37 and 34; 2,048 rows 1.8 ms by pairs and 2.0 without).
 int ctas_for(int rows) { return rows <= BM || (rows > 2 * BM && rows <= 3 * BM) ? 1 : 2; }
 // the rows of a launch: all, or equal parts where there are more row blocks than groups
 int rows_a_launch(int rows, int ctas) {
