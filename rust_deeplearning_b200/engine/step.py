@@ -36,8 +36,15 @@ def _next_pow2(n: int) -> int:
 _retired: List[tuple] = []
 
 
+def _over(event) -> bool:
+    try:
+        return event is not None and event.query()
+    except Exception:                  # recorded into a graph that captured the engine's stream: nobody can tell
+        return False
+
+
 def _release_retired():
-    _retired[:] = [r for r in _retired if r[1] is None or not r[1].query()]
+    _retired[:] = [r for r in _retired if not _over(r[1])]
 
 
 class _Graph:

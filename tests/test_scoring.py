@@ -387,6 +387,23 @@ def test_a_dropped_engine_waits_for_its_uploads(tmp_path, monkeypatch):
     assert len(waited) == 2
 
 
+def test_status_words_nobody_can_vouch_for_are_kept(monkeypatch):
+    from rust_deeplearning_b200.engine import step
+
+    class Event:
+        def __init__(self, answer):
+            self.answer = answer
+
+        def query(self):
+            if self.answer is None:
+                raise RuntimeError("the event was captured")
+            return self.answer
+    kept = [("a", Event(False)), ("b", None), ("c", Event(None))]
+    monkeypatch.setattr(step, "_retired", [kept[0], ("d", Event(True)), kept[1], kept[2]])
+    step._release_retired()
+    assert step._retired == kept
+
+
 def test_perplexity():
     from rust_deeplearning_b200 import ScoredText
     inf = float("inf")
