@@ -1261,9 +1261,10 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
     """`token_logprobs` of the logits scale * softcap(x W^T) of rows x [rows, in] behind an output head [vocab, in] (a tensor of x's type, or
     `Mx4Weight`), without keeping the logits.
 
-    More than 16 bfloat16 rows that meet `linear`'s alignment rules, and more than 256 that do not (by way of copies that do), run in one kernel that forms the statistics as it takes the products out of
-    tensor memory (its work space: a few MB, up to 250 MB for 32 alternatives); others form pieces of the logits by `linear`, 256 MB
-    at a time.  softcap: cap * tanh(. / cap) of the products, before scale (both numbers that float32 holds).  The weight is a constant, as `linear` has it."""
+    More than 16 bfloat16 rows that meet `linear`'s alignment rules, and more than 256 that do not (by way of copies that do), run in one kernel
+    that forms the statistics as it takes the products out of tensor memory.  Its work space goes by the device's blocks rather than by the rows: 1 MB without
+    alternatives, 25 to 50 MB for five, 130 to 260 MB for 32.  Others form pieces of the logits by `linear`, 256 MB at a time.  softcap: cap * tanh(. / cap) of
+    the products, before scale (both numbers that float32 holds).  The weight is a constant, as `linear` has it."""
     _need(x.dim() == 2 and len(weight.shape) == 2 and x.shape[1] == weight.shape[1] and x.shape[1] > 0,
           f"linear_logprobs: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not fit")
     _need(type(weight) is Mx4Weight or x.dtype is weight.dtype, "linear_logprobs: rows and weight of one type")
@@ -1294,6 +1295,7 @@ def linear_logprobs(x: torch.Tensor, weight, targets: Optional[torch.Tensor] = N
             if scale != 1.0:
                 scale_(z, scale)
             _token_logprobs(z, targets, out, r, top, status)
+            del z                                # before the next piece is made
     return out
 
 
@@ -1330,7 +1332,8 @@ def copy_rows(moves):
 
     Tensors are [sets, rows, ...] (the pages of a cache, or its states, of all layer runs) of any type, on one device; a row's own
     elements are contiguous, sets and rows may lie apart.  src and dst are lists of row numbers on the host, read before the call returns.  No
-    row may be the destination of two copies, or source of one and destination of another, and the tensors may not overlap."""
+    row may be the destination of two copies, or source of one and destination of another, and no tensor may begin before another one ends (two that
+    interleave are refused even where they share no byte: give them as one)."""
     moves = list(moves)
     if not moves:
         return

@@ -490,3 +490,17 @@ def test_many_rows_of_odd_widths_take_the_kernel(monkeypatch, rows, width, vocab
     monkeypatch.setattr(torch, "mm", refuse)
     t = targets_of(rows, vocab, 6)
     ref.check(ops.linear_logprobs(x, w, t, 7), f64(x) @ f64(w).T, t.cpu().numpy(), 7, "an odd width")
+
+
+def test_pieces_of_logits_are_held_one_at_a_time(monkeypatch):
+    x, w = head_case(1200, 320, 5000, torch.bfloat16, 22)
+    packed = ops.pack_mx4(w)
+    monkeypatch.setattr(ops, "LOGPROBS_PIECE", 400 * 5000)
+    want = ops.linear_logprobs(x, packed, None, 3)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = ops.linear_logprobs(x, packed, None, 3)
+    # a piece of logits is 8 MB; its rows in 8 bits and the results are less than one
+    assert torch.cuda.max_memory_allocated() - held < 10e6
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
