@@ -588,7 +588,8 @@ long long rdl_linear_logprobs_work_bytes(int rows, int vocab, int top);
 
 // Rows copied within tensors: row dst of every set becomes row src, for each tensor's list of pairs: list + 2 first_pair holds
 // `pairs` sources, then as many destinations; tensors may share a list.  Strides in bytes, tensors and list in host memory (read before the call returns).  No destination may be a source or
-// another pair's destination, and tensors may not overlap; row numbers are the caller's to check.
+// another pair's destination, and tensors may not overlap; row numbers are the caller's to check.  A tensor whose one row takes more than 2^31 - 1 blocks of 32 KB,
+// over all sets, is refused before anything is copied.
 #define RDL_COPY_ROWS_MAX_TENSORS 64
 typedef struct {
     void* base;

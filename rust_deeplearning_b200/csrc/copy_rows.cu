@@ -1,8 +1,8 @@
 // Rows of tensors copied within them: in tensors [sets][rows][...], row dst[i] of every set becomes row src[i] of that set, for several
 // tensors and lists of rows in one launch (the pages and states of a cache, of all layer runs).
 //
-// Nothing but memory bounds it: 872 MB in keys and values of 26 layers copied in 257 us, 6.8 TB/s read and written; a page of 13 layers in 2.7 us, a
-// launch and a trip to memory.  The description (where each tensor lies, which rows) travels in the kernel's parameters, so that
+// Nothing but memory bounds it: 872 MB in keys and values of 26 layers copied in 257 us, 6.8 TB/s read and written (calls in a graph; a
+// call among others 266); a page of 13 layers in 2.2 us, a launch and a trip to memory.  The description (where each tensor lies, which rows) travels in the kernel's parameters, so that
 // nothing has to be copied to the device ahead of it and nothing in host memory has to outlive the call.
 #include "api.h"
 #include "common.cuh"

@@ -4,10 +4,11 @@
 // or 8 where there are fewer rows than the device has room for blocks.  A thread copies what it looks at into shared memory of its own,
 // LP_RING batches ahead (cp.async), so that memory is kept busy while lists are sorted, and no thread waits for another's copy.
 //
-// Measured in a row of calls on the device: 2,048 rows of 256,000, float32 299 us without alternatives (7.0 TB/s), 295 with five, 314 with 20 (a logit
-// takes 12 to 16 instructions, so that the multiprocessors are busy three quarters of the time); bfloat16 195 and 231, bound by those instructions;
-// seconds of it at 1,000 W, float32 355 with five.  8,192 rows of 32,000, float32 151 us, 165 and 216; of 1,000 9, 20 and 31 us.  One row of 32,000
-// 6.1 us; eight of 256,000 6.2 us, with 20 alternatives 11.4: latency, of the lists at last.
+// Measured, calls in a graph, replayed once a while and (behind the stroke) for seconds, at the clock then sampled: 2,048 rows of 256,000, float32 303 / 302 us
+// without alternatives (6.9 TB/s; 1.60 GHz), 314 / 322 with five (1.69), 323 / 345 with 20 (1.74; a logit takes 12 to 16 instructions, so that the
+// multiprocessors are busy three quarters of the time); bfloat16 215 / 207, 240 / 229 and 322 / 309, at 1.85 to 1.97 GHz: those instructions.  8,192 rows of
+// 32,000, float32 154, 173 and 231 us; of 1,000 10, 20 and 29 us.  One row of 32,000 3.9 us, with five alternatives 6.3; eight of 256,000 6.2 us, with 20 12:
+// latency, of the lists at last.
 #include "api.h"
 #include "launch.cuh"
 #include "logprobs.cuh"

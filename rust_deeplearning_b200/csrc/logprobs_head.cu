@@ -16,10 +16,11 @@
 // tensor memory, half of the columns each, a row a thread.  Logits that may be among a row's largest are put aside in memory (`seen` below
 // says which), and the second kernel looks among them.
 //
-// Measured, 256,000 tokens, k 2,304, soft-cap: 8,192 rows and five alternatives 6.5 ms, 1.48 PFLOP/s; 2,048 rows, none, 1.56 ms, 1.54 PFLOP/s: a
-// tile's products take 18,432 cycles and a tile 18,450 to 19,500, at the clock that the power limit leaves (1.25 to 1.4 GHz).  What
-// is done with a tile takes 5,000 cycles (9,000 with a soft-cap, up to 15,000 with alternatives) beside them.  64 rows: 190 us, 208 with
-// alternatives (a kernel more, a longer second kernel), 6.2 and 5.7 TB/s of weights.
+// Measured, 256,000 tokens, k 2,304, soft-cap, calls in a graph, replayed once a while and (behind the stroke) for seconds: 8,192 rows and five alternatives
+// 5.5 / 6.3 ms, 1.75 / 1.54 PFLOP/s; 2,048 rows, none, 1.37 / 1.58 ms, 1.76 / 1.53 PFLOP/s.  Over seconds the power limit leaves 1.43 to 1.49 GHz
+// (sampled), at which a tile takes 20,600 to 21,700 cycles, its products 18,432.  What is done with a tile takes 5,000 cycles (9,000 with a soft-cap, up to
+// 15,000 with alternatives) beside them.  64 rows: 187 us, 202 with 20 alternatives (a kernel more, a longer second kernel), 6.3 and 5.9 TB/s of weights.
+// With alternatives a thread would like more than its 168 registers (three warps on a scheduler): 160 bytes a thread go to memory and back.
 //
 // Every wait is bounded; a block that gives up sets `status` and every path ends in the common tear-down.  A block takes all of a
 // multiprocessor's shared memory (see "Tensor memory" in mx_tensor.cuh: nothing that holds tensor memory fits beside it).
