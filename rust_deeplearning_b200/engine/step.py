@@ -33,7 +33,7 @@ def _next_pow2(n: int) -> int:
 
 # Status words of engines that were dropped, each with an event behind the engine's last step: a kernel of it that is still to run may write its
 # word, and the allocator of pinned memory, which knows nothing of that, must not hand it to anybody else.
-_retired: List[tuple] = []
+_retired: Dict[int, tuple] = {}         # by the word's address; engines may be dropped (by any thread, by the collector) while it is gone through
 
 
 def _over(event) -> bool:
@@ -44,7 +44,9 @@ def _over(event) -> bool:
 
 
 def _release_retired():
-    _retired[:] = [r for r in _retired if not _over(r[1])]
+    for address, (_, event) in list(_retired.items()):
+        if _over(event):
+            _retired.pop(address, None)
 
 
 class _Graph:
@@ -104,7 +106,7 @@ class Engine:
                 event.record(self._last_stream)
             except Exception:
                 event = None           # kept for good
-            _retired.append((self.status, event))
+            _retired[self.status.data_ptr()] = (self.status, event)
 
     # ---- sequences ----
     def new_sequence(self) -> int:

@@ -108,11 +108,11 @@ def test_the_status_word_of_a_dropped_engine_is_nobody_elses():
             torch.cuda._sleep(200_000_000)                   # stands for what is left of the step: a tenth of a second
         del eng
         held = [torch.zeros(1, dtype=torch.int32).pin_memory() for _ in range(20)]
-        assert all(t.data_ptr() != word for t in held) and any(r[0].data_ptr() == word for r in step._retired)
+        assert all(t.data_ptr() != word for t in held) and word in step._retired
         torch.cuda.synchronize()
         del held
         other = Engine(model, max_tokens=64)
-        assert not any(r[0].data_ptr() == word for r in step._retired)
+        assert word not in step._retired
         other.check_status()
 
 

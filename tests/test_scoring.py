@@ -398,10 +398,22 @@ def test_status_words_nobody_can_vouch_for_are_kept(monkeypatch):
             if self.answer is None:
                 raise RuntimeError("the event was captured")
             return self.answer
-    kept = [("a", Event(False)), ("b", None), ("c", Event(None))]
-    monkeypatch.setattr(step, "_retired", [kept[0], ("d", Event(True)), kept[1], kept[2]])
+    kept = {1: ("a", Event(False)), 3: ("b", None), 4: ("c", Event(None))}
+    monkeypatch.setattr(step, "_retired", {**kept, 2: ("d", Event(True))})
     step._release_retired()
     assert step._retired == kept
+
+
+def test_an_engine_dropped_while_status_words_are_gone_through(monkeypatch):
+    from rust_deeplearning_b200.engine import step
+
+    class Event:
+        def query(self):
+            step._retired[9] = ("another engine's", None)      # as the collector may do at any time
+            return True
+    monkeypatch.setattr(step, "_retired", {1: ("a", Event()), 2: ("b", Event())})
+    step._release_retired()
+    assert step._retired == {9: ("another engine's", None)}
 
 
 def test_perplexity():
